@@ -382,6 +382,104 @@ int qq_kv_scatter(void* k_layer, void* v_layer, int buf_dtype, int64_t kv_rows, 
                   const void* v, int src_dtype, const int64_t* locs, int n, int64_t row_elems,
                   void* stream);
 
+/* ------------------------------------------------- paged rows (blocks of 64 tokens)
+ * The device form of TokenToKVPoolAllocator.alloc / free with ReqToTokenPool
+ * (src/qwenquest/memory.py:28-76) for rows handed out in blocks of 64: block b is pool rows
+ * 64 b .. 64 b + 63, block 0 is padding.  held [max_reqs] counts a request's blocks,
+ * block_table [max_reqs, block_table_stride] lists them; the free blocks are a stack,
+ * free_blocks[0 .. *free_count), of free_cap entries. */
+
+/* Rows for the next new_lens[i] tokens of request req_pool_indices[i] behind its first
+ * lens[i]: the blocks it lacks for lens[i] + new_lens[i] tokens come off the stack (request
+ * order, then block order), block_table and held are brought up to date, and for every new
+ * token, request after request, loc gets its row, pos its position and
+ * req_to_token[request, position] its row; loc and pos past the requests' tokens get 0 (the
+ * padding row).  new_lens NULL: a decode batch, one token at position lens[i] - 1 each
+ * (total == bs; an entry with lens[i] < 1 is padding and gets row 0).  An entry without new
+ * tokens is ignored.  Asked again for the same lengths it takes nothing and answers the same.
+ * Refused as a whole, on the device, with every loc and pos 0 and nothing taken: bit 1 of
+ * *error_flags (and of error_mirror, device-accessible host memory, or NULL) when the stack
+ * has too few blocks, 2 for a request or a length outside its table, 4 for a request listed
+ * twice, 8 for more than `total` tokens.  workspace: qq_block_workspace_bytes(bs), this call's
+ * alone until its launches are done; a decode batch needs none. */
+int qq_block_assign(const int64_t* req_pool_indices, const int64_t* lens, const int64_t* new_lens, int bs,
+                    int64_t total, int32_t* block_table, int64_t block_table_stride, int32_t* req_to_token,
+                    int64_t req_to_token_stride, int64_t max_context_len, int max_reqs, int32_t* held,
+                    int32_t* free_blocks, int32_t* free_count, int64_t free_cap, int64_t* loc, int64_t* pos,
+                    int32_t* error_flags, int32_t* error_mirror, void* workspace, int64_t workspace_bytes,
+                    void* stream);
+
+/* The listed requests' blocks back on the stack (what assigning them in this order took off
+ * it lies there as before), their block_table entries and req_to_token positions cleared,
+ * held 0.  Refused as a whole with bits 2, 4 and 8 (more blocks than the stack has room for). */
+int qq_block_release(const int64_t* req_pool_indices, int bs, int32_t* block_table, int64_t block_table_stride,
+                     int32_t* req_to_token, int64_t req_to_token_stride, int64_t max_context_len, int max_reqs,
+                     int32_t* held, int32_t* free_blocks, int32_t* free_count, int64_t free_cap,
+                     int32_t* error_flags, int32_t* error_mirror, void* workspace, int64_t workspace_bytes,
+                     void* stream);
+int64_t qq_block_workspace_bytes(int bs);
+
+/* ---------------------------------------------------------- 8-bit K/V cache
+ * A cache of num_blocks blocks of 64 tokens (block 0 is padding: never written): of each
+ * layer k_codes / v_codes [num_blocks, kv_heads, 64 * head_dim] e4m3 codes in the kernels'
+ * order (csrc/qq_fp8.h) and k_scale / v_scale [num_blocks, kv_heads] floats, powers of two;
+ * a value is code * scale.  head_dim 64 or 128.  Pool row r is token r % 64 of block r / 64. */
+
+/* The form of MHATokenToKVPool.set_kv_buffer (src/qwenquest/memory.py:114-120) for this
+ * cache: k[i], v[i] ([n, kv_heads, head_dim] bf16 or fp32, 16-byte aligned) go to row loc[i].
+ * Per (block, head), K and V apart: the scale becomes 2^e, e the largest of its exponent
+ * before and the least e >= -110 with max |value written| <= 448 * 2^e; codes are rounded to
+ * nearest even; when e grows the block's other codes are re-rounded.  A call that writes a
+ * block's first row begins the block: its earlier codes (set to 0) and scale are void.  A
+ * value that is not finite makes the scale NaN until the block is begun again.  Rows of
+ * block 0 and outside the cache are skipped.  The entries of one block stand next to each
+ * other in loc (two runs of one block in a call leave it undefined); of a row listed twice
+ * in a run the last entry counts. */
+int qq_fp8_store(uint8_t* k_codes, uint8_t* v_codes, float* k_scale, float* v_scale, int num_blocks,
+                 int kv_heads, int head_dim, const void* k, const void* v, int src_dtype, const int64_t* loc,
+                 int64_t n, void* stream);
+
+/* k[i], v[i] = the values of row loc[i] ([n, kv_heads, head_dim]; exact in bf16 as in fp32);
+ * NaN for a row outside the cache. */
+int qq_fp8_rows(const uint8_t* k_codes, const uint8_t* v_codes, const float* k_scale, const float* v_scale,
+                int num_blocks, int kv_heads, int head_dim, const int64_t* loc, int64_t n, void* k, void* v,
+                int dst_dtype, void* stream);
+
+/* Page bounds (page_k_bounds, as qq_quest_prefill_bounds writes them) from the cache's codes
+ * for n_layers layers, the cache and the bounds given from the first of them (layer strides in
+ * elements): of request req_pool_indices[i] the pages [prefix_lens[i] / 64, seq_lens[i] / 64)
+ * (prefix_lens NULL: from 0; max_new, if not 0, is at least every seq - prefix), or with
+ * decode != 0 the page that the token at seq_lens[i] - 2 completes, if it does
+ * (src/qwenquest/quest.py:231-280 and 284-321 in one form: nothing runs along).  Blocks come
+ * from block_table; requests outside it are skipped, a block outside the cache gives NaN. */
+int qq_fp8_page_bounds(const uint8_t* k_codes, int64_t codes_layer_stride, const float* k_scale,
+                       int64_t scale_layer_stride, int num_blocks, int kv_heads, int head_dim,
+                       const int32_t* block_table, int64_t block_table_stride, int block_table_rows,
+                       int block_table_cols, const int64_t* req_pool_indices, const int64_t* seq_lens,
+                       const int64_t* prefix_lens, int bs, int decode, int64_t max_new, int n_layers,
+                       uint16_t* page_k_bounds, int max_reqs, int max_pages, void* stream);
+
+/* One layer's decode over the 8-bit cache (src/qwenquest/attention/dense.py:26-42 and
+ * quest_only.py:149-159 over it): with k_new the new tokens are stored first
+ * (qq_fp8_store(k_new, v_new, out_cache_loc), [bs, kv_heads, head_dim] new_dtype); then
+ * request i's q[i] ([bs, H, head_dim] bf16 or fp32, 16-byte aligned, batch stride a multiple
+ * of 8 elements) attends positions 0 .. seq_lens[i] - 1, or with `positions` and
+ * seq_lens[i] > top_k the pages positions[i, 64 u] / 64, u < top_k / 64 - 1, and the last 64
+ * positions (the layout of qq_quest_retrieve_topk; duplicates counted).  out [bs, H * head_dim]
+ * in q's dtype: zeros for an empty context; NaN for a request outside the table, and where a
+ * block is padding or outside the cache.  A context is cut to the table's columns.  Any
+ * H / kv_heads.  workspace: qq_fp8_decode_workspace_bytes, of any contents, this call's alone
+ * until its launches are done. */
+int qq_fp8_decode_attention(const void* q, int q_dtype, int64_t q_batch_stride, int num_q_heads,
+                            const void* k_new, const void* v_new, int new_dtype, const int64_t* out_cache_loc,
+                            uint8_t* k_codes, uint8_t* v_codes, float* k_scale, float* v_scale, int num_blocks,
+                            int kv_heads, int head_dim, const int32_t* block_table, int64_t block_table_stride,
+                            int block_table_rows, int block_table_cols, const int64_t* req_pool_indices,
+                            const int64_t* seq_lens, int bs, const int32_t* positions, int64_t positions_stride,
+                            int top_k, float scale, void* out, void* workspace, int64_t workspace_bytes,
+                            void* stream);
+int64_t qq_fp8_decode_workspace_bytes(int bs, int num_q_heads, int kv_heads, int head_dim);
+
 /* ------------------------------------------------------------- HiSparse tier
  * Layouts of the reference HiSparseCoordinator (src/qwenquest/hisparse/coordinator.py:103-131):
  * device_k/v[layer] [R*(buf+1), KV, D] (request r owns rows r*(buf+1) + slot,

@@ -101,6 +101,24 @@ SIGNATURES: dict[str, tuple] = {
     ),
     "qq_extend_attention_workspace_bytes": (_L, [_L, _I, _I, _I, _L]),
     "qq_kv_scatter": (_I, [_P, _P, _I, _L, _P, _P, _I, _P, _I, _L, _P]),
+    "qq_block_assign": (
+        _I,
+        [_P, _P, _P, _I, _L, _P, _L, _P, _L, _L, _I, _P, _P, _P, _L, _P, _P, _P, _P, _P, _L, _P],
+    ),
+    "qq_block_release": (_I, [_P, _I, _P, _L, _P, _L, _L, _I, _P, _P, _P, _L, _P, _P, _P, _L, _P]),
+    "qq_block_workspace_bytes": (_L, [_I]),
+    "qq_fp8_store": (_I, [_P, _P, _P, _P, _I, _I, _I, _P, _P, _I, _P, _L, _P]),
+    "qq_fp8_rows": (_I, [_P, _P, _P, _P, _I, _I, _I, _P, _L, _P, _P, _I, _P]),
+    "qq_fp8_page_bounds": (
+        _I,
+        [_P, _L, _P, _L, _I, _I, _I, _P, _L, _I, _I, _P, _P, _P, _I, _I, _L, _I, _P, _I, _I, _P],
+    ),
+    "qq_fp8_decode_attention": (
+        _I,
+        [_P, _I, _L, _I, _P, _P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _P, _L, _I, _I, _P, _P, _I, _P, _L, _I, _F,
+         _P, _P, _L, _P],
+    ),
+    "qq_fp8_decode_workspace_bytes": (_L, [_I, _I, _I, _I]),
     "qq_hisparse_swap_in": (
         _I,
         [_P, _L, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _L, _P, _P, _P, _P, _L, _L, _P, _P, _P,

@@ -14,6 +14,7 @@ import torch
 from torch.autograd import forward_ad
 
 from qwenquest_amd.attention.ops import extend_attention, extend_attention_batch, extend_attention_batch_checked
+from qwenquest_amd.paged import BlockReqToTokenPool, Fp8TokenToKVPool
 
 if TYPE_CHECKING:
     from qwenquest_amd.batch import ForwardBatch
@@ -40,6 +41,14 @@ class AttentionBackend(ABC):
     def __init__(self, req_to_token_pool: ReqToTokenPool, token_to_kv_pool: MHATokenToKVPool):
         self.req_to_token_pool = req_to_token_pool
         self.token_to_kv_pool = token_to_kv_pool
+        #: whether the pool holds 8-bit blocks
+        self.fp8 = isinstance(token_to_kv_pool, Fp8TokenToKVPool)
+        if self.fp8:
+            if not isinstance(req_to_token_pool, BlockReqToTokenPool):
+                raise ValueError("an Fp8TokenToKVPool needs a BlockReqToTokenPool")
+            if req_to_token_pool.num_blocks > token_to_kv_pool.num_blocks:
+                raise ValueError(f"the request pool hands out {req_to_token_pool.num_blocks} blocks, the K/V pool has "
+                                 f"{token_to_kv_pool.num_blocks}")
 
     @property
     def req_to_token(self) -> torch.Tensor:
@@ -66,6 +75,8 @@ class AttentionBackend(ABC):
         assert batch.out_cache_loc is not None and batch.extend_prefix_lens is not None
         pool = self.token_to_kv_pool
         pool.set_kv_buffer(layer.layer_id, batch.out_cache_loc, k, v)
+        if self.fp8:
+            return self._forward_extend_fp8(q, layer, batch)
         k_buf, v_buf = pool.get_kv_buffer(layer.layer_id)
         if self._extend_fast(q, k_buf, v_buf, layer.scaling, batch):
             attend = (extend_attention_batch if torch.cuda.is_current_stream_capturing()
@@ -84,6 +95,20 @@ class AttentionBackend(ABC):
                 extend_attention(q[offsets[i] : offsets[i + 1]], k_buf[locs], v_buf[locs],
                                  prefix_len=int(batch.extend_prefix_lens[i]), scaling=layer.scaling)
             )
+        return torch.cat(outputs, dim=0)
+
+    def _forward_extend_fp8(self, q: torch.Tensor, layer: Any, batch: ForwardBatch) -> torch.Tensor:
+        """forward_extend over an 8-bit pool, which holds the new K/V: every token attends the
+        pool's values, its own included."""
+        pool = self.token_to_kv_pool
+        q = q.reshape(q.shape[0], -1, pool.head_dim)
+        offsets = batch.extend_token_offsets()
+        outputs = []
+        for i in range(batch.batch_size):
+            locs = self.req_to_token[int(batch.req_pool_indices[i]), : int(batch.seq_lens[i])]
+            k, v = pool.get_rows(layer.layer_id, locs, torch.float32)
+            outputs.append(extend_attention(q[offsets[i] : offsets[i + 1]], k, v,
+                                            prefix_len=int(batch.extend_prefix_lens[i]), scaling=layer.scaling))
         return torch.cat(outputs, dim=0)
 
     def _extend_fast(self, q: torch.Tensor, k_buf: torch.Tensor, v_buf: torch.Tensor, scaling: float,

@@ -5,7 +5,9 @@ Every decode step attends each request's whole KV history in the device token
 pool.  bf16 with 4 KV heads x 128 runs one C call (``qq_dense_forward_decode``:
 the new K/V store, then the attention kernel of the Quest layer step over all
 of a request's rows); other shapes store the new K/V and run the split-K
-attention over the explicit row list ``req_to_token[req, :seq_len]``.
+attention over the explicit row list ``req_to_token[req, :seq_len]``.  Over an 8-bit pool
+(``Fp8TokenToKVPool``) one C call does both for every shape the pool takes
+(``qq_fp8_decode_attention``).
 """
 
 from __future__ import annotations
@@ -16,7 +18,7 @@ import torch
 
 from qwenquest_amd import _lib
 from qwenquest_amd.attention.base import AttentionBackend
-from qwenquest_amd.attention.ops import AttentionWorkspace, decode_attention_rows
+from qwenquest_amd.attention.ops import AttentionWorkspace, decode_attention_rows, fp8_decode_attention
 
 if TYPE_CHECKING:
     from qwenquest_amd.batch import ForwardBatch
@@ -50,6 +52,10 @@ class DenseBackend(AttentionBackend):
         bs = batch.batch_size
         dim = pool.head_dim
         q3 = q.reshape(bs, -1, dim)
+        if self.fp8:
+            return fp8_decode_attention(q3, pool, layer.layer_id, self.req_to_token_pool.block_table,
+                                        batch.req_pool_indices, batch.seq_lens, layer.scaling,
+                                        new=(batch.out_cache_loc, k, v))
         heads = q3.shape[1]
         rpi = batch.req_pool_indices.to(device=q3.device, dtype=torch.int64).contiguous()
         seq = batch.seq_lens.to(device=q3.device, dtype=torch.int64).contiguous()

@@ -1,6 +1,7 @@
 """Attention math (reference ``src/qwenquest/attention/ops.py``).
 
 ``decode_attention`` runs the HIP split-K kernel over an explicit row list;
+``fp8_decode_attention`` runs the HIP kernel over an 8-bit block cache;
 ``extend_attention_batch`` runs a whole prefill batch (bf16, head_dim 128) in the HIP
 prefill kernel; ``extend_attention``, one request of any shape, uses torch's SDPA on the
 device, in float32.
@@ -8,12 +9,18 @@ device, in float32.
 
 from __future__ import annotations
 
+from typing import TYPE_CHECKING
+
 import torch
 import torch.nn.functional as F
 
 from qwenquest_amd import _lib
 
-__all__ = ["decode_attention", "extend_attention", "extend_attention_batch", "AttentionWorkspace"]
+if TYPE_CHECKING:
+    from qwenquest_amd.paged import Fp8TokenToKVPool
+
+__all__ = ["decode_attention", "extend_attention", "extend_attention_batch", "fp8_decode_attention",
+           "AttentionWorkspace"]
 
 
 class AttentionWorkspace:
@@ -195,3 +202,91 @@ def extend_attention_batch_checked(
         return None
     tokens = verdict // 2
     return out if tokens >= out.shape[0] else out[:tokens]
+
+
+def _block_table(block_table: torch.Tensor, device: torch.device) -> torch.Tensor:
+    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.stride(1) != 1:
+        raise ValueError("block_table must be a 2-D int32 tensor with unit column stride")
+    if block_table.device != device:
+        raise ValueError(f"block_table lies on {block_table.device}, the pool on {device}")
+    if block_table.shape[0] > 1 and block_table.stride(0) < block_table.shape[1]:
+        raise ValueError("block_table's rows must not overlap")
+    return block_table
+
+
+def _table_args(bt: torch.Tensor) -> tuple:
+    return _lib.ptr(bt), max(bt.stride(0), bt.shape[1]), bt.shape[0], bt.shape[1]
+
+
+def _lengths(t: torch.Tensor, n: int, device: torch.device, what: str) -> torch.Tensor:
+    if t.dim() != 1 or t.shape[0] != n:
+        raise ValueError(f"{what} must have {n} entries, got {tuple(t.shape)}")
+    if t.dtype == torch.int64 and t.device == device and t.is_contiguous():
+        return t
+    return t.to(device=device, dtype=torch.int64).contiguous()
+
+
+def _queries(q: torch.Tensor, pool: Fp8TokenToKVPool) -> torch.Tensor:
+    """``q [n, H, D]`` (or ``[n, H*D]``) dense and 16-byte aligned."""
+    dim = pool.head_dim
+    if q.device != pool.device:
+        raise ValueError(f"q lies on {q.device}, the pool on {pool.device}")
+    if q.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"unsupported dtype {q.dtype}; the kernels take bfloat16 or float32")
+    if q.dim() == 2 and q.shape[1] % dim == 0:
+        q = q.reshape(q.shape[0], q.shape[1] // dim, dim)
+    if q.dim() != 3 or q.shape[2] != dim:
+        raise ValueError(f"queries must be [n, heads, {dim}], got {tuple(q.shape)}")
+    if q.shape[1] == 0 or q.shape[1] % pool.kv_heads:
+        raise ValueError(f"q_heads {q.shape[1]} not divisible by kv_heads {pool.kv_heads}")
+    q = q.detach().contiguous()
+    return q.clone() if q.data_ptr() % 16 else q
+
+
+def fp8_decode_attention(
+    q: torch.Tensor,
+    pool: Fp8TokenToKVPool,
+    layer_id: int,
+    block_table: torch.Tensor,
+    req_pool_indices: torch.Tensor,
+    seq_lens: torch.Tensor,
+    scaling: float,
+    *,
+    positions: torch.Tensor | None = None,
+    top_k: int = 0,
+    new: tuple[torch.Tensor, torch.Tensor, torch.Tensor] | None = None,
+) -> torch.Tensor:
+    """Decode over an 8-bit pool: request ``i`` attends ``q[i] [H, D]`` over its first ``seq_lens[i]``
+    tokens in the blocks ``block_table[req_pool_indices[i]]``, or, with ``positions [bs, >= top_k]``
+    (``QuestAlgorithm.retrieve_topk``) and a longer context than ``top_k``, over the pages listed
+    there and the last 64 tokens.  ``new``: ``(loc, k, v)`` of the batch's new tokens, stored first.
+    Returns ``[bs, H*D]`` in q's dtype (bf16 or fp32): zeros for an empty context, NaN for a request
+    outside the table or a context past its blocks."""
+    dev = pool.device
+    q = _queries(q, pool)
+    bs, heads, dim = q.shape
+    bt = _block_table(block_table, dev)
+    rpi = _lengths(req_pool_indices, bs, dev, "req_pool_indices")
+    seq = _lengths(seq_lens, bs, dev, "seq_lens")
+    if positions is not None:
+        if (positions.dim() != 2 or positions.dtype != torch.int32 or positions.device != dev
+                or positions.shape[0] < bs or positions.shape[1] < top_k or positions.stride(1) != 1):
+            raise ValueError(f"positions must be an int32 tensor [>= {bs}, >= {top_k}] on {dev}")
+    loc = kn = vn = None
+    if new is not None:
+        loc = _lengths(new[0], bs, dev, "out_cache_loc")
+        kn, vn = pool.new_rows(new[1], new[2], bs)
+    out = torch.empty((bs, heads * dim), dtype=q.dtype, device=dev)
+    need = int(_lib.load().qq_fp8_decode_workspace_bytes(bs, heads, pool.kv_heads, dim))
+    # of this call alone: it holds the division of the batch, which a graph's replay or a call on
+    # another stream must not find replaced
+    ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        _lib.call(
+            "qq_fp8_decode_attention", _lib.ptr(q), _lib.dtype_code(q.dtype), q.stride(0), heads, _lib.ptr(kn),
+            _lib.ptr(vn), _lib.DTYPE_BF16 if kn is None else _lib.dtype_code(kn.dtype), _lib.ptr(loc),
+            *pool.layer_args(layer_id), *_table_args(bt), _lib.ptr(rpi), _lib.ptr(seq), bs, _lib.ptr(positions),
+            0 if positions is None else max(positions.stride(0), positions.shape[1]), int(top_k), float(scaling),
+            _lib.ptr(out), _lib.ptr(ws), need, _lib.stream(dev),
+        )
+    return out

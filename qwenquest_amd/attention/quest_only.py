@@ -9,6 +9,10 @@ Per decode step::
                             [Q4] prepare_step
     forward_decode (x L):   save new K/V -> [Q6] retrieve_topk (score + select + layout)
                             -> [Q7] req_to_token gather + split-K attention
+
+Over an 8-bit pool (``Fp8TokenToKVPool``) pages are the pool's blocks: a page's bounds are taken
+from its codes when its last token is in (no running bounds), and the attention takes the
+selected pages by block.
 """
 
 from __future__ import annotations
@@ -20,8 +24,9 @@ import torch
 
 from qwenquest_amd import _lib
 from qwenquest_amd.attention.base import AttentionBackend
-from qwenquest_amd.attention.ops import AttentionWorkspace
+from qwenquest_amd.attention.ops import AttentionWorkspace, fp8_decode_attention
 from qwenquest_amd.config import SparseConfig, parse_hisparse_config
+from qwenquest_amd.paged import BLOCK_TOKENS
 from qwenquest_amd.quest import QuestAlgorithm
 
 if TYPE_CHECKING:
@@ -47,6 +52,9 @@ class QuestOnlyBackend(AttentionBackend):
         cfg = parse_hisparse_config(sparse_config)
         if cfg.algorithm != "quest" or cfg.quest_page_size is None:
             raise ValueError("Quest backends require hisparse_config with algorithm='quest'")
+        if self.fp8 and cfg.quest_page_size != BLOCK_TOKENS:
+            raise ValueError(f"an Fp8TokenToKVPool's pages are its blocks of {BLOCK_TOKENS} tokens: "
+                             f"quest_page_size must be {BLOCK_TOKENS}, got {cfg.quest_page_size}")
         self.sparse_config = cfg
         device = token_to_kv_pool.device
         self.quest = QuestAlgorithm(
@@ -82,6 +90,10 @@ class QuestOnlyBackend(AttentionBackend):
             bs = int(batch.req_pool_indices.numel())
             if bs > self._step_locs.numel():
                 raise ValueError(f"batch {bs} exceeds the request pool ({self._step_locs.numel()})")
+            if self.fp8:
+                self.quest.decode_step_blocks(batch.req_pool_indices, batch.seq_lens, self.token_to_kv_pool,
+                                              self.req_to_token_pool.block_table)
+                return
             self.quest.decode_step(batch.req_pool_indices, batch.seq_lens, self.token_to_kv_pool.k_all,
                                    self.req_to_token, self._skip_first_decode_update, self._decode_sync,
                                    self._step_locs[:bs])
@@ -116,6 +128,10 @@ class QuestOnlyBackend(AttentionBackend):
 
     def _update_quest_for_extend(self, batch: ForwardBatch) -> None:
         """[Q2] Per request: bounds of positions ``0 .. seq_len-1`` at every layer (quest_only.py:115-128)."""
+        if self.fp8:
+            self.quest.update_prefill_representations_blocks(batch.req_pool_indices, batch.seq_lens,
+                                                             self.token_to_kv_pool, self.req_to_token_pool.block_table)
+            return
         for req_idx, seq_len in zip(batch.req_pool_indices.tolist(), batch.seq_lens.tolist(), strict=True):
             prefill_indices = self.req_to_token[req_idx, :seq_len]
             self.quest.update_prefill_representations_fused(req_idx, self.token_to_kv_pool.k_all, prefill_indices)
@@ -142,6 +158,8 @@ class QuestOnlyBackend(AttentionBackend):
         heads, dim = q3.shape[1], pool.head_dim
         if step.seq_lens.shape[0] != bs:
             raise ValueError("batch size differs from the one given to prepare_step()")
+        if self.fp8:
+            return self._forward_decode_fp8(q3, k, v, layer, batch, phase)
         kn = k.reshape(bs, pool.kv_heads * dim)
         vn = v.reshape(bs, pool.kv_heads * dim)
         if kn.dtype != vn.dtype or kn.dtype not in (torch.bfloat16, torch.float32):
@@ -173,10 +191,26 @@ class QuestOnlyBackend(AttentionBackend):
             quest._record(layer.layer_id, rpi, step, self._positions[:bs])
         return out
 
+    def _forward_decode_fp8(self, q3, k, v, layer, batch: ForwardBatch, phase: int) -> torch.Tensor:
+        """forward_decode_phase over an 8-bit pool: 1 = scoring and selection, 2 = new-token store and
+        attention."""
+        if phase not in (1, 2, 3):
+            raise ValueError(f"phase must be 1, 2 or 3, got {phase}")
+        quest, pool, bs = self.quest, self.token_to_kv_pool, batch.batch_size
+        if phase & 1:
+            quest.retrieve_topk(q3, layer.layer_id, batch.req_pool_indices, quest._step.seq_lens, out=self._positions)
+        if not phase & 2:
+            return torch.empty((bs, q3.shape[1] * pool.head_dim), dtype=q3.dtype, device=q3.device)
+        return fp8_decode_attention(q3, pool, layer.layer_id, self.req_to_token_pool.block_table,
+                                    batch.req_pool_indices, quest._step.seq_lens, layer.scaling,
+                                    positions=self._positions, top_k=quest.top_k, new=(batch.out_cache_loc, k, v))
+
     def sparse_attention(self, q, layer, req_pool_indices, positions, actual, bs) -> torch.Tensor:
         """[Q7] rows = req_to_token[req, positions[:n]] -> attention over exactly those rows."""
         heads = q.shape[1] if q.dim() == 3 else q.shape[1] // self.token_to_kv_pool.head_dim
         dim = self.token_to_kv_pool.head_dim
+        if self.fp8:
+            raise ValueError("an Fp8TokenToKVPool is attended by block: fp8_decode_attention takes the positions")
         q3 = q.reshape(bs, heads, dim).contiguous()
         k_buf, v_buf = self.token_to_kv_pool.get_kv_buffer(layer.layer_id)
         rpi = req_pool_indices

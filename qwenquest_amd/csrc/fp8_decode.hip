@@ -1,0 +1,528 @@
+// Decode attention over the 8-bit K/V cache (layout: qq_fp8.h), dense or over the pages that
+// Quest selected (reference src/qwenquest/attention/dense.py:26-42, quest_only.py:132-159,
+// ops.py:48-66 over that cache).  With ks, vs the scales of token j's block and kc, vc its codes
+//   t_j = scale * log2(e) * ks * (q . kc_j),  p_j = 2^(t_j - max t),  out = sum p_j vs vc_j / sum p_j.
+//
+// The work comes in units, a (partial) block of the cache: of a dense request its blocks in
+// order, of one with selected pages those and the one or two blocks of its recent window.  All
+// requests' units in a row are cut into equal slices, one to a thread block per (KV head, tile
+// of 16 query heads), so that any mix of lengths fills the chip evenly in one round; a
+// request that lies in one slice is finished there, the others' (m, l, o) parts are merged.
+//
+// A wave takes a unit at a time: K and V codes straight from memory to registers in the
+// operands' order (1 KiB runs), converted to bf16 (exact), S^T = K Q^T, the softmax in
+// registers, O^T += V^T P^T, with P's values scaled by vs as bf16 pieces: two for bf16 output
+// (16 significand bits), three for fp32 (all 24).  fp32 queries go in as three bf16 pieces, too.
+// Bound: HBM, the codes once.
+#include "qq_fp8.h"
+#include "qq_quest_dev.h"
+#include "qq_rules.h"
+
+namespace qq {
+namespace {
+
+constexpr int kTile = 16;      // query heads of a tile
+constexpr int kDecWaves = 4;
+constexpr int kDecParts = 64;  // slices of a request, at most: the merge's table of weights
+
+struct DecPlan {
+  int32_t total, len, slices, pad;  // units of the batch, units of a slice, slices
+};
+
+struct DecArgs {
+  const void* q;  // [bs, H, D]
+  int64_t q_bstride;
+  int H, G, tiles;  // query heads, of a KV head, tiles of those
+  Fp8Cache c;
+  const int32_t* table;
+  int64_t table_stride;
+  int table_rows, table_cols;
+  const int64_t* rpi;
+  const int64_t* seq;
+  int bs;
+  const int32_t* positions;  // nullptr: dense
+  int64_t pos_stride;
+  int top_k;
+  float sl2;  // scale * log2(e)
+  void* out;  // [bs, H, D]
+  int max_slices, heads;  // heads: KV * tiles
+  DecPlan* plan;
+  int32_t* cu;       // [bs + 1] units before each request
+  int32_t* first;    // [max_slices] request of each slice's first unit
+  float* part_o;     // [max_slices, 2, heads, 16, D]
+  float* part_ml;    // [max_slices, 2, heads, 16, 2]
+};
+
+__device__ inline int context_of(const DecArgs& a, int b) {
+  return (int)min(max(a.seq[b], (int64_t)0), (int64_t)a.table_cols * kCacheTokens);
+}
+__device__ inline bool is_sparse(const DecArgs& a, int s) { return a.positions && s > a.top_k; }
+__device__ inline int units_of(const DecArgs& a, int s) {
+  if (is_sparse(a, s)) return a.top_k / 64 + (s % 64 ? 1 : 0);
+  return max((s + 63) / 64, 1);  // an empty context: one unit without tokens, which writes its zeros
+}
+
+__global__ __launch_bounds__(1024) void fp8_plan_kernel(DecArgs a) {
+  __shared__ int s_sum[16], s_long[16];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  int base = 0, longest = 0;
+  for (int b0 = 0; b0 < a.bs; b0 += 1024) {
+    const int b = b0 + tid;
+    const int u = b < a.bs ? units_of(a, context_of(a, b)) : 0;
+    int x = u;
+    longest = max(longest, u);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int y = __shfl_up(x, d, 64);
+      if (lane >= d) x += y;
+    }
+    __syncthreads();
+    if (lane == 63) s_sum[wave] = x;
+    __syncthreads();
+    int before = base;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+      if (w < wave) before += s_sum[w];
+      base += s_sum[w];
+    }
+    if (b < a.bs) a.cu[b] = before + x - u;
+  }
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) longest = max(longest, __shfl_xor(longest, d, 64));
+  if (lane == 0) s_long[wave] = longest;
+  if (tid == 0) a.cu[a.bs] = base;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 16; ++w) longest = max(longest, s_long[w]);
+  const int len = rules::fp8_slice_len(base, longest, a.max_slices);
+  const int slices = (base + len - 1) / len;
+  if (tid == 0) *a.plan = {base, len, slices, 0};
+  for (int i = tid; i < slices; i += 1024) {
+    const int at = i * len;
+    int lo = 0, hi = a.bs;  // the last request that begins at or before this unit
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (a.cu[mid] <= at) lo = mid;
+      else hi = mid;
+    }
+    a.first[i] = lo;
+  }
+}
+
+__device__ inline float trunc_bf16(float x) { return __uint_as_float(__float_as_uint(x) & 0xFFFF0000u); }
+__device__ inline uint32_t pack_trunc(float even, float odd) {
+  return __builtin_amdgcn_perm(__float_as_uint(odd), __float_as_uint(even), 0x07060302u);
+}
+
+// Eight codes as bf16.
+__device__ inline bf16x8_t codes8(uint32_t a, uint32_t b) {
+  u32x4_t w;
+  w.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, false));
+  w.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, true));
+  w.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, false));
+  w.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true));
+  return __builtin_bit_cast(bf16x8_t, w);
+}
+
+__device__ inline void store4(uint16_t* p, float a, float b, float c, float d) {
+  *reinterpret_cast<uint2*>(p) = make_uint2((uint32_t)f2bf(a) | ((uint32_t)f2bf(b) << 16),
+                                            (uint32_t)f2bf(c) | ((uint32_t)f2bf(d) << 16));
+}
+__device__ inline void store4(float* p, float a, float b, float c, float d) {
+  *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
+}
+
+// Channels d0 .. d0 + 7 of a query row as P bf16 pieces.
+template <int P>
+__device__ inline void load_query(const void* q, int64_t at, bool in, bf16x8_t (&f)[P]) {
+  if constexpr (P == 1) {
+    u32x4_t w = {0, 0, 0, 0};
+    if (in) w = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(q) + at);
+    f[0] = __builtin_bit_cast(bf16x8_t, w);
+  } else {
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = in ? static_cast<const float*>(q)[at + i] : 0.0f;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      u32x4_t w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        w[i] = pack_trunc(x[2 * i], x[2 * i + 1]);
+        // what is left of an infinity is nothing (not NaN): its first piece says it all
+        const float a = x[2 * i] - trunc_bf16(x[2 * i]), b = x[2 * i + 1] - trunc_bf16(x[2 * i + 1]);
+        x[2 * i] = fabsf(x[2 * i]) == INFINITY ? 0.0f : a;
+        x[2 * i + 1] = fabsf(x[2 * i + 1]) == INFINITY ? 0.0f : b;
+      }
+      f[p] = __builtin_bit_cast(bf16x8_t, w);
+    }
+  }
+}
+
+template <int D>
+struct DecSmem {
+  float m[kDecWaves][kTile], l[kDecWaves][kTile];
+  float o[kDecWaves][kTile][D + 4];
+};
+
+template <int D, typename T>
+__global__ __launch_bounds__(64 * kDecWaves, 2) void fp8_attend_kernel(DecArgs a) {
+  constexpr int QP = sizeof(T) == 2 ? 1 : 3, PP = sizeof(T) == 2 ? 2 : 3;  // pieces of q and of the weights
+  constexpr int KL = D / 64, VL = D / 16;  // 16-byte loads a lane: per 16 tokens of K, per block of V
+  __shared__ DecSmem<D> sm;
+  const DecPlan plan = *a.plan;
+  const int head = blockIdx.x % a.heads, slice = blockIdx.x / a.heads;
+  if (slice >= plan.slices) return;
+  const int h = head / a.tiles, tile = head - h * a.tiles;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int m16 = lane & 15, g = lane >> 4;
+  const int rows = min(a.G - tile * kTile, kTile);  // query heads of this tile
+  const int q_head = h * a.G + tile * kTile;
+  const int end = min((slice + 1) * plan.len, plan.total);
+  int at = slice * plan.len;
+  for (int b = a.first[slice]; at < end; ++b) {
+    const int c0 = a.cu[b], c1 = a.cu[b + 1];
+    const int u0 = at - c0, u1 = min(end, c1) - c0;  // this slice's units of request b
+    const int seq = context_of(a, b);
+    const bool sparse = is_sparse(a, seq);
+    const int64_t req = a.rpi[b];
+    const bool known = req >= 0 && req < a.table_rows;
+    const int32_t* tr = a.table + (known ? req : 0) * a.table_stride;
+    const int picked = a.top_k / 64 - 1;  // selected pages
+    const int win = seq & 63;             // the window's first token in its first block
+
+    bf16x8_t qf[2 * KL][QP];
+#pragma unroll
+    for (int i = 0; i < 2 * KL; ++i) {
+      const int d = ((i >> 1) * 4 + g) * 16 + (i & 1) * 8;
+      load_query<QP>(a.q, (int64_t)b * a.q_bstride + (int64_t)(q_head + min(m16, rows - 1)) * D + d, m16 < rows, qf[i]);
+    }
+    // lane j looks up this wave's unit j0 + j: u0 + wave + 4 (j0 + j)
+    const int n = u1 - u0 > wave ? (u1 - u0 - wave + kDecWaves - 1) / kDecWaves : 0;
+    int blk = 0;
+    float ks = 0.0f, vs = 0.0f;
+    bool bad = !known;
+    auto resolve = [&](int j0) {
+      const int u = u0 + wave + kDecWaves * (j0 + lane);
+      blk = 0;
+      if (j0 + lane < n && seq > 0 && known) {
+        int page = u;
+        if (sparse) page = u < picked ? a.positions[(int64_t)b * a.pos_stride + u * 64] >> 6 : (seq - 64) / 64 + (u - picked);
+        const int x = page >= 0 && page < a.table_cols ? tr[page] : 0;
+        if (x > 0 && x < a.c.blocks) blk = x;
+        else bad = true;  // no block there: no answer
+      }
+      const int64_t e = (int64_t)blk * a.c.KV + h;
+      ks = a.c.ks[e] * a.sl2;
+      vs = a.c.vs[e];
+    };
+    uint4 kr[4][KL], vr[VL];
+    auto head_of = [&](int j) { return ((int64_t)__builtin_amdgcn_readlane(blk, j & 63) * a.c.KV + h) * (64 * D) + lane * 16; };
+    auto load_k = [&](int j) {
+      const uint8_t* p = a.c.kc + head_of(j);
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < KL; ++i) kr[t][i] = *reinterpret_cast<const uint4*>(p + (t * KL + i) * 1024);
+    };
+    auto load_v = [&](int j) {
+      const uint8_t* p = a.c.vc + head_of(j);
+#pragma unroll
+      for (int i = 0; i < VL; ++i) vr[i] = *reinterpret_cast<const uint4*>(p + i * 1024);
+    };
+    float4_t o[VL];
+#pragma unroll
+    for (int i = 0; i < VL; ++i) o[i] = float4_t{0.f, 0.f, 0.f, 0.f};
+    float M = -INFINITY, L = 0.0f;
+    if (n > 0) {
+      resolve(0);
+      load_k(0);
+      load_v(0);
+    }
+    for (int j = 0; j < n; ++j) {
+      const float kscale = __shfl(ks, j & 63, 64), vscale = __shfl(vs, j & 63, 64);
+      // tokens of this unit
+      const int u = u0 + wave + kDecWaves * j;
+      int lo = 0, hi = 64;
+      if (!sparse) hi = min(64, seq - u * 64);
+      else if (u == picked) lo = win;
+      else if (u > picked) hi = win;
+      const bool last = j + 1 >= n, next_set = ((j + 1) & 63) == 0;
+      float4_t s[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        s[t] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < KL; ++i) {
+          const bf16x8_t k0 = codes8(kr[t][i].x, kr[t][i].y), k1 = codes8(kr[t][i].z, kr[t][i].w);
+#pragma unroll
+          for (int p = 0; p < QP; ++p) {
+            s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, qf[2 * i][p], s[t], 0, 0, 0);
+            s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, qf[2 * i + 1][p], s[t], 0, 0, 0);
+          }
+        }
+      }
+      if (!last && !next_set) load_k(j + 1);
+      float mx = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int tok = t * 16 + g * 4 + i;
+          s[t][i] = tok >= lo && tok < hi ? s[t][i] * kscale : -INFINITY;
+          mx = fmaxf(mx, s[t][i]);
+        }
+      mx = fmaxf(mx, lane_xor16(mx, lane));
+      mx = fmaxf(mx, lane_xor32(mx, lane));
+      const float Mn = fmaxf(M, mx);
+      const float mb = Mn == -INFINITY ? 0.0f : Mn;
+      const float alpha = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - mb);
+      M = Mn;
+      float sum = 0.0f;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float p = __builtin_amdgcn_exp2f(s[t][i] - mb);
+          sum += p;
+          // a masked token weighs nothing whatever its block's scale is
+          s[t][i] = s[t][i] == -INFINITY ? 0.0f : p * vscale;
+        }
+      L = L * alpha + sum;
+#pragma unroll
+      for (int i = 0; i < VL; ++i)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) o[i][x] *= alpha;
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        bf16x8_t pw[PP];
+#pragma unroll
+        for (int p = 0; p < PP; ++p) {
+          u32x4_t w;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const float e = s[2 * st + (x >> 1)][(x & 1) * 2], f = s[2 * st + (x >> 1)][(x & 1) * 2 + 1];
+            w[x] = pack_trunc(e, f);
+            s[2 * st + (x >> 1)][(x & 1) * 2] = e - trunc_bf16(e);
+            s[2 * st + (x >> 1)][(x & 1) * 2 + 1] = f - trunc_bf16(f);
+          }
+          pw[p] = __builtin_bit_cast(bf16x8_t, w);
+        }
+#pragma unroll
+        for (int i = 0; i < VL; ++i) {
+          const uint32_t x[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
+          const bf16x8_t vb = codes8(x[2 * st], x[2 * st + 1]);
+#pragma unroll
+          for (int p = 0; p < PP; ++p) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb, pw[p], o[i], 0, 0, 0);
+        }
+      }
+      if (!last) {
+        if (next_set) {
+          resolve(j + 1);
+          load_k(j + 1);
+        }
+        load_v(j + 1);
+      }
+    }
+    L += lane_xor16(L, lane);
+    L += lane_xor32(L, lane);
+    if (__any(bad)) L = __builtin_nanf("");
+
+    __syncthreads();  // the request before has been read out of sm
+    if (g == 0) {
+      sm.m[wave][m16] = M;
+      sm.l[wave][m16] = L;
+    }
+#pragma unroll
+    for (int i = 0; i < VL; ++i)
+      *reinterpret_cast<float4_t*>(&sm.o[wave][m16][i * 16 + g * 4]) = o[i];
+    __syncthreads();
+    const bool whole = u0 == 0 && c1 <= end;
+    const int64_t part = ((int64_t)(slice * 2 + (u0 == 0 ? 1 : 0)) * a.heads + head) * kTile;
+    for (int it = tid; it < rows * (D / 4); it += 64 * kDecWaves) {
+      const int r = it / (D / 4), d = (it - r * (D / 4)) * 4;
+      float Mx = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kDecWaves; ++w) Mx = fmaxf(Mx, sm.m[w][r]);
+      float Ls = 0.0f;
+      float4 Os = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kDecWaves; ++w) {
+        const float wt = sm.m[w][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm.m[w][r] - Mx);
+        const float lw = sm.l[w][r];
+        Ls += lw != lw ? lw : wt * lw;
+        const float4 x = *reinterpret_cast<const float4*>(&sm.o[w][r][d]);
+        Os.x += wt * x.x;
+        Os.y += wt * x.y;
+        Os.z += wt * x.z;
+        Os.w += wt * x.w;
+      }
+      if (whole) {
+        const float inv = Ls <= 0.0f ? 0.0f : 1.0f / Ls;  // nothing attended: zeros
+        store4(static_cast<T*>(a.out) + ((int64_t)b * a.H + q_head + r) * D + d, Os.x * inv, Os.y * inv, Os.z * inv, Os.w * inv);
+      } else {
+        *reinterpret_cast<float4*>(a.part_o + (part + r) * D + d) = Os;
+        if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (part + r) * 2) = make_float2(Mx, Ls);
+      }
+    }
+    at = c0 + u1;
+  }
+}
+
+// The parts of a request added up: a thread block per (request, query head), a thread per 4
+// channels and every (256 / (D / 4))-th part.
+template <int D, typename T>
+__global__ __launch_bounds__(256) void fp8_merge_kernel(DecArgs a) {
+  constexpr int DG = D / 4, NG = 256 / DG;
+  __shared__ float s_w[kDecParts];
+  __shared__ float4 s_o[256];
+  const DecPlan plan = *a.plan;
+  const int b = blockIdx.x, q_head = blockIdx.y;
+  const int c0 = a.cu[b], c1 = a.cu[b + 1];
+  const int first = c0 / plan.len, parts = (c1 - 1) / plan.len - first + 1;
+  if (parts <= 1) return;
+  const int h = q_head / a.G, r = (q_head - h * a.G) % kTile, head = h * a.tiles + (q_head - h * a.G) / kTile;
+  const int tid = threadIdx.x, grp = tid / DG, d = (tid % DG) * 4;
+  // part i: of slice first + i, the part that begins its request in the slice, or goes on in it
+  auto row_of = [&](int i) { return ((int64_t)((first + i) * 2 + (i == 0 ? 1 : 0)) * a.heads + head) * kTile + r; };
+  const int lane = tid & 63;
+  const float2 ml = lane < parts ? *reinterpret_cast<const float2*>(a.part_ml + row_of(lane) * 2) : make_float2(-INFINITY, 0.0f);
+  float Mx = ml.x;
+#pragma unroll
+  for (int x = 32; x >= 1; x >>= 1) Mx = fmaxf(Mx, __shfl_xor(Mx, x, 64));
+  const float wt = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - Mx);
+  float Ls = ml.y != ml.y ? ml.y : wt * ml.y;
+#pragma unroll
+  for (int x = 32; x >= 1; x >>= 1) Ls += __shfl_xor(Ls, x, 64);
+  if (tid < 64) s_w[tid] = wt;
+  __syncthreads();
+  float4 Os = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = grp; i < parts; i += NG) {
+    const float w = s_w[i];
+    const float4 x = *reinterpret_cast<const float4*>(a.part_o + row_of(i) * D + d);
+    Os.x += w * x.x;
+    Os.y += w * x.y;
+    Os.z += w * x.z;
+    Os.w += w * x.w;
+  }
+  s_o[tid] = Os;
+  __syncthreads();
+  if (grp) return;
+#pragma unroll
+  for (int k = 1; k < NG; ++k) {
+    const float4 x = s_o[tid + k * DG];
+    Os.x += x.x;
+    Os.y += x.y;
+    Os.z += x.z;
+    Os.w += x.w;
+  }
+  const float inv = Ls <= 0.0f ? 0.0f : 1.0f / Ls;
+  store4(static_cast<T*>(a.out) + ((int64_t)b * a.H + q_head) * D + d, Os.x * inv, Os.y * inv, Os.z * inv, Os.w * inv);
+}
+
+// The workspace's parts, in order; offsets are multiples of 256 bytes.
+struct DecSpace {
+  int64_t cu, first, part_o, part_ml, bytes;
+  int max_slices;
+};
+DecSpace decode_space(int bs, int H, int KV, int D) {
+  auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
+  const int tiles = (H / KV + kTile - 1) / kTile, heads = KV * tiles;
+  DecSpace s;
+  s.max_slices = rules::fp8_max_slices(heads);
+  s.cu = up(sizeof(DecPlan));
+  s.first = s.cu + up((int64_t)(bs + 1) * 4);
+  s.part_o = s.first + up((int64_t)s.max_slices * 4);
+  s.part_ml = s.part_o + (int64_t)s.max_slices * 2 * heads * kTile * D * 4;
+  s.bytes = s.part_ml + (int64_t)s.max_slices * 2 * heads * kTile * 2 * 4;
+  return s;
+}
+
+template <int D, typename T>
+void launch(const DecArgs& a, hipStream_t s) {
+  fp8_plan_kernel<<<1, 1024, 0, s>>>(a);
+  fp8_attend_kernel<D, T><<<a.max_slices * a.heads, 64 * kDecWaves, 0, s>>>(a);
+  fp8_merge_kernel<D, T><<<dim3(a.bs, a.H), 256, 0, s>>>(a);
+}
+
+}  // namespace
+}  // namespace qq
+
+using namespace qq;
+
+extern "C" int64_t qq_fp8_decode_workspace_bytes(int bs, int num_q_heads, int kv_heads, int head_dim) {
+  if (bs <= 0 || kv_heads <= 0 || num_q_heads < kv_heads || num_q_heads % kv_heads || !fp8_dim_ok(head_dim)) return 0;
+  return decode_space(bs, num_q_heads, kv_heads, head_dim).bytes;
+}
+
+extern "C" int qq_fp8_decode_attention(const void* q, int q_dtype, int64_t q_batch_stride, int num_q_heads,
+                                       const void* k_new, const void* v_new, int new_dtype, const int64_t* out_cache_loc,
+                                       uint8_t* k_codes, uint8_t* v_codes, float* k_scale, float* v_scale,
+                                       int num_blocks, int kv_heads, int head_dim, const int32_t* block_table,
+                                       int64_t block_table_stride, int block_table_rows, int block_table_cols,
+                                       const int64_t* req_pool_indices, const int64_t* seq_lens, int bs,
+                                       const int32_t* positions, int64_t positions_stride, int top_k, float scale,
+                                       void* out, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* what = "qq_fp8_decode_attention";
+  const Fp8Cache c{k_codes, v_codes, k_scale, v_scale, num_blocks, kv_heads, head_dim};
+  int st = check_cache(c, what);
+  if (st != QQ_OK) return st;
+  QQ_REQUIRE(dtype_ok(q_dtype), "%s: bad dtype", what);
+  QQ_REQUIRE(num_q_heads > 0 && num_q_heads % kv_heads == 0 && num_q_heads < 65536,
+             "%s: q_heads %d not divisible by kv_heads %d", what, num_q_heads, kv_heads);
+  QQ_REQUIRE(bs >= 0 && block_table_rows > 0 && block_table_cols > 0 && block_table_cols <= kMaxPoolBlocks &&
+                 block_table_stride >= block_table_cols,
+             "%s: bad sizes", what);
+  QQ_REQUIRE(!positions || (top_k > 0 && top_k % 64 == 0 && positions_stride >= top_k),
+             "%s: top_k %d is not a multiple of the block of 64", what, top_k);
+  const int64_t units = positions ? max((int64_t)1, min((int64_t)block_table_cols, (int64_t)top_k / 64 + 1)) : block_table_cols;
+  QQ_REQUIRE(units * bs < (int64_t)1 << 30, "%s: too many units of work", what);
+  if (bs == 0) return QQ_OK;
+  QQ_REQUIRE(q && block_table && req_pool_indices && seq_lens && out, "%s: null pointer", what);
+  QQ_REQUIRE((uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0 && q_batch_stride % 8 == 0,
+             "%s: q and out must be 16-byte aligned", what);
+  const DecSpace sp = decode_space(bs, num_q_heads, kv_heads, head_dim);
+  QQ_REQUIRE(workspace && workspace_bytes >= sp.bytes, "%s: workspace %lld bytes < %lld needed", what,
+             (long long)workspace_bytes, (long long)sp.bytes);
+  if (k_new) {
+    st = qq_fp8_store(k_codes, v_codes, k_scale, v_scale, num_blocks, kv_heads, head_dim, k_new, v_new, new_dtype,
+                      out_cache_loc, bs, stream);
+    if (st != QQ_OK) return st;
+  }
+  char* ws = static_cast<char*>(workspace);
+  DecArgs a{};
+  a.q = q;
+  a.q_bstride = q_batch_stride;
+  a.H = num_q_heads;
+  a.G = num_q_heads / kv_heads;
+  a.tiles = (a.G + kTile - 1) / kTile;
+  a.c = c;
+  a.table = block_table;
+  a.table_stride = block_table_stride;
+  a.table_rows = block_table_rows;
+  a.table_cols = block_table_cols;
+  a.rpi = req_pool_indices;
+  a.seq = seq_lens;
+  a.bs = bs;
+  a.positions = positions;
+  a.pos_stride = positions_stride;
+  a.top_k = positions ? top_k : 64;
+  a.sl2 = scale * 1.44269504088896340736f;
+  a.out = out;
+  a.max_slices = sp.max_slices;
+  a.heads = kv_heads * a.tiles;
+  a.plan = reinterpret_cast<DecPlan*>(ws);
+  a.cu = reinterpret_cast<int32_t*>(ws + sp.cu);
+  a.first = reinterpret_cast<int32_t*>(ws + sp.first);
+  a.part_o = reinterpret_cast<float*>(ws + sp.part_o);
+  a.part_ml = reinterpret_cast<float*>(ws + sp.part_ml);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (head_dim == 128) {
+    if (q_dtype == QQ_DTYPE_BF16) launch<128, uint16_t>(a, s);
+    else launch<128, float>(a, s);
+  } else {
+    if (q_dtype == QQ_DTYPE_BF16) launch<64, uint16_t>(a, s);
+    else launch<64, float>(a, s);
+  }
+  return check_launch(what);
+}

@@ -149,6 +149,20 @@ constexpr bool dense_all_whole(int total, int longest, int bs, int round) {
 // first, so that a round's end does not wait for a long one.
 constexpr bool dense_first(int units, int parts, int len) { return 2 * ((units + parts - 1) / parts) > len; }
 
+// ------------------------------------------------- attention over the 8-bit cache
+constexpr int kFp8Blocks = 512;    // 4-wave blocks of a round: two on every CU
+constexpr int kFp8Parts = 64;      // slices of a request, at most: the merge's table of weights
+constexpr int kFp8MinLen = 4;      // units of a slice, at least: one to a wave
+
+// Slices that the grid holds for each of `heads` (KV head, tile of query heads) pairs.
+constexpr int fp8_max_slices(int heads) { return (int)most(kFp8Blocks / heads, 1); }
+
+// Units of a slice: equal slices of the whole batch in one round.
+constexpr int fp8_slice_len(int64_t total, int64_t longest, int64_t max_slices) {
+  const int64_t even = ceil_of(total, max_slices), parts = ceil_of(longest, kFp8Parts - 1);
+  return (int)most(most(even, parts), kFp8MinLen);
+}
+
 // ------------------------------------------------------------------ prefill
 constexpr int kExtRows = 128;      // query rows per block
 constexpr int kExtTile = 64;       // tokens per K/V tile

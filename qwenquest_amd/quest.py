@@ -22,10 +22,14 @@ order and ties go to the lowest page index (the reference leaves both to torch).
 from __future__ import annotations
 
 from dataclasses import dataclass, field
+from typing import TYPE_CHECKING
 
 import torch
 
 from qwenquest_amd import _lib
+
+if TYPE_CHECKING:
+    from qwenquest_amd.paged import Fp8TokenToKVPool
 
 __all__ = ["QuestAlgorithm", "QuestSelection", "QuestTrace", "StepLayout"]
 
@@ -356,6 +360,55 @@ class QuestAlgorithm:
         )
         self._step = StepLayout(seq, actual, limit, self.page_size, self.top_k)
         return self._step
+
+    # -------------------------------------------- pages of an 8-bit block pool
+
+    def _page_bounds(self, pool: Fp8TokenToKVPool, block_table, reqs, seq_lens, prefix_lens, decode: bool,
+                     max_new: int) -> torch.Tensor:
+        if self.page_size != 64:
+            raise ValueError(f"an 8-bit pool's pages are its blocks of 64 tokens, not of {self.page_size}")
+        if pool.kv_heads != self.kv_heads or pool.head_dim != self.head_dim or pool.num_layers < self.end_layer:
+            raise ValueError(f"the pool ({pool.num_layers} layers, {pool.kv_heads} x {pool.head_dim}) does not hold the "
+                             f"Quest layers' keys ({self.end_layer} layers, {self.kv_heads} x {self.head_dim})")
+        if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.stride(1) != 1:
+            raise ValueError("block_table must be a 2-D int32 tensor with unit column stride")
+        lens = [t if t is None else t.to(device=self.device, dtype=torch.int64).contiguous()
+                for t in (reqs, seq_lens, prefix_lens)]
+        bs = int(lens[0].numel())
+        if any(t is not None and t.numel() != bs for t in lens):
+            raise ValueError("req_indices, seq_lens and prefix_lens differ in length")
+        codes, _, scale, _, *geometry = pool.layer_args(self.start_layer)
+        with torch.cuda.device(self.device):
+            _lib.call(
+                "qq_fp8_page_bounds", codes, pool.k_codes.stride(0), scale, pool.k_scale.stride(0), *geometry,
+                _lib.ptr(block_table), max(block_table.stride(0), block_table.shape[1]), block_table.shape[0],
+                block_table.shape[1], *(_lib.ptr(t) for t in lens), bs, int(decode), int(max_new), self.num_layers,
+                _lib.ptr(self.page_k_bounds), self.max_reqs, self.max_pages_per_req, _lib.stream(self.device),
+            )
+        return lens[1]
+
+    def update_prefill_representations_blocks(
+        self,
+        req_indices: torch.Tensor,
+        seq_lens: torch.Tensor,
+        pool: Fp8TokenToKVPool,
+        block_table: torch.Tensor,
+        *,
+        prefix_lens: torch.Tensor | None = None,
+        max_new: int = 0,
+    ) -> None:
+        """[Q2] for a batch over an 8-bit pool, every Quest layer in one launch: bounds of the pages
+        that the first ``seq_lens[i]`` tokens of each request complete, from ``prefix_lens[i]``'s
+        page on if given (``max_new``: the most new tokens of a request, where the caller knows it,
+        sizes the launch).  A page is complete or has no bounds: nothing is kept for the tail."""
+        self._page_bounds(pool, block_table, req_indices, seq_lens, prefix_lens, False, max_new)
+
+    def decode_step_blocks(self, req_indices: torch.Tensor, seq_lens: torch.Tensor, pool: Fp8TokenToKVPool,
+                           block_table: torch.Tensor) -> StepLayout:
+        """[Q3] + [Q4] over an 8-bit pool: bounds of the pages that the previous step's tokens
+        completed, at every layer, then the step layout."""
+        seq = self._page_bounds(pool, block_table, req_indices, seq_lens, None, True, 0)
+        return self.prepare_step(seq)
 
     # ---------------------------------------------------- [Q5] page criticality
 
