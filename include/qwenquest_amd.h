@@ -480,6 +480,26 @@ int qq_fp8_decode_attention(const void* q, int q_dtype, int64_t q_batch_stride, 
                             void* stream);
 int64_t qq_fp8_decode_workspace_bytes(int bs, int num_q_heads, int kv_heads, int head_dim);
 
+/* The batch form of AttentionBackend.forward_extend (src/qwenquest/attention/base.py:65-93) over
+ * the 8-bit cache, the new K/V being in it: request i's extend_lens[i] new tokens (q
+ * [n, H, head_dim] bf16, request after request, 16-byte aligned) attend positions
+ * 0 .. prefix_lens[i] + t of its blocks, at most seq_lens[i] -> out [n, H * head_dim] bf16.  The
+ * lengths are read on the device only.  H divisible by kv_heads, scale > 0.  A negative request
+ * index counts from the table's end.  NaN: a request outside the table, the query tiles (128 rows
+ * of one KV head's query heads) that attend a block which is padding or outside the cache, rows
+ * that attend nothing, and rows of q past the requests' tokens.  workspace >=
+ * qq_fp8_extend_workspace_bytes, of any contents: (m, l, o) partials, when few query rows meet a
+ * wide table. */
+int qq_fp8_extend_attention(const void* q, int num_q_heads, const uint8_t* k_codes, const uint8_t* v_codes,
+                            const float* k_scale, const float* v_scale, int num_blocks, int kv_heads,
+                            int head_dim, const int32_t* block_table, int64_t block_table_stride,
+                            int block_table_rows, int block_table_cols, const int64_t* req_pool_indices,
+                            const int64_t* seq_lens, const int64_t* prefix_lens, const int64_t* extend_lens,
+                            int bs, int64_t n, float scale, void* out, void* workspace,
+                            int64_t workspace_bytes, void* stream);
+int64_t qq_fp8_extend_workspace_bytes(int64_t n, int bs, int num_q_heads, int kv_heads, int head_dim,
+                                      int block_table_cols);
+
 /* ------------------------------------------------------------- HiSparse tier
  * Layouts of the reference HiSparseCoordinator (src/qwenquest/hisparse/coordinator.py:103-131):
  * device_k/v[layer] [R*(buf+1), KV, D] (request r owns rows r*(buf+1) + slot,

@@ -119,6 +119,11 @@ SIGNATURES: dict[str, tuple] = {
          _P, _P, _L, _P],
     ),
     "qq_fp8_decode_workspace_bytes": (_L, [_I, _I, _I, _I]),
+    "qq_fp8_extend_attention": (
+        _I,
+        [_P, _I, _P, _P, _P, _P, _I, _I, _I, _P, _L, _I, _I, _P, _P, _P, _P, _I, _L, _F, _P, _P, _L, _P],
+    ),
+    "qq_fp8_extend_workspace_bytes": (_L, [_L, _I, _I, _I, _I, _I]),
     "qq_hisparse_swap_in": (
         _I,
         [_P, _L, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _L, _P, _P, _P, _P, _L, _L, _P, _P, _P,

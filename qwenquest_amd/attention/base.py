@@ -13,7 +13,12 @@ from typing import TYPE_CHECKING, Any
 import torch
 from torch.autograd import forward_ad
 
-from qwenquest_amd.attention.ops import extend_attention, extend_attention_batch, extend_attention_batch_checked
+from qwenquest_amd.attention.ops import (
+    extend_attention,
+    extend_attention_batch,
+    extend_attention_batch_checked,
+    fp8_extend_attention,
+)
 from qwenquest_amd.paged import BlockReqToTokenPool, Fp8TokenToKVPool
 
 if TYPE_CHECKING:
@@ -99,9 +104,17 @@ class AttentionBackend(ABC):
 
     def _forward_extend_fp8(self, q: torch.Tensor, layer: Any, batch: ForwardBatch) -> torch.Tensor:
         """forward_extend over an 8-bit pool, which holds the new K/V: every token attends the
-        pool's values, its own included."""
+        pool's values, its own included.  bf16 queries with a positive scale run the whole batch in
+        one launch that reads the lengths on the device (NaN where the loop would refuse a request
+        index, and for rows of q past the requests' tokens); others go request by request over the
+        values."""
         pool = self.token_to_kv_pool
         q = q.reshape(q.shape[0], -1, pool.head_dim)
+        if (q.dtype == torch.bfloat16 and 0.0 < float(layer.scaling) < float("inf") and _plain(q)
+                and batch.extend_seq_lens is not None):
+            return fp8_extend_attention(q, pool, layer.layer_id, self.req_to_token_pool.block_table,
+                                        batch.req_pool_indices, batch.seq_lens, batch.extend_prefix_lens,
+                                        batch.extend_seq_lens, float(layer.scaling))
         offsets = batch.extend_token_offsets()
         outputs = []
         for i in range(batch.batch_size):

@@ -1,7 +1,7 @@
 """Attention math (reference ``src/qwenquest/attention/ops.py``).
 
 ``decode_attention`` runs the HIP split-K kernel over an explicit row list;
-``fp8_decode_attention`` runs the HIP kernel over an 8-bit block cache;
+``fp8_decode_attention`` and ``fp8_extend_attention`` run the HIP kernels over an 8-bit block cache;
 ``extend_attention_batch`` runs a whole prefill batch (bf16, head_dim 128) in the HIP
 prefill kernel; ``extend_attention``, one request of any shape, uses torch's SDPA on the
 device, in float32.
@@ -20,7 +20,7 @@ if TYPE_CHECKING:
     from qwenquest_amd.paged import Fp8TokenToKVPool
 
 __all__ = ["decode_attention", "extend_attention", "extend_attention_batch", "fp8_decode_attention",
-           "AttentionWorkspace"]
+           "fp8_extend_attention", "AttentionWorkspace"]
 
 
 class AttentionWorkspace:
@@ -288,5 +288,45 @@ def fp8_decode_attention(
             *pool.layer_args(layer_id), *_table_args(bt), _lib.ptr(rpi), _lib.ptr(seq), bs, _lib.ptr(positions),
             0 if positions is None else max(positions.stride(0), positions.shape[1]), int(top_k), float(scaling),
             _lib.ptr(out), _lib.ptr(ws), need, _lib.stream(dev),
+        )
+    return out
+
+
+def fp8_extend_attention(
+    q: torch.Tensor,
+    pool: Fp8TokenToKVPool,
+    layer_id: int,
+    block_table: torch.Tensor,
+    req_pool_indices: torch.Tensor,
+    seq_lens: torch.Tensor,
+    prefix_lens: torch.Tensor,
+    extend_lens: torch.Tensor,
+    scaling: float,
+) -> torch.Tensor:
+    """Causal prefill of a batch over an 8-bit pool that holds the new K/V: ``q [n, H, D]`` (bf16)
+    holds the requests' new tokens one request after the other; token ``t`` of request ``i`` attends
+    positions ``0 .. prefix_lens[i] + t``.  Returns ``[n, H*D]``; the lengths are read on the device
+    only.  NaN: a request outside the table, a query tile that attends a block which is not there,
+    rows of q past the requests' tokens."""
+    dev = pool.device
+    if q.dtype != torch.bfloat16:
+        raise ValueError(f"unsupported dtype {q.dtype}; the prefill kernel takes bfloat16")
+    q = _queries(q, pool)
+    n, heads, dim = q.shape
+    bt = _block_table(block_table, dev)
+    bs = int(req_pool_indices.shape[0])
+    rpi, seq, prefix, ext = (_lengths(t, bs, dev, what) for t, what in (
+        (req_pool_indices, "req_pool_indices"), (seq_lens, "seq_lens"), (prefix_lens, "prefix_lens"),
+        (extend_lens, "extend_lens")))
+    if bs == 0 and n:
+        raise ValueError(f"{n} tokens of no request")
+    need = int(_lib.load().qq_fp8_extend_workspace_bytes(n, bs, heads, pool.kv_heads, dim, bt.shape[1]))
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    out = torch.empty((n, heads * dim), dtype=q.dtype, device=dev)
+    with torch.cuda.device(dev):
+        _lib.call(
+            "qq_fp8_extend_attention", _lib.ptr(q), heads, *pool.layer_args(layer_id), *_table_args(bt), _lib.ptr(rpi),
+            _lib.ptr(seq), _lib.ptr(prefix), _lib.ptr(ext), bs, n, float(scaling), _lib.ptr(out), _lib.ptr(ws), need,
+            _lib.stream(dev),
         )
     return out

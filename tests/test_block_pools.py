@@ -112,6 +112,18 @@ def test_decode_refuses(lib, kw, said):
     refused(lib.qq_fp8_decode_attention(*a.values(), None), lib, said)
 
 
+@pytest.mark.parametrize("kw, said", BAD_CACHE + [
+    (dict(H=30), b"divisible"), (dict(scale=0.0), b"positive"), (dict(scale=float("nan")), b"positive"),
+    (dict(scale=float("inf")), b"positive"), (dict(bs=-1), b"bad sizes"), (dict(n=1 << 28), b"bad sizes"),
+    (dict(tstride=3), b"bad sizes"), (dict(q=None), b"null"), (dict(ext=None), b"null"), (dict(out=ctypes.c_void_p(4104)), b"aligned"),
+    (dict(n=8, tcols=1 << 12, tstride=1 << 12, ws=None), b"workspace")])
+def test_extend_refuses(lib, kw, said):
+    a = dict(q=FAKE, H=32, **CACHE, table=FAKE, tstride=4, trows=2, tcols=4, rpi=FAKE, seq=FAKE, prefix=FAKE, ext=FAKE, bs=2, n=10,
+             scale=0.1, out=FAKE, ws=FAKE, bytes=1 << 30)
+    a.update(kw)
+    refused(lib.qq_fp8_extend_attention(*a.values(), None), lib, said)
+
+
 def test_decode_workspace(lib):
     assert lib.qq_fp8_decode_workspace_bytes(0, 32, 4, 128) == 0
     assert lib.qq_fp8_decode_workspace_bytes(2, 30, 4, 128) == 0

@@ -1,0 +1,269 @@
+"""The paged request pool, the 8-bit cache and the backends together, as an engine runs them: admission,
+chunked prefill, decode steps, requests that finish and slots that are used again - against the
+cache and the attention by their definitions on the host."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import bf16
+from oracle import fp8_cache as of
+from oracle import quest as oq
+from qwenquest_amd.attention import DenseBackend, QuestHiSparseBackend, QuestOnlyBackend
+from qwenquest_amd.batch import ForwardBatch, ForwardMode
+from qwenquest_amd.memory import MHATokenToKVPool, ReqToTokenPool
+from qwenquest_amd.paged import BlockReqToTokenPool, Fp8TokenToKVPool
+from qwenquest_amd.quest import QuestTrace
+
+pytestmark = pytest.mark.gpu
+
+
+class Layer:
+    def __init__(self, layer_id, dim):
+        self.layer_id, self.scaling = layer_id, dim**-0.5
+
+
+def i64(x, dev):
+    return torch.as_tensor(np.asarray(x), dtype=torch.int64).to(dev)
+
+
+class Engine:
+    """What an engine keeps, and the same on the host: tokens of each request per layer."""
+
+    def __init__(self, dev, backend, layers, heads, kv, dim, dtype, reqs, width, blocks, top_k=256, avoid=False, seed=0):
+        self.dev, self.layers, self.heads, self.kv, self.dim, self.dtype = dev, layers, heads, kv, dim, dtype
+        self.rtp = BlockReqToTokenPool(reqs, width, blocks, dev)
+        self.kvp = Fp8TokenToKVPool(blocks, layers, kv, dim, dev)
+        self.top_k = top_k
+        if backend == "quest":
+            self.be = QuestOnlyBackend(self.rtp, self.kvp, {"algorithm": "quest", "top_k": top_k, "quest_page_size": 64,
+                                                            "avoid_recent_overlap": avoid})
+            self.be.quest.trace = QuestTrace()
+        else:
+            self.be = DenseBackend(self.rtp, self.kvp)
+        self.avoid = avoid
+        self.gen = torch.Generator(device=dev).manual_seed(seed)
+        self.cache = [of.Cache(blocks, kv, dim) for _ in range(layers)]
+        self.lens = {}
+        self.mods = [Layer(i, dim) for i in range(layers)]
+
+    def rand(self, *shape):
+        return torch.empty(shape, device=self.dev).normal_(generator=self.gen).to(self.dtype)
+
+    def check(self, out, q, ks, scale=None):
+        k, v = ks
+        qn = q.double().cpu().numpy()
+        want, spread, size = of.attend(qn, k, v, self.dim**-0.5)
+        bf = self.dtype == torch.bfloat16
+        # 12 bits of a weight cover the prefill's rounding as well as the decode's
+        tol = of.attend_tolerance(want, spread, size, len(k), self.dim, bf, 12 if bf else 22)
+        err = np.abs(out.double().cpu().numpy().reshape(want.shape) - want)
+        assert (err <= tol).all(), (err / tol).max()
+
+    def prefill(self, reqs, new):
+        prefix = [self.lens.get(r, 0) for r in reqs]
+        rpi, pre, ext = i64(reqs, self.dev), i64(prefix, self.dev), i64(new, self.dev)
+        n = sum(new)
+        loc, pos = self.rtp.assign(rpi, pre, ext, n)
+        batch = ForwardBatch(ForwardMode.EXTEND, None, pos, rpi, pre + ext, loc, self.rtp, self.kvp, self.be,
+                             extend_prefix_lens=pre, extend_seq_lens=ext)
+        self.be.init_forward_metadata(batch)
+        for layer in self.mods:
+            q, k, v = self.rand(n, self.heads, self.dim), self.rand(n, self.kv, self.dim) * 2, self.rand(n, self.kv, self.dim)
+            out = self.be.forward(q, k, v, layer, batch)
+            assert out.shape == (n, self.heads * self.dim) and out.dtype == q.dtype
+            self.cache[layer.layer_id].write(loc.cpu().numpy(), k.float().cpu().numpy(), v.float().cpu().numpy())
+            at = 0
+            for r, p, m in zip(reqs, prefix, new):
+                for t in sorted({0, m // 2, m - 1}) if m else []:
+                    self.check(out[at + t], q[at + t], self.cache[layer.layer_id].rows(self.rows(r, p + t + 1)))
+                at += m
+        self.be.on_extend_finished(batch)
+        for r, p, m in zip(reqs, prefix, new):
+            self.lens[r] = p + m
+
+    def rows(self, r, n):
+        return self.rtp.req_to_token[r, :n].long().cpu().numpy()
+
+    def decode(self, reqs):
+        """One eager step of these requests; the attended positions come from the definition."""
+        seq = [self.lens[r] + 1 for r in reqs]
+        rpi, sl = i64(reqs, self.dev), i64(seq, self.dev)
+        loc, pos = self.rtp.assign_decode(rpi, sl)
+        batch = ForwardBatch(ForwardMode.DECODE, None, pos, rpi, sl, loc, self.rtp, self.kvp, self.be)
+        bounds = [self.bounds(layer, reqs, seq) for layer in range(self.layers)]
+        self.be.init_forward_metadata(batch)
+        for layer in self.mods:
+            q, k, v = self.rand(len(reqs), self.heads, self.dim), self.rand(len(reqs), self.kv, self.dim), self.rand(len(reqs), self.kv, self.dim)
+            out = self.be.forward(q, k, v, layer, batch)
+            c = self.cache[layer.layer_id]
+            c.write(loc.cpu().numpy(), k.float().cpu().numpy(), v.float().cpu().numpy())
+            for i, (r, s) in enumerate(zip(reqs, seq)):
+                at = np.arange(s)
+                if isinstance(self.be, QuestOnlyBackend):
+                    at = self.selected(q[i], bounds[layer.layer_id][i], s)
+                    got = self.be.quest.trace.records[-len(reqs) + i]
+                    assert got.layer_id == layer.layer_id and got.positions.tolist() == at.tolist()
+                self.check(out[i], q[i], c.rows(self.rows(r, s)[at]))
+        for r, s in zip(reqs, seq):
+            self.lens[r] = s
+
+    def bounds(self, layer, reqs, seq):
+        """Bounds of the pages that are complete before the step's own token, bf16 bits."""
+        out = []
+        for r, s in zip(reqs, seq):
+            full = (s - 1) // 64
+            k = self.cache[layer].rows(self.rows(r, full * 64))[0].reshape(full, 64, self.kv, self.dim)
+            lo, hi = (bf16.from_f32(x.astype(np.float32)) for x in (k.min(1), k.max(1))) if full else (np.zeros((0, self.kv, self.dim), np.uint16),) * 2
+            out.append(np.stack([lo, hi], -1))
+        return out
+
+    def selected(self, q, bounds, s):
+        if s <= self.top_k:
+            return np.arange(s)
+        qbar = oq.group_queries(q.float().cpu().numpy()[None], self.kv, self.dim, self.dtype == torch.bfloat16)
+        scores = oq.page_scores(qbar, bounds[None])[0]
+        limit = s // 64 - 1 if self.avoid else s // 64
+        pages = oq.topk_pages(scores, min(limit, len(scores)), self.top_k // 64 - 1)
+        return np.concatenate([(pages[:, None] * 64 + np.arange(64)).reshape(-1), np.arange(s - 64, s)])
+
+    def finish(self, r):
+        self.be.on_request_finished(r)
+        self.rtp.release(i64([r], self.dev))
+        del self.lens[r]
+
+
+@pytest.mark.parametrize("backend, heads, kv, dim, dtype, avoid", [
+    ("quest", 16, 4, 128, torch.bfloat16, False), ("quest", 6, 2, 128, torch.bfloat16, True),
+    ("quest", 8, 2, 64, torch.float32, False), ("dense", 10, 2, 128, torch.bfloat16, False), ("dense", 3, 3, 64, torch.float32, False)])
+def test_a_server_s_life(cuda, backend, heads, kv, dim, dtype, avoid):
+    e = Engine(cuda, backend, 2, heads, kv, dim, dtype, 4, 900, 50, avoid=avoid)
+    e.prefill([2, 0], [300, 40])
+    for _ in range(3):
+        e.decode([0, 2])
+    e.prefill([2, 3], [250, 64])  # a second chunk, and another request
+    for i in range(70):
+        e.decode([3, 2, 0] if i % 2 else [2, 3])
+    e.finish(2)
+    e.prefill([2], [500])  # the slot again, over blocks that were used
+    for _ in range(4):
+        e.decode([2, 0])
+    e.rtp.check_errors()
+
+
+def test_decode_steps_in_a_replayed_graph(cuda):
+    """A captured step of every layer, replayed as lengths grow in place; eager steps between."""
+    e, w = (Engine(cuda, "quest", 2, 8, 2, 128, torch.bfloat16, 3, 900, 50, seed=5) for _ in range(2))
+    for x in (e, w):
+        x.be.quest.trace = None
+        x.prefill([0, 1, 2], [400, 63, 255])
+    rpi, seq = torch.arange(3, device=cuda), i64([401, 64, 256], cuda)
+    q, k, v = (torch.zeros(2, 3, h, 128, device=cuda, dtype=torch.bfloat16) for h in (8, 2, 2))
+
+    def step(x):
+        loc, pos = x.rtp.assign_decode(rpi, seq)
+        batch = ForwardBatch(ForwardMode.DECODE, None, pos, rpi, seq, loc, x.rtp, x.kvp, x.be)
+        x.be.init_forward_metadata(batch)
+        return [x.be.forward(q[i], k[i], v[i], x.mods[i], batch) for i in range(2)]
+
+    for t in (q, k, v):
+        t.normal_(generator=e.gen)
+    step(e), step(w)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step(e)
+    for _ in range(6):
+        seq += 1
+        for t in (q, k, v):
+            t.normal_(generator=e.gen)
+        graph.replay()
+        want = step(w)
+        assert all(torch.equal(a, b) and not a.isnan().any() for a, b in zip(outs, want))
+        assert torch.equal(e.kvp.k_codes, w.kvp.k_codes) and torch.equal(e.be.quest.page_k_bounds, w.be.quest.page_k_bounds)
+    e.rtp.poll_errors()
+
+
+def test_padded_entries_of_a_decode_batch(cuda):
+    """seq_lens 0: no row, no token stored, an output of zeros."""
+    e = Engine(cuda, "dense", 1, 4, 2, 128, torch.bfloat16, 3, 300, 20)
+    e.prefill([0, 1], [100, 30])
+    rpi, seq = i64([0, 0, 1], cuda), i64([101, 0, 31], cuda)
+    loc, pos = e.rtp.assign_decode(rpi, seq)
+    assert loc[1] == 0
+    batch = ForwardBatch(ForwardMode.DECODE, None, pos, rpi, seq, loc, e.rtp, e.kvp, e.be)
+    q, k, v = e.rand(3, 4, 128), e.rand(3, 2, 128), e.rand(3, 2, 128)
+    out = e.be.forward(q, k, v, e.mods[0], batch)
+    e.cache[0].write(loc.cpu().numpy(), k.float().cpu().numpy(), v.float().cpu().numpy())
+    for i in (0, 2):
+        e.check(out[i], q[i], e.cache[0].rows(e.rows(int(rpi[i]), int(seq[i]))))
+    assert not out[1].any() and not e.kvp.k_codes[0, 0].any()
+
+
+def test_phases_are_the_step_in_two(cuda):
+    e = Engine(cuda, "quest", 1, 8, 2, 128, torch.bfloat16, 2, 900, 30)
+    e.prefill([0, 1], [500, 70])
+    rpi, seq = i64([0, 1], cuda), i64([501, 71], cuda)
+    loc, pos = e.rtp.assign_decode(rpi, seq)
+    batch = ForwardBatch(ForwardMode.DECODE, None, pos, rpi, seq, loc, e.rtp, e.kvp, e.be)
+    e.be.init_forward_metadata(batch)
+    q, k, v = e.rand(2, 8, 128), e.rand(2, 2, 128), e.rand(2, 2, 128)
+    whole = e.be.forward(q, k, v, e.mods[0], batch)
+    e.be.forward_decode_phase(q, k, v, e.mods[0], batch, 1)
+    assert torch.equal(whole, e.be.forward_decode_phase(q, k, v, e.mods[0], batch, 2))
+    with pytest.raises(ValueError, match="phase"):
+        e.be.forward_decode_phase(q, k, v, e.mods[0], batch, 4)
+    with pytest.raises(ValueError, match="block"):
+        e.be.sparse_attention(q, e.mods[0], rpi, torch.zeros(2, 256, dtype=torch.int32, device=cuda), seq.int(), 2)
+
+
+def test_pools_that_do_not_go_together(cuda):
+    paged, rows = BlockReqToTokenPool(2, 300, 9, cuda), ReqToTokenPool(2, 300, cuda)
+    fp8, plain = Fp8TokenToKVPool(9, 1, 2, 128, cuda), MHATokenToKVPool(600, 1, 2, 128, torch.bfloat16, cuda)
+    cfg = {"algorithm": "quest", "top_k": 128, "quest_page_size": 64}
+    with pytest.raises(ValueError, match="BlockReqToTokenPool"):
+        DenseBackend(rows, fp8)
+    with pytest.raises(ValueError, match="blocks"):
+        DenseBackend(BlockReqToTokenPool(2, 300, 10, cuda), fp8)
+    with pytest.raises(ValueError, match="quest_page_size must be 64"):
+        QuestOnlyBackend(paged, fp8, {**cfg, "quest_page_size": 32})
+    with pytest.raises(ValueError, match="MHATokenToKVPool"):
+        QuestHiSparseBackend(paged, fp8, cfg, host_pool_size=100)
+    DenseBackend(paged, plain)
+
+
+@pytest.mark.parametrize("backend", ["dense", "quest"])
+def test_paged_rows_serve_the_bf16_pool(cuda, backend):
+    """The slot maps with an MHATokenToKVPool: the same outputs as with rows handed out by hand."""
+    outs = []
+    for paged in (True, False):
+        gen = torch.Generator(device=cuda).manual_seed(1)
+        rtp = BlockReqToTokenPool(2, 600, 20, cuda) if paged else ReqToTokenPool(2, 600, cuda)
+        kvp = MHATokenToKVPool(20 * 64, 1, 4, 128, torch.bfloat16, cuda)
+        be = (DenseBackend(rtp, kvp) if backend == "dense" else
+              QuestOnlyBackend(rtp, kvp, {"algorithm": "quest", "top_k": 128, "quest_page_size": 64}))
+        rpi, pre, ext = i64([1, 0], cuda), i64([0, 0], cuda), i64([300, 90], cuda)
+        if paged:
+            loc, _ = rtp.assign(rpi, pre, ext, 390)
+        else:
+            loc = torch.arange(1, 391, device=cuda)
+            rtp.req_to_token[1, :300], rtp.req_to_token[0, :90] = loc[:300].int(), loc[300:].int()
+        batch = ForwardBatch(ForwardMode.EXTEND, None, None, rpi, ext, loc, rtp, kvp, be, extend_prefix_lens=pre, extend_seq_lens=ext)
+
+        def rand(*shape):
+            return torch.empty(shape, device=cuda).normal_(generator=gen).to(torch.bfloat16)
+
+        got = [be.forward(rand(390, 16, 128), rand(390, 4, 128), rand(390, 4, 128), Layer(0, 128), batch)]
+        seq = i64([301, 91], cuda)
+        if paged:
+            loc, _ = rtp.assign_decode(rpi, seq)
+        else:
+            loc = i64([500, 501], cuda)
+            rtp.req_to_token[rpi, seq - 1] = loc.int()
+        batch = ForwardBatch(ForwardMode.DECODE, None, None, rpi, seq, loc, rtp, kvp, be)
+        be.init_forward_metadata(batch)
+        got.append(be.forward(rand(2, 16, 128), rand(2, 4, 128), rand(2, 4, 128), Layer(0, 128), batch))
+        outs.append(got)
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
