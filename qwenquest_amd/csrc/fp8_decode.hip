@@ -4,17 +4,20 @@
 //   t_j = scale * log2(e) * ks * (q . kc_j),  p_j = 2^(t_j - max t),  out = sum p_j vs vc_j / sum p_j.
 //
 // The work comes in units, a (partial) block of the cache: of a dense request its blocks in
-// order, of one with selected pages those and the one or two blocks of its recent window.  All
+// order, of one with selected pages those and its recent window (the last 64 tokens, which lie at
+// 64 different places of two blocks: a place comes from one or the other).  All
 // requests' units in a row are cut into equal slices, one to a thread block per (KV head, tile
 // of 16 query heads), so that any mix of lengths fills the chip evenly in one round; a
-// request that lies in one slice is finished there, the others' (m, l, o) parts are merged.
+// request that lies in one slice is finished there, the others' (m, l, o) parts are merged by
+// the block that completes them.  Two launches: fp8_begin_kernel cuts the slices and stores the
+// new tokens, fp8_attend_kernel does the rest.
 //
 // A wave takes a unit at a time: K and V codes straight from memory to registers in the
 // operands' order (1 KiB runs), converted to bf16 (exact), S^T = K Q^T, the softmax in
 // registers, O^T += V^T P^T, with P's values scaled by vs as bf16 pieces: two for bf16 output
 // (16 significand bits), three for fp32 (all 24).  fp32 queries go in as three bf16 pieces, too.
 // Bound: HBM, the codes once.
-#include "qq_fp8.h"
+#include "qq_fp8_store.h"
 #include "qq_quest_dev.h"
 #include "qq_rules.h"
 
@@ -27,6 +30,10 @@ constexpr int kDecParts = 64;  // slices of a request, at most: the merge's tabl
 
 struct DecPlan {
   int32_t total, len, slices, pad;  // units of the batch, units of a slice, slices
+};
+struct DecItem {  // a slice's first request: its units are [c0, c1) of the batch's
+  int32_t b, c0, c1, seq;
+  int32_t req, pad[3];  // its table row, or -1: outside the table
 };
 
 struct DecArgs {
@@ -48,7 +55,8 @@ struct DecArgs {
   int max_slices, heads;  // heads: KV * tiles
   DecPlan* plan;
   int32_t* cu;       // [bs + 1] units before each request
-  int32_t* first;    // [max_slices] request of each slice's first unit
+  DecItem* items;    // [max_slices]
+  uint32_t* done;    // [max_slices, heads] parts finished of the request that goes on behind a slice
   float* part_o;     // [max_slices, 2, heads, 16, D]
   float* part_ml;    // [max_slices, 2, heads, 16, 2]
 };
@@ -56,17 +64,23 @@ struct DecArgs {
 __device__ inline int context_of(const DecArgs& a, int b) {
   return (int)min(max(a.seq[b], (int64_t)0), (int64_t)a.table_cols * kCacheTokens);
 }
+__device__ inline int table_row(const DecArgs& a, int b) {
+  const int64_t req = a.rpi[b];
+  return req >= 0 && req < a.table_rows ? (int)req : -1;
+}
 __device__ inline bool is_sparse(const DecArgs& a, int s) { return a.positions && s > a.top_k; }
 __device__ inline int units_of(const DecArgs& a, int s) {
-  if (is_sparse(a, s)) return a.top_k / 64 + (s % 64 ? 1 : 0);
+  if (is_sparse(a, s)) return a.top_k / 64;
   return max((s + 63) / 64, 1);  // an empty context: one unit without tokens, which writes its zeros
 }
 
-__global__ __launch_bounds__(1024) void fp8_plan_kernel(DecArgs a) {
-  __shared__ int s_sum[16], s_long[16];
+// Cuts the batch's units into slices; 256 threads.
+__device__ inline void plan_slices(const DecArgs& a) {
+  __shared__ int s_sum[4], s_long[4];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  for (int i = tid; i < a.max_slices * a.heads; i += 256) a.done[i] = 0u;
   int base = 0, longest = 0;
-  for (int b0 = 0; b0 < a.bs; b0 += 1024) {
+  for (int b0 = 0; b0 < a.bs; b0 += 256) {
     const int b = b0 + tid;
     const int u = b < a.bs ? units_of(a, context_of(a, b)) : 0;
     int x = u;
@@ -81,7 +95,7 @@ __global__ __launch_bounds__(1024) void fp8_plan_kernel(DecArgs a) {
     __syncthreads();
     int before = base;
 #pragma unroll
-    for (int w = 0; w < 16; ++w) {
+    for (int w = 0; w < 4; ++w) {
       if (w < wave) before += s_sum[w];
       base += s_sum[w];
     }
@@ -92,12 +106,11 @@ __global__ __launch_bounds__(1024) void fp8_plan_kernel(DecArgs a) {
   if (lane == 0) s_long[wave] = longest;
   if (tid == 0) a.cu[a.bs] = base;
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < 16; ++w) longest = max(longest, s_long[w]);
+  longest = max(max(s_long[0], s_long[1]), max(s_long[2], s_long[3]));
   const int len = rules::fp8_slice_len(base, longest, a.max_slices);
   const int slices = (base + len - 1) / len;
   if (tid == 0) *a.plan = {base, len, slices, 0};
-  for (int i = tid; i < slices; i += 1024) {
+  for (int i = tid; i < slices; i += 256) {
     const int at = i * len;
     int lo = 0, hi = a.bs;  // the last request that begins at or before this unit
     while (hi - lo > 1) {
@@ -105,8 +118,21 @@ __global__ __launch_bounds__(1024) void fp8_plan_kernel(DecArgs a) {
       if (a.cu[mid] <= at) lo = mid;
       else hi = mid;
     }
-    a.first[i] = lo;
+    a.items[i] = {lo, a.cu[lo], a.cu[lo + 1], context_of(a, lo), table_row(a, lo), {0, 0, 0}};
   }
+}
+
+// Block 0: the slices; then a block per new token, head, and K or V.
+template <int D, typename SRC>
+__global__ __launch_bounds__(256) void fp8_begin_kernel(DecArgs a, StoreArgs st) {
+  __shared__ StoreSmem<D> sm;
+  if (blockIdx.x == 0) {
+    plan_slices(a);
+    return;
+  }
+  const int i = (blockIdx.x - 1) >> 1, h = i % a.c.KV;
+  if (blockIdx.x & 1) store_segment<D, SRC, false>(st, sm, i / a.c.KV, h);
+  else store_segment<D, SRC, true>(st, sm, i / a.c.KV, h);
 }
 
 __device__ inline float trunc_bf16(float x) { return __uint_as_float(__float_as_uint(x) & 0xFFFF0000u); }
@@ -161,17 +187,103 @@ __device__ inline void load_query(const void* q, int64_t at, bool in, bf16x8_t (
 
 template <int D>
 struct DecSmem {
-  float m[kDecWaves][kTile], l[kDecWaves][kTile];
-  float o[kDecWaves][kTile][D + 4];
+  union {
+    struct {
+      float m[kDecWaves][kTile], l[kDecWaves][kTile];
+      float o[kDecWaves][kTile][D + 4];
+    };
+    struct {
+      float w[kTile][kDecParts], sum[kTile];
+      float4 red[64 * kDecWaves];
+    } merge;
+  };
+  uint32_t last;
 };
+
+// The parts of a request's tile added up, by the block that finished the last of them: a wave
+// per query head and a lane per part for the weights, then a thread per 4 channels of a head,
+// and where those are few, of every ng-th part.
+template <int D, typename T>
+__device__ inline void merge_parts(const DecArgs& a, DecSmem<D>& sm, int head, int first, int parts, int rows, T* out) {
+  constexpr int NT = 64 * kDecWaves;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  // row r of part i: of slice first + i, the part that begins its request there, or goes on in it
+  auto row_of = [&](int i) { return ((first + i) * 2 + (i == 0 ? 1 : 0)) * a.heads + head; };
+  const uint64_t* ml = reinterpret_cast<const uint64_t*>(a.part_ml);
+  const int items = rows * (D / 4), ng = max(NT / items, 1);
+  const int grp = items <= NT ? tid / items : 0;
+  const int it0 = tid - grp * items;
+  const __amdgpu_buffer_rsrc_t ro =
+      agent_rsrc(a.part_o, (uint32_t)((int64_t)a.max_slices * 2 * a.heads * kTile * D * (int)sizeof(float)));
+  // a batch of an item's parts; past the last part they re-read it.  The first go out before the
+  // weights are known
+  constexpr int kBatch = 8;
+  float4 x[kBatch];
+  auto load_parts = [&](int it, int i0) {
+    const int r = it / (D / 4), d = (it - r * (D / 4)) * 4;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u)
+      x[u] = ld_agent_x4(ro, (uint32_t)(((row_of(min(i0 + u * ng, parts - 1)) * kTile + r) * D + d) * (int)sizeof(float)));
+  };
+  load_parts(min(it0, items - 1), grp);
+  for (int r = wave; r < rows; r += kDecWaves) {
+    const uint64_t e = lane < parts ? ld_agent(ml + (int64_t)row_of(lane) * kTile + r) : (uint64_t)0xFF800000u;  // (-inf, 0)
+    const float m = __uint_as_float((uint32_t)e), l = __uint_as_float((uint32_t)(e >> 32));
+    float Mx = m;
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) Mx = fmaxf(Mx, __shfl_xor(Mx, d, 64));
+    const float w = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - Mx);
+    float Ls = l != l ? l : w * l;
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) Ls += __shfl_xor(Ls, d, 64);
+    sm.merge.w[r][lane] = w;
+    if (lane == 0) sm.merge.sum[r] = Ls;
+  }
+  lds_barrier();
+  if (ng == 1 && grp > 0) return;  // threads past the items
+  for (int it = it0; it < items; it += NT) {  // once where ng > 1
+    const int r = it / (D / 4), d = (it - r * (D / 4)) * 4;
+    float4 Os = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (grp < ng) {
+      for (int i0 = grp; i0 < parts; i0 += kBatch * ng) {
+        if (it != it0 || i0 != grp) load_parts(it, i0);
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          if (i0 + u * ng >= parts) break;
+          const float w = sm.merge.w[r][i0 + u * ng];
+          Os.x += w * x[u].x;
+          Os.y += w * x[u].y;
+          Os.z += w * x[u].z;
+          Os.w += w * x[u].w;
+        }
+      }
+    }
+    if (ng > 1) {  // block-uniform
+      sm.merge.red[tid] = Os;
+      __syncthreads();
+      if (grp != 0) return;
+      for (int g = 1; g < ng; ++g) {
+        const float4 y = sm.merge.red[tid + g * items];
+        Os.x += y.x;
+        Os.y += y.y;
+        Os.z += y.z;
+        Os.w += y.w;
+      }
+    }
+    const float Ls = sm.merge.sum[r];
+    const float inv = Ls <= 0.0f ? 0.0f : 1.0f / Ls;
+    store4(out + (int64_t)r * D + d, Os.x * inv, Os.y * inv, Os.z * inv, Os.w * inv);
+  }
+}
 
 template <int D, typename T>
 __global__ __launch_bounds__(64 * kDecWaves, 2) void fp8_attend_kernel(DecArgs a) {
   constexpr int QP = sizeof(T) == 2 ? 1 : 3, PP = sizeof(T) == 2 ? 2 : 3;  // pieces of q and of the weights
   constexpr int KL = D / 64, VL = D / 16;  // 16-byte loads a lane: per 16 tokens of K, per block of V
   __shared__ DecSmem<D> sm;
-  const DecPlan plan = *a.plan;
   const int head = blockIdx.x % a.heads, slice = blockIdx.x / a.heads;
+  const DecPlan plan = *a.plan;
+  const DecItem item = a.items[slice];  // both in one round trip; stale past the last slice
   if (slice >= plan.slices) return;
   const int h = head / a.tiles, tile = head - h * a.tiles;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -180,16 +292,13 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void fp8_attend_kernel(DecArgs a
   const int q_head = h * a.G + tile * kTile;
   const int end = min((slice + 1) * plan.len, plan.total);
   int at = slice * plan.len;
-  for (int b = a.first[slice]; at < end; ++b) {
-    const int c0 = a.cu[b], c1 = a.cu[b + 1];
+  int b = item.b, c0 = item.c0, c1 = item.c1, seq = item.seq, req = item.req;
+  for (;;) {
     const int u0 = at - c0, u1 = min(end, c1) - c0;  // this slice's units of request b
-    const int seq = context_of(a, b);
     const bool sparse = is_sparse(a, seq);
-    const int64_t req = a.rpi[b];
-    const bool known = req >= 0 && req < a.table_rows;
-    const int32_t* tr = a.table + (known ? req : 0) * a.table_stride;
-    const int picked = a.top_k / 64 - 1;  // selected pages
-    const int win = seq & 63;             // the window's first token in its first block
+    const bool known = req >= 0;
+    const int32_t* tr = a.table + (int64_t)max(req, 0) * a.table_stride;
+    const int picked = a.top_k / 64 - 1;  // selected pages; the unit after them is the window
 
     bf16x8_t qf[2 * KL][QP];
 #pragma unroll
@@ -199,36 +308,50 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void fp8_attend_kernel(DecArgs a
     }
     // lane j looks up this wave's unit j0 + j: u0 + wave + 4 (j0 + j)
     const int n = u1 - u0 > wave ? (u1 - u0 - wave + kDecWaves - 1) / kDecWaves : 0;
-    int blk = 0;
-    float ks = 0.0f, vs = 0.0f;
+    int blk = 0, blk2 = 0;  // blk2: the window's second block
+    float ks = 0.0f, vs = 0.0f, ks2 = 0.0f, vs2 = 0.0f;
     bool bad = !known;
+    auto block_at = [&](int page) {
+      const int x = page >= 0 && page < a.table_cols ? tr[page] : 0;
+      if (x > 0 && x < a.c.blocks) return x;
+      bad = true;  // no block there: no answer
+      return 0;
+    };
     auto resolve = [&](int j0) {
       const int u = u0 + wave + kDecWaves * (j0 + lane);
-      blk = 0;
+      blk = blk2 = 0;
+      const bool win = sparse && u == picked;
       if (j0 + lane < n && seq > 0 && known) {
-        int page = u;
-        if (sparse) page = u < picked ? a.positions[(int64_t)b * a.pos_stride + u * 64] >> 6 : (seq - 64) / 64 + (u - picked);
-        const int x = page >= 0 && page < a.table_cols ? tr[page] : 0;
-        if (x > 0 && x < a.c.blocks) blk = x;
-        else bad = true;  // no block there: no answer
+        blk = block_at(!sparse ? u : win ? (seq - 64) >> 6 : a.positions[(int64_t)b * a.pos_stride + u * 64] >> 6);
+        blk2 = win && (seq & 63) ? block_at(seq >> 6) : blk;
       }
-      const int64_t e = (int64_t)blk * a.c.KV + h;
-      ks = a.c.ks[e] * a.sl2;
+      const int64_t e = (int64_t)blk * a.c.KV + h, e2 = (int64_t)blk2 * a.c.KV + h;
+      ks = a.c.ks[e];
       vs = a.c.vs[e];
+      if (sparse) {
+        ks2 = a.c.ks[e2];
+        vs2 = a.c.vs[e2];
+      }
     };
     uint4 kr[4][KL], vr[VL];
-    auto head_of = [&](int j) { return ((int64_t)__builtin_amdgcn_readlane(blk, j & 63) * a.c.KV + h) * (64 * D) + lane * 16; };
-    auto load_k = [&](int j) {
-      const uint8_t* p = a.c.kc + head_of(j);
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int i = 0; i < KL; ++i) kr[t][i] = *reinterpret_cast<const uint4*>(p + (t * KL + i) * 1024);
+    auto head_at = [&](int blocks, int j) {
+      return ((int64_t)__builtin_amdgcn_readlane(blocks, j & 63) * a.c.KV + h) * (64 * D) + lane * 16;
     };
-    auto load_v = [&](int j) {
-      const uint8_t* p = a.c.vc + head_of(j);
+    // K of unit j: a window's tokens before place seq % 64 come from its second block
+    auto load_k = [&](int j) {
+      const uint8_t* p = a.c.kc + head_at(blk, j);
+      const uint8_t* p2 = a.c.kc + head_at(blk2, j);
 #pragma unroll
-      for (int i = 0; i < VL; ++i) vr[i] = *reinterpret_cast<const uint4*>(p + i * 1024);
+      for (int t = 0; t < 4; ++t) {
+        const uint8_t* pt = t * 16 + m16 < (seq & 63) ? p2 : p;
+#pragma unroll
+        for (int i = 0; i < KL; ++i) kr[t][i] = *reinterpret_cast<const uint4*>(pt + (t * KL + i) * 1024);
+      }
+    };
+    auto load_v = [&](const int blocks, int j, uint4* v) {
+      const uint8_t* p = a.c.vc + head_at(blocks, j);
+#pragma unroll
+      for (int i = 0; i < VL; ++i) v[i] = *reinterpret_cast<const uint4*>(p + i * 1024);
     };
     float4_t o[VL];
 #pragma unroll
@@ -237,16 +360,14 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void fp8_attend_kernel(DecArgs a
     if (n > 0) {
       resolve(0);
       load_k(0);
-      load_v(0);
+      load_v(blk, 0, vr);
     }
     for (int j = 0; j < n; ++j) {
-      const float kscale = __shfl(ks, j & 63, 64), vscale = __shfl(vs, j & 63, 64);
-      // tokens of this unit
       const int u = u0 + wave + kDecWaves * j;
-      int lo = 0, hi = 64;
-      if (!sparse) hi = min(64, seq - u * 64);
-      else if (u == picked) lo = win;
-      else if (u > picked) hi = win;
+      const bool win = sparse && u == picked;
+      const int hi = sparse ? 64 : min(64, seq - u * 64);  // tokens of this unit
+      const float kscale = __shfl(ks, j & 63, 64) * a.sl2, vscale = __shfl(vs, j & 63, 64);
+      const float kscale2 = win ? __shfl(ks2, j & 63, 64) * a.sl2 : kscale, vscale2 = win ? __shfl(vs2, j & 63, 64) : vscale;
       const bool last = j + 1 >= n, next_set = ((j + 1) & 63) == 0;
       float4_t s[4];
 #pragma unroll
@@ -262,14 +383,16 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void fp8_attend_kernel(DecArgs a
           }
         }
       }
-      if (!last && !next_set) load_k(j + 1);
+      // the next unit's K under this one's softmax and values; a window's second V goes there instead
+      if (win) load_v(blk2, j, &kr[0][0]);
+      else if (!last && !next_set) load_k(j + 1);
       float mx = -INFINITY;
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int tok = t * 16 + g * 4 + i;
-          s[t][i] = tok >= lo && tok < hi ? s[t][i] * kscale : -INFINITY;
+          s[t][i] = tok < hi ? s[t][i] * (tok < (seq & 63) ? kscale2 : kscale) : -INFINITY;
           mx = fmaxf(mx, s[t][i]);
         }
       mx = fmaxf(mx, lane_xor16(mx, lane));
@@ -286,8 +409,20 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void fp8_attend_kernel(DecArgs a
           const float p = __builtin_amdgcn_exp2f(s[t][i] - mb);
           sum += p;
           // a masked token weighs nothing whatever its block's scale is
-          s[t][i] = s[t][i] == -INFINITY ? 0.0f : p * vscale;
+          s[t][i] = s[t][i] == -INFINITY ? 0.0f : p * (t * 16 + g * 4 + i < (seq & 63) ? vscale2 : vscale);
         }
+      if (win) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const int from2 = min(max((seq & 63) - t * 16 - g * 4, 0), 4);  // of the word's four tokens
+          const uint32_t mask = from2 >= 4 ? 0xFFFFFFFFu : (1u << (8 * from2)) - 1u;
+#pragma unroll
+          for (int i = 0; i < VL; ++i) {
+            uint32_t& w = reinterpret_cast<uint32_t*>(&vr[i])[t];
+            w = (reinterpret_cast<const uint32_t*>(&kr[0][0])[i * 4 + t] & mask) | (w & ~mask);
+          }
+        }
+      }
       L = L * alpha + sum;
 #pragma unroll
       for (int i = 0; i < VL; ++i)
@@ -317,11 +452,9 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void fp8_attend_kernel(DecArgs a
         }
       }
       if (!last) {
-        if (next_set) {
-          resolve(j + 1);
-          load_k(j + 1);
-        }
-        load_v(j + 1);
+        if (next_set) resolve(j + 1);
+        if (next_set || win) load_k(j + 1);
+        load_v(blk, j + 1, vr);
       }
     }
     L += lane_xor16(L, lane);
@@ -338,7 +471,9 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void fp8_attend_kernel(DecArgs a
       *reinterpret_cast<float4_t*>(&sm.o[wave][m16][i * 16 + g * 4]) = o[i];
     __syncthreads();
     const bool whole = u0 == 0 && c1 <= end;
-    const int64_t part = ((int64_t)(slice * 2 + (u0 == 0 ? 1 : 0)) * a.heads + head) * kTile;
+    T* out = static_cast<T*>(a.out) + ((int64_t)b * a.H + q_head) * D;
+    const int part = ((slice * 2 + (u0 == 0 ? 1 : 0)) * a.heads + head) * kTile;
+    const __amdgpu_buffer_rsrc_t po = agent_rsrc(a.part_o + (int64_t)part * D, (uint32_t)(kTile * D * sizeof(float)));
     for (int it = tid; it < rows * (D / 4); it += 64 * kDecWaves) {
       const int r = it / (D / 4), d = (it - r * (D / 4)) * 4;
       float Mx = -INFINITY;
@@ -359,70 +494,36 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void fp8_attend_kernel(DecArgs a
       }
       if (whole) {
         const float inv = Ls <= 0.0f ? 0.0f : 1.0f / Ls;  // nothing attended: zeros
-        store4(static_cast<T*>(a.out) + ((int64_t)b * a.H + q_head + r) * D + d, Os.x * inv, Os.y * inv, Os.z * inv, Os.w * inv);
+        store4(out + (int64_t)r * D + d, Os.x * inv, Os.y * inv, Os.z * inv, Os.w * inv);
       } else {
-        *reinterpret_cast<float4*>(a.part_o + (part + r) * D + d) = Os;
-        if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (part + r) * 2) = make_float2(Mx, Ls);
+        st_agent_x4(po, (uint32_t)((r * D + d) * sizeof(float)), Os);
+        if (d == 0) {
+          st_agent(a.part_ml + (int64_t)(part + r) * 2, Mx);
+          st_agent(a.part_ml + (int64_t)(part + r) * 2 + 1, Ls);
+        }
       }
     }
+    if (!whole) {
+      const int first = c0 / plan.len, parts = (c1 - 1) / plan.len - first + 1;
+      wait_memory();
+      __syncthreads();
+      if (tid == 0) sm.last = add_agent(&a.done[first * a.heads + head], 1u) == (uint32_t)parts - 1;
+      __syncthreads();
+      if (sm.last) merge_parts<D, T>(a, sm, head, first, parts, rows, out);
+    }
     at = c0 + u1;
+    if (at >= end) return;
+    ++b;
+    c0 = c1;
+    c1 = a.cu[b + 1];
+    seq = context_of(a, b);
+    req = table_row(a, b);
   }
-}
-
-// The parts of a request added up: a thread block per (request, query head), a thread per 4
-// channels and every (256 / (D / 4))-th part.
-template <int D, typename T>
-__global__ __launch_bounds__(256) void fp8_merge_kernel(DecArgs a) {
-  constexpr int DG = D / 4, NG = 256 / DG;
-  __shared__ float s_w[kDecParts];
-  __shared__ float4 s_o[256];
-  const DecPlan plan = *a.plan;
-  const int b = blockIdx.x, q_head = blockIdx.y;
-  const int c0 = a.cu[b], c1 = a.cu[b + 1];
-  const int first = c0 / plan.len, parts = (c1 - 1) / plan.len - first + 1;
-  if (parts <= 1) return;
-  const int h = q_head / a.G, r = (q_head - h * a.G) % kTile, head = h * a.tiles + (q_head - h * a.G) / kTile;
-  const int tid = threadIdx.x, grp = tid / DG, d = (tid % DG) * 4;
-  // part i: of slice first + i, the part that begins its request in the slice, or goes on in it
-  auto row_of = [&](int i) { return ((int64_t)((first + i) * 2 + (i == 0 ? 1 : 0)) * a.heads + head) * kTile + r; };
-  const int lane = tid & 63;
-  const float2 ml = lane < parts ? *reinterpret_cast<const float2*>(a.part_ml + row_of(lane) * 2) : make_float2(-INFINITY, 0.0f);
-  float Mx = ml.x;
-#pragma unroll
-  for (int x = 32; x >= 1; x >>= 1) Mx = fmaxf(Mx, __shfl_xor(Mx, x, 64));
-  const float wt = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - Mx);
-  float Ls = ml.y != ml.y ? ml.y : wt * ml.y;
-#pragma unroll
-  for (int x = 32; x >= 1; x >>= 1) Ls += __shfl_xor(Ls, x, 64);
-  if (tid < 64) s_w[tid] = wt;
-  __syncthreads();
-  float4 Os = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i = grp; i < parts; i += NG) {
-    const float w = s_w[i];
-    const float4 x = *reinterpret_cast<const float4*>(a.part_o + row_of(i) * D + d);
-    Os.x += w * x.x;
-    Os.y += w * x.y;
-    Os.z += w * x.z;
-    Os.w += w * x.w;
-  }
-  s_o[tid] = Os;
-  __syncthreads();
-  if (grp) return;
-#pragma unroll
-  for (int k = 1; k < NG; ++k) {
-    const float4 x = s_o[tid + k * DG];
-    Os.x += x.x;
-    Os.y += x.y;
-    Os.z += x.z;
-    Os.w += x.w;
-  }
-  const float inv = Ls <= 0.0f ? 0.0f : 1.0f / Ls;
-  store4(static_cast<T*>(a.out) + ((int64_t)b * a.H + q_head) * D + d, Os.x * inv, Os.y * inv, Os.z * inv, Os.w * inv);
 }
 
 // The workspace's parts, in order; offsets are multiples of 256 bytes.
 struct DecSpace {
-  int64_t cu, first, part_o, part_ml, bytes;
+  int64_t cu, items, done, part_o, part_ml, bytes;
   int max_slices;
 };
 DecSpace decode_space(int bs, int H, int KV, int D) {
@@ -431,18 +532,20 @@ DecSpace decode_space(int bs, int H, int KV, int D) {
   DecSpace s;
   s.max_slices = rules::fp8_max_slices(heads);
   s.cu = up(sizeof(DecPlan));
-  s.first = s.cu + up((int64_t)(bs + 1) * 4);
-  s.part_o = s.first + up((int64_t)s.max_slices * 4);
+  s.items = s.cu + up((int64_t)(bs + 1) * 4);
+  s.done = s.items + up((int64_t)s.max_slices * sizeof(DecItem));
+  s.part_o = s.done + up((int64_t)s.max_slices * heads * 4);
   s.part_ml = s.part_o + (int64_t)s.max_slices * 2 * heads * kTile * D * 4;
   s.bytes = s.part_ml + (int64_t)s.max_slices * 2 * heads * kTile * 2 * 4;
   return s;
 }
 
 template <int D, typename T>
-void launch(const DecArgs& a, hipStream_t s) {
-  fp8_plan_kernel<<<1, 1024, 0, s>>>(a);
+void launch(const DecArgs& a, const StoreArgs& st, hipStream_t s) {
+  const unsigned begin = 1 + (st.k ? 2u * a.bs * a.c.KV : 0);
+  if (st.dtype == QQ_DTYPE_BF16) fp8_begin_kernel<D, uint16_t><<<begin, 256, 0, s>>>(a, st);
+  else fp8_begin_kernel<D, float><<<begin, 256, 0, s>>>(a, st);
   fp8_attend_kernel<D, T><<<a.max_slices * a.heads, 64 * kDecWaves, 0, s>>>(a);
-  fp8_merge_kernel<D, T><<<dim3(a.bs, a.H), 256, 0, s>>>(a);
 }
 
 }  // namespace
@@ -465,8 +568,8 @@ extern "C" int qq_fp8_decode_attention(const void* q, int q_dtype, int64_t q_bat
                                        void* out, void* workspace, int64_t workspace_bytes, void* stream) {
   const char* what = "qq_fp8_decode_attention";
   const Fp8Cache c{k_codes, v_codes, k_scale, v_scale, num_blocks, kv_heads, head_dim};
-  int st = check_cache(c, what);
-  if (st != QQ_OK) return st;
+  const int ok = check_cache(c, what);
+  if (ok != QQ_OK) return ok;
   QQ_REQUIRE(dtype_ok(q_dtype), "%s: bad dtype", what);
   QQ_REQUIRE(num_q_heads > 0 && num_q_heads % kv_heads == 0 && num_q_heads < 65536,
              "%s: q_heads %d not divisible by kv_heads %d", what, num_q_heads, kv_heads);
@@ -484,11 +587,10 @@ extern "C" int qq_fp8_decode_attention(const void* q, int q_dtype, int64_t q_bat
   const DecSpace sp = decode_space(bs, num_q_heads, kv_heads, head_dim);
   QQ_REQUIRE(workspace && workspace_bytes >= sp.bytes, "%s: workspace %lld bytes < %lld needed", what,
              (long long)workspace_bytes, (long long)sp.bytes);
-  if (k_new) {
-    st = qq_fp8_store(k_codes, v_codes, k_scale, v_scale, num_blocks, kv_heads, head_dim, k_new, v_new, new_dtype,
-                      out_cache_loc, bs, stream);
-    if (st != QQ_OK) return st;
-  }
+  QQ_REQUIRE(!k_new || (v_new && out_cache_loc), "%s: null pointer", what);
+  QQ_REQUIRE(!k_new || dtype_ok(new_dtype), "%s: bad dtype", what);
+  QQ_REQUIRE(((uintptr_t)k_new | (uintptr_t)v_new) % 16 == 0, "%s: k_new and v_new must be 16-byte aligned", what);
+  QQ_REQUIRE(!k_new || (int64_t)bs * kv_heads < (int64_t)1 << 30, "%s: bad sizes", what);
   char* ws = static_cast<char*>(workspace);
   DecArgs a{};
   a.q = q;
@@ -513,16 +615,18 @@ extern "C" int qq_fp8_decode_attention(const void* q, int q_dtype, int64_t q_bat
   a.heads = kv_heads * a.tiles;
   a.plan = reinterpret_cast<DecPlan*>(ws);
   a.cu = reinterpret_cast<int32_t*>(ws + sp.cu);
-  a.first = reinterpret_cast<int32_t*>(ws + sp.first);
+  a.items = reinterpret_cast<DecItem*>(ws + sp.items);
+  a.done = reinterpret_cast<uint32_t*>(ws + sp.done);
   a.part_o = reinterpret_cast<float*>(ws + sp.part_o);
   a.part_ml = reinterpret_cast<float*>(ws + sp.part_ml);
+  const StoreArgs st{c, k_new, v_new, new_dtype, out_cache_loc, bs, 1};
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (head_dim == 128) {
-    if (q_dtype == QQ_DTYPE_BF16) launch<128, uint16_t>(a, s);
-    else launch<128, float>(a, s);
+    if (q_dtype == QQ_DTYPE_BF16) launch<128, uint16_t>(a, st, s);
+    else launch<128, float>(a, st, s);
   } else {
-    if (q_dtype == QQ_DTYPE_BF16) launch<64, uint16_t>(a, s);
-    else launch<64, float>(a, s);
+    if (q_dtype == QQ_DTYPE_BF16) launch<64, uint16_t>(a, st, s);
+    else launch<64, float>(a, st, s);
   }
   return check_launch(what);
 }
