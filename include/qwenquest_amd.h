@@ -451,13 +451,16 @@ int qq_fp8_rows(const uint8_t* k_codes, const uint8_t* v_codes, const float* k_s
  * (prefix_lens NULL: from 0; max_new, if not 0, is at least every seq - prefix), or with
  * decode != 0 the page that the token at seq_lens[i] - 2 completes, if it does
  * (src/qwenquest/quest.py:231-280 and 284-321 in one form: nothing runs along).  Blocks come
- * from block_table; requests outside it are skipped, a block outside the cache gives NaN. */
+ * from block_table; requests outside it are skipped, a block outside the cache gives NaN.
+ * actual_lens and candidate_limit (both or neither): qq_quest_prepare_step's outputs for pages
+ * of 64, in the same launch. */
 int qq_fp8_page_bounds(const uint8_t* k_codes, int64_t codes_layer_stride, const float* k_scale,
                        int64_t scale_layer_stride, int num_blocks, int kv_heads, int head_dim,
                        const int32_t* block_table, int64_t block_table_stride, int block_table_rows,
                        int block_table_cols, const int64_t* req_pool_indices, const int64_t* seq_lens,
                        const int64_t* prefix_lens, int bs, int decode, int64_t max_new, int n_layers,
-                       uint16_t* page_k_bounds, int max_reqs, int max_pages, void* stream);
+                       uint16_t* page_k_bounds, int max_reqs, int max_pages, int top_k,
+                       int avoid_recent_overlap, int32_t* actual_lens, int32_t* candidate_limit, void* stream);
 
 /* One layer's decode over the 8-bit cache (src/qwenquest/attention/dense.py:26-42 and
  * quest_only.py:149-159 over it): with k_new the new tokens are stored first
@@ -479,6 +482,22 @@ int qq_fp8_decode_attention(const void* q, int q_dtype, int64_t q_batch_stride, 
                             int top_k, float scale, void* out, void* workspace, int64_t workspace_bytes,
                             void* stream);
 int64_t qq_fp8_decode_workspace_bytes(int bs, int num_q_heads, int kv_heads, int head_dim);
+
+/* QuestOnlyBackend.forward_decode (src/qwenquest/attention/quest_only.py:132-159) for one layer
+ * over the 8-bit cache: page scores and selection from page_k_bounds (as qq_quest_retrieve_topk,
+ * pages of 64; scores_ws [bs, max_pages], positions [bs, top_k] written), the new tokens' store
+ * and the attention over the selected pages (as qq_fp8_decode_attention).  Three launches: the
+ * scores; the selection with the store; the attention.  phase 1 = scores and selection, 2 = store
+ * and attention over the positions that phase 1 left, 3 = both. */
+int qq_fp8_quest_step(const void* q, int q_dtype, int64_t q_batch_stride, int num_q_heads, const void* k_new,
+                      const void* v_new, int new_dtype, const int64_t* out_cache_loc, uint8_t* k_codes,
+                      uint8_t* v_codes, float* k_scale, float* v_scale, int num_blocks, int kv_heads, int head_dim,
+                      const int32_t* block_table, int64_t block_table_stride, int block_table_rows,
+                      int block_table_cols, const uint16_t* page_k_bounds, int layer,
+                      const int64_t* req_pool_indices, const int64_t* seq_lens, const int32_t* candidate_limit,
+                      int bs, int max_reqs, int max_pages, int top_k, float scale, float* scores_ws,
+                      int32_t* positions, void* out, void* workspace, int64_t workspace_bytes, int phase,
+                      void* stream);
 
 /* The batch form of AttentionBackend.forward_extend (src/qwenquest/attention/base.py:65-93) over
  * the 8-bit cache, the new K/V being in it: request i's extend_lens[i] new tokens (q

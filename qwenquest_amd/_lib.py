@@ -111,7 +111,7 @@ SIGNATURES: dict[str, tuple] = {
     "qq_fp8_rows": (_I, [_P, _P, _P, _P, _I, _I, _I, _P, _L, _P, _P, _I, _P]),
     "qq_fp8_page_bounds": (
         _I,
-        [_P, _L, _P, _L, _I, _I, _I, _P, _L, _I, _I, _P, _P, _P, _I, _I, _L, _I, _P, _I, _I, _P],
+        [_P, _L, _P, _L, _I, _I, _I, _P, _L, _I, _I, _P, _P, _P, _I, _I, _L, _I, _P, _I, _I, _I, _I, _P, _P, _P],
     ),
     "qq_fp8_decode_attention": (
         _I,
@@ -119,6 +119,11 @@ SIGNATURES: dict[str, tuple] = {
          _P, _P, _L, _P],
     ),
     "qq_fp8_decode_workspace_bytes": (_L, [_I, _I, _I, _I]),
+    "qq_fp8_quest_step": (
+        _I,
+        [_P, _I, _L, _I, _P, _P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _P, _L, _I, _I, _P, _I, _P, _P, _P, _I, _I, _I,
+         _I, _F, _P, _P, _P, _P, _L, _I, _P],
+    ),
     "qq_fp8_extend_attention": (
         _I,
         [_P, _I, _P, _P, _P, _P, _I, _I, _I, _P, _L, _I, _I, _P, _P, _P, _P, _I, _L, _F, _P, _P, _L, _P],
@@ -205,3 +210,25 @@ def stream(device: torch.device | None = None) -> int:
     index = device.index if device is not None else None
     # the handle alone: a Stream object for it costs a call 2 us
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
+
+
+class _Same:
+    """A context that changes nothing."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_SAME = _Same()
+
+
+def on(device: torch.device):
+    """A context with `device` current, for launches on its streams; entering the one that is
+    already current costs nothing (torch.cuda.device: 2 us a call)."""
+    index = device.index
+    if index is None or index == torch._C._cuda_getDevice():
+        return _SAME
+    return torch.cuda.device(device)

@@ -18,9 +18,10 @@ from qwenquest_amd import _lib
 
 if TYPE_CHECKING:
     from qwenquest_amd.paged import Fp8TokenToKVPool
+    from qwenquest_amd.quest import QuestAlgorithm
 
 __all__ = ["decode_attention", "extend_attention", "extend_attention_batch", "fp8_decode_attention",
-           "fp8_extend_attention", "AttentionWorkspace"]
+           "fp8_extend_attention", "fp8_quest_step", "AttentionWorkspace"]
 
 
 class AttentionWorkspace:
@@ -281,13 +282,67 @@ def fp8_decode_attention(
     # of this call alone: it holds the division of the batch, which a graph's replay or a call on
     # another stream must not find replaced
     ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
+    with _lib.on(dev):
         _lib.call(
             "qq_fp8_decode_attention", _lib.ptr(q), _lib.dtype_code(q.dtype), q.stride(0), heads, _lib.ptr(kn),
             _lib.ptr(vn), _lib.DTYPE_BF16 if kn is None else _lib.dtype_code(kn.dtype), _lib.ptr(loc),
             *pool.layer_args(layer_id), *_table_args(bt), _lib.ptr(rpi), _lib.ptr(seq), bs, _lib.ptr(positions),
             0 if positions is None else max(positions.stride(0), positions.shape[1]), int(top_k), float(scaling),
             _lib.ptr(out), _lib.ptr(ws), need, _lib.stream(dev),
+        )
+    return out
+
+
+def fp8_quest_step(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    loc: torch.Tensor,
+    pool: Fp8TokenToKVPool,
+    layer_id: int,
+    block_table: torch.Tensor,
+    quest: QuestAlgorithm,
+    req_pool_indices: torch.Tensor,
+    positions: torch.Tensor,
+    scaling: float,
+    phase: int = 3,
+) -> torch.Tensor:
+    """One layer of Quest decode over an 8-bit pool, after ``quest.decode_step_blocks``: the new tokens
+    ``k``/``v`` go to rows ``loc``, the page scores select (``positions [>= bs, top_k]`` int32 is
+    written, as ``QuestAlgorithm.retrieve_topk`` writes it), and ``q [bs, H, D]`` attends the selected
+    pages.  ``phase``: 1 = scoring and selection, 2 = store and attention after phase 1, 3 = both.
+    Returns ``[bs, H*D]`` (complete after phase 2)."""
+    dev, step = pool.device, quest._step
+    if step is None:
+        raise RuntimeError("decode_step_blocks() must be called once per decode step first")
+    q = _queries(q, pool)
+    bs, heads, dim = q.shape
+    if step.seq_lens.shape[0] != bs:
+        raise ValueError("batch size differs from the one given to decode_step_blocks()")
+    if bs > quest.max_reqs:
+        raise ValueError(f"batch {bs} exceeds max_reqs {quest.max_reqs}")
+    if quest.page_size != 64 or quest.kv_heads != pool.kv_heads or quest.head_dim != dim:
+        raise ValueError("the Quest state is not of this pool's pages and heads")
+    if not quest.start_layer <= layer_id < quest.end_layer:
+        raise IndexError(f"layer {layer_id} is no Quest layer ({quest.start_layer} .. {quest.end_layer - 1})")
+    if (positions.dtype != torch.int32 or positions.device != dev or not positions.is_contiguous()
+            or positions.dim() != 2 or positions.shape[0] < bs or positions.shape[1] != quest.top_k):
+        raise ValueError(f"positions must be a contiguous int32 tensor [>= {bs}, {quest.top_k}] on {dev}")
+    bt = _block_table(block_table, dev)
+    rpi = _lengths(req_pool_indices, bs, dev, "req_pool_indices")
+    loc = _lengths(loc, bs, dev, "out_cache_loc")
+    kn, vn = pool.new_rows(k, v, bs)
+    out = torch.empty((bs, heads * dim), dtype=q.dtype, device=dev)
+    need = int(_lib.load().qq_fp8_decode_workspace_bytes(bs, heads, pool.kv_heads, dim))
+    ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)  # of this call alone
+    with _lib.on(dev):
+        _lib.call(
+            "qq_fp8_quest_step", _lib.ptr(q), _lib.dtype_code(q.dtype), q.stride(0), heads, _lib.ptr(kn), _lib.ptr(vn),
+            _lib.dtype_code(kn.dtype), _lib.ptr(loc), *pool.layer_args(layer_id), *_table_args(bt),
+            _lib.ptr(quest.page_k_bounds), layer_id - quest.start_layer, _lib.ptr(rpi), _lib.ptr(step.seq_lens),
+            _lib.ptr(step.candidate_limit_i32), bs, quest.max_reqs, quest.max_pages_per_req, quest.top_k, float(scaling),
+            _lib.ptr(quest._scores_ws), _lib.ptr(positions), _lib.ptr(out), _lib.ptr(ws), need, int(phase),
+            _lib.stream(dev),
         )
     return out
 
@@ -323,7 +378,7 @@ def fp8_extend_attention(
     need = int(_lib.load().qq_fp8_extend_workspace_bytes(n, bs, heads, pool.kv_heads, dim, bt.shape[1]))
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     out = torch.empty((n, heads * dim), dtype=q.dtype, device=dev)
-    with torch.cuda.device(dev):
+    with _lib.on(dev):
         _lib.call(
             "qq_fp8_extend_attention", _lib.ptr(q), heads, *pool.layer_args(layer_id), *_table_args(bt), _lib.ptr(rpi),
             _lib.ptr(seq), _lib.ptr(prefix), _lib.ptr(ext), bs, n, float(scaling), _lib.ptr(out), _lib.ptr(ws), need,

@@ -24,7 +24,7 @@ import torch
 
 from qwenquest_amd import _lib
 from qwenquest_amd.attention.base import AttentionBackend
-from qwenquest_amd.attention.ops import AttentionWorkspace, fp8_decode_attention
+from qwenquest_amd.attention.ops import AttentionWorkspace, fp8_quest_step
 from qwenquest_amd.config import SparseConfig, parse_hisparse_config
 from qwenquest_amd.paged import BLOCK_TOKENS
 from qwenquest_amd.quest import QuestAlgorithm
@@ -192,18 +192,14 @@ class QuestOnlyBackend(AttentionBackend):
         return out
 
     def _forward_decode_fp8(self, q3, k, v, layer, batch: ForwardBatch, phase: int) -> torch.Tensor:
-        """forward_decode_phase over an 8-bit pool: 1 = scoring and selection, 2 = new-token store and
-        attention."""
-        if phase not in (1, 2, 3):
-            raise ValueError(f"phase must be 1, 2 or 3, got {phase}")
-        quest, pool, bs = self.quest, self.token_to_kv_pool, batch.batch_size
-        if phase & 1:
-            quest.retrieve_topk(q3, layer.layer_id, batch.req_pool_indices, quest._step.seq_lens, out=self._positions)
-        if not phase & 2:
-            return torch.empty((bs, q3.shape[1] * pool.head_dim), dtype=q3.dtype, device=q3.device)
-        return fp8_decode_attention(q3, pool, layer.layer_id, self.req_to_token_pool.block_table,
-                                    batch.req_pool_indices, quest._step.seq_lens, layer.scaling,
-                                    positions=self._positions, top_k=quest.top_k, new=(batch.out_cache_loc, k, v))
+        """forward_decode_phase over an 8-bit pool in one C call: 1 = scoring and selection, 2 = new-token
+        store and attention."""
+        quest, rpi = self.quest, batch.req_pool_indices
+        out = fp8_quest_step(q3, k, v, batch.out_cache_loc, self.token_to_kv_pool, layer.layer_id,
+                             self.req_to_token_pool.block_table, quest, rpi, self._positions, layer.scaling, phase)
+        if quest.trace is not None and phase & 1:
+            quest._record(layer.layer_id, rpi, quest._step, self._positions[: batch.batch_size])
+        return out
 
     def sparse_attention(self, q, layer, req_pool_indices, positions, actual, bs) -> torch.Tensor:
         """[Q7] rows = req_to_token[req, positions[:n]] -> attention over exactly those rows."""

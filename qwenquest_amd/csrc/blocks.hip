@@ -13,7 +13,8 @@
 //
 // assign_plan_kernel: one block; a thread per request (a loop over more), two block-wide
 // prefix sums (tokens, blocks).  All requests are judged before anything is written, so a
-// refused call leaves the pool as it was and answers the padding row.  assign_fill_kernel:
+// refused call leaves the pool as it was and answers the padding row.  Up to a request per
+// thread, what the judging read stays in registers.  assign_fill_kernel:
 // a thread per token and per new block, each finding its request by bisection of the
 // prefix sums; a thread per token writes 20 bytes, coalesced.
 // Bound: launches and the latency of dependent loads at decode sizes, the 20 bytes a token
@@ -23,8 +24,7 @@
 namespace qq {
 namespace {
 
-constexpr int kPlan = 1024;      // threads of the planning block
-constexpr int kPlanWaves = kPlan / 64;
+constexpr int kPlan = 1024;      // threads of the planning block, at most
 constexpr int kErrExhausted = 1, kErrRequest = 2, kErrTwice = 4, kErrTotal = 8;
 constexpr int kMaxPoolReqs = 1 << 18;  // the planning block's bitmap of requests: 32 KiB
 
@@ -60,14 +60,16 @@ struct BlockArgs {
   int32_t* err_mirror;
   PlanHead* head;
   PlanRow* rows;
+  int here;  // the planning block writes the slots itself
 };
 
 struct PlanSmem {
-  int64_t a[kPlanWaves], b[kPlanWaves];
+  int64_t a[kPlan / 64], b[kPlan / 64];
   int32_t err;
 };
 
 // Exclusive prefix sums of (a, b) over the block's threads; the totals come back in ta, tb.
+template <int NT>
 __device__ inline void block_sums(PlanSmem& sm, int64_t& a, int64_t& b, int64_t& ta, int64_t& tb) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   int64_t x = a, y = b;
@@ -88,7 +90,7 @@ __device__ inline void block_sums(PlanSmem& sm, int64_t& a, int64_t& b, int64_t&
   int64_t ba = 0, bb = 0;
   ta = tb = 0;
 #pragma unroll
-  for (int w = 0; w < kPlanWaves; ++w) {
+  for (int w = 0; w < NT / 64; ++w) {
     const int64_t u = sm.a[w], v = sm.b[w];
     if (w < wave) {
       ba += u;
@@ -136,82 +138,7 @@ __device__ inline void report(const BlockArgs& a, int err) {
   if (a.err_mirror) *a.err_mirror |= err;
 }
 
-__global__ __launch_bounds__(kPlan) void assign_plan_kernel(BlockArgs a) {
-  extern __shared__ uint32_t seen[];
-  __shared__ PlanSmem sm;
-  const int tid = threadIdx.x;
-  for (int i = tid; i < (a.reqs + 31) / 32; i += kPlan) seen[i] = 0;
-  if (tid == 0) sm.err = 0;
-  const int count = *a.count;
-  __syncthreads();
-  int64_t tokens = 0, blocks = 0;
-  int err = 0;
-  for (int i0 = 0; i0 < a.bs; i0 += kPlan) {
-    const Asked q = asked(a, i0 + tid);
-    int64_t t = 0, b = 0, tt, tb;
-    if (q.n != 0) {
-      if (!sound(a, q)) {
-        err |= kErrRequest;
-      } else {
-        if (mark(seen, q.req)) err |= kErrTwice;
-        t = q.n;
-        b = max(0, blocks_of(q.prefix + q.n) - a.held[q.req]);
-      }
-    }
-    block_sums(sm, t, b, tt, tb);
-    tokens += tt;
-    blocks += tb;
-  }
-  if (err) atomicOr(&sm.err, err);
-  if (tid == 0) {
-    if (blocks > count) atomicOr(&sm.err, kErrExhausted);
-    if (a.fresh && tokens > a.total) atomicOr(&sm.err, kErrTotal);
-  }
-  __syncthreads();
-  err = sm.err;
-  if (tid == 0) {
-    if (err) report(a, err);
-    else *a.count = count - (int)blocks;
-    if (a.fresh) *a.head = {err == 0, count, err ? 0 : (int)tokens, err ? 0 : (int)blocks, {0, 0, 0, 0}};
-  }
-  if (err) {
-    if (!a.fresh)
-      for (int i = tid; i < a.bs; i += kPlan) a.loc[i] = a.pos[i] = 0;
-    return;
-  }
-  int64_t t0 = 0, b0 = 0;
-  for (int i0 = 0; i0 < a.bs; i0 += kPlan) {
-    const int i = i0 + tid;
-    const Asked q = asked(a, i);
-    const int held = q.n > 0 ? a.held[q.req] : 0;
-    const int need = q.n > 0 ? max(0, blocks_of(q.prefix + q.n) - held) : 0;
-    int64_t t = q.n, b = need, tt, tb;
-    block_sums(sm, t, b, tt, tb);
-    t += t0;
-    b += b0;
-    t0 += tt;
-    b0 += tb;
-    if (i >= a.bs) continue;
-    if (need > 0) a.held[q.req] = held + need;
-    if (a.fresh) {
-      a.rows[i] = {(int)t, (int)b, (int)q.req, (int)q.prefix, held, {0, 0, 0}};
-      continue;
-    }
-    // decode: the request's one token here and now
-    int64_t row = 0;
-    if (q.n) {
-      int32_t* tr = a.table + q.req * a.table_stride;
-      int32_t block = need ? 0 : tr[q.prefix >> 6];
-      for (int j = 0; j < need; ++j) tr[held + j] = block = a.stack[count - 1 - (b + j)];
-      row = (int64_t)block * 64 + (q.prefix & 63);
-      a.r2t[q.req * a.r2t_stride + q.prefix] = (int32_t)row;
-    }
-    a.loc[i] = row;
-    a.pos[i] = q.n ? q.prefix : 0;
-  }
-}
-
-// The last request whose first token (blk: block) is at or before `at`, among those with any.
+// The last request whose first token (BLK: block) is at or before `at`, among those with any.
 template <bool BLK>
 __device__ inline int find_row(const PlanRow* rows, int bs, int at) {
   int lo = 0, hi = bs;
@@ -223,9 +150,8 @@ __device__ inline int find_row(const PlanRow* rows, int bs, int at) {
   return lo;
 }
 
-__global__ __launch_bounds__(256) void assign_fill_kernel(BlockArgs a) {
-  const PlanHead h = *a.head;
-  const int64_t step = (int64_t)gridDim.x * 256, first = (int64_t)blockIdx.x * 256 + threadIdx.x;
+// Table entries and slots of a planned call, item by item from `first`.
+__device__ inline void fill_slots(const BlockArgs& a, const PlanHead& h, int64_t first, int64_t step) {
   for (int64_t k = first; k < h.blocks; k += step) {
     const PlanRow r = a.rows[find_row<true>(a.rows, a.bs, (int)k)];
     a.table[r.req * a.table_stride + r.held + (k - r.blk)] = a.stack[h.count - 1 - k];
@@ -242,6 +168,109 @@ __global__ __launch_bounds__(256) void assign_fill_kernel(BlockArgs a) {
     }
     a.loc[t] = row;
     a.pos[t] = p;
+  }
+}
+
+__global__ __launch_bounds__(256) void assign_fill_kernel(BlockArgs a) {
+  fill_slots(a, *a.head, (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256);
+}
+
+// What request i takes: its tokens and the blocks it lacks (after a call: none).
+struct Taken {
+  Asked q;
+  int held, need;
+};
+
+template <int NT>
+__global__ __launch_bounds__(NT) void assign_plan_kernel(BlockArgs a) {
+  extern __shared__ uint32_t seen[];
+  __shared__ PlanSmem sm;
+  const int tid = threadIdx.x;
+  auto look = [&](int i, int& err) {
+    Taken t{asked(a, i), 0, 0};
+    if (t.q.n == 0) return t;
+    if (sound(a, t.q)) {
+      t.held = a.held[t.q.req];
+      t.need = max(0, blocks_of(t.q.prefix + t.q.n) - t.held);
+    } else {
+      err |= kErrRequest;
+      t.q.n = 0;
+    }
+    return t;
+  };
+  int err = 0;
+  const Taken mine = look(tid, err);  // in flight while the bitmap is cleared
+  const int count = *a.count;
+  for (int i = tid; i < (a.reqs + 31) / 32; i += NT) seen[i] = 0;
+  if (tid == 0) sm.err = 0;
+  __syncthreads();
+  int64_t tokens = 0, blocks = 0;
+  int64_t t0 = 0, b0 = 0;  // before this thread's request, in the only round
+  for (int i0 = 0; i0 < a.bs; i0 += NT) {
+    const Taken x = i0 == 0 ? mine : look(i0 + tid, err);
+    if (x.q.n > 0 && mark(seen, x.q.req)) err |= kErrTwice;
+    int64_t t = x.q.n, b = x.need, tt, tb;
+    block_sums<NT>(sm, t, b, tt, tb);
+    tokens += tt;
+    blocks += tb;
+    t0 = t;
+    b0 = b;
+  }
+  if (err) atomicOr(&sm.err, err);
+  if (tid == 0) {
+    if (blocks > count) atomicOr(&sm.err, kErrExhausted);
+    if (a.fresh && tokens > a.total) atomicOr(&sm.err, kErrTotal);
+  }
+  __syncthreads();
+  err = sm.err;
+  if (tid == 0) {
+    if (err) report(a, err);
+    else *a.count = count - (int)blocks;
+    if (a.fresh) *a.head = {err == 0, count, err ? 0 : (int)tokens, err ? 0 : (int)blocks, {0, 0, 0, 0}};
+  }
+  if (err) {
+    if (a.here)
+      for (int64_t i = tid; i < a.total; i += NT) a.loc[i] = a.pos[i] = 0;
+    return;
+  }
+  const PlanHead planned{1, count, (int)tokens, (int)blocks, {0, 0, 0, 0}};
+  tokens = blocks = 0;
+  for (int i0 = 0; i0 < a.bs; i0 += NT) {
+    const int i = i0 + tid;
+    const Taken x = i0 == 0 ? mine : look(i, err);
+    int64_t t = t0, b = b0;
+    if (a.bs > NT) {  // block-uniform
+      int64_t tt, tb;
+      t = x.q.n;
+      b = x.need;
+      block_sums<NT>(sm, t, b, tt, tb);
+      t += tokens;
+      b += blocks;
+      tokens += tt;
+      blocks += tb;
+    }
+    if (i >= a.bs) continue;
+    const Asked& q = x.q;
+    if (x.need > 0) a.held[q.req] = x.held + x.need;
+    if (a.fresh) {
+      a.rows[i] = {(int)t, (int)b, (int)q.req, (int)q.prefix, x.held, {0, 0, 0}};
+      continue;
+    }
+    // decode: the request's one token here and now
+    int64_t row = 0;
+    if (q.n) {
+      int32_t* tr = a.table + q.req * a.table_stride;
+      int32_t block = x.need ? 0 : tr[q.prefix >> 6];
+      for (int j = 0; j < x.need; ++j) tr[x.held + j] = block = a.stack[count - 1 - (b + j)];
+      row = (int64_t)block * 64 + (q.prefix & 63);
+      a.r2t[q.req * a.r2t_stride + q.prefix] = (int32_t)row;
+    }
+    a.loc[i] = row;
+    a.pos[i] = q.n ? q.prefix : 0;
+  }
+  if (a.fresh && a.here) {
+    __syncthreads();  // the records are written
+    fill_slots(a, planned, tid, NT);
   }
 }
 
@@ -267,7 +296,7 @@ __global__ __launch_bounds__(kPlan) void release_plan_kernel(BlockArgs a) {
       else held = a.held[req];
     }
     int64_t t = 0, b = held, tt, tb;
-    block_sums(sm, t, b, tt, tb);
+    block_sums<kPlan>(sm, t, b, tt, tb);
     if (i < a.bs) a.rows[i] = {0, (int)(blocks + b), (int)req, 0, (int)held, {0, 0, 0}};
     blocks += tb;
   }
@@ -342,7 +371,7 @@ extern "C" int qq_block_assign(const int64_t* req_pool_indices, const int64_t* l
   const char* what = "qq_block_assign";
   BlockArgs a{req_pool_indices, lens, new_lens, bs, total, block_table, block_table_stride, req_to_token,
               req_to_token_stride, max_context_len, max_reqs, held, free_blocks, free_count, free_cap, loc, pos,
-              error_flags, error_mirror, nullptr, nullptr};
+              error_flags, error_mirror, nullptr, nullptr, 0};
   int st = check_pool(a, what);
   if (st != QQ_OK) return st;
   QQ_REQUIRE(bs == 0 || lens, "%s: null pointer", what);
@@ -352,8 +381,12 @@ extern "C" int qq_block_assign(const int64_t* req_pool_indices, const int64_t* l
   QQ_REQUIRE(bs > 0, "%s: %lld tokens of no request", what, (long long)total);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (new_lens && (st = set_workspace(a, workspace, workspace_bytes, what)) != QQ_OK) return st;
-  assign_plan_kernel<<<1, kPlan, seen_bytes(a), s>>>(a);
-  if (new_lens) assign_fill_kernel<<<fill_blocks(total), 256, 0, s>>>(a);
+  // a launch less is worth up to four tokens a thread of the planning block
+  a.here = !new_lens || total <= 4 * (bs <= 256 ? 256 : kPlan);
+  // one round of threads where that is enough; few waves meet at a barrier sooner
+  if (bs <= 256) assign_plan_kernel<256><<<1, 256, seen_bytes(a), s>>>(a);
+  else assign_plan_kernel<kPlan><<<1, kPlan, seen_bytes(a), s>>>(a);
+  if (!a.here) assign_fill_kernel<<<fill_blocks(total), 256, 0, s>>>(a);
   return check_launch(what);
 }
 
@@ -365,7 +398,7 @@ extern "C" int qq_block_release(const int64_t* req_pool_indices, int bs, int32_t
   const char* what = "qq_block_release";
   BlockArgs a{req_pool_indices, nullptr, nullptr, bs, 0, block_table, block_table_stride, req_to_token,
               req_to_token_stride, max_context_len, max_reqs, held, free_blocks, free_count, free_cap, nullptr, nullptr,
-              error_flags, error_mirror, nullptr, nullptr};
+              error_flags, error_mirror, nullptr, nullptr, 0};
   int st = check_pool(a, what);
   if (st != QQ_OK) return st;
   if (bs == 0) return QQ_OK;

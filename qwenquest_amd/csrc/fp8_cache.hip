@@ -29,19 +29,20 @@ __device__ inline void write8(float* out, uint32_t a, uint32_t b, float s) {
   *reinterpret_cast<float4*>(out + 4) = make_float4(y.x * s, y.y * s, y.z * s, y.w * s);
 }
 
-// Values of listed rows: a thread block takes 64 entries of one head, a thread 8 channels of every
-// 16th entry.  K is read in place (8 bytes of a token's 16-byte pieces; the entries' neighbours
+// Values of listed rows: a thread block takes `per` entries (16 or 64) of one head, a thread 8
+// channels of every 16th entry.  K is read in place (8 bytes of a token's 16-byte pieces; the entries' neighbours
 // share the lines).  A channel's tokens of V lie together, a token's channels 16 bytes apart: a
 // run of entries of one block reads the block through the LDS, a few entries their bytes.
 // Bound: HBM.
 template <int D, typename DST>
-__global__ __launch_bounds__(2 * D) void fp8_rows_kernel(Fp8Cache c, const int64_t* loc, int64_t n, DST* k, DST* v) {
+__global__ __launch_bounds__(2 * D) void fp8_rows_kernel(Fp8Cache c, const int64_t* loc, int64_t n, int per, DST* k,
+                                                          DST* v) {
   constexpr int NT = 2 * D, DG = D / 8, kRows = 64 * D / 256;
   __shared__ __align__(16) uint8_t codes[kRows * 272];  // 256-byte rows, 16 bytes apart: see StoreSmem
   const int tid = threadIdx.x, lane = tid & 63, h = blockIdx.y;
   const int dg = tid % DG, sub = tid / DG;
-  const int64_t e0 = (int64_t)blockIdx.x * 64;
-  const int count = (int)min((int64_t)64, n - e0);
+  const int64_t e0 = (int64_t)blockIdx.x * per;
+  const int count = (int)min((int64_t)per, n - e0);
   const int64_t row = lane < count ? loc[e0 + lane] : -1;
   const bool in = row >= 0 && (row >> 6) < c.blocks;
   const int blk = in ? (int)(row >> 6) : -1, slot = (int)(row & 63);
@@ -49,8 +50,7 @@ __global__ __launch_bounds__(2 * D) void fp8_rows_kernel(Fp8Cache c, const int64
   const int64_t at = (int64_t)max(blk, 0) * c.KV + h;
   const float nan = __builtin_nanf("");
   const float ks = in ? c.ks[at] : nan, vs = in ? c.vs[at] : nan;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i * 16 < per; ++i) {
     const int e = sub + 16 * i;
     const int b = max(__shfl(blk, e, 64), 0), t = __shfl(slot, e, 64);
     const float s = __shfl(ks, e, 64);
@@ -73,7 +73,7 @@ __global__ __launch_bounds__(2 * D) void fp8_rows_kernel(Fp8Cache c, const int64
       }
       __syncthreads();
     }
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i * 16 < per; ++i) {
       const int e = sub + 16 * i;
       const int t = __shfl(slot, e, 64);
       const float s = __shfl(vs, e, 64);
@@ -105,6 +105,9 @@ struct PageArgs {
   int decode;
   uint32_t* bounds;  // [layers, R, MP, KV * D] (min, max) words
   int R, MP;
+  int top_k, avoid;
+  int32_t* actual;  // nullptr, or the step's layout: actual_lens, candidate_limit
+  int32_t* limit;
 };
 
 // Min and max of a page's keys per channel, a wave per (page, head, layer).  A scale is
@@ -116,7 +119,11 @@ template <int D>
 __global__ __launch_bounds__(256) void fp8_page_bounds_kernel(PageArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int b = blockIdx.y, layer = blockIdx.z;
-  const int64_t req = a.rpi[b], s = max(a.seq[b], (int64_t)0);
+  const int64_t req = a.rpi[b], seq = a.seq[b], s = max(seq, (int64_t)0);
+  if (a.actual && layer == 0 && blockIdx.x == 0 && threadIdx.x == 0) {
+    a.actual[b] = (int32_t)min(seq, (int64_t)a.top_k);  // quest.py:343-352
+    a.limit[b] = (int32_t)(a.avoid ? max(seq / 64 - 1, (int64_t)0) : seq / 64);
+  }
   if (req < 0 || req >= a.R || req >= a.table_rows) return;
   int64_t lo, hi;  // pages
   if (a.decode) {  // the page that the token before the newest completes
@@ -232,17 +239,20 @@ extern "C" int qq_fp8_rows(const uint8_t* k_codes, const uint8_t* v_codes, const
   QQ_REQUIRE(n >= 0 && n < (int64_t)1 << 31, "%s: bad sizes", what);
   if (n == 0) return QQ_OK;
   QQ_REQUIRE(loc && k && v, "%s: null pointer", what);
-  const dim3 grid((unsigned)((n + 63) / 64), kv_heads);
+  // a block's run is read by as many thread blocks as its entries are dealt to; few entries give
+  // more thread blocks of a run or two each (1000 entries of 32 requests 10.5 us in 64s)
+  const int per = n * kv_heads <= 16384 ? 16 : 64;
+  const dim3 grid((unsigned)((n + per - 1) / per), kv_heads);
   hipStream_t s = static_cast<hipStream_t>(stream);
   uint16_t *kb = static_cast<uint16_t*>(k), *vb = static_cast<uint16_t*>(v);
   float *kf = static_cast<float*>(k), *vf = static_cast<float*>(v);
   const bool bf = dst_dtype == QQ_DTYPE_BF16;
   if (head_dim == 128) {
-    if (bf) fp8_rows_kernel<128><<<grid, 256, 0, s>>>(c, loc, n, kb, vb);
-    else fp8_rows_kernel<128><<<grid, 256, 0, s>>>(c, loc, n, kf, vf);
+    if (bf) fp8_rows_kernel<128><<<grid, 256, 0, s>>>(c, loc, n, per, kb, vb);
+    else fp8_rows_kernel<128><<<grid, 256, 0, s>>>(c, loc, n, per, kf, vf);
   } else {
-    if (bf) fp8_rows_kernel<64><<<grid, 128, 0, s>>>(c, loc, n, kb, vb);
-    else fp8_rows_kernel<64><<<grid, 128, 0, s>>>(c, loc, n, kf, vf);
+    if (bf) fp8_rows_kernel<64><<<grid, 128, 0, s>>>(c, loc, n, per, kb, vb);
+    else fp8_rows_kernel<64><<<grid, 128, 0, s>>>(c, loc, n, per, kf, vf);
   }
   return check_launch(what);
 }
@@ -252,7 +262,8 @@ extern "C" int qq_fp8_page_bounds(const uint8_t* k_codes, int64_t codes_layer_st
                                   const int32_t* block_table, int64_t block_table_stride, int block_table_rows,
                                   int block_table_cols, const int64_t* req_pool_indices, const int64_t* seq_lens,
                                   const int64_t* prefix_lens, int bs, int decode, int64_t max_new, int n_layers,
-                                  uint16_t* page_k_bounds, int max_reqs, int max_pages, void* stream) {
+                                  uint16_t* page_k_bounds, int max_reqs, int max_pages, int top_k,
+                                  int avoid_recent_overlap, int32_t* actual_lens, int32_t* candidate_limit, void* stream) {
   const char* what = "qq_fp8_page_bounds";
   const Fp8Cache c{const_cast<uint8_t*>(k_codes), const_cast<uint8_t*>(k_codes), const_cast<float*>(k_scale),
                    const_cast<float*>(k_scale), num_blocks, kv_heads, head_dim};
@@ -261,11 +272,13 @@ extern "C" int qq_fp8_page_bounds(const uint8_t* k_codes, int64_t codes_layer_st
   QQ_REQUIRE(bs >= 0 && bs < 65536 && n_layers > 0 && n_layers < 65536 && max_reqs > 0 && max_pages > 0 && max_new >= 0 &&
                  block_table_cols > 0 && block_table_stride >= block_table_cols && block_table_rows > 0,
              "%s: bad sizes", what);
+  QQ_REQUIRE(!actual_lens == !candidate_limit, "%s: one of the layout's outputs is missing", what);
   if (bs == 0) return QQ_OK;
   QQ_REQUIRE(block_table && req_pool_indices && seq_lens && page_k_bounds, "%s: null pointer", what);
   PageArgs a{k_codes, k_scale, codes_layer_stride, scale_layer_stride, num_blocks, kv_heads, block_table, block_table_stride,
              block_table_rows, block_table_cols, req_pool_indices, seq_lens, prefix_lens, decode,
-             reinterpret_cast<uint32_t*>(page_k_bounds), max_reqs, max_pages};
+             reinterpret_cast<uint32_t*>(page_k_bounds), max_reqs, max_pages, top_k, avoid_recent_overlap, actual_lens,
+             candidate_limit};
   // pages of a request, at most: those its new tokens can complete
   const int64_t pages = decode ? 1 : min((int64_t)max_pages, max_new > 0 && prefix_lens ? max_new / 64 + 1 : (int64_t)max_pages);
   const int64_t need = (pages * kv_heads + 3) / 4, fill = max((int64_t)1, (int64_t)16384 / ((int64_t)bs * n_layers));

@@ -122,17 +122,30 @@ __device__ inline void plan_slices(const DecArgs& a) {
   }
 }
 
-// Block 0: the slices; then a block per new token, head, and K or V.
-template <int D, typename SRC>
-__global__ __launch_bounds__(256) void fp8_begin_kernel(DecArgs a, StoreArgs st) {
-  __shared__ StoreSmem<D> sm;
+// Block 0: the slices; then a block per request that selects its pages (KPT > 0: scores per
+// thread), and a block per new token, head, and K or V.
+template <int D, typename SRC, int KPT>
+__global__ __launch_bounds__(256) void fp8_begin_kernel(DecArgs a, StoreArgs st, SelectArgs sel) {
+  __shared__ union Smem {
+    StoreSmem<D> st;
+    SelectSmem<(KPT > 0 ? KPT : 1)> sel;
+    __device__ Smem() {}
+  } sm;
   if (blockIdx.x == 0) {
     plan_slices(a);
     return;
   }
-  const int i = (blockIdx.x - 1) >> 1, h = i % a.c.KV;
-  if (blockIdx.x & 1) store_segment<D, SRC, false>(st, sm, i / a.c.KV, h);
-  else store_segment<D, SRC, true>(st, sm, i / a.c.KV, h);
+  int i = blockIdx.x - 1;
+  if constexpr (KPT > 0) {
+    if (i < a.bs) {
+      select_filter_block<KPT>(sel, i, sm.sel);
+      return;
+    }
+    i -= a.bs;
+  }
+  const int tok = i / (2 * a.c.KV), rest = i - tok * 2 * a.c.KV;
+  if (rest & 1) store_segment<D, SRC, true>(st, sm.st, tok, rest >> 1);
+  else store_segment<D, SRC, false>(st, sm.st, tok, rest >> 1);
 }
 
 __device__ inline float trunc_bf16(float x) { return __uint_as_float(__float_as_uint(x) & 0xFFFF0000u); }
@@ -540,12 +553,88 @@ DecSpace decode_space(int bs, int H, int KV, int D) {
   return s;
 }
 
-template <int D, typename T>
-void launch(const DecArgs& a, const StoreArgs& st, hipStream_t s) {
-  const unsigned begin = 1 + (st.k ? 2u * a.bs * a.c.KV : 0);
-  if (st.dtype == QQ_DTYPE_BF16) fp8_begin_kernel<D, uint16_t><<<begin, 256, 0, s>>>(a, st);
-  else fp8_begin_kernel<D, float><<<begin, 256, 0, s>>>(a, st);
-  fp8_attend_kernel<D, T><<<a.max_slices * a.heads, 64 * kDecWaves, 0, s>>>(a);
+template <int D, int KPT>
+void begin(const DecArgs& a, const StoreArgs& st, const SelectArgs& sel, hipStream_t s) {
+  const unsigned blocks = 1 + (KPT > 0 ? a.bs : 0) + (st.k ? 2u * a.bs * a.c.KV : 0);
+  if (st.dtype == QQ_DTYPE_BF16) fp8_begin_kernel<D, uint16_t, KPT><<<blocks, 256, 0, s>>>(a, st, sel);
+  else fp8_begin_kernel<D, float, KPT><<<blocks, 256, 0, s>>>(a, st, sel);
+}
+
+// `sel`: with k_sel > 0 the pages are selected first, from scores that are there.
+template <int D>
+void launch(const DecArgs& a, const StoreArgs& st, const SelectArgs& sel, int q_dtype, hipStream_t s) {
+  const int n = max(sel.MP, sel.k_sel);
+  if (!sel.positions) begin<D, 0>(a, st, sel, s);
+  else if (sel.k_sel <= 64 && n <= 4 * 256) begin<D, 4>(a, st, sel, s);
+  else if (sel.k_sel <= 64 && n <= 9 * 256) begin<D, 9>(a, st, sel, s);
+  else if (sel.k_sel <= 64 && n <= 16 * 256) begin<D, 16>(a, st, sel, s);
+  else {
+    launch_select(sel, a.bs, sel.MP, sel.k_sel, s);
+    begin<D, 0>(a, st, sel, s);
+  }
+  const int grid = a.max_slices * a.heads;
+  if (q_dtype == QQ_DTYPE_BF16) fp8_attend_kernel<D, uint16_t><<<grid, 64 * kDecWaves, 0, s>>>(a);
+  else fp8_attend_kernel<D, float><<<grid, 64 * kDecWaves, 0, s>>>(a);
+}
+
+// Everything of a call but its launches; `what` refuses.
+int set_args(DecArgs& a, StoreArgs& st, const char* what, const void* q, int q_dtype, int64_t q_batch_stride,
+             int num_q_heads, const void* k_new, const void* v_new, int new_dtype, const int64_t* out_cache_loc,
+             const Fp8Cache& c, const int32_t* block_table, int64_t block_table_stride, int block_table_rows,
+             int block_table_cols, const int64_t* req_pool_indices, const int64_t* seq_lens, int bs,
+             const int32_t* positions, int64_t positions_stride, int top_k, float scale, void* out, void* workspace,
+             int64_t workspace_bytes) {
+  const int ok = check_cache(c, what);
+  if (ok != QQ_OK) return ok;
+  QQ_REQUIRE(dtype_ok(q_dtype), "%s: bad dtype", what);
+  QQ_REQUIRE(num_q_heads > 0 && num_q_heads % c.KV == 0 && num_q_heads < 65536,
+             "%s: q_heads %d not divisible by kv_heads %d", what, num_q_heads, c.KV);
+  QQ_REQUIRE(bs >= 0 && block_table_rows > 0 && block_table_cols > 0 && block_table_cols <= kMaxPoolBlocks &&
+                 block_table_stride >= block_table_cols,
+             "%s: bad sizes", what);
+  QQ_REQUIRE(!positions || (top_k > 0 && top_k % 64 == 0 && positions_stride >= top_k),
+             "%s: top_k %d is not a multiple of the block of 64", what, top_k);
+  QQ_REQUIRE((int64_t)block_table_cols * bs < (int64_t)1 << 30, "%s: too many units of work", what);
+  if (bs == 0) return QQ_OK;
+  QQ_REQUIRE(q && block_table && req_pool_indices && seq_lens && out, "%s: null pointer", what);
+  QQ_REQUIRE((uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0 && q_batch_stride % 8 == 0,
+             "%s: q and out must be 16-byte aligned", what);
+  QQ_REQUIRE(!k_new || (v_new && out_cache_loc), "%s: null pointer", what);
+  QQ_REQUIRE(!k_new || dtype_ok(new_dtype), "%s: bad dtype", what);
+  QQ_REQUIRE(((uintptr_t)k_new | (uintptr_t)v_new) % 16 == 0, "%s: k_new and v_new must be 16-byte aligned", what);
+  QQ_REQUIRE(!k_new || (int64_t)bs * c.KV < (int64_t)1 << 29, "%s: bad sizes", what);
+  const DecSpace sp = decode_space(bs, num_q_heads, c.KV, c.D);
+  QQ_REQUIRE(workspace && workspace_bytes >= sp.bytes, "%s: workspace %lld bytes < %lld needed", what,
+             (long long)workspace_bytes, (long long)sp.bytes);
+  char* ws = static_cast<char*>(workspace);
+  a.q = q;
+  a.q_bstride = q_batch_stride;
+  a.H = num_q_heads;
+  a.G = num_q_heads / c.KV;
+  a.tiles = (a.G + kTile - 1) / kTile;
+  a.c = c;
+  a.table = block_table;
+  a.table_stride = block_table_stride;
+  a.table_rows = block_table_rows;
+  a.table_cols = block_table_cols;
+  a.rpi = req_pool_indices;
+  a.seq = seq_lens;
+  a.bs = bs;
+  a.positions = positions;
+  a.pos_stride = positions_stride;
+  a.top_k = positions ? top_k : 64;
+  a.sl2 = scale * kLog2e;
+  a.out = out;
+  a.max_slices = sp.max_slices;
+  a.heads = c.KV * a.tiles;
+  a.plan = reinterpret_cast<DecPlan*>(ws);
+  a.cu = reinterpret_cast<int32_t*>(ws + sp.cu);
+  a.items = reinterpret_cast<DecItem*>(ws + sp.items);
+  a.done = reinterpret_cast<uint32_t*>(ws + sp.done);
+  a.part_o = reinterpret_cast<float*>(ws + sp.part_o);
+  a.part_ml = reinterpret_cast<float*>(ws + sp.part_ml);
+  st = StoreArgs{c, k_new, v_new, new_dtype, out_cache_loc, bs, 1};
+  return QQ_OK;
 }
 
 }  // namespace
@@ -567,66 +656,72 @@ extern "C" int qq_fp8_decode_attention(const void* q, int q_dtype, int64_t q_bat
                                        const int32_t* positions, int64_t positions_stride, int top_k, float scale,
                                        void* out, void* workspace, int64_t workspace_bytes, void* stream) {
   const char* what = "qq_fp8_decode_attention";
-  const Fp8Cache c{k_codes, v_codes, k_scale, v_scale, num_blocks, kv_heads, head_dim};
-  const int ok = check_cache(c, what);
-  if (ok != QQ_OK) return ok;
-  QQ_REQUIRE(dtype_ok(q_dtype), "%s: bad dtype", what);
-  QQ_REQUIRE(num_q_heads > 0 && num_q_heads % kv_heads == 0 && num_q_heads < 65536,
-             "%s: q_heads %d not divisible by kv_heads %d", what, num_q_heads, kv_heads);
-  QQ_REQUIRE(bs >= 0 && block_table_rows > 0 && block_table_cols > 0 && block_table_cols <= kMaxPoolBlocks &&
-                 block_table_stride >= block_table_cols,
-             "%s: bad sizes", what);
-  QQ_REQUIRE(!positions || (top_k > 0 && top_k % 64 == 0 && positions_stride >= top_k),
-             "%s: top_k %d is not a multiple of the block of 64", what, top_k);
-  const int64_t units = positions ? max((int64_t)1, min((int64_t)block_table_cols, (int64_t)top_k / 64 + 1)) : block_table_cols;
-  QQ_REQUIRE(units * bs < (int64_t)1 << 30, "%s: too many units of work", what);
-  if (bs == 0) return QQ_OK;
-  QQ_REQUIRE(q && block_table && req_pool_indices && seq_lens && out, "%s: null pointer", what);
-  QQ_REQUIRE((uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0 && q_batch_stride % 8 == 0,
-             "%s: q and out must be 16-byte aligned", what);
-  const DecSpace sp = decode_space(bs, num_q_heads, kv_heads, head_dim);
-  QQ_REQUIRE(workspace && workspace_bytes >= sp.bytes, "%s: workspace %lld bytes < %lld needed", what,
-             (long long)workspace_bytes, (long long)sp.bytes);
-  QQ_REQUIRE(!k_new || (v_new && out_cache_loc), "%s: null pointer", what);
-  QQ_REQUIRE(!k_new || dtype_ok(new_dtype), "%s: bad dtype", what);
-  QQ_REQUIRE(((uintptr_t)k_new | (uintptr_t)v_new) % 16 == 0, "%s: k_new and v_new must be 16-byte aligned", what);
-  QQ_REQUIRE(!k_new || (int64_t)bs * kv_heads < (int64_t)1 << 30, "%s: bad sizes", what);
-  char* ws = static_cast<char*>(workspace);
   DecArgs a{};
-  a.q = q;
-  a.q_bstride = q_batch_stride;
-  a.H = num_q_heads;
-  a.G = num_q_heads / kv_heads;
-  a.tiles = (a.G + kTile - 1) / kTile;
-  a.c = c;
-  a.table = block_table;
-  a.table_stride = block_table_stride;
-  a.table_rows = block_table_rows;
-  a.table_cols = block_table_cols;
-  a.rpi = req_pool_indices;
-  a.seq = seq_lens;
-  a.bs = bs;
-  a.positions = positions;
-  a.pos_stride = positions_stride;
-  a.top_k = positions ? top_k : 64;
-  a.sl2 = scale * 1.44269504088896340736f;
-  a.out = out;
-  a.max_slices = sp.max_slices;
-  a.heads = kv_heads * a.tiles;
-  a.plan = reinterpret_cast<DecPlan*>(ws);
-  a.cu = reinterpret_cast<int32_t*>(ws + sp.cu);
-  a.items = reinterpret_cast<DecItem*>(ws + sp.items);
-  a.done = reinterpret_cast<uint32_t*>(ws + sp.done);
-  a.part_o = reinterpret_cast<float*>(ws + sp.part_o);
-  a.part_ml = reinterpret_cast<float*>(ws + sp.part_ml);
-  const StoreArgs st{c, k_new, v_new, new_dtype, out_cache_loc, bs, 1};
+  StoreArgs st{};
+  const int ok = set_args(a, st, what, q, q_dtype, q_batch_stride, num_q_heads, k_new, v_new, new_dtype, out_cache_loc,
+                          {k_codes, v_codes, k_scale, v_scale, num_blocks, kv_heads, head_dim}, block_table,
+                          block_table_stride, block_table_rows, block_table_cols, req_pool_indices, seq_lens, bs, positions,
+                          positions_stride, top_k, scale, out, workspace, workspace_bytes);
+  if (ok != QQ_OK || bs == 0) return ok;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (head_dim == 128) {
-    if (q_dtype == QQ_DTYPE_BF16) launch<128, uint16_t>(a, st, s);
-    else launch<128, float>(a, st, s);
+  if (head_dim == 128) launch<128>(a, st, SelectArgs{}, q_dtype, s);
+  else launch<64>(a, st, SelectArgs{}, q_dtype, s);
+  return check_launch(what);
+}
+
+extern "C" int qq_fp8_quest_step(const void* q, int q_dtype, int64_t q_batch_stride, int num_q_heads, const void* k_new,
+                                 const void* v_new, int new_dtype, const int64_t* out_cache_loc, uint8_t* k_codes,
+                                 uint8_t* v_codes, float* k_scale, float* v_scale, int num_blocks, int kv_heads,
+                                 int head_dim, const int32_t* block_table, int64_t block_table_stride,
+                                 int block_table_rows, int block_table_cols, const uint16_t* page_k_bounds, int layer,
+                                 const int64_t* req_pool_indices, const int64_t* seq_lens, const int32_t* candidate_limit,
+                                 int bs, int max_reqs, int max_pages, int top_k, float scale, float* scores_ws,
+                                 int32_t* positions, void* out, void* workspace, int64_t workspace_bytes, int phase,
+                                 void* stream) {
+  const char* what = "qq_fp8_quest_step";
+  QQ_REQUIRE(phase >= 1 && phase <= 3, "%s: phase must be 1, 2 or 3, got %d", what, phase);
+  QQ_REQUIRE(bs == 0 || (page_k_bounds && candidate_limit && scores_ws && positions), "%s: null pointer", what);
+  QQ_REQUIRE(layer >= 0 && max_reqs > 0 && max_pages >= 0, "%s: bad sizes", what);
+  DecArgs a{};
+  StoreArgs st{};
+  const int ok = set_args(a, st, what, q, q_dtype, q_batch_stride, num_q_heads, k_new, v_new, new_dtype, out_cache_loc,
+                          {k_codes, v_codes, k_scale, v_scale, num_blocks, kv_heads, head_dim}, block_table,
+                          block_table_stride, block_table_rows, block_table_cols, req_pool_indices, seq_lens, bs, positions,
+                          top_k, top_k, scale, out, workspace, workspace_bytes);
+  if (ok != QQ_OK || bs == 0) return ok;
+  const int C = kv_heads * head_dim, k_sel = top_k / 64 - 1;
+  QQ_REQUIRE(C <= kMaxC, "%s: kv_heads*head_dim %d exceeds %d", what, C, kMaxC);
+  QQ_REQUIRE(k_sel <= 1024, "%s: %d selected pages exceed 1024", what, k_sel);
+  SelectArgs sel{};
+  sel.q = q;
+  sel.q_dtype = q_dtype;
+  sel.q_bstride = q_batch_stride;
+  sel.H = num_q_heads;
+  sel.bounds_layer = reinterpret_cast<const uint32_t*>(page_k_bounds) + (int64_t)layer * max_reqs * max_pages * C;
+  sel.rpi = req_pool_indices;
+  sel.seq = seq_lens;
+  sel.limit = candidate_limit;
+  sel.R = max_reqs;
+  sel.MP = max_pages;
+  sel.KV = kv_heads;
+  sel.D = head_dim;
+  sel.C = C;
+  sel.m = (C + 63) / 64;
+  sel.P = 64;
+  sel.top_k = top_k;
+  sel.k_sel = k_sel;
+  sel.ppb = 32;
+  sel.scores = scores_ws;
+  sel.positions = positions;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (phase == 1) return launch_retrieve(sel, bs, s);
+  if (phase == 3) {
+    const int scored = launch_score(sel, bs, false, s);
+    if (scored != QQ_OK) return scored;
   } else {
-    if (q_dtype == QQ_DTYPE_BF16) launch<64, uint16_t>(a, st, s);
-    else launch<64, float>(a, st, s);
+    sel = SelectArgs{};  // phase 1 left the positions
   }
+  if (head_dim == 128) launch<128>(a, st, sel, q_dtype, s);
+  else launch<64>(a, st, sel, q_dtype, s);
   return check_launch(what);
 }

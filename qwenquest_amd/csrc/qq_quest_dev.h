@@ -634,6 +634,45 @@ __device__ inline void select_ranked(const float (&sv)[KPT], int lim, int n_eff,
   my_row0 = (page_rows && my_page >= 0 && my_page < max_pages) ? page_rows[my_page] : -1;
 }
 
+// Top k <= 64 pages of n_eff <= 256*KPT keys of request b by a block of 256 threads
+// (select_topk_block), then the layout.
+template <int KPT>
+__device__ inline void select_filter_block(const SelectArgs& a, int b, SelectSmem<KPT>& sm) {
+  const int tid = threadIdx.x;
+  // Every load of the selection is issued up front: the request words and all
+  // of the request's score slots (those past the candidate limit are masked
+  // below), so the block waits for one memory round trip, not three.
+  const int64_t s = a.seq[b];
+  const int64_t req = a.rpi[b];
+  const int lim_raw = a.limit[b];
+  const float* sc = a.scores + (int64_t)b * a.MP;
+  float sv[KPT];
+#pragma unroll
+  for (int i = 0; i < KPT; ++i) {
+    const int p = tid + kBlock * i;
+    sv[i] = p < a.MP ? sc[p] : 0.0f;
+  }
+  int32_t* pos = a.positions + (int64_t)b * a.top_k;
+  const int k = a.k_sel;
+  if (s <= a.top_k || k == 0) {
+    store_new_token(a, b);
+    if (s <= a.top_k)
+      write_dense(pos, s, a.top_k);
+    else
+      write_recent(pos, s, a.P);
+    return;
+  }
+  const int lim = (req >= 0 && req < a.R) ? min(lim_raw, a.MP) : 0;
+  select_topk_block<KPT>(sv, lim, max(lim, k), k, sm);
+  const int P = a.P;
+  for (int slot = tid; slot < k * P; slot += kBlock) {
+    const int r = slot / P;
+    pos[slot] = sm.order[r] * P + (slot - r * P);
+  }
+  write_recent(pos + (int64_t)k * P, s, P);
+  store_new_token(a, b);  // the attention launch that reads the pool comes after this one
+}
+
 // ----------------------------------------------------------------- attention
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));

@@ -473,45 +473,11 @@ __global__ __launch_bounds__(kThreads) void select_layout_kernel(SelectArgs a) {
   write_recent(pos + (int64_t)k * P, s, P);
 }
 
-// Top k <= 64 pages of n_eff <= 256*KPT keys, one block per request
-// (select_topk_block), then the layout.
+// select_filter_block, one block per request.
 template <int KPT>
 __global__ __launch_bounds__(kThreads) void select_filter_kernel(SelectArgs a) {
-  const int b = blockIdx.x;
-  const int tid = threadIdx.x;
-  // Every load of the selection is issued up front: the request words and all
-  // of the request's score slots (those past the candidate limit are masked
-  // below), so the block waits for one memory round trip, not three.
-  const int64_t s = a.seq[b];
-  const int64_t req = a.rpi[b];
-  const int lim_raw = a.limit[b];
-  const float* sc = a.scores + (int64_t)b * a.MP;
-  float sv[KPT];
-#pragma unroll
-  for (int i = 0; i < KPT; ++i) {
-    const int p = tid + kThreads * i;
-    sv[i] = p < a.MP ? sc[p] : 0.0f;
-  }
-  int32_t* pos = a.positions + (int64_t)b * a.top_k;
-  const int k = a.k_sel;
-  if (s <= a.top_k || k == 0) {
-    store_new_token(a, b);
-    if (s <= a.top_k)
-      write_dense(pos, s, a.top_k);
-    else
-      write_recent(pos, s, a.P);
-    return;
-  }
-  const int lim = (req >= 0 && req < a.R) ? min(lim_raw, a.MP) : 0;
   __shared__ SelectSmem<KPT> sm;
-  select_topk_block<KPT>(sv, lim, max(lim, k), k, sm);
-  const int P = a.P;
-  for (int slot = tid; slot < k * P; slot += kThreads) {
-    const int r = slot / P;
-    pos[slot] = sm.order[r] * P + (slot - r * P);
-  }
-  write_recent(pos + (int64_t)k * P, s, P);
-  store_new_token(a, b);  // the attention launch that reads the pool comes after this one
+  select_filter_block<KPT>(a, blockIdx.x, sm);
 }
 
 // group_queries (quest.py:366-391) as its own kernel: out [bs, C] in q's dtype.

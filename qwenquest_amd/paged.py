@@ -22,7 +22,17 @@ BLOCK_TOKENS = 64
 _ERR_EXHAUSTED, _ERR_REQUEST, _ERR_TWICE, _ERR_TOTAL = 1, 2, 4, 8
 
 
+def _indexed(device: torch.device | str) -> torch.device:
+    """``cuda`` as the device it stands for now: the pool's tensors lie there from now on."""
+    device = torch.device(device)
+    if device.type == "cuda" and device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    return device
+
+
 def _device_i64(t: torch.Tensor, device: torch.device, what: str) -> torch.Tensor:
+    if t.dtype is torch.int64 and t.dim() == 1 and t.device == device and t.is_contiguous():
+        return t
     if t.dim() != 1:
         raise ValueError(f"{what} must be one-dimensional, got {tuple(t.shape)}")
     if t.dtype.is_floating_point or t.dtype == torch.bool:
@@ -42,7 +52,7 @@ class BlockReqToTokenPool(ReqToTokenPool):
     """
 
     def __init__(self, size: int, max_context_len: int, num_blocks: int, device: torch.device | str):
-        super().__init__(size, max_context_len, device)
+        super().__init__(size, max_context_len, _indexed(device))
         if self.device.type != "cuda":
             raise RuntimeError("qwenquest_amd.BlockReqToTokenPool needs a GPU device (no CPU path)")
         if num_blocks < 1:
@@ -57,15 +67,14 @@ class BlockReqToTokenPool(ReqToTokenPool):
         self._err = torch.zeros(1, dtype=torch.int32, device=dev)
         self._err_host = pinned_zeros((1,), torch.int32)
         self._err_host_dev = HiSparseCoordinator._device_address(self._err_host)
+        # the C entries' view of the pool, whose tensors stay where they are
+        r2t, bt = self.req_to_token, self.block_table
+        self._args = (_lib.ptr(bt), bt.stride(0), _lib.ptr(r2t), r2t.stride(0), r2t.shape[1], r2t.shape[0],
+                      _lib.ptr(self.held), _lib.ptr(self.free_blocks), _lib.ptr(self.free_count), self.free_blocks.numel())
 
     def available_blocks(self) -> int:
         """Free blocks (reads the device: a synchronisation)."""
         return int(self.free_count.item())
-
-    def _pool_args(self) -> tuple:
-        r2t, bt = self.req_to_token, self.block_table
-        return (_lib.ptr(bt), bt.stride(0), _lib.ptr(r2t), r2t.stride(0), r2t.shape[1], r2t.shape[0],
-                _lib.ptr(self.held), _lib.ptr(self.free_blocks), _lib.ptr(self.free_count), self.free_blocks.numel())
 
     def _workspace(self, bs: int) -> torch.Tensor:
         # of this call alone: a graph's replay must not find another call's plan in it
@@ -73,13 +82,12 @@ class BlockReqToTokenPool(ReqToTokenPool):
         return torch.empty(max(need, 1), dtype=torch.uint8, device=self.device)
 
     def _assign(self, rpi, lens, new_lens, total: int) -> tuple[torch.Tensor, torch.Tensor]:
-        loc = torch.empty(total, dtype=torch.int64, device=self.device)
-        pos = torch.empty(total, dtype=torch.int64, device=self.device)
+        loc, pos = torch.empty((2, total), dtype=torch.int64, device=self.device).unbind(0)
         ws = self._workspace(rpi.numel()) if new_lens is not None else None
-        with torch.cuda.device(self.device):
+        with _lib.on(self.device):
             _lib.call(
                 "qq_block_assign", _lib.ptr(rpi), _lib.ptr(lens), _lib.ptr(new_lens), int(rpi.numel()), total,
-                *self._pool_args(), _lib.ptr(loc), _lib.ptr(pos), _lib.ptr(self._err), self._err_host_dev, _lib.ptr(ws),
+                *self._args, _lib.ptr(loc), _lib.ptr(pos), _lib.ptr(self._err), self._err_host_dev, _lib.ptr(ws),
                 0 if ws is None else ws.numel(), _lib.stream(self.device),
             )
         return loc, pos
@@ -113,8 +121,8 @@ class BlockReqToTokenPool(ReqToTokenPool):
         """Give the listed requests' blocks back and clear their tables."""
         rpi = _device_i64(req_pool_indices, self.device, "req_pool_indices")
         ws = self._workspace(rpi.numel())
-        with torch.cuda.device(self.device):
-            _lib.call("qq_block_release", _lib.ptr(rpi), int(rpi.numel()), *self._pool_args(), _lib.ptr(self._err),
+        with _lib.on(self.device):
+            _lib.call("qq_block_release", _lib.ptr(rpi), int(rpi.numel()), *self._args, _lib.ptr(self._err),
                       self._err_host_dev, _lib.ptr(ws), ws.numel(), _lib.stream(self.device))
 
     def free(self, req_pool_idx: int) -> None:
@@ -162,7 +170,7 @@ class Fp8TokenToKVPool:
     dtype = torch.float8_e4m3fn
 
     def __init__(self, num_blocks: int, num_layers: int, kv_heads: int, head_dim: int, device: torch.device | str):
-        self.device = torch.device(device)
+        self.device = _indexed(device)
         if self.device.type != "cuda":
             raise RuntimeError("qwenquest_amd.Fp8TokenToKVPool needs a GPU device (no CPU path)")
         if head_dim not in (64, 128):
@@ -217,7 +225,7 @@ class Fp8TokenToKVPool:
         if n == 0:
             return
         k, v = self.new_rows(k, v, n)
-        with torch.cuda.device(self.device):
+        with _lib.on(self.device):
             _lib.call("qq_fp8_store", *self.layer_args(layer_id), _lib.ptr(k), _lib.ptr(v), _lib.dtype_code(k.dtype),
                       _lib.ptr(loc), n, _lib.stream(self.device))
 
@@ -231,7 +239,7 @@ class Fp8TokenToKVPool:
         k = torch.empty((n, self.kv_heads, self.head_dim), dtype=dtype, device=self.device)
         v = torch.empty_like(k)
         if n:
-            with torch.cuda.device(self.device):
+            with _lib.on(self.device):
                 _lib.call("qq_fp8_rows", *self.layer_args(layer_id), _lib.ptr(loc), n, _lib.ptr(k), _lib.ptr(v), code,
                           _lib.stream(self.device))
         return k, v

@@ -364,7 +364,7 @@ class QuestAlgorithm:
     # -------------------------------------------- pages of an 8-bit block pool
 
     def _page_bounds(self, pool: Fp8TokenToKVPool, block_table, reqs, seq_lens, prefix_lens, decode: bool,
-                     max_new: int) -> torch.Tensor:
+                     max_new: int) -> StepLayout | None:
         if self.page_size != 64:
             raise ValueError(f"an 8-bit pool's pages are its blocks of 64 tokens, not of {self.page_size}")
         if pool.kv_heads != self.kv_heads or pool.head_dim != self.head_dim or pool.num_layers < self.end_layer:
@@ -378,14 +378,18 @@ class QuestAlgorithm:
         if any(t is not None and t.numel() != bs for t in lens):
             raise ValueError("req_indices, seq_lens and prefix_lens differ in length")
         codes, _, scale, _, *geometry = pool.layer_args(self.start_layer)
-        with torch.cuda.device(self.device):
+        actual = limit = None
+        if decode:
+            actual, limit = torch.empty((2, bs), dtype=torch.int32, device=self.device).unbind(0)
+        with _lib.on(self.device):
             _lib.call(
                 "qq_fp8_page_bounds", codes, pool.k_codes.stride(0), scale, pool.k_scale.stride(0), *geometry,
                 _lib.ptr(block_table), max(block_table.stride(0), block_table.shape[1]), block_table.shape[0],
                 block_table.shape[1], *(_lib.ptr(t) for t in lens), bs, int(decode), int(max_new), self.num_layers,
-                _lib.ptr(self.page_k_bounds), self.max_reqs, self.max_pages_per_req, _lib.stream(self.device),
+                _lib.ptr(self.page_k_bounds), self.max_reqs, self.max_pages_per_req, self.top_k,
+                int(self.avoid_recent_overlap), _lib.ptr(actual), _lib.ptr(limit), _lib.stream(self.device),
             )
-        return lens[1]
+        return StepLayout(lens[1], actual, limit, self.page_size, self.top_k) if decode else None
 
     def update_prefill_representations_blocks(
         self,
@@ -405,10 +409,10 @@ class QuestAlgorithm:
 
     def decode_step_blocks(self, req_indices: torch.Tensor, seq_lens: torch.Tensor, pool: Fp8TokenToKVPool,
                            block_table: torch.Tensor) -> StepLayout:
-        """[Q3] + [Q4] over an 8-bit pool: bounds of the pages that the previous step's tokens
-        completed, at every layer, then the step layout."""
-        seq = self._page_bounds(pool, block_table, req_indices, seq_lens, None, True, 0)
-        return self.prepare_step(seq)
+        """[Q3] + [Q4] over an 8-bit pool in one launch: bounds of the pages that the previous step's
+        tokens completed, at every layer, and the step layout."""
+        self._step = self._page_bounds(pool, block_table, req_indices, seq_lens, None, True, 0)
+        return self._step
 
     # ---------------------------------------------------- [Q5] page criticality
 

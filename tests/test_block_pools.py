@@ -91,10 +91,11 @@ def test_rows_refuses(lib, kw, said):
 @pytest.mark.parametrize("kw, said", [
     (dict(kc=None), b"null cache"), (dict(dim=80), b"head_dim"), (dict(bs=-1), b"bad sizes"), (dict(bs=65536), b"bad sizes"),
     (dict(layers=0), b"bad sizes"), (dict(reqs=0), b"bad sizes"), (dict(mp=0), b"bad sizes"), (dict(tstride=3), b"bad sizes"),
-    (dict(seq=None), b"null"), (dict(bounds=None), b"null"), (dict(table=None), b"null")])
+    (dict(seq=None), b"null"), (dict(bounds=None), b"null"), (dict(table=None), b"null"), (dict(actual=FAKE), b"layout")])
 def test_page_bounds_refuses(lib, kw, said):
     a = dict(kc=FAKE, kst=100, ks=FAKE, sst=10, blocks=5, kv=4, dim=128, table=FAKE, tstride=4, trows=2, tcols=4, rpi=FAKE,
-             seq=FAKE, prefix=None, bs=2, decode=0, max_new=0, layers=1, bounds=FAKE, reqs=2, mp=4)
+             seq=FAKE, prefix=None, bs=2, decode=0, max_new=0, layers=1, bounds=FAKE, reqs=2, mp=4, top_k=128,
+             avoid=0, actual=None, limit=None)
     a.update(kw)
     refused(lib.qq_fp8_page_bounds(*a.values(), None), lib, said)
 
@@ -110,6 +111,19 @@ def test_decode_refuses(lib, kw, said):
              rpi=FAKE, seq=FAKE, bs=2, pos=None, pstride=0, top_k=0, scale=0.1, out=FAKE, ws=FAKE, bytes=1 << 30)
     a.update(kw)
     refused(lib.qq_fp8_decode_attention(*a.values(), None), lib, said)
+
+
+@pytest.mark.parametrize("kw, said", BAD_CACHE + [
+    (dict(phase=0), b"phase"), (dict(phase=4), b"phase"), (dict(bounds=None), b"null"), (dict(scores=None), b"null"),
+    (dict(pos=None), b"null"), (dict(limit=None), b"null"), (dict(layer=-1), b"bad sizes"), (dict(reqs=0), b"bad sizes"),
+    (dict(top_k=100), b"multiple"), (dict(top_k=64 * 1026), b"selected pages"), (dict(kv=16, H=32), b"exceeds"),
+    (dict(loc=None), b"null"), (dict(nd=7), b"dtype"), (dict(kn=ctypes.c_void_p(4104)), b"aligned"), (dict(bytes=64), b"workspace")])
+def test_quest_step_refuses(lib, kw, said):
+    a = dict(q=FAKE, qd=0, qst=4096, H=32, kn=FAKE, vn=FAKE, nd=0, loc=FAKE, **CACHE, table=FAKE, tstride=4, trows=2, tcols=4,
+             bounds=FAKE, layer=0, rpi=FAKE, seq=FAKE, limit=FAKE, bs=2, reqs=2, mp=4, top_k=128, scale=0.1, scores=FAKE, pos=FAKE,
+             out=FAKE, ws=FAKE, bytes=1 << 30, phase=3)
+    a.update(kw)
+    refused(lib.qq_fp8_quest_step(*a.values(), None), lib, said)
 
 
 @pytest.mark.parametrize("kw, said", BAD_CACHE + [
