@@ -12,7 +12,11 @@
 // the block that completes them.  Two launches: fp8_begin_kernel cuts the slices and stores the
 // new tokens, fp8_attend_kernel does the rest.
 //
-// A wave takes a unit at a time: K and V codes straight from memory to registers in the
+// Of its block's slice a wave takes a quarter, units in a row, and goes through their requests on
+// its own; what a request's end finds in one wave is written by that wave, the rest meets in the
+// LDS.  A slice of many short requests thus has four of them in work at once, their blocks
+// looked up together, and a request's first unit is loaded under the one before it.  A wave
+// takes a unit at a time: K and V codes straight from memory to registers in the
 // operands' order (1 KiB runs), converted to bf16 (exact), S^T = K Q^T, the softmax in
 // registers, O^T += V^T P^T, with P's values scaled by vs as bf16 pieces: two for bf16 output
 // (16 significand bits), three for fp32 (all 24).  fp32 queries go in as three bf16 pieces, too.
@@ -198,12 +202,16 @@ __device__ inline void load_query(const void* q, int64_t at, bool in, bf16x8_t (
   }
 }
 
-template <int D>
+// What waves leave for the block to add up: slot 2 w of wave w for the request that goes on in its
+// units, 2 w + 1 for the one that goes on behind them.
+constexpr int kSlots = 2 * kDecWaves;
 struct DecSmem {
   union {
     struct {
-      float m[kDecWaves][kTile], l[kDecWaves][kTile];
-      float o[kDecWaves][kTile][D + 4];
+      float m[kSlots][kTile], l[kSlots][kTile];
+      int32_t b[kSlots];      // request, or -1: nothing there
+      int32_t c0[kSlots], c1[kSlots];
+      int32_t ended[kSlots];  // its last unit is among them
     };
     struct {
       float w[kTile][kDecParts], sum[kTile];
@@ -211,13 +219,16 @@ struct DecSmem {
     } merge;
   };
   uint32_t last;
+  float4 o[1];  // [kSlots][rows][D + 4] floats
 };
+constexpr int dec_row_floats(int D) { return D + 4; }
+inline size_t dec_smem_bytes(int rows, int D) { return sizeof(DecSmem) + (size_t)kSlots * rows * dec_row_floats(D) * 4; }
 
 // The parts of a request's tile added up, by the block that finished the last of them: a wave
 // per query head and a lane per part for the weights, then a thread per 4 channels of a head,
 // and where those are few, of every ng-th part.
 template <int D, typename T>
-__device__ inline void merge_parts(const DecArgs& a, DecSmem<D>& sm, int head, int first, int parts, int rows, T* out) {
+__device__ inline void merge_parts(const DecArgs& a, DecSmem& sm, int head, int first, int parts, int rows, T* out) {
   constexpr int NT = 64 * kDecWaves;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   // row r of part i: of slice first + i, the part that begins its request there, or goes on in it
@@ -293,7 +304,10 @@ template <int D, typename T>
 __global__ __launch_bounds__(64 * kDecWaves, 2) void fp8_attend_kernel(DecArgs a) {
   constexpr int QP = sizeof(T) == 2 ? 1 : 3, PP = sizeof(T) == 2 ? 2 : 3;  // pieces of q and of the weights
   constexpr int KL = D / 64, VL = D / 16;  // 16-byte loads a lane: per 16 tokens of K, per block of V
-  __shared__ DecSmem<D> sm;
+  constexpr int RF = dec_row_floats(D);
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  DecSmem& sm = *reinterpret_cast<DecSmem*>(smem_raw);
+  float* sm_o = reinterpret_cast<float*>(sm.o);
   const int head = blockIdx.x % a.heads, slice = blockIdx.x / a.heads;
   const DecPlan plan = *a.plan;
   const DecItem item = a.items[slice];  // both in one round trip; stale past the last slice
@@ -303,210 +317,290 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void fp8_attend_kernel(DecArgs a
   const int m16 = lane & 15, g = lane >> 4;
   const int rows = min(a.G - tile * kTile, kTile);  // query heads of this tile
   const int q_head = h * a.G + tile * kTile;
-  const int end = min((slice + 1) * plan.len, plan.total);
-  int at = slice * plan.len;
-  int b = item.b, c0 = item.c0, c1 = item.c1, seq = item.seq, req = item.req;
-  for (;;) {
-    const int u0 = at - c0, u1 = min(end, c1) - c0;  // this slice's units of request b
-    const bool sparse = is_sparse(a, seq);
-    const bool known = req >= 0;
-    const int32_t* tr = a.table + (int64_t)max(req, 0) * a.table_stride;
-    const int picked = a.top_k / 64 - 1;  // selected pages; the unit after them is the window
+  const int at = slice * plan.len, end = min(at + plan.len, plan.total);
+  // this wave's units
+  const int s0 = at + (int)((int64_t)(end - at) * wave / kDecWaves), s1 = at + (int)((int64_t)(end - at) * (wave + 1) / kDecWaves);
+  const int picked = a.top_k / 64 - 1;  // selected pages; the unit after them is the window
+  if (lane < 2) sm.b[2 * wave + lane] = -1;
 
-    bf16x8_t qf[2 * KL][QP];
+  // Of unit u0 + lane: its request, place in it, block and scales; a window has two blocks.  64 units
+  // belong to 64 requests at most, from request rb on.
+  int rb = item.b;
+  int u_b = 0, u_c0 = 0, u_c1 = 0, u_seq = 0, blk = 0, blk2 = 0;
+  bool u_bad = false;
+  float ks = 0.0f, vs = 0.0f, ks2 = 0.0f, vs2 = 0.0f;
+  auto resolve = [&](int u0) {
+    const int u = u0 + lane, u_end = min(u0 + 64, s1);
+    int row = item.req;
+    if (rb == item.b && u_end <= item.c1) {  // all of them the slice's first request's
+      u_b = rb;
+      u_c0 = item.c0;
+      u_c1 = item.c1;
+      u_seq = item.seq;
+    } else {
+      int begins;  // unit where request rb + lane begins
+      for (;;) {
+        const int r = rb + lane;
+        begins = r <= a.bs ? a.cu[r] : 0x7FFFFFFF;
+        const int skip = __popcll(__ballot(begins <= u0)) - 1;  // those that begin before: a run of lanes from 0
+        if (skip == 0) break;
+        rb += skip;
+      }
+      const int r = rb + lane;
+      const int my_seq = r < a.bs ? context_of(a, r) : 0, my_row = r < a.bs ? table_row(a, r) : -1;
+      int i = 0;  // of the window's requests
+      for (int x = 1; x < 64; ++x) {
+        const int c = __builtin_amdgcn_readlane(begins, x);
+        if (c >= u_end) break;
+        i += u >= c ? 1 : 0;
+      }
+      u_b = rb + i;
+      u_c0 = __shfl(begins, i, 64);
+      u_seq = __shfl(my_seq, i, 64);
+      row = __shfl(my_row, i, 64);
+      u_c1 = u_c0 + units_of(a, u_seq);
+    }
+    blk = blk2 = 0;
+    u_bad = row < 0;
+    const int32_t* tr = a.table + (int64_t)max(row, 0) * a.table_stride;
+    auto block_at = [&](int page) {
+      const int x = page >= 0 && page < a.table_cols ? tr[page] : 0;
+      if (x > 0 && x < a.c.blocks) return x;
+      u_bad = true;  // no block there: no answer
+      return 0;
+    };
+    const bool sparse = is_sparse(a, u_seq), win = sparse && u - u_c0 == picked;
+    if (u < u_end && u_seq > 0 && row >= 0) {
+      const int place = u - u_c0;
+      blk = block_at(!sparse ? place : win ? (u_seq - 64) >> 6 : a.positions[(int64_t)u_b * a.pos_stride + place * 64] >> 6);
+      blk2 = win && (u_seq & 63) ? block_at(u_seq >> 6) : blk;
+    }
+    const int64_t e = (int64_t)blk * a.c.KV + h, e2 = (int64_t)blk2 * a.c.KV + h;
+    ks = a.c.ks[e];
+    vs = a.c.vs[e];
+    if (a.positions) {
+      ks2 = a.c.ks[e2];
+      vs2 = a.c.vs[e2];
+    }
+  };
+  uint4 kr[4][KL], vr[VL];
+  auto head_at = [&](int blocks, int j) {
+    return ((int64_t)__builtin_amdgcn_readlane(blocks, j) * a.c.KV + h) * (64 * D) + lane * 16;
+  };
+  // K of lane j's unit: a window's tokens before place seq % 64 come from its second block
+  auto load_k = [&](int j) {
+    const uint8_t* p = a.c.kc + head_at(blk, j);
+    const uint8_t* p2 = a.c.kc + head_at(blk2, j);
+    const int from2 = __builtin_amdgcn_readlane(u_seq, j) & 63;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const uint8_t* pt = t * 16 + m16 < from2 ? p2 : p;
+#pragma unroll
+      for (int i = 0; i < KL; ++i) kr[t][i] = *reinterpret_cast<const uint4*>(pt + (t * KL + i) * 1024);
+    }
+  };
+  auto load_v = [&](int blocks, int j, uint4* v) {
+    const uint8_t* p = a.c.vc + head_at(blocks, j);
+#pragma unroll
+    for (int i = 0; i < VL; ++i) v[i] = *reinterpret_cast<const uint4*>(p + i * 1024);
+  };
+  bf16x8_t qf[2 * KL][QP];
+  float4_t o[VL];
+  float M = -INFINITY, L = 0.0f;
+  bool bad = false;
+  int first = s0;  // this request's first unit here
+  auto load_q = [&](int b) {
 #pragma unroll
     for (int i = 0; i < 2 * KL; ++i) {
       const int d = ((i >> 1) * 4 + g) * 16 + (i & 1) * 8;
       load_query<QP>(a.q, (int64_t)b * a.q_bstride + (int64_t)(q_head + min(m16, rows - 1)) * D + d, m16 < rows, qf[i]);
     }
-    // lane j looks up this wave's unit j0 + j: u0 + wave + 4 (j0 + j)
-    const int n = u1 - u0 > wave ? (u1 - u0 - wave + kDecWaves - 1) / kDecWaves : 0;
-    int blk = 0, blk2 = 0;  // blk2: the window's second block
-    float ks = 0.0f, vs = 0.0f, ks2 = 0.0f, vs2 = 0.0f;
-    bool bad = !known;
-    auto block_at = [&](int page) {
-      const int x = page >= 0 && page < a.table_cols ? tr[page] : 0;
-      if (x > 0 && x < a.c.blocks) return x;
-      bad = true;  // no block there: no answer
-      return 0;
-    };
-    auto resolve = [&](int j0) {
-      const int u = u0 + wave + kDecWaves * (j0 + lane);
-      blk = blk2 = 0;
-      const bool win = sparse && u == picked;
-      if (j0 + lane < n && seq > 0 && known) {
-        blk = block_at(!sparse ? u : win ? (seq - 64) >> 6 : a.positions[(int64_t)b * a.pos_stride + u * 64] >> 6);
-        blk2 = win && (seq & 63) ? block_at(seq >> 6) : blk;
-      }
-      const int64_t e = (int64_t)blk * a.c.KV + h, e2 = (int64_t)blk2 * a.c.KV + h;
-      ks = a.c.ks[e];
-      vs = a.c.vs[e];
-      if (sparse) {
-        ks2 = a.c.ks[e2];
-        vs2 = a.c.vs[e2];
-      }
-    };
-    uint4 kr[4][KL], vr[VL];
-    auto head_at = [&](int blocks, int j) {
-      return ((int64_t)__builtin_amdgcn_readlane(blocks, j & 63) * a.c.KV + h) * (64 * D) + lane * 16;
-    };
-    // K of unit j: a window's tokens before place seq % 64 come from its second block
-    auto load_k = [&](int j) {
-      const uint8_t* p = a.c.kc + head_at(blk, j);
-      const uint8_t* p2 = a.c.kc + head_at(blk2, j);
+  };
+  // loads come back in order: the queries before the keys, the keys before the values
+  if (s0 < s1) {
+    resolve(s0);
+    load_q(__builtin_amdgcn_readlane(u_b, 0));
+    load_k(0);
+    load_v(blk, 0, vr);
+  }
+  for (int u = s0; u < s1; ++u) {
+    const int j = (u - s0) & 63;
+    const int b = __builtin_amdgcn_readlane(u_b, j), c0 = __builtin_amdgcn_readlane(u_c0, j), c1 = __builtin_amdgcn_readlane(u_c1, j);
+    const int seq = __builtin_amdgcn_readlane(u_seq, j);
+    if (u == s0 || u == c0) {  // a request begins here
+      first = u;
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const uint8_t* pt = t * 16 + m16 < (seq & 63) ? p2 : p;
-#pragma unroll
-        for (int i = 0; i < KL; ++i) kr[t][i] = *reinterpret_cast<const uint4*>(pt + (t * KL + i) * 1024);
-      }
-    };
-    auto load_v = [&](const int blocks, int j, uint4* v) {
-      const uint8_t* p = a.c.vc + head_at(blocks, j);
-#pragma unroll
-      for (int i = 0; i < VL; ++i) v[i] = *reinterpret_cast<const uint4*>(p + i * 1024);
-    };
-    float4_t o[VL];
-#pragma unroll
-    for (int i = 0; i < VL; ++i) o[i] = float4_t{0.f, 0.f, 0.f, 0.f};
-    float M = -INFINITY, L = 0.0f;
-    if (n > 0) {
-      resolve(0);
-      load_k(0);
-      load_v(blk, 0, vr);
+      for (int i = 0; i < VL; ++i) o[i] = float4_t{0.f, 0.f, 0.f, 0.f};
+      M = -INFINITY;
+      L = 0.0f;
+      bad = false;
     }
-    for (int j = 0; j < n; ++j) {
-      const int u = u0 + wave + kDecWaves * j;
-      const bool win = sparse && u == picked;
-      const int hi = sparse ? 64 : min(64, seq - u * 64);  // tokens of this unit
-      const float kscale = __shfl(ks, j & 63, 64) * a.sl2, vscale = __shfl(vs, j & 63, 64);
-      const float kscale2 = win ? __shfl(ks2, j & 63, 64) * a.sl2 : kscale, vscale2 = win ? __shfl(vs2, j & 63, 64) : vscale;
-      const bool last = j + 1 >= n, next_set = ((j + 1) & 63) == 0;
-      float4_t s[4];
+    const bool sparse = is_sparse(a, seq), win = sparse && u - c0 == picked;
+    const int hi = sparse ? 64 : min(64, seq - (u - c0) * 64);  // tokens of this unit
+    const float kscale = __shfl(ks, j, 64) * a.sl2, vscale = __shfl(vs, j, 64);
+    const float kscale2 = win ? __shfl(ks2, j, 64) * a.sl2 : kscale, vscale2 = win ? __shfl(vs2, j, 64) : vscale;
+    bad |= (bool)__builtin_amdgcn_readlane((int)u_bad, j);
+    const bool last = u + 1 >= s1, next_set = j == 63;
+    float4_t s[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      s[t] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < KL; ++i) {
+        const bf16x8_t k0 = codes8(kr[t][i].x, kr[t][i].y), k1 = codes8(kr[t][i].z, kr[t][i].w);
+#pragma unroll
+        for (int p = 0; p < QP; ++p) {
+          s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, qf[2 * i][p], s[t], 0, 0, 0);
+          s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, qf[2 * i + 1][p], s[t], 0, 0, 0);
+        }
+      }
+    }
+    if (!last && u + 1 == c1) load_q(b + 1);
+    // the next unit's K under this one's softmax and values; a window's second V goes there instead
+    if (win) load_v(blk2, j, &kr[0][0]);
+    else if (!last && !next_set) load_k(j + 1);
+    float mx = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int tok = t * 16 + g * 4 + i;
+        s[t][i] = tok < hi ? s[t][i] * (tok < (seq & 63) ? kscale2 : kscale) : -INFINITY;
+        mx = fmaxf(mx, s[t][i]);
+      }
+    mx = fmaxf(mx, lane_xor16(mx, lane));
+    mx = fmaxf(mx, lane_xor32(mx, lane));
+    const float Mn = fmaxf(M, mx);
+    const float mb = Mn == -INFINITY ? 0.0f : Mn;
+    const float alpha = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - mb);
+    M = Mn;
+    float sum = 0.0f;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float p = __builtin_amdgcn_exp2f(s[t][i] - mb);
+        sum += p;
+        // a masked token weighs nothing whatever its block's scale is
+        s[t][i] = s[t][i] == -INFINITY ? 0.0f : p * (t * 16 + g * 4 + i < (seq & 63) ? vscale2 : vscale);
+      }
+    if (win) {
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        s[t] = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < KL; ++i) {
-          const bf16x8_t k0 = codes8(kr[t][i].x, kr[t][i].y), k1 = codes8(kr[t][i].z, kr[t][i].w);
-#pragma unroll
-          for (int p = 0; p < QP; ++p) {
-            s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, qf[2 * i][p], s[t], 0, 0, 0);
-            s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, qf[2 * i + 1][p], s[t], 0, 0, 0);
-          }
-        }
-      }
-      // the next unit's K under this one's softmax and values; a window's second V goes there instead
-      if (win) load_v(blk2, j, &kr[0][0]);
-      else if (!last && !next_set) load_k(j + 1);
-      float mx = -INFINITY;
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int tok = t * 16 + g * 4 + i;
-          s[t][i] = tok < hi ? s[t][i] * (tok < (seq & 63) ? kscale2 : kscale) : -INFINITY;
-          mx = fmaxf(mx, s[t][i]);
-        }
-      mx = fmaxf(mx, lane_xor16(mx, lane));
-      mx = fmaxf(mx, lane_xor32(mx, lane));
-      const float Mn = fmaxf(M, mx);
-      const float mb = Mn == -INFINITY ? 0.0f : Mn;
-      const float alpha = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - mb);
-      M = Mn;
-      float sum = 0.0f;
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float p = __builtin_amdgcn_exp2f(s[t][i] - mb);
-          sum += p;
-          // a masked token weighs nothing whatever its block's scale is
-          s[t][i] = s[t][i] == -INFINITY ? 0.0f : p * (t * 16 + g * 4 + i < (seq & 63) ? vscale2 : vscale);
-        }
-      if (win) {
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const int from2 = min(max((seq & 63) - t * 16 - g * 4, 0), 4);  // of the word's four tokens
-          const uint32_t mask = from2 >= 4 ? 0xFFFFFFFFu : (1u << (8 * from2)) - 1u;
-#pragma unroll
-          for (int i = 0; i < VL; ++i) {
-            uint32_t& w = reinterpret_cast<uint32_t*>(&vr[i])[t];
-            w = (reinterpret_cast<const uint32_t*>(&kr[0][0])[i * 4 + t] & mask) | (w & ~mask);
-          }
-        }
-      }
-      L = L * alpha + sum;
-#pragma unroll
-      for (int i = 0; i < VL; ++i)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) o[i][x] *= alpha;
-#pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        bf16x8_t pw[PP];
-#pragma unroll
-        for (int p = 0; p < PP; ++p) {
-          u32x4_t w;
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const float e = s[2 * st + (x >> 1)][(x & 1) * 2], f = s[2 * st + (x >> 1)][(x & 1) * 2 + 1];
-            w[x] = pack_trunc(e, f);
-            s[2 * st + (x >> 1)][(x & 1) * 2] = e - trunc_bf16(e);
-            s[2 * st + (x >> 1)][(x & 1) * 2 + 1] = f - trunc_bf16(f);
-          }
-          pw[p] = __builtin_bit_cast(bf16x8_t, w);
-        }
+        const int from2 = min(max((seq & 63) - t * 16 - g * 4, 0), 4);  // of the word's four tokens
+        const uint32_t mask = from2 >= 4 ? 0xFFFFFFFFu : (1u << (8 * from2)) - 1u;
 #pragma unroll
         for (int i = 0; i < VL; ++i) {
-          const uint32_t x[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
-          const bf16x8_t vb = codes8(x[2 * st], x[2 * st + 1]);
-#pragma unroll
-          for (int p = 0; p < PP; ++p) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb, pw[p], o[i], 0, 0, 0);
+          uint32_t& w = reinterpret_cast<uint32_t*>(&vr[i])[t];
+          w = (reinterpret_cast<const uint32_t*>(&kr[0][0])[i * 4 + t] & mask) | (w & ~mask);
         }
       }
-      if (!last) {
-        if (next_set) resolve(j + 1);
-        if (next_set || win) load_k(j + 1);
-        load_v(blk, j + 1, vr);
-      }
     }
-    L += lane_xor16(L, lane);
-    L += lane_xor32(L, lane);
-    if (__any(bad)) L = __builtin_nanf("");
-
-    __syncthreads();  // the request before has been read out of sm
-    if (g == 0) {
-      sm.m[wave][m16] = M;
-      sm.l[wave][m16] = L;
-    }
+    L = L * alpha + sum;
 #pragma unroll
     for (int i = 0; i < VL; ++i)
-      *reinterpret_cast<float4_t*>(&sm.o[wave][m16][i * 16 + g * 4]) = o[i];
-    __syncthreads();
-    const bool whole = u0 == 0 && c1 <= end;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) o[i][x] *= alpha;
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      bf16x8_t pw[PP];
+#pragma unroll
+      for (int p = 0; p < PP; ++p) {
+        u32x4_t w;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const float e = s[2 * st + (x >> 1)][(x & 1) * 2], f = s[2 * st + (x >> 1)][(x & 1) * 2 + 1];
+          w[x] = pack_trunc(e, f);
+          s[2 * st + (x >> 1)][(x & 1) * 2] = e - trunc_bf16(e);
+          s[2 * st + (x >> 1)][(x & 1) * 2 + 1] = f - trunc_bf16(f);
+        }
+        pw[p] = __builtin_bit_cast(bf16x8_t, w);
+      }
+#pragma unroll
+      for (int i = 0; i < VL; ++i) {
+        const uint32_t x[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
+        const bf16x8_t vb = codes8(x[2 * st], x[2 * st + 1]);
+#pragma unroll
+        for (int p = 0; p < PP; ++p) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb, pw[p], o[i], 0, 0, 0);
+      }
+    }
+    if (!last) {
+      if (next_set) resolve(u + 1);
+      if (next_set || win) load_k(next_set ? 0 : j + 1);
+      load_v(blk, next_set ? 0 : j + 1, vr);
+    }
+    if (!last && u + 1 < c1) continue;
+    // the request's units here are done
+    float l = L + lane_xor16(L, lane);
+    l += lane_xor32(l, lane);
+    if (bad) l = __builtin_nanf("");
+    const bool began = first == c0, ended = u + 1 == c1;
+    if (began && ended) {
+      const float inv = l <= 0.0f ? 0.0f : 1.0f / l;  // nothing attended: zeros
+      if (m16 < rows) {
+        T* out = static_cast<T*>(a.out) + ((int64_t)b * a.H + q_head + m16) * D + g * 4;
+#pragma unroll
+        for (int i = 0; i < VL; ++i) store4(out + i * 16, o[i][0] * inv, o[i][1] * inv, o[i][2] * inv, o[i][3] * inv);
+      }
+      continue;
+    }
+    const int slot = 2 * wave + (began ? 1 : 0);
+    if (lane == 0) {
+      sm.b[slot] = b;
+      sm.c0[slot] = c0;
+      sm.c1[slot] = c1;
+      sm.ended[slot] = ended;
+    }
+    if (g == 0) {
+      sm.m[slot][m16] = M;
+      sm.l[slot][m16] = l;
+    }
+    if (m16 < rows) {
+#pragma unroll
+      for (int i = 0; i < VL; ++i) *reinterpret_cast<float4_t*>(sm_o + (slot * rows + m16) * RF + i * 16 + g * 4) = o[i];
+    }
+  }
+  __syncthreads();
+  // The requests that more than one wave has, or that go on in another slice: their slots follow one
+  // another, from the one where the request begins here to the one where it ends (or the slice).
+  const int sl = lane & (kSlots - 1);
+  const int sl_b = sm.b[sl], sl_c0 = sm.c0[sl], sl_c1 = sm.c1[sl];
+  uint32_t left = (uint32_t)__ballot(sl_b >= 0) & ((1u << kSlots) - 1u);
+  const uint32_t ends = (uint32_t)__ballot(sm.ended[sl] != 0) & left;
+  bool handed = false;
+  int next_b = -1, next_c0 = 0, next_c1 = 0;  // the request that goes on in the next slice
+  while (left) {
+    const int f = __builtin_ctz(left);
+    const uint32_t stop = ends & ~((1u << f) - 1u);
+    const bool ended = stop != 0;
+    const uint32_t mask = ended ? left & ((2u << __builtin_ctz(stop)) - 1u) : left;
+    left &= ~mask;
+    const int b = __builtin_amdgcn_readlane(sl_b, f), c0 = __builtin_amdgcn_readlane(sl_c0, f), c1 = __builtin_amdgcn_readlane(sl_c1, f);
+    const bool whole = c0 >= at && ended;
     T* out = static_cast<T*>(a.out) + ((int64_t)b * a.H + q_head) * D;
-    const int part = ((slice * 2 + (u0 == 0 ? 1 : 0)) * a.heads + head) * kTile;
+    const int part = ((slice * 2 + (c0 >= at ? 1 : 0)) * a.heads + head) * kTile;
     const __amdgpu_buffer_rsrc_t po = agent_rsrc(a.part_o + (int64_t)part * D, (uint32_t)(kTile * D * sizeof(float)));
     for (int it = tid; it < rows * (D / 4); it += 64 * kDecWaves) {
       const int r = it / (D / 4), d = (it - r * (D / 4)) * 4;
       float Mx = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < kDecWaves; ++w) Mx = fmaxf(Mx, sm.m[w][r]);
+      for (int w = 0; w < kSlots; ++w) Mx = mask >> w & 1 ? fmaxf(Mx, sm.m[w][r]) : Mx;
       float Ls = 0.0f;
       float4 Os = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < kDecWaves; ++w) {
+      for (int w = 0; w < kSlots; ++w) {
+        if (!(mask >> w & 1)) continue;  // block-uniform
         const float wt = sm.m[w][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm.m[w][r] - Mx);
         const float lw = sm.l[w][r];
         Ls += lw != lw ? lw : wt * lw;
-        const float4 x = *reinterpret_cast<const float4*>(&sm.o[w][r][d]);
+        const float4 x = *reinterpret_cast<const float4*>(sm_o + (w * rows + r) * RF + d);
         Os.x += wt * x.x;
         Os.y += wt * x.y;
         Os.z += wt * x.z;
         Os.w += wt * x.w;
       }
       if (whole) {
-        const float inv = Ls <= 0.0f ? 0.0f : 1.0f / Ls;  // nothing attended: zeros
+        const float inv = Ls <= 0.0f ? 0.0f : 1.0f / Ls;
         store4(out + (int64_t)r * D + d, Os.x * inv, Os.y * inv, Os.z * inv, Os.w * inv);
       } else {
         st_agent_x4(po, (uint32_t)((r * D + d) * sizeof(float)), Os);
@@ -516,21 +610,27 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void fp8_attend_kernel(DecArgs a
         }
       }
     }
-    if (!whole) {
-      const int first = c0 / plan.len, parts = (c1 - 1) / plan.len - first + 1;
-      wait_memory();
-      __syncthreads();
-      if (tid == 0) sm.last = add_agent(&a.done[first * a.heads + head], 1u) == (uint32_t)parts - 1;
-      __syncthreads();
-      if (sm.last) merge_parts<D, T>(a, sm, head, first, parts, rows, out);
+    handed |= !whole;
+    if (c0 >= at && !ended) {
+      next_b = b;
+      next_c0 = c0;
+      next_c1 = c1;
     }
-    at = c0 + u1;
-    if (at >= end) return;
-    ++b;
-    c0 = c1;
-    c1 = a.cu[b + 1];
-    seq = context_of(a, b);
-    req = table_row(a, b);
+  }
+  if (!handed) return;
+  // parts handed out: of the request that comes from the slice before, and of the one that goes on in
+  // the next; the block that finishes a request's last part adds them up
+  wait_memory();
+  for (int x = 0; x < 2; ++x) {
+    const int b = x ? next_b : item.c0 < at ? item.b : -1;
+    if (b < 0) continue;  // block-uniform
+    const int c0 = x ? next_c0 : item.c0, c1 = x ? next_c1 : item.c1;
+    const int first_slice = c0 / plan.len, parts = (c1 - 1) / plan.len - first_slice + 1;
+    __syncthreads();
+    if (tid == 0) sm.last = add_agent(&a.done[first_slice * a.heads + head], 1u) == (uint32_t)parts - 1;
+    __syncthreads();
+    if (sm.last)
+      merge_parts<D, T>(a, sm, head, first_slice, parts, rows, static_cast<T*>(a.out) + ((int64_t)b * a.H + q_head) * D);
   }
 }
 
@@ -560,6 +660,22 @@ void begin(const DecArgs& a, const StoreArgs& st, const SelectArgs& sel, hipStre
   else fp8_begin_kernel<D, float, KPT><<<blocks, 256, 0, s>>>(a, st, sel);
 }
 
+// LDS past the 64 KiB default (tiles of more than 15 heads of 128): opted in once per device.
+template <int D, typename T>
+void attend(const DecArgs& a, hipStream_t s) {
+  const size_t bytes = dec_smem_bytes(min(a.G, kTile), D);
+  if (bytes > 64 * 1024) {
+    static bool opted[64] = {false};
+    int dev = 0;
+    if (hipGetDevice(&dev) == hipSuccess && dev >= 0 && dev < 64 && !opted[dev]) {
+      (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&fp8_attend_kernel<D, T>),
+                                hipFuncAttributeMaxDynamicSharedMemorySize, (int)dec_smem_bytes(kTile, D));
+      opted[dev] = true;
+    }
+  }
+  fp8_attend_kernel<D, T><<<a.max_slices * a.heads, 64 * kDecWaves, bytes, s>>>(a);
+}
+
 // `sel`: with k_sel > 0 the pages are selected first, from scores that are there.
 template <int D>
 void launch(const DecArgs& a, const StoreArgs& st, const SelectArgs& sel, int q_dtype, hipStream_t s) {
@@ -572,9 +688,8 @@ void launch(const DecArgs& a, const StoreArgs& st, const SelectArgs& sel, int q_
     launch_select(sel, a.bs, sel.MP, sel.k_sel, s);
     begin<D, 0>(a, st, sel, s);
   }
-  const int grid = a.max_slices * a.heads;
-  if (q_dtype == QQ_DTYPE_BF16) fp8_attend_kernel<D, uint16_t><<<grid, 64 * kDecWaves, 0, s>>>(a);
-  else fp8_attend_kernel<D, float><<<grid, 64 * kDecWaves, 0, s>>>(a);
+  if (q_dtype == QQ_DTYPE_BF16) attend<D, uint16_t>(a, s);
+  else attend<D, float>(a, s);
 }
 
 // Everything of a call but its launches; `what` refuses.
