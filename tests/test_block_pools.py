@@ -178,7 +178,7 @@ def test_slices_cover_the_batch_within_the_grid_and_the_merge(rules):
         total, most = sum(units), rules.slices_(heads)
         n = rules.len_(total, max(units), most)
         slices = -(-total // n)
-        assert 1 <= slices <= most and (heads * most <= 512 or most == 1)
+        assert 1 <= slices <= most and (heads * most <= 256 or most == 1)  # a block per CU
         at = 0
         for u in units:  # parts of a request
             assert (at + u - 1) // n - at // n + 1 <= rules.parts_()
