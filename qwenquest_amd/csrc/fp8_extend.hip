@@ -9,11 +9,12 @@
 // its token (K) or channel (V): no bank conflicts and nothing transposed.
 //   S^T = K Q^T  v_mfma_f32_32x32x16_bf16, K's codes to bf16 (exact)
 //   O^T += V^T W^T  v_mfma_f32_32x32x16_f16, V's codes to f16 (exact)
-// With t = scale log2(e) ks (q . kc), M the running maximum of t, and R the largest exponent of a
-// V scale so far (one number per wave), a weight goes into the product as
-//   w = 2^(t - M + lv - R + 15),  vs = 2^lv,
-// so V's scale costs nothing per element, w fills f16's range from the top (the 15) and what
-// another block's far larger values leave of it is lost only under 2^-40 of those.  w goes to f16's
+// With t = scale log2(e) ks (q . kc), M a running maximum of t that is let lag by 8 (the sums are
+// rescaled once it lags more), and R the largest exponent of a V scale so far (one number per
+// wave), a weight goes into the product as
+//   w = 2^(t - M + lv - R + 7),  vs = 2^lv,
+// so V's scale costs nothing per element, w fills f16's range from the top (7 + 8) and what
+// another block's far larger values leave of it is lost only under 2^-32 of those.  w goes to f16's
 // 11 bits by truncation (one instruction for two weights) of w (1 + 0.72 * 2^-11): truncation takes
 // half a step on average, 2^-10 / 2 over the significand's 1 .. 2, in the mean 0.72 * 2^-11.
 // A weight is off by 0.64 * 2^-10 at most, an output by that of sum p |v|, where its own rounding
@@ -26,7 +27,7 @@ namespace {
 
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 
-constexpr int kLift = 15;           // w <= 2^15 * kRound < f16's 65504
+constexpr int kLift = 7, kSlack = 8;  // w <= 2^(7 + 8) * kRound < f16's 65504
 constexpr float kRound = 1.0003516f, kRoundLog2 = 5.0713e-4f;  // 1 + 0.72 * 2^-11
 constexpr int kExpFloor = -60;      // of lv - R: f16 has nothing left of such weights, their fp32 sum has
 
@@ -71,6 +72,17 @@ __device__ inline f16x8_t codes_f16(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(f16x8_t, w);
 }
 
+// find_tile's answer is the same in every lane; in scalar registers it makes the K/V loop's control
+// and its lookups scalar.
+__device__ inline ExtendTile uniform_tile(const ExtendTile& t) {
+  auto u = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  return {u(t.b), u(t.tile), u(t.q0), u(t.n), u(t.past), u(t.req), u(t.kv_len), u(t.prefix)};
+}
+
+// Words that this launch does not write, through the scalar cache.
+typedef const __attribute__((address_space(4))) int32_t* scalar_words_t;
+typedef const __attribute__((address_space(4))) float* scalar_floats_t;
+
 template <int D>
 __global__ __launch_bounds__(64 * kExtWaves, 2) void fp8_extend_kernel(Fp8ExtendArgs a) {
   constexpr int KI = D / 32, NC = D / 32;  // pairs of 16-channel pieces of K, 32-channel tiles of the output
@@ -88,7 +100,7 @@ __global__ __launch_bounds__(64 * kExtWaves, 2) void fp8_extend_kernel(Fp8Extend
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int lo = lane & 31, hf = lane >> 5;
-  const ExtendTile et = find_tile(a, t_lin);
+  const ExtendTile et = uniform_tile(find_tile(a, t_lin));
   const int64_t row_out = (int64_t)a.H * D;
   if (et.b < 0) {
     // rows of q past the requests' tokens have no answer: NaN, in 8-byte pieces, shared by the
@@ -124,14 +136,14 @@ __global__ __launch_bounds__(64 * kExtWaves, 2) void fp8_extend_kernel(Fp8Extend
   for (int i = 0; i < 2 * KI; ++i)
     qb[i] = *reinterpret_cast<const bf16x8_t*>(qp + ((i >> 1) * 2 + hf) * 16 + (i & 1) * 8);
 
-  const int32_t* bt = a.table + (int64_t)max(et.req, 0) * a.table_stride;
+  const scalar_words_t bt = (scalar_words_t)(uintptr_t)(a.table + (int64_t)max(et.req, 0) * a.table_stride);
+  const scalar_floats_t ksp = (scalar_floats_t)(uintptr_t)(a.c.ks + h), vsp = (scalar_floats_t)(uintptr_t)(a.c.vs + h);
   bool bad = et.req < 0;
-  // the scalars of a tile: its block's scales, and where its codes are
-  auto block_at = [&](int j) {
-    const int b = bt[j];
-    const bool ok = b > 0 && b < a.c.blocks;
+  // a tile's block; padding and ids outside the cache are read as padding, and spoil the answer
+  auto block_of_word = [&](int word) {
+    const bool ok = word > 0 && word < a.c.blocks;
     bad |= !ok;
-    return ok ? b : 0;
+    return ok ? word : 0;
   };
   auto load_tile = [&](int buf, int blk) {
     const int64_t at = ((int64_t)blk * a.KV + h) * kHead + wave * (kHead / 4) + lane * 16;
@@ -153,30 +165,37 @@ __global__ __launch_bounds__(64 * kExtWaves, 2) void fp8_extend_kernel(Fp8Extend
   // tile of 32, token groups hf and hf + 2
   const int k_off = (lo >> 4) * 16 * D + (lo & 15) * 16 + hf * 256;
   const int v_off = (lo >> 4) * 1024 + (lo & 15) * 16 + hf * 256;
-  int blk_next = 0, buf = 0;
+  int word = 0, buf = 0;  // the table's word of the tile after the one in flight
   float ks = 0.0f, vs = 0.0f, ks_next = 0.0f, vs_next = 0.0f;
   if (j_begin < j_end) {
-    const int blk = block_at(j_begin);
-    ks_next = a.c.ks[(int64_t)blk * a.KV + h];
-    vs_next = a.c.vs[(int64_t)blk * a.KV + h];
+    const int blk = block_of_word(bt[j_begin]);
+    ks_next = ksp[(int64_t)blk * a.KV];
+    vs_next = vsp[(int64_t)blk * a.KV];
     load_tile(0, blk);
-    if (j_begin + 1 < j_end) blk_next = block_at(j_begin + 1);
+    word = bt[min(j_begin + 1, j_end - 1)];
   }
   for (int j = j_begin; j < j_end; ++j) {
     ks = ks_next;
     vs = vs_next;
     tile_barrier();
     if (j + 1 < j_end) {
-      load_tile(buf ^ 1, blk_next);
-      ks_next = a.c.ks[(int64_t)blk_next * a.KV + h];
-      vs_next = a.c.vs[(int64_t)blk_next * a.KV + h];
-      if (j + 2 < j_end) blk_next = block_at(j + 2);
+      const int blk = block_of_word(word);
+      load_tile(buf ^ 1, blk);
+      ks_next = ksp[(int64_t)blk * a.KV];
+      vs_next = vsp[(int64_t)blk * a.KV];
+      word = bt[min(j + 2, j_end - 1)];
     }
     const unsigned char* sk = sm + buf * 2 * kHead + k_off;
     const unsigned char* sv = sm + buf * 2 * kHead + kHead + v_off;
     buf ^= 1;
     // S^T[token 32 t + 8 (i / 4) + 4 hf + i % 4][row lo] in s[t][i]
     float16_t s[2];
+    uint4 kw[2][KI], vw[NC][2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < KI; ++i) kw[t][i] = *reinterpret_cast<const uint4*>(sk + t * 32 * D + i * 512);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
 #pragma unroll
@@ -184,11 +203,19 @@ __global__ __launch_bounds__(64 * kExtWaves, 2) void fp8_extend_kernel(Fp8Extend
 #pragma unroll
       for (int i = 0; i < KI; ++i) {
         bf16x8_t k0, k1;
-        codes16(*reinterpret_cast<const uint4*>(sk + t * 32 * D + i * 512), k0, k1);
+        codes16(kw[t][i], k0, k1);
         s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k0, qb[2 * i], s[t], 0, 0, 0);
         s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k1, qb[2 * i + 1], s[t], 0, 0, 0);
       }
     }
+    // the values' codes arrive under the softmax
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int x = 0; x < NC; ++x) {
+      vw[x][0] = *reinterpret_cast<const uint4*>(sv + x * 2048);
+      vw[x][1] = *reinterpret_cast<const uint4*>(sv + x * 2048 + 512);
+    }
+    __builtin_amdgcn_sched_barrier(0);
     const bool edge = (j + 1) * kExtTile > lim_full;  // block-uniform: some row's limit is inside this tile
     const int left = lim - j * kExtTile - 4 * hf;
     if (edge) {
@@ -207,7 +234,7 @@ __global__ __launch_bounds__(64 * kExtWaves, 2) void fp8_extend_kernel(Fp8Extend
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[t][i]);
     mx = fmaxf(mx, lane_xor32(mx, lane)) * c;
     const int lv = vs != vs ? R : exponent_of(vs);
-    if (__any(mx > M) || lv > R) {
+    if (__any(mx > M + kSlack) || lv > R) {
       const float Mn = fmaxf(M, mx);
       const float am = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - Mn);
       const int Rn = max(R, lv);
@@ -239,7 +266,7 @@ __global__ __launch_bounds__(64 * kExtWaves, 2) void fp8_extend_kernel(Fp8Extend
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int i = 0; i < 16; ++i) sum += s[t][i];
-    L = __builtin_fmaf(sum, pow2f(-lift) / kRound, L);
+    L = __builtin_fmaf(sum, pow2f(-lift) * (1.0f / kRound), L);
     // O^T += V^T W^T, 16 tokens at a time
     u32x4_t wv[4];
 #pragma unroll
@@ -249,7 +276,7 @@ __global__ __launch_bounds__(64 * kExtWaves, 2) void fp8_extend_kernel(Fp8Extend
         wv[u][x] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(s[u >> 1][(u & 1) * 8 + 2 * x], s[u >> 1][(u & 1) * 8 + 2 * x + 1]));
 #pragma unroll
     for (int x = 0; x < NC; ++x) {
-      const uint4 va = *reinterpret_cast<const uint4*>(sv + x * 2048), vb = *reinterpret_cast<const uint4*>(sv + x * 2048 + 512);
+      const uint4 va = vw[x][0], vb = vw[x][1];
       const uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vb.x, vb.y, vb.z, vb.w};
 #pragma unroll
       for (int u = 0; u < 4; ++u)
