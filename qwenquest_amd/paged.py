@@ -187,6 +187,12 @@ class Fp8TokenToKVPool:
         self.v_codes = torch.zeros(codes, dtype=torch.uint8, device=self.device)
         self.k_scale = torch.full(codes[:3], 2.0**-110, dtype=torch.float32, device=self.device)
         self.v_scale = torch.full(codes[:3], 2.0**-110, dtype=torch.float32, device=self.device)
+        # one layer's codes and scales with the geometry, as the C entries take them; the tensors
+        # stay where they are
+        code_step, scale_step = self.k_codes.stride(0), self.k_scale.stride(0) * 4
+        base = [_lib.ptr(t) for t in (self.k_codes, self.v_codes, self.k_scale, self.v_scale)]
+        self._layers = [(base[0] + i * code_step, base[1] + i * code_step, base[2] + i * scale_step,
+                         base[3] + i * scale_step, num_blocks, kv_heads, head_dim) for i in range(num_layers)]
 
     @property
     def rows(self) -> int:
@@ -199,9 +205,7 @@ class Fp8TokenToKVPool:
         """One layer's codes and scales with the geometry, as the C entries take them."""
         if not 0 <= layer_id < self.num_layers:
             raise IndexError(f"layer {layer_id} of {self.num_layers}")
-        codes, scales = layer_id * self.k_codes.stride(0), layer_id * self.k_scale.stride(0) * 4
-        return (_lib.ptr(self.k_codes) + codes, _lib.ptr(self.v_codes) + codes, _lib.ptr(self.k_scale) + scales,
-                _lib.ptr(self.v_scale) + scales, self.num_blocks, self.kv_heads, self.head_dim)
+        return self._layers[layer_id]
 
     def new_rows(self, k: torch.Tensor, v: torch.Tensor, n: int) -> tuple[torch.Tensor, torch.Tensor]:
         """``k`` and ``v`` of n tokens as the C entries take them: one bf16 or fp32 type, dense,
@@ -212,7 +216,8 @@ class Fp8TokenToKVPool:
         for x in (k, v):
             if x.numel() != n * self.kv_heads * self.head_dim:
                 raise ValueError(f"expected {n} rows of {self.kv_heads} x {self.head_dim}, got {tuple(x.shape)}")
-            x = x.detach().reshape(n, self.kv_heads, self.head_dim).contiguous()
+            if not x.is_contiguous():
+                x = x.contiguous()
             out.append(x.clone() if x.data_ptr() % 16 else x)
         return out[0], out[1]
 
@@ -236,8 +241,7 @@ class Fp8TokenToKVPool:
         code = _lib.dtype_code(dtype)
         loc = _device_i64(loc, self.device, "loc")
         n = int(loc.numel())
-        k = torch.empty((n, self.kv_heads, self.head_dim), dtype=dtype, device=self.device)
-        v = torch.empty_like(k)
+        k, v = torch.empty((2, n, self.kv_heads, self.head_dim), dtype=dtype, device=self.device).unbind(0)
         if n:
             with _lib.on(self.device):
                 _lib.call("qq_fp8_rows", *self.layer_args(layer_id), _lib.ptr(loc), n, _lib.ptr(k), _lib.ptr(v), code,
