@@ -55,8 +55,10 @@ class BlockReqToTokenPool(ReqToTokenPool):
         super().__init__(size, max_context_len, _indexed(device))
         if self.device.type != "cuda":
             raise RuntimeError("qwenquest_amd.BlockReqToTokenPool needs a GPU device (no CPU path)")
-        if num_blocks < 1:
-            raise ValueError(f"num_blocks must be at least 1 (the padding block), got {num_blocks}")
+        if not 1 <= num_blocks <= 1 << 24:
+            raise ValueError(f"num_blocks must be at least 1 (the padding block) and at most 2^24, got {num_blocks}")
+        if not 1 <= size <= 1 << 18 or not 1 <= max_context_len < 1 << 30:
+            raise ValueError(f"at most 2^18 requests of under 2^30 tokens, got {size} of {max_context_len}")
         dev = self.device
         self.num_blocks = num_blocks
         self.max_blocks = (max_context_len + BLOCK_TOKENS - 1) // BLOCK_TOKENS
@@ -128,7 +130,7 @@ class BlockReqToTokenPool(ReqToTokenPool):
     def free(self, req_pool_idx: int) -> None:
         """Release the request's blocks, then its slot (memory.py:44-50)."""
         self.release(torch.tensor([req_pool_idx], dtype=torch.int64))
-        self._free_slots.append(req_pool_idx)
+        super().free(req_pool_idx)
 
     def check_errors(self, sync: bool = True) -> None:
         """Raise what a call refused on the device: RuntimeError when the blocks ran out, ValueError
@@ -175,8 +177,9 @@ class Fp8TokenToKVPool:
             raise RuntimeError("qwenquest_amd.Fp8TokenToKVPool needs a GPU device (no CPU path)")
         if head_dim not in (64, 128):
             raise ValueError(f"head_dim must be 64 or 128, got {head_dim}")
-        if num_blocks < 1 or num_layers < 1 or kv_heads < 1:
-            raise ValueError("num_blocks, num_layers and kv_heads must be at least 1")
+        if not 1 <= num_blocks <= 1 << 24 or num_layers < 1 or not 1 <= kv_heads <= 1024:
+            raise ValueError(f"num_blocks must be 1 .. 2^24, kv_heads 1 .. 1024 and num_layers at least 1, got {num_blocks}, "
+                             f"{kv_heads} and {num_layers}")
         self.num_blocks = num_blocks
         self.num_layers = num_layers
         self.kv_heads = kv_heads

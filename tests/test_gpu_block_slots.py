@@ -170,8 +170,9 @@ def test_arguments_are_checked(cuda):
         pool.assign_decode(two, two.float())
     with pytest.raises(ValueError, match="total"):
         pool.assign(one, one, one, -1)
-    with pytest.raises(ValueError, match="num_blocks"):
-        BlockReqToTokenPool(2, 500, 0, cuda)
+    for bad in ((2, 500, 0), (2, 500, (1 << 24) + 1), (0, 500, 4), ((1 << 18) + 1, 1, 4), (2, 0, 4), (2, 1 << 30, 4)):
+        with pytest.raises(ValueError):
+            BlockReqToTokenPool(*bad, cuda)
 
 
 def test_slots_and_blocks_come_back_together(cuda):

@@ -267,3 +267,39 @@ def test_paged_rows_serve_the_bf16_pool(cuda, backend):
         got.append(be.forward(rand(2, 16, 128), rand(2, 4, 128), rand(2, 4, 128), Layer(0, 128), batch))
         outs.append(got)
     assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
+def test_blocks_past_32_bit_offsets(cuda):
+    """A layer of more than 2^32 bytes of codes: its last blocks written, read, bounded and attended."""
+    from qwenquest_amd.attention.ops import fp8_decode_attention, fp8_extend_attention
+
+    kv, dim, blocks = 8, 128, 70_000  # 65536 bytes a block
+    pool = Fp8TokenToKVPool(blocks, 1, kv, dim, cuda)
+    assert pool.k_codes[0].numel() > 1 << 32
+    ids = [blocks - 1, 1, blocks - 2, blocks // 2]
+    table = torch.tensor([ids], dtype=torch.int32, device=cuda)
+    gen = torch.Generator(device=cuda).manual_seed(0)
+    loc = torch.tensor([b * 64 + t for b in ids for t in range(64)], device=cuda)
+    k, v = (torch.empty((256, kv, dim), device=cuda).normal_(generator=gen).to(torch.bfloat16) for _ in range(2))
+    pool.set_kv_buffer(0, loc, k, v)
+    cache = of.Cache(5, kv, dim)  # the same in small blocks
+    cache.write(torch.arange(64, 320).numpy(), k.float().cpu().numpy(), v.float().cpu().numpy())
+    kw, vw = cache.rows(np.arange(64, 320))
+    got = pool.get_rows(0, loc, torch.float32)
+    assert np.array_equal(got[0].cpu().numpy(), kw) and np.array_equal(got[1].cpu().numpy(), vw)
+    q = torch.empty((2, 16, dim), device=cuda).normal_(generator=gen).to(torch.bfloat16)
+    scale, n = dim**-0.5, 230
+    for out, row, seen in (
+            (fp8_decode_attention(q[:1], pool, 0, table, i64([0], cuda), i64([n], cuda), scale), q[0], n),
+            (fp8_extend_attention(q, pool, 0, table, i64([0], cuda), i64([n], cuda), i64([n - 2], cuda), i64([2], cuda), scale)[1:], q[1], n)):
+        want, spread, size = of.attend(row.double().cpu().numpy(), kw[:seen], vw[:seen], scale)
+        tol = of.attend_tolerance(want, spread, size, seen, dim, True, 12)
+        assert (np.abs(out[0].double().cpu().numpy().reshape(want.shape) - want) <= tol).all()
+    from qwenquest_amd.quest import QuestAlgorithm
+
+    quest = QuestAlgorithm(128, 64, cuda)
+    quest.init_storage(0, 1, 1, 256, kv, dim)
+    quest.update_prefill_representations_blocks(i64([0], cuda), i64([256], cuda), pool, table)
+    b = quest.page_k_bounds[0, 0].float().cpu().numpy()
+    pages = kw.reshape(4, 64, kv, dim)
+    assert np.array_equal(b[..., 0], pages.min(1)) and np.array_equal(b[..., 1], pages.max(1))
