@@ -464,7 +464,8 @@ int qq_fp8_page_bounds(const uint8_t* k_codes, int64_t codes_layer_stride, const
 
 /* One layer's decode over the 8-bit cache (src/qwenquest/attention/dense.py:26-42 and
  * quest_only.py:149-159 over it): with k_new the new tokens are stored first
- * (qq_fp8_store(k_new, v_new, out_cache_loc), [bs, kv_heads, head_dim] new_dtype); then
+ * (qq_fp8_store(k_new, v_new, out_cache_loc), [bs, kv_heads, head_dim] new_dtype; each in the last
+ * block of its own request's context, or in none); then
  * request i's q[i] ([bs, H, head_dim] bf16 or fp32, 16-byte aligned, batch stride a multiple
  * of 8 elements) attends positions 0 .. seq_lens[i] - 1, or with `positions` and
  * seq_lens[i] > top_k the pages positions[i, 64 u] / 64, u < top_k / 64 - 1, and the last 64
@@ -480,8 +481,17 @@ int qq_fp8_decode_attention(const void* q, int q_dtype, int64_t q_batch_stride, 
                             int block_table_rows, int block_table_cols, const int64_t* req_pool_indices,
                             const int64_t* seq_lens, int bs, const int32_t* positions, int64_t positions_stride,
                             int top_k, float scale, void* out, void* workspace, int64_t workspace_bytes,
-                            void* stream);
+                            int planned, void* stream);
 int64_t qq_fp8_decode_workspace_bytes(int bs, int num_q_heads, int kv_heads, int head_dim);
+
+/* The part of qq_fp8_decode_attention that depends on a step's lengths alone, once for its layers:
+ * divides the batch into `workspace` (>= qq_fp8_decode_workspace_bytes(bs, kv_heads, kv_heads,
+ * head_dim)), with which calls for the same requests, lengths, table and cache geometry, without
+ * positions, on the same stream pass planned != 0 and run as one launch each, at up to 16 query
+ * heads per KV head (others as without a plan, with a workspace of their own size). */
+int qq_fp8_decode_plan(int num_blocks, int kv_heads, int head_dim, int block_table_rows, int block_table_cols,
+                       const int64_t* req_pool_indices, const int64_t* seq_lens, int bs, void* workspace,
+                       int64_t workspace_bytes, void* stream);
 
 /* QuestOnlyBackend.forward_decode (src/qwenquest/attention/quest_only.py:132-159) for one layer
  * over the 8-bit cache: page scores and selection from page_k_bounds (as qq_quest_retrieve_topk,

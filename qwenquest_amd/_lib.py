@@ -116,8 +116,9 @@ SIGNATURES: dict[str, tuple] = {
     "qq_fp8_decode_attention": (
         _I,
         [_P, _I, _L, _I, _P, _P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _P, _L, _I, _I, _P, _P, _I, _P, _L, _I, _F,
-         _P, _P, _L, _P],
+         _P, _P, _L, _I, _P],
     ),
+    "qq_fp8_decode_plan": (_I, [_I, _I, _I, _I, _I, _P, _P, _I, _P, _L, _P]),
     "qq_fp8_decode_workspace_bytes": (_L, [_I, _I, _I, _I]),
     "qq_fp8_quest_step": (
         _I,

@@ -7,7 +7,7 @@ the new K/V store, then the attention kernel of the Quest layer step over all
 of a request's rows); other shapes store the new K/V and run the split-K
 attention over the explicit row list ``req_to_token[req, :seq_len]``.  Over an 8-bit pool
 (``Fp8TokenToKVPool``) one C call does both for every shape the pool takes
-(``qq_fp8_decode_attention``).
+(``qq_fp8_decode_attention``), after ``init_forward_metadata`` as one launch.
 """
 
 from __future__ import annotations
@@ -18,7 +18,12 @@ import torch
 
 from qwenquest_amd import _lib
 from qwenquest_amd.attention.base import AttentionBackend
-from qwenquest_amd.attention.ops import AttentionWorkspace, decode_attention_rows, fp8_decode_attention
+from qwenquest_amd.attention.ops import (
+    AttentionWorkspace,
+    decode_attention_rows,
+    fp8_decode_attention,
+    fp8_decode_plan,
+)
 
 if TYPE_CHECKING:
     from qwenquest_amd.batch import ForwardBatch
@@ -45,6 +50,13 @@ class DenseBackend(AttentionBackend):
         return (q3.dtype == torch.bfloat16 and pool.dtype == torch.bfloat16 and pool.kv_heads == 4
                 and pool.head_dim == 128 and heads % 4 == 0 and heads // 4 <= 16)
 
+    def init_forward_metadata(self, batch: ForwardBatch) -> None:
+        """Over an 8-bit pool: the step's division of the decode batch, for all of its layers.  It stays
+        with the batch, whose requests and lengths it is of."""
+        if self.fp8 and batch.forward_mode.is_decode():
+            batch.decode_plan = fp8_decode_plan(self.token_to_kv_pool, self.req_to_token_pool.block_table,
+                                                batch.req_pool_indices, batch.seq_lens)
+
     def forward_decode(self, q, k, v, layer, batch: ForwardBatch) -> torch.Tensor:
         """dense.py:26-42: set_kv_buffer, then attention over req_to_token[req, :seq_len]."""
         assert batch.out_cache_loc is not None
@@ -55,7 +67,7 @@ class DenseBackend(AttentionBackend):
         if self.fp8:
             return fp8_decode_attention(q3, pool, layer.layer_id, self.req_to_token_pool.block_table,
                                         batch.req_pool_indices, batch.seq_lens, layer.scaling,
-                                        new=(batch.out_cache_loc, k, v))
+                                        new=(batch.out_cache_loc, k, v), plan=batch.decode_plan)
         heads = q3.shape[1]
         rpi = batch.req_pool_indices.to(device=q3.device, dtype=torch.int64).contiguous()
         seq = batch.seq_lens.to(device=q3.device, dtype=torch.int64).contiguous()

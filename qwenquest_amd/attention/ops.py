@@ -9,7 +9,7 @@ device, in float32.
 
 from __future__ import annotations
 
-from typing import TYPE_CHECKING
+from typing import TYPE_CHECKING, NamedTuple
 
 import torch
 import torch.nn.functional as F
@@ -244,6 +244,30 @@ def _queries(q: torch.Tensor, pool: Fp8TokenToKVPool) -> torch.Tensor:
     return q.clone() if q.data_ptr() % 16 else q
 
 
+class Fp8DecodePlan(NamedTuple):
+    """A decode batch of ``bs`` requests divided for the chip (``fp8_decode_plan``)."""
+
+    bs: int
+    workspace: torch.Tensor
+
+
+def fp8_decode_plan(pool: Fp8TokenToKVPool, block_table: torch.Tensor, req_pool_indices: torch.Tensor,
+                    seq_lens: torch.Tensor) -> Fp8DecodePlan:
+    """What ``fp8_decode_attention`` over whole contexts makes of a step's lengths, once for the step's
+    layers, on the current stream."""
+    dev = pool.device
+    bs = int(req_pool_indices.shape[0])
+    bt = _block_table(block_table, dev)
+    rpi = _lengths(req_pool_indices, bs, dev, "req_pool_indices")
+    seq = _lengths(seq_lens, bs, dev, "seq_lens")
+    need = int(_lib.load().qq_fp8_decode_workspace_bytes(bs, pool.kv_heads, pool.kv_heads, pool.head_dim))
+    ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+    with _lib.on(dev):
+        _lib.call("qq_fp8_decode_plan", pool.num_blocks, pool.kv_heads, pool.head_dim, bt.shape[0], bt.shape[1],
+                  _lib.ptr(rpi), _lib.ptr(seq), bs, _lib.ptr(ws), need, _lib.stream(dev))
+    return Fp8DecodePlan(bs, ws)
+
+
 def fp8_decode_attention(
     q: torch.Tensor,
     pool: Fp8TokenToKVPool,
@@ -256,11 +280,15 @@ def fp8_decode_attention(
     positions: torch.Tensor | None = None,
     top_k: int = 0,
     new: tuple[torch.Tensor, torch.Tensor, torch.Tensor] | None = None,
+    plan: Fp8DecodePlan | None = None,
 ) -> torch.Tensor:
     """Decode over an 8-bit pool: request ``i`` attends ``q[i] [H, D]`` over its first ``seq_lens[i]``
     tokens in the blocks ``block_table[req_pool_indices[i]]``, or, with ``positions [bs, >= top_k]``
     (``QuestAlgorithm.retrieve_topk``) and a longer context than ``top_k``, over the pages listed
-    there and the last 64 tokens.  ``new``: ``(loc, k, v)`` of the batch's new tokens, stored first.
+    there and the last 64 tokens.  ``new``: ``(loc, k, v)`` of the batch's new tokens, stored first,
+    each in the last block of its own request's context (or in the void block 0).  ``plan``: this
+    step's ``fp8_decode_plan`` (of the same pool, table, requests and lengths, on the same stream; not
+    with ``positions``): up to 16 query heads per KV head then run as one launch.
     Returns ``[bs, H*D]`` in q's dtype (bf16 or fp32): zeros for an empty context, NaN for a request
     outside the table or a context past its blocks."""
     dev = pool.device
@@ -278,17 +306,24 @@ def fp8_decode_attention(
         loc = _lengths(new[0], bs, dev, "out_cache_loc")
         kn, vn = pool.new_rows(new[1], new[2], bs)
     out = torch.empty((bs, heads * dim), dtype=q.dtype, device=dev)
+    if plan is not None and positions is not None:
+        raise ValueError("a plan is of whole contexts, not of selected pages")
     need = int(_lib.load().qq_fp8_decode_workspace_bytes(bs, heads, pool.kv_heads, dim))
-    # of this call alone: it holds the division of the batch, which a graph's replay or a call on
-    # another stream must not find replaced
-    ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+    if plan is not None and heads <= 16 * pool.kv_heads:
+        ws = plan.workspace
+        if plan.bs != bs or ws.device != dev or ws.numel() != max(need, 1):
+            raise ValueError("plan is not fp8_decode_plan's of this batch and pool")
+    else:
+        # of this call alone: it holds the division of the batch, which a graph's replay or a call on
+        # another stream must not find replaced
+        ws, plan = torch.empty(max(need, 1), dtype=torch.uint8, device=dev), None
     with _lib.on(dev):
         _lib.call(
             "qq_fp8_decode_attention", _lib.ptr(q), _lib.dtype_code(q.dtype), q.stride(0), heads, _lib.ptr(kn),
             _lib.ptr(vn), _lib.DTYPE_BF16 if kn is None else _lib.dtype_code(kn.dtype), _lib.ptr(loc),
             *pool.layer_args(layer_id), *_table_args(bt), _lib.ptr(rpi), _lib.ptr(seq), bs, _lib.ptr(positions),
             0 if positions is None else max(positions.stride(0), positions.shape[1]), int(top_k), float(scaling),
-            _lib.ptr(out), _lib.ptr(ws), need, _lib.stream(dev),
+            _lib.ptr(out), _lib.ptr(ws), need, int(plan is not None), _lib.stream(dev),
         )
     return out
 

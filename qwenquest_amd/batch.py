@@ -40,6 +40,8 @@ class ForwardBatch:
     attn_backend: Any
     extend_prefix_lens: torch.Tensor | None = None
     extend_seq_lens: torch.Tensor | None = None
+    #: set by a backend's init_forward_metadata: a decode step's work, divided once for its layers
+    decode_plan: Any = None
 
     @property
     def batch_size(self) -> int:

@@ -10,7 +10,9 @@
 // of 16 query heads), so that any mix of lengths fills the chip evenly in one round; a
 // request that lies in one slice is finished there, the others' (m, l, o) parts are merged by
 // the block that completes them.  Two launches: fp8_begin_kernel cuts the slices and stores the
-// new tokens, fp8_attend_kernel does the rest.
+// new tokens, fp8_attend_kernel does the rest.  The slices depend on the lengths alone: cut once
+// for a step (fp8_plan_kernel), its layers are one launch each, in which the wave that has a
+// request's last block stores the request's new token into it first.
 //
 // Of its block's slice a wave takes an eighth, units in a row, and goes through their requests on
 // its own; what a request's end finds in one wave is written by that wave, the rest meets in the
@@ -33,7 +35,7 @@ constexpr int kDecWaves = 8;
 constexpr int kDecParts = rules::kFp8Parts;  // slices of a request, at most: the merge's table of weights
 
 struct DecPlan {
-  int32_t total, len, slices, pad;  // units of the batch, units of a slice, slices
+  int32_t total, len, slices, bs;  // units of the batch, units of a slice, slices, requests
 };
 struct DecItem {  // a slice's first request: its units are [c0, c1) of the batch's
   int32_t b, c0, c1, seq;
@@ -60,7 +62,7 @@ struct DecArgs {
   DecPlan* plan;
   int32_t* cu;       // [bs + 1] units before each request
   DecItem* items;    // [max_slices]
-  uint32_t* done;    // [max_slices, heads] parts finished of the request that goes on behind a slice
+  uint32_t* done;    // [max_slices, heads] parts finished of the request that goes on behind a slice; left 0
   float* part_o;     // [max_slices, 2, heads, 16, D]
   float* part_ml;    // [max_slices, 2, heads, 16, 2]
 };
@@ -113,7 +115,7 @@ __device__ inline void plan_slices(const DecArgs& a) {
   longest = max(max(s_long[0], s_long[1]), max(s_long[2], s_long[3]));
   const int len = rules::fp8_slice_len(base, longest, a.max_slices);
   const int slices = (base + len - 1) / len;
-  if (tid == 0) *a.plan = {base, len, slices, 0};
+  if (tid == 0) *a.plan = {base, len, slices, a.bs};
   for (int i = tid; i < slices; i += 256) {
     const int at = i * len;
     int lo = 0, hi = a.bs;  // the last request that begins at or before this unit
@@ -125,6 +127,8 @@ __device__ inline void plan_slices(const DecArgs& a) {
     a.items[i] = {lo, a.cu[lo], a.cu[lo + 1], context_of(a, lo), table_row(a, lo), {0, 0, 0}};
   }
 }
+
+__global__ __launch_bounds__(256) void fp8_plan_kernel(DecArgs a) { plan_slices(a); }
 
 // Block 0: the slices; then a block per request that selects its pages (KPT > 0: scores per
 // thread), and a block per new token, head, and K or V.
@@ -313,7 +317,7 @@ __device__ inline void merge_parts(const DecArgs& a, DecSmem& sm, int head, int 
 }
 
 template <int D, typename T>
-__global__ __launch_bounds__(64 * kDecWaves, 2) void fp8_attend_kernel(DecArgs a) {
+__global__ __launch_bounds__(64 * kDecWaves, 2) void fp8_attend_kernel(DecArgs a, StoreArgs st) {
   constexpr int QP = sizeof(T) == 2 ? 1 : 3, PP = sizeof(T) == 2 ? 2 : 3;  // pieces of q and of the weights
   constexpr int KL = D / 64, VL = D / 16;  // 16-byte loads a lane: per 16 tokens of K, per block of V
   constexpr int RF = dec_row_floats(D);
@@ -323,7 +327,7 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void fp8_attend_kernel(DecArgs a
   const int head = blockIdx.x % a.heads, slice = blockIdx.x / a.heads;
   const DecPlan plan = *a.plan;
   const DecItem item = a.items[slice];  // both in one round trip; stale past the last slice
-  if (slice >= plan.slices) return;
+  if (slice >= plan.slices || plan.bs != a.bs) return;  // a plan of another batch answers nothing
   const int h = head / a.tiles, tile = head - h * a.tiles;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int m16 = lane & 15, g = lane >> 4;
@@ -334,6 +338,22 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void fp8_attend_kernel(DecArgs a
   const int s0 = at + (int)((int64_t)(end - at) * wave / kDecWaves), s1 = at + (int)((int64_t)(end - at) * (wave + 1) / kDecWaves);
   const int picked = a.top_k / 64 - 1;  // selected pages; the unit after them is the window
   if (lane < 2) sm.b[2 * wave + lane] = -1;
+
+  // New tokens of the requests that end among this wave's units, each in its request's last block,
+  // which no other wave of this head reads.
+  if (st.k && s1 >= item.c1) {
+    bool more = true;
+    for (int r0 = item.b; more; r0 += 64) {
+      const int r = r0 + lane;
+      int c1 = 0x7FFFFFFF;
+      if (r == item.b) c1 = item.c1;
+      else if (s1 > item.c1 && r < a.bs) c1 = a.cu[r + 1];
+      for (uint64_t tails = __ballot(c1 > s0 && c1 <= s1); tails; tails &= tails - 1)
+        store_token<D>(st, r0 + __builtin_ctzll(tails), h);
+      more = __builtin_amdgcn_readlane(c1, 63) < s1;
+    }
+    wait_memory();
+  }
 
   // Of unit u0 + lane: its request, place in it, block and scales; a window has two blocks.  64 units
   // belong to 64 requests at most, from request rb on.
@@ -350,10 +370,11 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void fp8_attend_kernel(DecArgs a
       u_c1 = item.c1;
       u_seq = item.seq;
     } else {
-      int begins;  // unit where request rb + lane begins
+      int begins, ends;  // units of request rb + lane
       for (;;) {
         const int r = rb + lane;
         begins = r <= a.bs ? a.cu[r] : 0x7FFFFFFF;
+        ends = r < a.bs ? a.cu[r + 1] : 0x7FFFFFFF;
         const int skip = __popcll(__ballot(begins <= u0)) - 1;  // those that begin before: a run of lanes from 0
         if (skip == 0) break;
         rb += skip;
@@ -370,7 +391,7 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void fp8_attend_kernel(DecArgs a
       u_c0 = __shfl(begins, i, 64);
       u_seq = __shfl(my_seq, i, 64);
       row = __shfl(my_row, i, 64);
-      u_c1 = u_c0 + units_of(a, u_seq);
+      u_c1 = __shfl(ends, i, 64);
     }
     blk = blk2 = 0;
     u_bad = row < 0;
@@ -636,7 +657,11 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void fp8_attend_kernel(DecArgs a
     const int c0 = x ? next_c0 : item.c0, c1 = x ? next_c1 : item.c1;
     const int first_slice = c0 / plan.len, parts = (c1 - 1) / plan.len - first_slice + 1;
     __syncthreads();
-    if (tid == 0) sm.last = add_agent(&a.done[first_slice * a.heads + head], 1u) == (uint32_t)parts - 1;
+    if (tid == 0) {
+      uint32_t* done = &a.done[first_slice * a.heads + head];
+      sm.last = add_agent(done, 1u) == (uint32_t)parts - 1;
+      if (sm.last) st_agent(done, 0u);  // for the step's next layer
+    }
     __syncthreads();
     if (sm.last)
       merge_parts<D, T>(a, sm, head, first_slice, parts, rows, static_cast<T*>(a.out) + ((int64_t)b * a.H + q_head) * D);
@@ -671,7 +696,7 @@ void begin(const DecArgs& a, const StoreArgs& st, const SelectArgs& sel, hipStre
 
 // LDS past the 64 KiB default (tiles of more than 15 heads of 128): opted in once per device.
 template <int D, typename T>
-void attend(const DecArgs& a, hipStream_t s) {
+void attend(const DecArgs& a, const StoreArgs& st, hipStream_t s) {
   const size_t bytes = dec_smem_bytes(min(a.G, kTile), D);
   if (bytes > 64 * 1024) {
     static bool opted[64] = {false};
@@ -682,14 +707,17 @@ void attend(const DecArgs& a, hipStream_t s) {
       opted[dev] = true;
     }
   }
-  fp8_attend_kernel<D, T><<<a.max_slices * a.heads, 64 * kDecWaves, bytes, s>>>(a);
+  fp8_attend_kernel<D, T><<<a.max_slices * a.heads, 64 * kDecWaves, bytes, s>>>(a, st);
 }
 
-// `sel`: with k_sel > 0 the pages are selected first, from scores that are there.
+// `sel`: with k_sel > 0 the pages are selected first, from scores that are there.  planned: the
+// workspace holds the slices, and nothing of another head tile waits for the new tokens.
 template <int D>
-void launch(const DecArgs& a, const StoreArgs& st, const SelectArgs& sel, int q_dtype, hipStream_t s) {
+void launch(const DecArgs& a, const StoreArgs& st, const SelectArgs& sel, bool planned, int q_dtype, hipStream_t s) {
   const int n = max(sel.MP, sel.k_sel);
-  if (!sel.positions) begin<D, 0>(a, st, sel, s);
+  StoreArgs in{};  // what is left to store for the attention
+  if (planned) in = st;
+  else if (!sel.positions) begin<D, 0>(a, st, sel, s);
   else if (sel.k_sel <= 64 && n <= 4 * 256) begin<D, 4>(a, st, sel, s);
   else if (sel.k_sel <= 64 && n <= 9 * 256) begin<D, 9>(a, st, sel, s);
   else if (sel.k_sel <= 64 && n <= 16 * 256) begin<D, 16>(a, st, sel, s);
@@ -697,8 +725,8 @@ void launch(const DecArgs& a, const StoreArgs& st, const SelectArgs& sel, int q_
     launch_select(sel, a.bs, sel.MP, sel.k_sel, s);
     begin<D, 0>(a, st, sel, s);
   }
-  if (q_dtype == QQ_DTYPE_BF16) attend<D, uint16_t>(a, s);
-  else attend<D, float>(a, s);
+  if (q_dtype == QQ_DTYPE_BF16) attend<D, uint16_t>(a, in, s);
+  else attend<D, float>(a, in, s);
 }
 
 // Everything of a call but its launches; `what` refuses.
@@ -778,7 +806,8 @@ extern "C" int qq_fp8_decode_attention(const void* q, int q_dtype, int64_t q_bat
                                        int64_t block_table_stride, int block_table_rows, int block_table_cols,
                                        const int64_t* req_pool_indices, const int64_t* seq_lens, int bs,
                                        const int32_t* positions, int64_t positions_stride, int top_k, float scale,
-                                       void* out, void* workspace, int64_t workspace_bytes, void* stream) {
+                                       void* out, void* workspace, int64_t workspace_bytes, int planned,
+                                       void* stream) {
   const char* what = "qq_fp8_decode_attention";
   DecArgs a{};
   StoreArgs st{};
@@ -787,9 +816,31 @@ extern "C" int qq_fp8_decode_attention(const void* q, int q_dtype, int64_t q_bat
                           block_table_stride, block_table_rows, block_table_cols, req_pool_indices, seq_lens, bs, positions,
                           positions_stride, top_k, scale, out, workspace, workspace_bytes);
   if (ok != QQ_OK || bs == 0) return ok;
+  QQ_REQUIRE(!planned || !positions, "%s: a plan is of whole contexts, not of selected pages", what);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (head_dim == 128) launch<128>(a, st, SelectArgs{}, q_dtype, s);
-  else launch<64>(a, st, SelectArgs{}, q_dtype, s);
+  const bool one = planned && a.tiles == 1;
+  if (head_dim == 128) launch<128>(a, st, SelectArgs{}, one, q_dtype, s);
+  else launch<64>(a, st, SelectArgs{}, one, q_dtype, s);
+  return check_launch(what);
+}
+
+extern "C" int qq_fp8_decode_plan(int num_blocks, int kv_heads, int head_dim, int block_table_rows, int block_table_cols,
+                                  const int64_t* req_pool_indices, const int64_t* seq_lens, int bs, void* workspace,
+                                  int64_t workspace_bytes, void* stream) {
+  const char* what = "qq_fp8_decode_plan";
+  // what the slices do not depend on stands in for itself
+  uint8_t* any = reinterpret_cast<uint8_t*>(workspace);
+  float* any_scale = static_cast<float*>(workspace);
+  DecArgs a{};
+  StoreArgs st{};
+  QQ_REQUIRE(bs <= 0 || workspace, "%s: null pointer", what);
+  if (bs == 0) return QQ_OK;
+  const int ok = set_args(a, st, what, any, QQ_DTYPE_BF16, 0, kv_heads, nullptr, nullptr, QQ_DTYPE_BF16, nullptr,
+                          {any, any, any_scale, any_scale, num_blocks, kv_heads, head_dim},
+                          static_cast<const int32_t*>(workspace), block_table_cols, block_table_rows, block_table_cols,
+                          req_pool_indices, seq_lens, bs, nullptr, 0, 0, 1.0f, workspace, workspace, workspace_bytes);
+  if (ok != QQ_OK) return ok;
+  fp8_plan_kernel<<<1, 256, 0, static_cast<hipStream_t>(stream)>>>(a);
   return check_launch(what);
 }
 
@@ -845,7 +896,7 @@ extern "C" int qq_fp8_quest_step(const void* q, int q_dtype, int64_t q_batch_str
   } else {
     sel = SelectArgs{};  // phase 1 left the positions
   }
-  if (head_dim == 128) launch<128>(a, st, sel, q_dtype, s);
-  else launch<64>(a, st, sel, q_dtype, s);
+  if (head_dim == 128) launch<128>(a, st, sel, false, q_dtype, s);
+  else launch<64>(a, st, sel, false, q_dtype, s);
   return check_launch(what);
 }

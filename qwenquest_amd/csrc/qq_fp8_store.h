@@ -236,5 +236,81 @@ __device__ inline void store_segment(const StoreArgs& a, StoreSmem<D>& sm, int64
   }
 }
 
+// One entry by one wave, K in its first D / 8 lanes and V in the next ones: what store_segment does
+// for a run of one entry.  Its writes are under way when it returns.
+template <int D>
+__device__ inline void store_token(const StoreArgs& a, int64_t i, int h) {
+  constexpr int DG = D / 8;
+  const int lane = threadIdx.x & 63, dg = lane % DG;
+  const bool mine = lane < 2 * DG, isv = lane >= DG;
+  const int64_t row = a.loc[i];
+  const int block = block_of(row, a.c.blocks), t = (int)(row & 63);
+  if (block == 0) return;  // wave-uniform
+  const int64_t at = (int64_t)block * a.c.KV + h, from = ((int64_t)i * a.c.KV + h) * D + dg * 8;
+  uint8_t *kc = a.c.kc + at * (64 * D), *vc = a.c.vc + at * (64 * D);
+  float* scale = (isv ? a.c.vs : a.c.ks) + at;
+  const float before = *scale;
+  float x[8];
+  if (a.dtype == QQ_DTYPE_BF16) {
+    Values8<uint16_t> v;
+    v.load(isv ? a.v : a.k, from);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = v[j];
+  } else {
+    Values8<float> v;
+    v.load(isv ? a.v : a.k, from);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = v[j];
+  }
+  const bool begun = t == 0;
+  float m = 0.0f;
+  bool bad = false;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const bool ok = is_finite(x[j]);
+    bad |= !ok;
+    x[j] = ok ? x[j] : 0.0f;
+    m = fmaxf(m, fabsf(x[j]));
+  }
+#pragma unroll
+  for (int d = DG / 2; d >= 1; d >>= 1) {
+    m = fmaxf(m, __shfl_xor(m, d, 64));
+    bad |= (bool)__shfl_xor((int)bad, d, 64);
+  }
+  const bool lost = !begun && before != before;
+  const int e_old = begun || lost ? kScaleMin : exponent_of(before);
+  const int e = max(e_old, scale_exponent(m));
+  const float inv = pow2f(-e);
+  const uint32_t lo = encode4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+  const uint32_t hi = encode4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
+  // the block's other codes: void, or rounded again
+  const float f = begun ? 0.0f : e > e_old ? pow2f(max(e_old - e, -126)) : 1.0f;
+  bool whole = false;
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const float fc = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), c ? DG : 0));
+    if (fc == 1.0f) continue;
+    whole = true;
+    uint8_t* codes = c ? vc : kc;
+    for (int q = lane; q < 4 * D; q += 64) {
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (fc != 0.0f) {
+        w = *reinterpret_cast<const uint4*>(codes + q * 16);
+        w = make_uint4(rescale4(w.x, fc), rescale4(w.y, fc), rescale4(w.z, fc), rescale4(w.w, fc));
+      }
+      *reinterpret_cast<uint4*>(codes + q * 16) = w;
+    }
+  }
+  if (whole) __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the entry's own codes come after them
+  if (!mine) return;
+  if (dg == 0) *scale = bad || lost ? __builtin_nanf("") : pow2f(e);
+  if (!isv) {
+    *reinterpret_cast<uint2*>(kc + k_offset(D, t, dg * 8)) = make_uint2(lo, hi);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) vc[v_offset(t, dg * 8 + j)] = (uint8_t)((j < 4 ? lo : hi) >> (8 * (j & 3)));
+  }
+}
+
 }  // namespace
 }  // namespace qq

@@ -105,12 +105,23 @@ def test_page_bounds_refuses(lib, kw, said):
     (dict(tstride=3), b"bad sizes"), (dict(trows=0), b"bad sizes"), (dict(pos=FAKE, top_k=100), b"multiple"),
     (dict(pos=FAKE, top_k=128, pstride=64), b"multiple"), (dict(q=None), b"null"), (dict(out=None), b"null"),
     (dict(q=ctypes.c_void_p(4104)), b"aligned"), (dict(qst=4100), b"aligned"), (dict(bytes=64), b"workspace"),
-    (dict(bs=1 << 20, tcols=1 << 24, tstride=1 << 24), b"units")])
+    (dict(bs=1 << 20, tcols=1 << 24, tstride=1 << 24), b"units"), (dict(planned=1, pos=FAKE, top_k=128, pstride=128), b"whole")])
 def test_decode_refuses(lib, kw, said):
     a = dict(q=FAKE, qd=0, qst=4096, H=32, kn=None, vn=None, nd=0, loc=None, **CACHE, table=FAKE, tstride=4, trows=2, tcols=4,
-             rpi=FAKE, seq=FAKE, bs=2, pos=None, pstride=0, top_k=0, scale=0.1, out=FAKE, ws=FAKE, bytes=1 << 30)
+             rpi=FAKE, seq=FAKE, bs=2, pos=None, pstride=0, top_k=0, scale=0.1, out=FAKE, ws=FAKE, bytes=1 << 30,
+             planned=0)
     a.update(kw)
     refused(lib.qq_fp8_decode_attention(*a.values(), None), lib, said)
+
+
+@pytest.mark.parametrize("kw, said", [
+    (dict(blocks=0), b"blocks"), (dict(kv=0), b"KV heads"), (dict(dim=80), b"head_dim"), (dict(trows=0), b"bad sizes"),
+    (dict(tcols=0), b"bad sizes"), (dict(bs=-1), b"bad sizes"), (dict(rpi=None), b"null"), (dict(seq=None), b"null"),
+    (dict(ws=None), b"null"), (dict(bytes=64), b"workspace"), (dict(bs=1 << 20, tcols=1 << 24), b"units")])
+def test_decode_plan_refuses(lib, kw, said):
+    a = dict(blocks=5, kv=4, dim=128, trows=2, tcols=4, rpi=FAKE, seq=FAKE, bs=2, ws=FAKE, bytes=1 << 30)
+    a.update(kw)
+    refused(lib.qq_fp8_decode_plan(*a.values(), None), lib, said)
 
 
 @pytest.mark.parametrize("kw, said", BAD_CACHE + [

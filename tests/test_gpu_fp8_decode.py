@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from oracle import fp8_cache as of
-from qwenquest_amd.attention.ops import fp8_decode_attention
+from qwenquest_amd.attention.ops import fp8_decode_attention, fp8_decode_plan
 from qwenquest_amd.paged import Fp8TokenToKVPool
 
 pytestmark = pytest.mark.gpu
@@ -226,6 +226,55 @@ def test_new_tokens_are_stored_and_attended(cuda):
     want.pool.set_kv_buffer(want.layer, loc, k, v)
     assert torch.equal(s.pool.k_codes, want.pool.k_codes) and torch.equal(s.pool.v_scale, want.pool.v_scale)
     s.check(out, q, 0.1)
+
+
+@pytest.mark.parametrize("heads, kv, dim, dtype, lens", [
+    (32, 4, 128, torch.bfloat16, [1, 64, 65, 128, 0, 700, 4097, 5000, 2]), (3, 3, 64, torch.float32, [129, 192, 1, 1000]),
+    (16, 1, 128, torch.float32, [1 + i % 70 for i in range(600)]), (34, 2, 64, torch.bfloat16, [100, 64, 1]),
+    (4, 1, 64, torch.bfloat16, [1 + i * 37 % 65 for i in range(2500)]), (8, 4, 128, torch.bfloat16, [20000]),
+    (8, 4, 128, torch.bfloat16, [64 * 40] * 48)])
+def test_a_step_divided_once_for_its_layers(cuda, heads, kv, dim, dtype, lens):
+    """Layers of one plan leave the cache and the answers, to the bit, that calls without one do: new
+    tokens that begin a block, make its scale grow, are not finite or are nobody's (block 0)."""
+    ours, want = (Setup(cuda, lens, kv, dim, seed=7, layer=1) for _ in range(2))
+    n, reqs = i64(lens, cuda), torch.arange(len(lens), device=cuda)
+    loc = torch.cat([s_rows for s_rows in (ours.rows(r, [max(m, 1) - 1]) for r, m in enumerate(lens))])
+    loc[2::11] = 0
+    gen = torch.Generator(device=cuda).manual_seed(3)
+    for step in range(3):  # the same division three times over
+        plan = fp8_decode_plan(ours.pool, ours.table, reqs, n) if step != 1 else plan
+        for layer in (0, 1):  # layer 0: nothing there yet
+            q = ours.queries(heads, dtype, 10 * step + layer)
+            k, v = (torch.randn(len(lens), kv, dim, device=cuda, generator=gen) for _ in range(2))
+            k[::3] *= 2.0 ** (3 * step)
+            v[1::4] *= 2.0 ** (3 * step)
+            k[5::13, 0, 3], v[7::17, kv - 1, 60] = float("nan"), float("inf")
+            k, v = k.to(dtype), v.to(dtype)
+            a = fp8_decode_attention(q, ours.pool, layer, ours.table, reqs, n, 0.1, new=(loc, k, v), plan=plan)
+            b = fp8_decode_attention(q, want.pool, layer, want.table, reqs, n, 0.1, new=(loc, k, v))
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8)) or torch.equal(a.isnan(), b.isnan())
+            assert torch.equal(a.nan_to_num(), b.nan_to_num())
+            for x in ("k_codes", "v_codes", "k_scale", "v_scale"):
+                assert torch.equal(getattr(ours.pool, x)[layer].view(torch.uint8)[1:], getattr(want.pool, x)[layer].view(torch.uint8)[1:]), x
+    a = fp8_decode_attention(q, ours.pool, 1, ours.table, reqs, n, 0.1, plan=plan)  # nothing to store
+    assert torch.equal(a.nan_to_num(), b.nan_to_num())
+
+
+def test_a_plan_is_checked(cuda):
+    s = Setup(cuda, [100, 100], 2, 64)
+    q, r, n = s.queries(4, torch.bfloat16), torch.arange(2), i64([100, 100], cuda)
+    plan = fp8_decode_plan(s.pool, s.table, r, n)
+    others = i64(range(3), cuda) % 2
+    more = fp8_decode_plan(s.pool, s.table, others, n[:1].repeat(3))
+    wider = fp8_decode_plan(Setup(cuda, [100, 100], 4, 64).pool, s.table, r, n)
+    for bad in (more, wider, plan._replace(workspace=plan.workspace.cpu())):
+        with pytest.raises(ValueError, match="plan"):
+            fp8_decode_attention(q, s.pool, s.layer, s.table, r, n, 0.1, plan=bad)
+    with pytest.raises(ValueError, match="selected pages"):
+        fp8_decode_attention(q, s.pool, s.layer, s.table, r, n, 0.1, plan=plan, top_k=64,
+                             positions=torch.zeros(2, 64, dtype=torch.int32, device=cuda))
+    s.check(fp8_decode_attention(q, s.pool, s.layer, s.table, r, n, 0.1, plan=plan), q, 0.1)
+    assert fp8_decode_plan(s.pool, s.table, r[:0], n[:0]).bs == 0
 
 
 def test_arguments_are_checked(cuda):
