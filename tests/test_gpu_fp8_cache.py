@@ -97,6 +97,26 @@ def test_a_prompt_longer_than_one_round(cuda):
     check(pool, want)
 
 
+@pytest.mark.parametrize("n, kv", [(600, 2), (600, 5), (1500, 2), (1500, 6), (1500, 11), (1025, 1), (1024, 1)])
+def test_segments_of_every_length(cuda, n, kv):
+    """2 to 64 entries looked after together: runs of a block's whole length and of single entries."""
+    rng = np.random.default_rng(n * kv)
+    dim, blocks = 64, 260
+    pool, want = Fp8TokenToKVPool(blocks, 1, kv, dim, cuda), of.Cache(blocks, kv, dim)
+    loc = []
+    for b in rng.permutation(np.arange(1, blocks)):
+        first, many = int(rng.integers(0, 64)), int(rng.choice([1, 1, 2, 30, 64, 64]))
+        loc += [int(b) * 64 + t for t in range(first, min(first + many, 64))] + [0] * int(rng.random() < 0.1)
+    while len(loc) < n:
+        loc.append(loc[-1])  # the last row, over and over
+    loc = np.array(loc[-n:])
+    for _ in range(2):
+        k, v = (torch.from_numpy(values(rng, n, kv, dim)).to(cuda) for _ in range(2))
+        pool.set_kv_buffer(0, i64(loc, cuda), k, v)
+        want.write(loc, k.cpu().numpy(), v.cpu().numpy())
+        check(pool, want)
+
+
 def test_edges_of_the_format(cuda):
     """Ties, subnormal codes, the largest code, the least scale, zeros, signs."""
     kv, dim = 1, 64
