@@ -429,9 +429,10 @@ int64_t qq_block_workspace_bytes(int bs);
  * cache: k[i], v[i] ([n, kv_heads, head_dim] bf16 or fp32, 16-byte aligned) go to row loc[i].
  * Per (block, head), K and V apart: the scale becomes 2^e, e the largest of its exponent
  * before and the least e >= -110 with max |value written| <= 448 * 2^e; codes are rounded to
- * nearest even; when e grows the block's other codes are re-rounded.  A call that writes a
- * block's first row begins the block: its earlier codes (set to 0) and scale are void.  A
- * value that is not finite makes the scale NaN until the block is begun again.  Rows of
+ * nearest even (a value within 1/32 of float's largest may come back as infinity); when e grows
+ * the block's other codes are re-rounded.  A call that writes a block's first row begins the
+ * block: its earlier codes (set to 0) and scale are void.  A value that is not finite makes the
+ * scale NaN until the block is begun again.  Rows of
  * block 0 and outside the cache are skipped.  The entries of one block stand next to each
  * other in loc (two runs of one block in a call leave it undefined); of a row listed twice
  * in a run the last entry counts. */
@@ -464,9 +465,7 @@ int qq_fp8_page_bounds(const uint8_t* k_codes, int64_t codes_layer_stride, const
 
 /* One layer's decode over the 8-bit cache (src/qwenquest/attention/dense.py:26-42 and
  * quest_only.py:149-159 over it): with k_new the new tokens are stored first
- * (qq_fp8_store(k_new, v_new, out_cache_loc), [bs, kv_heads, head_dim] new_dtype; each in the last
- * block of its own request's context, or in none); then
- * request i's q[i] ([bs, H, head_dim] bf16 or fp32, 16-byte aligned, batch stride a multiple
+ * (qq_fp8_store(k_new, v_new, out_cache_loc), [bs, kv_heads, head_dim] new_dtype); then request i's q[i] ([bs, H, head_dim] bf16 or fp32, 16-byte aligned, batch stride a multiple
  * of 8 elements) attends positions 0 .. seq_lens[i] - 1, or with `positions` and
  * seq_lens[i] > top_k the pages positions[i, 64 u] / 64, u < top_k / 64 - 1, and the last 64
  * positions (the layout of qq_quest_retrieve_topk; duplicates counted).  out [bs, H * head_dim]
@@ -488,7 +487,9 @@ int64_t qq_fp8_decode_workspace_bytes(int bs, int num_q_heads, int kv_heads, int
  * divides the batch into `workspace` (>= qq_fp8_decode_workspace_bytes(bs, kv_heads, kv_heads,
  * head_dim)), with which calls for the same requests, lengths, table and cache geometry, without
  * positions, on the same stream pass planned != 0 and run as one launch each, at up to 16 query
- * heads per KV head (others as without a plan, with a workspace of their own size). */
+ * heads per KV head (others as without a plan, with a workspace of their own size).  In a planned
+ * call each new token lies in the last block of its own request's context, no two in one block,
+ * or in no block (rows of block 0).  A plan of another bs writes nothing. */
 int qq_fp8_decode_plan(int num_blocks, int kv_heads, int head_dim, int block_table_rows, int block_table_cols,
                        const int64_t* req_pool_indices, const int64_t* seq_lens, int bs, void* workspace,
                        int64_t workspace_bytes, void* stream);

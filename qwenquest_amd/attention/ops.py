@@ -285,10 +285,11 @@ def fp8_decode_attention(
     """Decode over an 8-bit pool: request ``i`` attends ``q[i] [H, D]`` over its first ``seq_lens[i]``
     tokens in the blocks ``block_table[req_pool_indices[i]]``, or, with ``positions [bs, >= top_k]``
     (``QuestAlgorithm.retrieve_topk``) and a longer context than ``top_k``, over the pages listed
-    there and the last 64 tokens.  ``new``: ``(loc, k, v)`` of the batch's new tokens, stored first,
-    each in the last block of its own request's context (or in the void block 0).  ``plan``: this
-    step's ``fp8_decode_plan`` (of the same pool, table, requests and lengths, on the same stream; not
-    with ``positions``): up to 16 query heads per KV head then run as one launch.
+    there and the last 64 tokens.  ``new``: ``(loc, k, v)`` of the batch's new tokens, stored first.
+    ``plan``: this step's ``fp8_decode_plan`` (of the same pool, table, requests and lengths, on the
+    same stream; not with ``positions``): up to 16 query heads per KV head then run as one launch,
+    for which each new token lies in the last block of its own request's context and no two in one
+    block (rows of block 0, the padding, aside).
     Returns ``[bs, H*D]`` in q's dtype (bf16 or fp32): zeros for an empty context, NaN for a request
     outside the table or a context past its blocks."""
     dev = pool.device

@@ -22,6 +22,11 @@
 // half a step on average, 2^-10 / 2 over the significand's 1 .. 2, in the mean 0.72 * 2^-11.
 // A weight is off by 0.64 * 2^-10 at most, an output by that of sum p |v|, where its own rounding
 // is 2^-8 of it; the weights' sum stays in fp32.
+//
+// Bound: the matrix cores and, beside them, the softmax's vector instructions.  Measured, 32 query
+// heads on 4 of 128: 8192 tokens behind 8192 1494 us (1.10 PFLOP/s of the formula's operations;
+// with bf16 scores 1639, with vector lookups 1797), 3440 tokens of 6 prompts 182 us, where the
+// longest tile chain is as long as the rest.
 #include "qq_extend_dev.h"
 #include "qq_fp8.h"
 

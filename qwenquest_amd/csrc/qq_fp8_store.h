@@ -7,7 +7,9 @@
 // value that is not finite makes the scale NaN until the block is begun again.
 //
 // One thread block per (run of entries of one cache block, head, K or V).  Bound at prompts: HBM;
-// at decode steps the chain entries -> values -> write, three round trips.
+// at decode steps the chain entries -> values -> write, three round trips.  Measured, 4 heads of
+// 128 from bf16: 131071 tokens 83 us (4.9 TB/s; 454 when one block did K and V and wrote the codes
+// as it had them instead of composing whole blocks in the LDS), 32 decode tokens 4.9 us.
 #pragma once
 
 #include "qq_fp8.h"
