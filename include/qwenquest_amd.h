@@ -454,14 +454,17 @@ int qq_fp8_rows(const uint8_t* k_codes, const uint8_t* v_codes, const float* k_s
  * (src/qwenquest/quest.py:231-280 and 284-321 in one form: nothing runs along).  Blocks come
  * from block_table; requests outside it are skipped, a block outside the cache gives NaN.
  * actual_lens and candidate_limit (both or neither): qq_quest_prepare_step's outputs for pages
- * of 64, in the same launch. */
+ * of 64, in the same launch.  plan (decode only, or NULL): a workspace of
+ * qq_fp8_decode_workspace_bytes(bs, kv_heads, kv_heads, head_dim), into which the step's
+ * selections of top_k tokens are divided for its qq_fp8_quest_step calls. */
 int qq_fp8_page_bounds(const uint8_t* k_codes, int64_t codes_layer_stride, const float* k_scale,
                        int64_t scale_layer_stride, int num_blocks, int kv_heads, int head_dim,
                        const int32_t* block_table, int64_t block_table_stride, int block_table_rows,
                        int block_table_cols, const int64_t* req_pool_indices, const int64_t* seq_lens,
                        const int64_t* prefix_lens, int bs, int decode, int64_t max_new, int n_layers,
                        uint16_t* page_k_bounds, int max_reqs, int max_pages, int top_k,
-                       int avoid_recent_overlap, int32_t* actual_lens, int32_t* candidate_limit, void* stream);
+                       int avoid_recent_overlap, int32_t* actual_lens, int32_t* candidate_limit, void* plan,
+                       int64_t plan_bytes, void* stream);
 
 /* One layer's decode over the 8-bit cache (src/qwenquest/attention/dense.py:26-42 and
  * quest_only.py:149-159 over it): with k_new the new tokens are stored first
@@ -498,7 +501,12 @@ int qq_fp8_decode_plan(int num_blocks, int kv_heads, int head_dim, int block_tab
  * over the 8-bit cache: page scores and selection from page_k_bounds (as qq_quest_retrieve_topk,
  * pages of 64; scores_ws [bs, max_pages], positions [bs, top_k] written), the new tokens' store
  * and the attention over the selected pages (as qq_fp8_decode_attention).  Three launches: the
- * scores; the selection with the store; the attention.  phase 1 = scores and selection, 2 = store
+ * scores; the selection with the store; the attention.  planned != 0: workspace is the plan that
+ * this step's qq_fp8_page_bounds made (same requests, lengths, table, geometry and top_k, on the same
+ * stream; up to 16 query heads per KV head, others as without), for which the new tokens lie as
+ * in a planned qq_fp8_decode_attention.  bf16 at 4 KV heads x 128 with 2 to 8 query heads each,
+ * top_k of 512 to 4160, up to 8192 pages and 64 requests then takes two launches: the scores with the
+ * store; the selection with the attention.  phase 1 = scores and selection, 2 = store
  * and attention over the positions that phase 1 left, 3 = both. */
 int qq_fp8_quest_step(const void* q, int q_dtype, int64_t q_batch_stride, int num_q_heads, const void* k_new,
                       const void* v_new, int new_dtype, const int64_t* out_cache_loc, uint8_t* k_codes,
@@ -508,7 +516,7 @@ int qq_fp8_quest_step(const void* q, int q_dtype, int64_t q_batch_stride, int nu
                       const int64_t* req_pool_indices, const int64_t* seq_lens, const int32_t* candidate_limit,
                       int bs, int max_reqs, int max_pages, int top_k, float scale, float* scores_ws,
                       int32_t* positions, void* out, void* workspace, int64_t workspace_bytes, int phase,
-                      void* stream);
+                      int planned, void* stream);
 
 /* The batch form of AttentionBackend.forward_extend (src/qwenquest/attention/base.py:65-93) over
  * the 8-bit cache, the new K/V being in it: request i's extend_lens[i] new tokens (q

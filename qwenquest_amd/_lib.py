@@ -111,7 +111,8 @@ SIGNATURES: dict[str, tuple] = {
     "qq_fp8_rows": (_I, [_P, _P, _P, _P, _I, _I, _I, _P, _L, _P, _P, _I, _P]),
     "qq_fp8_page_bounds": (
         _I,
-        [_P, _L, _P, _L, _I, _I, _I, _P, _L, _I, _I, _P, _P, _P, _I, _I, _L, _I, _P, _I, _I, _I, _I, _P, _P, _P],
+        [_P, _L, _P, _L, _I, _I, _I, _P, _L, _I, _I, _P, _P, _P, _I, _I, _L, _I, _P, _I, _I, _I, _I, _P, _P, _P,
+         _L, _P],
     ),
     "qq_fp8_decode_attention": (
         _I,
@@ -123,7 +124,7 @@ SIGNATURES: dict[str, tuple] = {
     "qq_fp8_quest_step": (
         _I,
         [_P, _I, _L, _I, _P, _P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _P, _L, _I, _I, _P, _I, _P, _P, _P, _I, _I, _I,
-         _I, _F, _P, _P, _P, _P, _L, _I, _P],
+         _I, _F, _P, _P, _P, _P, _L, _I, _I, _P],
     ),
     "qq_fp8_extend_attention": (
         _I,

@@ -346,7 +346,8 @@ def fp8_quest_step(
     """One layer of Quest decode over an 8-bit pool, after ``quest.decode_step_blocks``: the new tokens
     ``k``/``v`` go to rows ``loc``, the page scores select (``positions [>= bs, top_k]`` int32 is
     written, as ``QuestAlgorithm.retrieve_topk`` writes it), and ``q [bs, H, D]`` attends the selected
-    pages.  ``phase``: 1 = scoring and selection, 2 = store and attention after phase 1, 3 = both.
+    pages.  On the stream of ``decode_step_blocks``; each new token lies in the last block of its own
+    request's context and no two in one block (rows of block 0 aside).  ``phase``: 1 = scoring and selection, 2 = store and attention after phase 1, 3 = both.
     Returns ``[bs, H*D]`` (complete after phase 2)."""
     dev, step = pool.device, quest._step
     if step is None:
@@ -370,14 +371,15 @@ def fp8_quest_step(
     kn, vn = pool.new_rows(k, v, bs)
     out = torch.empty((bs, heads * dim), dtype=q.dtype, device=dev)
     need = int(_lib.load().qq_fp8_decode_workspace_bytes(bs, heads, pool.kv_heads, dim))
-    ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)  # of this call alone
+    planned = step.plan is not None and heads <= 16 * pool.kv_heads and step.top_k == quest.top_k
+    ws = step.plan if planned else torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
     with _lib.on(dev):
         _lib.call(
             "qq_fp8_quest_step", _lib.ptr(q), _lib.dtype_code(q.dtype), q.stride(0), heads, _lib.ptr(kn), _lib.ptr(vn),
             _lib.dtype_code(kn.dtype), _lib.ptr(loc), *pool.layer_args(layer_id), *_table_args(bt),
             _lib.ptr(quest.page_k_bounds), layer_id - quest.start_layer, _lib.ptr(rpi), _lib.ptr(step.seq_lens),
             _lib.ptr(step.candidate_limit_i32), bs, quest.max_reqs, quest.max_pages_per_req, quest.top_k, float(scaling),
-            _lib.ptr(quest._scores_ws), _lib.ptr(positions), _lib.ptr(out), _lib.ptr(ws), need, int(phase),
+            _lib.ptr(quest._scores_ws), _lib.ptr(positions), _lib.ptr(out), _lib.ptr(ws), need, int(phase), int(planned),
             _lib.stream(dev),
         )
     return out

@@ -2,6 +2,7 @@
 // MHATokenToKVPool.set_kv_buffer (reference src/qwenquest/memory.py:114-120) for blocks of e4m3
 // codes with a scale per block and KV head, the rows back as values, and the page bounds of
 // QuestAlgorithm (src/qwenquest/quest.py:231-321) from the codes.
+#include "qq_fp8_plan.h"
 #include "qq_fp8_store.h"
 
 namespace qq {
@@ -110,6 +111,8 @@ struct PageArgs {
   int top_k, avoid;
   int32_t* actual;  // nullptr, or the step's layout: actual_lens, candidate_limit
   int32_t* limit;
+  int layers;
+  PlanArgs plan;  // cu nullptr, or the step's division of the attention's work, by a block past the layers
 };
 
 // Min and max of a page's keys per channel, a wave per (page, head, layer).  A scale is
@@ -123,6 +126,10 @@ template <int D>
 __global__ __launch_bounds__(256) void fp8_page_bounds_kernel(PageArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int b = blockIdx.y, layer = blockIdx.z;
+  if (layer == a.layers) {
+    if (b == 0 && blockIdx.x == 0) plan_slices(a.plan);
+    return;
+  }
   const int64_t req = a.rpi[b], seq = a.seq[b], s = max(seq, (int64_t)0);
   if (a.actual && layer == 0 && blockIdx.x == 0 && threadIdx.x == 0) {
     a.actual[b] = (int32_t)min(seq, (int64_t)a.top_k);  // quest.py:343-352
@@ -270,13 +277,14 @@ extern "C" int qq_fp8_page_bounds(const uint8_t* k_codes, int64_t codes_layer_st
                                   int block_table_cols, const int64_t* req_pool_indices, const int64_t* seq_lens,
                                   const int64_t* prefix_lens, int bs, int decode, int64_t max_new, int n_layers,
                                   uint16_t* page_k_bounds, int max_reqs, int max_pages, int top_k,
-                                  int avoid_recent_overlap, int32_t* actual_lens, int32_t* candidate_limit, void* stream) {
+                                  int avoid_recent_overlap, int32_t* actual_lens, int32_t* candidate_limit, void* plan,
+                                  int64_t plan_bytes, void* stream) {
   const char* what = "qq_fp8_page_bounds";
   const Fp8Cache c{const_cast<uint8_t*>(k_codes), const_cast<uint8_t*>(k_codes), const_cast<float*>(k_scale),
                    const_cast<float*>(k_scale), num_blocks, kv_heads, head_dim};
   const int st = check_cache(c, what);
   if (st != QQ_OK) return st;
-  QQ_REQUIRE(bs >= 0 && bs < 65536 && n_layers > 0 && n_layers < 65536 && max_reqs > 0 && max_pages > 0 && max_new >= 0 &&
+  QQ_REQUIRE(bs >= 0 && bs < 65536 && n_layers > 0 && n_layers < 65535 && max_reqs > 0 && max_pages > 0 && max_new >= 0 &&
                  block_table_cols > 0 && block_table_stride >= block_table_cols && block_table_rows > 0,
              "%s: bad sizes", what);
   QQ_REQUIRE(!actual_lens == !candidate_limit, "%s: one of the layout's outputs is missing", what);
@@ -285,11 +293,18 @@ extern "C" int qq_fp8_page_bounds(const uint8_t* k_codes, int64_t codes_layer_st
   PageArgs a{k_codes, k_scale, codes_layer_stride, scale_layer_stride, num_blocks, kv_heads, block_table, block_table_stride,
              block_table_rows, block_table_cols, req_pool_indices, seq_lens, prefix_lens, decode,
              reinterpret_cast<uint32_t*>(page_k_bounds), max_reqs, max_pages, top_k, avoid_recent_overlap, actual_lens,
-             candidate_limit};
+             candidate_limit, n_layers, {}};
+  if (plan) {
+    QQ_REQUIRE(decode && top_k > 0 && top_k % 64 == 0, "%s: a plan is of a decode step's selections of whole pages", what);
+    QQ_REQUIRE((int64_t)block_table_cols * bs < (int64_t)1 << 30, "%s: too many units of work", what);
+    const DecSpace sp = decode_space(bs, kv_heads, kv_heads, head_dim);
+    QQ_REQUIRE(plan_bytes >= sp.bytes, "%s: workspace %lld bytes < %lld needed", what, (long long)plan_bytes, (long long)sp.bytes);
+    set_plan(a.plan, sp, plan, req_pool_indices, seq_lens, bs, block_table_rows, block_table_cols, top_k, kv_heads);
+  }
   // pages of a request, at most: those its new tokens can complete
   const int64_t pages = decode ? 1 : min((int64_t)max_pages, max_new > 0 && prefix_lens ? max_new / 64 + 1 : (int64_t)max_pages);
   const int64_t need = (pages * kv_heads + 3) / 4, fill = max((int64_t)1, (int64_t)16384 / ((int64_t)bs * n_layers));
-  const dim3 grid((unsigned)min(need, fill), bs, n_layers);
+  const dim3 grid((unsigned)min(need, fill), bs, n_layers + (plan ? 1 : 0));
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (head_dim == 128) fp8_page_bounds_kernel<128><<<grid, 256, 0, s>>>(a);
   else fp8_page_bounds_kernel<64><<<grid, 256, 0, s>>>(a);

@@ -27,6 +27,7 @@
 // words, scales and codes, partials, count, merge, ~1 us each): one request of 2000 tokens 10.6 us
 // a layer, 15.2 in two launches; the plan 4.4 us a step.  16 requests' 31 pages and window
 // 14.7 us behind a begin launch of 5.3 and the scores' 11.8.
+#include "qq_fp8_plan.h"
 #include "qq_fp8_store.h"
 #include "qq_quest_dev.h"
 #include "qq_rules.h"
@@ -34,103 +35,23 @@
 namespace qq {
 namespace {
 
-constexpr int kTile = 16;      // query heads of a tile
 constexpr int kDecWaves = 8;
 constexpr int kDecParts = rules::kFp8Parts;  // slices of a request, at most: the merge's table of weights
 
-struct DecPlan {
-  int32_t total, len, slices, bs;  // units of the batch, units of a slice, slices, requests
-};
-struct DecItem {  // a slice's first request: its units are [c0, c1) of the batch's
-  int32_t b, c0, c1, seq;
-  int32_t req, pad[3];  // its table row, or -1: outside the table
-};
-
-struct DecArgs {
+struct DecArgs : PlanArgs {
   const void* q;  // [bs, H, D]
   int64_t q_bstride;
   int H, G, tiles;  // query heads, of a KV head, tiles of those
   Fp8Cache c;
   const int32_t* table;
   int64_t table_stride;
-  int table_rows, table_cols;
-  const int64_t* rpi;
-  const int64_t* seq;
-  int bs;
-  const int32_t* positions;  // nullptr: dense
+  const int32_t* positions;  // nullptr: dense, or the attention selects
   int64_t pos_stride;
-  int top_k;
   float sl2;  // scale * log2(e)
   void* out;  // [bs, H, D]
-  int max_slices, heads;  // heads: KV * tiles
-  DecPlan* plan;
-  int32_t* cu;       // [bs + 1] units before each request
-  DecItem* items;    // [max_slices]
-  uint32_t* done;    // [max_slices, heads] parts finished of the request that goes on behind a slice; left 0
-  float* part_o;     // [max_slices, 2, heads, 16, D]
-  float* part_ml;    // [max_slices, 2, heads, 16, 2]
+  float* part_o;   // [max_slices, 2, heads, 16, D]
+  float* part_ml;  // [max_slices, 2, heads, 16, 2]
 };
-
-__device__ inline int context_of(const DecArgs& a, int b) {
-  return (int)min(max(a.seq[b], (int64_t)0), (int64_t)a.table_cols * kCacheTokens);
-}
-__device__ inline int table_row(const DecArgs& a, int b) {
-  const int64_t req = a.rpi[b];
-  return req >= 0 && req < a.table_rows ? (int)req : -1;
-}
-__device__ inline bool is_sparse(const DecArgs& a, int s) { return a.positions && s > a.top_k; }
-__device__ inline int units_of(const DecArgs& a, int s) {
-  if (is_sparse(a, s)) return a.top_k / 64;
-  return max((s + 63) / 64, 1);  // an empty context: one unit without tokens, which writes its zeros
-}
-
-// Cuts the batch's units into slices; 256 threads.
-__device__ inline void plan_slices(const DecArgs& a) {
-  __shared__ int s_sum[4], s_long[4];
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  for (int i = tid; i < a.max_slices * a.heads; i += 256) a.done[i] = 0u;
-  int base = 0, longest = 0;
-  for (int b0 = 0; b0 < a.bs; b0 += 256) {
-    const int b = b0 + tid;
-    const int u = b < a.bs ? units_of(a, context_of(a, b)) : 0;
-    int x = u;
-    longest = max(longest, u);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int y = __shfl_up(x, d, 64);
-      if (lane >= d) x += y;
-    }
-    __syncthreads();
-    if (lane == 63) s_sum[wave] = x;
-    __syncthreads();
-    int before = base;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      if (w < wave) before += s_sum[w];
-      base += s_sum[w];
-    }
-    if (b < a.bs) a.cu[b] = before + x - u;
-  }
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) longest = max(longest, __shfl_xor(longest, d, 64));
-  if (lane == 0) s_long[wave] = longest;
-  if (tid == 0) a.cu[a.bs] = base;
-  __syncthreads();
-  longest = max(max(s_long[0], s_long[1]), max(s_long[2], s_long[3]));
-  const int len = rules::fp8_slice_len(base, longest, a.max_slices);
-  const int slices = (base + len - 1) / len;
-  if (tid == 0) *a.plan = {base, len, slices, a.bs};
-  for (int i = tid; i < slices; i += 256) {
-    const int at = i * len;
-    int lo = 0, hi = a.bs;  // the last request that begins at or before this unit
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (a.cu[mid] <= at) lo = mid;
-      else hi = mid;
-    }
-    a.items[i] = {lo, a.cu[lo], a.cu[lo + 1], context_of(a, lo), table_row(a, lo), {0, 0, 0}};
-  }
-}
 
 __global__ __launch_bounds__(256) void fp8_plan_kernel(DecArgs a) { plan_slices(a); }
 
@@ -320,8 +241,26 @@ __device__ inline void merge_parts(const DecArgs& a, DecSmem& sm, int head, int 
   }
 }
 
-template <int D, typename T>
-__global__ __launch_bounds__(64 * kDecWaves, 2) void fp8_attend_kernel(DecArgs a, StoreArgs st) {
+// The pages that request b attends, by a whole block of 64 * kDecWaves threads: in the scores' order
+// into pages[0 .. k_sel).
+template <int KPT>
+__device__ inline void select_pages(const SelectArgs& sel, int b, RankSelectSmem<KPT, 64 * kDecWaves>& sm, int32_t* pages) {
+  constexpr int NT = 64 * kDecWaves;
+  const float* sc = sel.scores + (int64_t)b * sel.MP;
+  float sv[KPT];
+#pragma unroll
+  for (int i = 0; i < KPT; ++i) sv[i] = sc[min((int)threadIdx.x + NT * i, sel.MP - 1)];
+  const int64_t req = sel.rpi[b];
+  const int lim = req >= 0 && req < sel.R ? min(sel.limit[b], sel.MP) : 0;
+  int rank = -1, page = -1, row0 = -1;
+  select_ranked<KPT, NT>(sv, lim, max(lim, sel.k_sel), sel.k_sel, sm, nullptr, sel.MP, rank, page, row0);
+  if (threadIdx.x < 64 && rank >= 0 && rank < sel.k_sel) pages[rank] = page;
+  lds_barrier();
+}
+
+// KPT > 0: the requests' pages are selected here, KPT scores a thread.
+template <int D, typename T, int KPT>
+__global__ __launch_bounds__(64 * kDecWaves, 2) void fp8_attend_kernel(DecArgs a, StoreArgs st, SelectArgs sel) {
   constexpr int QP = sizeof(T) == 2 ? 1 : 3, PP = sizeof(T) == 2 ? 2 : 3;  // pieces of q and of the weights
   constexpr int KL = D / 64, VL = D / 16;  // 16-byte loads a lane: per 16 tokens of K, per block of V
   constexpr int RF = dec_row_floats(D);
@@ -331,7 +270,7 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void fp8_attend_kernel(DecArgs a
   const int head = blockIdx.x % a.heads, slice = blockIdx.x / a.heads;
   const DecPlan plan = *a.plan;
   const DecItem item = a.items[slice];  // both in one round trip; stale past the last slice
-  if (slice >= plan.slices || plan.bs != a.bs) return;  // a plan of another batch answers nothing
+  if (slice >= plan.slices || plan.bs != a.bs || plan.top_k != a.top_k) return;  // another batch's plan answers nothing
   const int h = head / a.tiles, tile = head - h * a.tiles;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int m16 = lane & 15, g = lane >> 4;
@@ -342,6 +281,38 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void fp8_attend_kernel(DecArgs a
   const int s0 = at + (int)((int64_t)(end - at) * wave / kDecWaves), s1 = at + (int)((int64_t)(end - at) * (wave + 1) / kDecWaves);
   const int picked = a.top_k / 64 - 1;  // selected pages; the unit after them is the window
   if (lane < 2) sm.b[2 * wave + lane] = -1;
+
+  // The selections of this slice's requests: a slice is no longer than one of them, so there are two
+  // at most.
+  __shared__ int32_t s_pages[KPT > 0 ? 2 : 1][64];
+  int sel_first = -1;  // the first of the two
+  // f(request lane, its units' begin, its context) of 64 requests from r0 on that begin in or before the slice
+  auto each_64 = [&](auto f) {
+    bool more = true;
+    for (int r0 = item.b; more; r0 += 64) {
+      const int r = r0 + lane;
+      int c0 = 0x7FFFFFFF, seq = 0;
+      if (r == item.b) {
+        c0 = item.c0;
+        seq = item.seq;
+      } else if (end > item.c1 && r < a.bs) {
+        c0 = a.cu[r];
+        seq = context_of(a, r);
+      }
+      f(r0, c0, seq);
+      more = __builtin_amdgcn_readlane(c0, 63) < end;
+    }
+  };
+  if constexpr (KPT > 0) {
+    auto& sm_sel = *reinterpret_cast<RankSelectSmem<KPT, 64 * kDecWaves>*>(sm.o);
+    each_64([&](int r0, int c0, int seq) {
+      for (uint64_t hits = __ballot(c0 < end && is_sparse(a, seq)); hits; hits &= hits - 1) {
+        const int b = r0 + __builtin_ctzll(hits);
+        select_pages<KPT>(sel, b, sm_sel, s_pages[sel_first >= 0 ? 1 : 0]);
+        if (sel_first < 0) sel_first = b;
+      }
+    });
+  }
 
   // New tokens of the requests that end among this wave's units, each in its request's last block,
   // which no other wave of this head reads.
@@ -409,13 +380,16 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void fp8_attend_kernel(DecArgs a
     const bool sparse = is_sparse(a, u_seq), win = sparse && u - u_c0 == picked;
     if (u < u_end && u_seq > 0 && row >= 0) {
       const int place = u - u_c0;
-      blk = block_at(!sparse ? place : win ? (u_seq - 64) >> 6 : a.positions[(int64_t)u_b * a.pos_stride + place * 64] >> 6);
+      int page = place;
+      if (win) page = (u_seq - 64) >> 6;
+      else if (sparse) page = KPT > 0 ? s_pages[u_b == sel_first ? 0 : 1][place] : a.positions[(int64_t)u_b * a.pos_stride + place * 64] >> 6;
+      blk = block_at(page);
       blk2 = win && (u_seq & 63) ? block_at(u_seq >> 6) : blk;
     }
     const int64_t e = (int64_t)blk * a.c.KV + h, e2 = (int64_t)blk2 * a.c.KV + h;
     ks = a.c.ks[e];
     vs = a.c.vs[e];
-    if (a.positions) {
+    if (a.top_k) {
       ks2 = a.c.ks[e2];
       vs2 = a.c.vs[e2];
     }
@@ -597,6 +571,23 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void fp8_attend_kernel(DecArgs a
       for (int i = 0; i < VL; ++i) *reinterpret_cast<float4_t*>(sm_o + (slot * rows + m16) * RF + i * 16 + g * 4) = o[i];
     }
   }
+  if constexpr (KPT > 0) {  // the layout of the requests that begin here, for those who read it
+    if (head == 0)
+      each_64([&](int r0, int c0, int seq) {
+        const uint64_t long_ones = __ballot(is_sparse(a, seq));
+        for (uint64_t hits = __ballot(c0 >= at && c0 < end); hits; hits &= hits - 1) {
+          const int i = __builtin_ctzll(hits), b = r0 + i;
+          int32_t* pos = sel.positions + (int64_t)b * sel.top_k;
+          if (!(long_ones >> i & 1)) {
+            write_dense(pos, a.seq[b], sel.top_k);
+            continue;
+          }
+          const int32_t* pages = s_pages[b == sel_first ? 0 : 1];
+          for (int slot = tid; slot < sel.k_sel * 64; slot += 64 * kDecWaves) pos[slot] = pages[slot >> 6] * 64 + (slot & 63);
+          write_recent(pos + (int64_t)sel.k_sel * 64, a.seq[b], 64);
+        }
+      });
+  }
   __syncthreads();
   // The requests that more than one wave has, or that go on in another slice: their slots follow one
   // another, from the one where the request begins here to the one where it ends (or the slice).
@@ -672,25 +663,6 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void fp8_attend_kernel(DecArgs a
   }
 }
 
-// The workspace's parts, in order; offsets are multiples of 256 bytes.
-struct DecSpace {
-  int64_t cu, items, done, part_o, part_ml, bytes;
-  int max_slices;
-};
-DecSpace decode_space(int bs, int H, int KV, int D) {
-  auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
-  const int tiles = (H / KV + kTile - 1) / kTile, heads = KV * tiles;
-  DecSpace s;
-  s.max_slices = rules::fp8_max_slices(heads);
-  s.cu = up(sizeof(DecPlan));
-  s.items = s.cu + up((int64_t)(bs + 1) * 4);
-  s.done = s.items + up((int64_t)s.max_slices * sizeof(DecItem));
-  s.part_o = s.done + up((int64_t)s.max_slices * heads * 4);
-  s.part_ml = s.part_o + (int64_t)s.max_slices * 2 * heads * kTile * D * 4;
-  s.bytes = s.part_ml + (int64_t)s.max_slices * 2 * heads * kTile * 2 * 4;
-  return s;
-}
-
 template <int D, int KPT>
 void begin(const DecArgs& a, const StoreArgs& st, const SelectArgs& sel, hipStream_t s) {
   const unsigned blocks = 1 + (KPT > 0 ? a.bs : 0) + (st.k ? 2u * a.bs * a.c.KV : 0);
@@ -698,20 +670,22 @@ void begin(const DecArgs& a, const StoreArgs& st, const SelectArgs& sel, hipStre
   else fp8_begin_kernel<D, float, KPT><<<blocks, 256, 0, s>>>(a, st, sel);
 }
 
-// LDS past the 64 KiB default (tiles of more than 15 heads of 128): opted in once per device.
-template <int D, typename T>
-void attend(const DecArgs& a, const StoreArgs& st, hipStream_t s) {
-  const size_t bytes = dec_smem_bytes(min(a.G, kTile), D);
-  if (bytes > 64 * 1024) {
+// LDS past the 64 KiB default (tiles of more than 15 heads of 128, large selections): opted in once
+// per device.
+template <int D, typename T, int KPT>
+void attend(const DecArgs& a, const StoreArgs& st, const SelectArgs& sel, hipStream_t s) {
+  size_t bytes = dec_smem_bytes(min(a.G, kTile), D);
+  if (KPT > 0) bytes = max(bytes, sizeof(DecSmem) + sizeof(RankSelectSmem<(KPT > 0 ? KPT : 1), 64 * kDecWaves>));
+  if (bytes > 60 * 1024) {
     static bool opted[64] = {false};
     int dev = 0;
     if (hipGetDevice(&dev) == hipSuccess && dev >= 0 && dev < 64 && !opted[dev]) {
-      (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&fp8_attend_kernel<D, T>),
-                                hipFuncAttributeMaxDynamicSharedMemorySize, (int)dec_smem_bytes(kTile, D));
+      (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&fp8_attend_kernel<D, T, KPT>),
+                                hipFuncAttributeMaxDynamicSharedMemorySize, (int)max(dec_smem_bytes(kTile, D), bytes));
       opted[dev] = true;
     }
   }
-  fp8_attend_kernel<D, T><<<a.max_slices * a.heads, 64 * kDecWaves, bytes, s>>>(a, st);
+  fp8_attend_kernel<D, T, KPT><<<a.max_slices * a.heads, 64 * kDecWaves, bytes, s>>>(a, st, sel);
 }
 
 // `sel`: with k_sel > 0 the pages are selected first, from scores that are there.  planned: the
@@ -729,8 +703,29 @@ void launch(const DecArgs& a, const StoreArgs& st, const SelectArgs& sel, bool p
     launch_select(sel, a.bs, sel.MP, sel.k_sel, s);
     begin<D, 0>(a, st, sel, s);
   }
-  if (q_dtype == QQ_DTYPE_BF16) attend<D, uint16_t>(a, in, s);
-  else attend<D, float>(a, in, s);
+  if (q_dtype == QQ_DTYPE_BF16) attend<D, uint16_t, 0>(a, in, sel, s);
+  else attend<D, float, 0>(a, in, sel, s);
+}
+
+// Whether a planned step of Quest runs as two launches: the scores with the new tokens, and an
+// attention that selects by itself.  A slice must not be longer than a request's selection (at
+// most as many requests as the grid has slices, and 8 units, fp8_slice_len's least), so that a block
+// selects for two requests at most.
+bool selects_itself(const DecArgs& a, const SelectArgs& sel, int q_dtype) {
+  return q_dtype == QQ_DTYPE_BF16 && a.c.D == 128 && a.tiles == 1 && a.bs <= a.max_slices && sel.top_k >= 8 * 64 &&
+         sel.k_sel <= 64 && sel.MP > 0 && max(sel.MP, sel.k_sel) <= 16 * 64 * kDecWaves &&
+         (int64_t)a.table_cols * kCacheTokens > sel.top_k;
+}
+
+void launch_selecting(DecArgs a, const SelectArgs& sel, hipStream_t s) {
+  const int n = max(sel.MP, sel.k_sel);
+  constexpr int NT = 64 * kDecWaves;
+  a.positions = nullptr;
+  const StoreArgs none{};
+  if (n <= NT) attend<128, uint16_t, 1>(a, none, sel, s);
+  else if (n <= 2 * NT) attend<128, uint16_t, 2>(a, none, sel, s);
+  else if (n <= 5 * NT) attend<128, uint16_t, 5>(a, none, sel, s);
+  else attend<128, uint16_t, 16>(a, none, sel, s);
 }
 
 // Everything of a call but its launches; `what` refuses.
@@ -771,22 +766,11 @@ int set_args(DecArgs& a, StoreArgs& st, const char* what, const void* q, int q_d
   a.c = c;
   a.table = block_table;
   a.table_stride = block_table_stride;
-  a.table_rows = block_table_rows;
-  a.table_cols = block_table_cols;
-  a.rpi = req_pool_indices;
-  a.seq = seq_lens;
-  a.bs = bs;
   a.positions = positions;
   a.pos_stride = positions_stride;
-  a.top_k = positions ? top_k : 64;
   a.sl2 = scale * kLog2e;
   a.out = out;
-  a.max_slices = sp.max_slices;
-  a.heads = c.KV * a.tiles;
-  a.plan = reinterpret_cast<DecPlan*>(ws);
-  a.cu = reinterpret_cast<int32_t*>(ws + sp.cu);
-  a.items = reinterpret_cast<DecItem*>(ws + sp.items);
-  a.done = reinterpret_cast<uint32_t*>(ws + sp.done);
+  set_plan(a, sp, ws, req_pool_indices, seq_lens, bs, block_table_rows, block_table_cols, positions ? top_k : 0, c.KV * a.tiles);
   a.part_o = reinterpret_cast<float*>(ws + sp.part_o);
   a.part_ml = reinterpret_cast<float*>(ws + sp.part_ml);
   st = StoreArgs{c, k_new, v_new, new_dtype, out_cache_loc, bs, 1};
@@ -856,7 +840,7 @@ extern "C" int qq_fp8_quest_step(const void* q, int q_dtype, int64_t q_batch_str
                                  const int64_t* req_pool_indices, const int64_t* seq_lens, const int32_t* candidate_limit,
                                  int bs, int max_reqs, int max_pages, int top_k, float scale, float* scores_ws,
                                  int32_t* positions, void* out, void* workspace, int64_t workspace_bytes, int phase,
-                                 void* stream) {
+                                 int planned, void* stream) {
   const char* what = "qq_fp8_quest_step";
   QQ_REQUIRE(phase >= 1 && phase <= 3, "%s: phase must be 1, 2 or 3, got %d", what, phase);
   QQ_REQUIRE(bs == 0 || (page_k_bounds && candidate_limit && scores_ws && positions), "%s: null pointer", what);
@@ -893,6 +877,14 @@ extern "C" int qq_fp8_quest_step(const void* q, int q_dtype, int64_t q_batch_str
   sel.scores = scores_ws;
   sel.positions = positions;
   hipStream_t s = static_cast<hipStream_t>(stream);
+  if (planned && phase == 3 && selects_itself(a, sel, q_dtype)) {
+    const int scored = launch_score_codes(sel, bs, a.c, k_new, v_new, new_dtype, out_cache_loc, s);
+    if (scored < 0) return scored;
+    if (scored == QQ_OK) {
+      launch_selecting(a, sel, s);
+      return check_launch(what);
+    }
+  }
   if (phase == 1) return launch_retrieve(sel, bs, s);
   if (phase == 3) {
     const int scored = launch_score(sel, bs, false, s);

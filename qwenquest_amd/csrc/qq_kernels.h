@@ -65,6 +65,12 @@ void launch_select(const SelectArgs& a, int bs, int max_pages, int k_sel, hipStr
 // `store_new` the new token's K/V is stored as well (blocks x == 0).
 int launch_score(const SelectArgs& a, int bs, bool store_new, hipStream_t stream);
 
+// Page scoring only, with the new tokens' store into an 8-bit cache (qq_fp8_store.h; k NULL: none) in
+// the same launch; 1: not for this shape.
+struct Fp8Cache;
+int launch_score_codes(const SelectArgs& a, int bs, const Fp8Cache& c, const void* k, const void* v, int dtype,
+                       const int64_t* loc, hipStream_t stream);
+
 // Chunk attention + merge; `workspace` holds the (m, l, o) partials.
 int launch_attention(AttnArgs& a, int kv_dtype, int bs, int64_t workspace_bytes, void* workspace,
                      hipStream_t stream, const char* what);

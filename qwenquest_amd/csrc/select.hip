@@ -17,6 +17,7 @@
 // per-thread maxima filters the keys, survivors are rank-counted; otherwise a 4-pass radix
 // select on order-preserving 32-bit keys with ties at the threshold to the
 // lowest page index.
+#include "qq_fp8_store.h"
 #include "qq_quest_dev.h"
 
 namespace qq {
@@ -280,12 +281,28 @@ __device__ inline float half_pages_partial(const uint4 (&w)[2], const float4 (&q
   return u;
 }
 
+// What the blocks of new tokens do: rows of a bf16 or fp32 pool, or codes of an 8-bit cache.
+struct NewRows {
+  int store;
+  __device__ inline void operator()(const SelectArgs& a, int b) const {
+    if (store) store_new_token(a, b);
+  }
+};
+struct NewCodes {
+  StoreArgs st;
+  __device__ inline void operator()(const SelectArgs& a, int b) const {
+    if (!st.k) return;
+    for (int h = threadIdx.x >> 6; h < a.KV; h += kThreads / 64) store_token<128>(st, b, h);
+  }
+};
+
+template <typename New>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(8, 8)))
-void score_pages_fast4_kernel(SelectArgs a, int store_new) {
+void score_pages_fast4_kernel(SelectArgs a, New store_new) {
   constexpr int C = 512, D = 128;
   const int b = blockIdx.y;
   if (blockIdx.x == 0) {  // the new token's block (its test needs no argument load)
-    if (store_new) store_new_token(a, b);
+    store_new(a, b);
     return;
   }
   // every argument of the scoring path in the first batch of argument loads; the
@@ -541,15 +558,27 @@ void launch_select(const SelectArgs& a, int bs, int max_pages, int k_sel, hipStr
     select_layout_kernel<<<bs, kThreads, 0, s>>>(a);
 }
 
+static bool fast4(const SelectArgs& a) {
+  const int G = a.KV > 0 ? a.H / a.KV : 0;
+  return a.C == 512 && a.D == 128 && a.q_dtype == QQ_DTYPE_BF16 && G >= 2 && G <= 8 && a.H == G * a.KV;
+}
+
+int launch_score_codes(const SelectArgs& a, int bs, const Fp8Cache& c, const void* k, const void* v, int dtype,
+                       const int64_t* loc, hipStream_t s) {
+  if (!fast4(a)) return 1;
+  const int tiles = max(1, ceil_div(a.MP, kPagesPerBlock4));
+  score_pages_fast4_kernel<<<dim3(tiles + 1, bs), kThreads, 0, s>>>(a, NewCodes{{c, k, v, dtype, loc, bs, 1}});
+  return check_launch("quest page scores");
+}
+
 int launch_score(const SelectArgs& a, int bs, bool store_new, hipStream_t s) {
   dim3 grid(max(1, ceil_div(a.MP, kPagesPerBlock)), bs);
   auto pages_grid = [&](int n) { return dim3(max(1, ceil_div(a.MP, kBlockWaves * n)), bs); };
   const int M = (a.C + 63) / 64;
   const int st = store_new ? 1 : 0;
-  const int G = a.KV > 0 ? a.H / a.KV : 0;
-  if (a.C == 512 && a.D == 128 && a.q_dtype == QQ_DTYPE_BF16 && G >= 2 && G <= 8 && a.H == G * a.KV) {
+  if (fast4(a)) {
     const int tiles = max(1, ceil_div(a.MP, kPagesPerBlock4));
-    score_pages_fast4_kernel<<<dim3(tiles + 1, bs), kThreads, 0, s>>>(a, st);
+    score_pages_fast4_kernel<<<dim3(tiles + 1, bs), kThreads, 0, s>>>(a, NewRows{st});
   } else if (a.C == 512)
     score_pages_fast_kernel<8, 8><<<grid, kThreads, 0, s>>>(a, st);
   // pages per wave: few of the larger pages, so that a small batch still has waves on

@@ -91,11 +91,13 @@ def test_rows_refuses(lib, kw, said):
 @pytest.mark.parametrize("kw, said", [
     (dict(kc=None), b"null cache"), (dict(dim=80), b"head_dim"), (dict(bs=-1), b"bad sizes"), (dict(bs=65536), b"bad sizes"),
     (dict(layers=0), b"bad sizes"), (dict(reqs=0), b"bad sizes"), (dict(mp=0), b"bad sizes"), (dict(tstride=3), b"bad sizes"),
-    (dict(seq=None), b"null"), (dict(bounds=None), b"null"), (dict(table=None), b"null"), (dict(actual=FAKE), b"layout")])
+    (dict(seq=None), b"null"), (dict(bounds=None), b"null"), (dict(table=None), b"null"), (dict(actual=FAKE), b"layout"), (dict(plan=FAKE, plan_bytes=1 << 30), b"decode step"),
+    (dict(plan=FAKE, plan_bytes=1 << 30, decode=1, top_k=100), b"decode step"), (dict(plan=FAKE, plan_bytes=9, decode=1), b"workspace"),
+    (dict(plan=FAKE, plan_bytes=1 << 30, decode=1, bs=65535, tcols=1 << 24, tstride=1 << 24), b"units")])
 def test_page_bounds_refuses(lib, kw, said):
     a = dict(kc=FAKE, kst=100, ks=FAKE, sst=10, blocks=5, kv=4, dim=128, table=FAKE, tstride=4, trows=2, tcols=4, rpi=FAKE,
              seq=FAKE, prefix=None, bs=2, decode=0, max_new=0, layers=1, bounds=FAKE, reqs=2, mp=4, top_k=128,
-             avoid=0, actual=None, limit=None)
+             avoid=0, actual=None, limit=None, plan=None, plan_bytes=0)
     a.update(kw)
     refused(lib.qq_fp8_page_bounds(*a.values(), None), lib, said)
 
@@ -132,7 +134,7 @@ def test_decode_plan_refuses(lib, kw, said):
 def test_quest_step_refuses(lib, kw, said):
     a = dict(q=FAKE, qd=0, qst=4096, H=32, kn=FAKE, vn=FAKE, nd=0, loc=FAKE, **CACHE, table=FAKE, tstride=4, trows=2, tcols=4,
              bounds=FAKE, layer=0, rpi=FAKE, seq=FAKE, limit=FAKE, bs=2, reqs=2, mp=4, top_k=128, scale=0.1, scores=FAKE, pos=FAKE,
-             out=FAKE, ws=FAKE, bytes=1 << 30, phase=3)
+             out=FAKE, ws=FAKE, bytes=1 << 30, phase=3, planned=0)
     a.update(kw)
     refused(lib.qq_fp8_quest_step(*a.values(), None), lib, said)
 

@@ -219,6 +219,49 @@ def test_phases_are_the_step_in_two(cuda):
         e.be.sparse_attention(q, e.mods[0], rpi, torch.zeros(2, 256, dtype=torch.int32, device=cuda), seq.int(), 2)
 
 
+@pytest.mark.parametrize("lens, top_k, width, heads, avoid", [
+    ([5000], 2048, 6000, 32, False), ([64 * 40 + 1, 64, 0, 700, 513, 512, 3000], 512, 4000, 8, True),
+    ([1500 + 97 * i for i in range(30)], 512, 66000, 24, False), ([600 + i for i in range(64)], 512, 700, 16, False),
+    ([1, 64, 130, 2000] * 16, 1024, 40000, 32, False), ([600] * 65, 512, 700, 16, False), ([9000, 4161, 4160], 4160, 9001, 32, True),
+    ([2000] * 5, 448, 3000, 32, False), ([70000, 300], 2048, 530000, 32, False), ([900, 500, 60], 512, 512, 8, False)])
+def test_a_divided_step_of_quest(cuda, lens, top_k, width, heads, avoid):
+    """With the step's division, at the shape of two launches and beside it: selections, cache and
+    answers, to the bit, of the three launches."""
+    kv, dim, bs = 4, 128, len(lens)
+    gen = torch.Generator(device=cuda).manual_seed(bs)
+    rtp = BlockReqToTokenPool(bs + 1, width, sum(n // 64 + 2 for n in lens) + 5, cuda)
+    kvp = Fp8TokenToKVPool(rtp.num_blocks, 1, kv, dim, cuda)
+    be = QuestOnlyBackend(rtp, kvp, {"algorithm": "quest", "top_k": top_k, "quest_page_size": 64, "avoid_recent_overlap": avoid})
+    be.quest.trace = QuestTrace()
+    reqs, had = torch.arange(bs, device=cuda) + 1, [min(max(n - 1, 0), width) for n in lens]
+    total = sum(had)
+    loc, _ = rtp.assign(reqs, i64([0] * bs, cuda), i64(had, cuda), total)
+    pages = torch.randn(total // 64 + 1, kv, dim, device=cuda, generator=gen).repeat_interleave(64, 0)[:total]
+    kvp.set_kv_buffer(0, loc, pages + torch.randn(total, kv, dim, device=cuda, generator=gen),
+                      torch.randn(total, kv, dim, device=cuda, generator=gen))
+    be.quest.update_prefill_representations_blocks(reqs, i64(had, cuda), kvp, rtp.block_table)
+    rtp.check_errors()
+    seq = i64([min(n, width) for n in lens], cuda)
+    for step in range(3):
+        loc, pos = rtp.assign_decode(reqs, seq)
+        batch = ForwardBatch(ForwardMode.DECODE, None, pos, reqs, seq, loc, rtp, kvp, be)
+        q, k, v = (torch.randn(bs, h, dim, device=cuda, generator=gen).bfloat16() for h in (heads, kv, kv))
+        if step == 2:
+            q[:] = 0  # every page scores alike
+        be.init_forward_metadata(batch)
+        be._positions.fill_(-7)
+        out = be.forward(q, k, v, Layer(0, dim), batch)
+        got = be._positions.clone(), kvp.k_codes.clone(), kvp.v_codes.clone(), kvp.k_scale.clone(), kvp.v_scale.clone()
+        be.quest._step.plan = None
+        be._positions.fill_(-7)
+        want = be.forward(q, k, v, Layer(0, dim), batch)
+        assert torch.equal(out, want) and not out.isnan().any()
+        for a, b in zip(got, (be._positions, kvp.k_codes, kvp.v_codes, kvp.k_scale, kvp.v_scale)):
+            assert torch.equal(a, b)
+        seq = torch.where((seq > 0) & (seq < width), seq + 1, seq)
+    rtp.check_errors()
+
+
 def test_pools_that_do_not_go_together(cuda):
     paged, rows = BlockReqToTokenPool(2, 300, 9, cuda), ReqToTokenPool(2, 300, cuda)
     fp8, plain = Fp8TokenToKVPool(9, 1, 2, 128, cuda), MHATokenToKVPool(600, 1, 2, 128, torch.bfloat16, cuda)
