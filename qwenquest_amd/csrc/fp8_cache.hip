@@ -121,7 +121,7 @@ struct PageArgs {
 // lane m has channel m: 15 exchanges for 16 channels instead of 64.
 // Bound: HBM, the codes once (64 * D bytes per page and head, read as they lie).  Measured: two
 // prompts of 16K tokens, 4 heads of 128, 48 layers 161 us (5.3 TB/s, reads and writes); a
-// decode step's page of one request, 8 layers 1.9 us.
+// decode step's page of one request, 8 layers 1.9 us, with the step's slices 3.4.
 template <int D>
 __global__ __launch_bounds__(256) void fp8_page_bounds_kernel(PageArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;

@@ -9,10 +9,14 @@
 // requests' units in a row are cut into equal slices, one to a thread block per (KV head, tile
 // of 16 query heads), so that any mix of lengths fills the chip evenly in one round; a
 // request that lies in one slice is finished there, the others' (m, l, o) parts are merged by
-// the block that completes them.  Two launches: fp8_begin_kernel cuts the slices and stores the
-// new tokens, fp8_attend_kernel does the rest.  The slices depend on the lengths alone: cut once
-// for a step (fp8_plan_kernel), its layers are one launch each, in which the wave that has a
-// request's last block stores the request's new token into it first.
+// the block that completes them.
+//
+// Launches: fp8_begin_kernel cuts the slices, stores the new tokens and selects pages,
+// fp8_attend_kernel does the rest.  The slices depend on the lengths alone: cut once for a step
+// (fp8_plan_kernel, or beside the page bounds), a dense layer is one launch, in which the wave that
+// has a request's last block stores the request's new token into it first; a layer of Quest stores
+// beside the page scores (a selected page may be the one that is written) and selects here, at
+// shapes where a block does that for two requests at most.
 //
 // Of its block's slice a wave takes an eighth, units in a row, and goes through their requests on
 // its own; what a request's end finds in one wave is written by that wave, the rest meets in the
@@ -25,8 +29,8 @@
 // Bound: HBM, the codes once, when they are many: 16 requests of 131072 tokens, 4 heads of 128,
 // 378 us (5.7 TB/s).  A small batch is bound by its chain of memory round trips (slice, table
 // words, scales and codes, partials, count, merge, ~1 us each): one request of 2000 tokens 10.6 us
-// a layer, 15.2 in two launches; the plan 4.4 us a step.  16 requests' 31 pages and window
-// 14.7 us behind a begin launch of 5.3 and the scores' 11.8.
+// a layer, 15.2 in two launches; the plan 4.4 us a step.  16 requests' 31 pages and window of
+// 131072 tokens 17.6 us with the selection, 14.7 behind a begin launch of 5.3.
 #include "qq_fp8_plan.h"
 #include "qq_fp8_store.h"
 #include "qq_quest_dev.h"
