@@ -67,7 +67,7 @@ class DenseBackend(AttentionBackend):
         if self.fp8:
             return fp8_decode_attention(q3, pool, layer.layer_id, self.req_to_token_pool.block_table,
                                         batch.req_pool_indices, batch.seq_lens, layer.scaling,
-                                        new=(batch.out_cache_loc, k, v), plan=batch.decode_plan)
+                                        new=(batch.out_cache_loc, k, v), plan=getattr(batch, "decode_plan", None))
         heads = q3.shape[1]
         rpi = batch.req_pool_indices.to(device=q3.device, dtype=torch.int64).contiguous()
         seq = batch.seq_lens.to(device=q3.device, dtype=torch.int64).contiguous()

@@ -285,6 +285,8 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void fp8_attend_kernel(DecArgs a
   const int s0 = at + (int)((int64_t)(end - at) * wave / kDecWaves), s1 = at + (int)((int64_t)(end - at) * (wave + 1) / kDecWaves);
   const int picked = a.top_k / 64 - 1;  // selected pages; the unit after them is the window
   if (lane < 2) sm.b[2 * wave + lane] = -1;
+  // lengths or requests that have changed since the plan: no answer (0.25 us a layer)
+  const bool stale = context_of(a, item.b) != item.seq || table_row(a, item.b) != item.req;
 
   // The selections of this slice's requests: a slice is no longer than one of them, so there are two
   // at most.
@@ -373,7 +375,7 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void fp8_attend_kernel(DecArgs a
       u_c1 = __shfl(ends, i, 64);
     }
     blk = blk2 = 0;
-    u_bad = row < 0;
+    u_bad = row < 0 || (u_b == item.b ? stale : units_of(a, u_seq) != u_c1 - u_c0);
     const int32_t* tr = a.table + (int64_t)max(row, 0) * a.table_stride;
     auto block_at = [&](int page) {
       const int x = page >= 0 && page < a.table_cols ? tr[page] : 0;

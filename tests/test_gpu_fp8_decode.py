@@ -260,6 +260,26 @@ def test_a_step_divided_once_for_its_layers(cuda, heads, kv, dim, dtype, lens):
     assert torch.equal(a.nan_to_num(), b.nan_to_num())
 
 
+def test_a_plan_of_other_lengths_answers_nothing_wrong(cuda):
+    """Lengths and requests that change behind the plan: the right answer or NaN."""
+    lens = [500, 64, 3000, 1, 200, 700]
+    s = Setup(cuda, lens, 2, 128, spare=4)
+    q, n, reqs = s.queries(8, torch.bfloat16), i64(lens, cuda), torch.arange(6, device=cuda)
+    plan = fp8_decode_plan(s.pool, s.table, reqs, n)
+    lone = [fp8_decode_plan(s.pool, s.table, reqs[i : i + 1], n[i : i + 1]) for i in range(6)]
+    changes = [(n + 1, reqs), (n + 64, reqs), (n - 1, reqs), (n // 2, reqs), (n.flip(0), reqs), (n * 0, reqs), (n, reqs.flip(0))]
+    for m, r in changes:
+        want = fp8_decode_attention(q, s.pool, s.layer, s.table, r, m, 0.1)
+        got = fp8_decode_attention(q, s.pool, s.layer, s.table, r, m, 0.1, plan=plan)
+        ok = got.isnan().all(1) | ((got.float() - want.float()).abs() <= 2**-7 * want.float().abs().amax(1, keepdim=True)).all(1)
+        assert ok.all(), (m, r, ok)
+        for i in range(6):
+            one = fp8_decode_attention(q[i : i + 1], s.pool, s.layer, s.table, r[i : i + 1], m[i : i + 1], 0.1, plan=lone[i])
+            assert one.isnan().all() or ((m[i] == n[i]) & (r[i] == reqs[i]))
+    again = fp8_decode_attention(q, s.pool, s.layer, s.table, reqs, n, 0.1, plan=plan)
+    s.check(again, q, 0.1)
+
+
 def test_a_plan_is_checked(cuda):
     s = Setup(cuda, [100, 100], 2, 64)
     q, r, n = s.queries(4, torch.bfloat16), torch.arange(2), i64([100, 100], cuda)
