@@ -219,6 +219,8 @@ class Fp8TokenToKVPool:
         for x in (k, v):
             if x.numel() != n * self.kv_heads * self.head_dim:
                 raise ValueError(f"expected {n} rows of {self.kv_heads} x {self.head_dim}, got {tuple(x.shape)}")
+            if x.is_cuda and x.device != self.device:
+                raise ValueError(f"k and v must lie on {self.device}, got {x.device}")
             if not x.is_contiguous():
                 x = x.contiguous()
             out.append(x.clone() if x.data_ptr() % 16 else x)
