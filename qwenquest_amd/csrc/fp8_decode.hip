@@ -329,8 +329,15 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void fp8_attend_kernel(DecArgs a
       int c1 = 0x7FFFFFFF;
       if (r == item.b) c1 = item.c1;
       else if (s1 > item.c1 && r < a.bs) c1 = a.cu[r + 1];
-      for (uint64_t tails = __ballot(c1 > s0 && c1 <= s1); tails; tails &= tails - 1)
-        store_token<D>(st, r0 + __builtin_ctzll(tails), h);
+      for (uint64_t tails = __ballot(c1 > s0 && c1 <= s1); tails;) {
+        int mine = -1;  // of the requests at hand, this lane group's
+#pragma unroll
+        for (int i = 0; i < 256 / D; ++i) {
+          if (lane / (D / 4) == i && tails) mine = __builtin_ctzll(tails);
+          tails &= tails - 1;  // (0 stays 0)
+        }
+        store_tokens<D>(st, r0 + mine, mine >= 0, h);
+      }
       more = __builtin_amdgcn_readlane(c1, 63) < s1;
     }
     wait_memory();

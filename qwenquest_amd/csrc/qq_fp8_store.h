@@ -238,18 +238,23 @@ __device__ inline void store_segment(const StoreArgs& a, StoreSmem<D>& sm, int64
   }
 }
 
-// One entry by one wave, K in its first D / 8 lanes and V in the next ones: what store_segment does
-// for a run of one entry.  Its writes are under way when it returns.
+// Single entries by one wave, each by a group of D / 4 lanes, K in the group's first half and V in the
+// second: what store_segment does for runs of one entry.  `i` is the group's entry, if `on`; no two
+// in one block.  The writes are under way when it returns.  Three round trips, for the entries of a
+// wave together (1024 requests of 100 tokens, 4 heads of 64: 23.7 us a layer, with one entry after
+// the other 24.4).
 template <int D>
-__device__ inline void store_token(const StoreArgs& a, int64_t i, int h) {
+__device__ inline void store_tokens(const StoreArgs& a, int64_t i, bool on, int h) {
   constexpr int DG = D / 8;
   const int lane = threadIdx.x & 63, dg = lane % DG;
-  const bool mine = lane < 2 * DG, isv = lane >= DG;
+  const bool isv = lane / DG & 1;
+  if (!on) i = 0;
   const int64_t row = a.loc[i];
-  const int block = block_of(row, a.c.blocks), t = (int)(row & 63);
-  if (block == 0) return;  // wave-uniform
-  const int64_t at = (int64_t)block * a.c.KV + h, from = ((int64_t)i * a.c.KV + h) * D + dg * 8;
-  uint8_t *kc = a.c.kc + at * (64 * D), *vc = a.c.vc + at * (64 * D);
+  const int block = on ? block_of(row, a.c.blocks) : 0, t = (int)(row & 63);
+  const bool mine = block > 0;
+  if (!__any(mine)) return;
+  const int64_t at = (int64_t)block * a.c.KV + h, from = (i * a.c.KV + h) * D + dg * 8;
+  uint8_t* codes = (isv ? a.c.vc : a.c.kc) + at * (64 * D);
   float* scale = (isv ? a.c.vs : a.c.ks) + at;
   const float before = *scale;
   float x[8];
@@ -285,32 +290,32 @@ __device__ inline void store_token(const StoreArgs& a, int64_t i, int h) {
   const float inv = pow2f(-e);
   const uint32_t lo = encode4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
   const uint32_t hi = encode4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
-  // the block's other codes: void, or rounded again
+  // a block's other codes: void, or rounded again; by the whole wave
   const float f = begun ? 0.0f : e > e_old ? pow2f(max(e_old - e, -126)) : 1.0f;
-  bool whole = false;
-#pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    const float fc = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), c ? DG : 0));
-    if (fc == 1.0f) continue;
-    whole = true;
-    uint8_t* codes = c ? vc : kc;
+  uint64_t blocks = __ballot(mine && dg == 0 && f != 1.0f);
+  const bool any = blocks != 0;
+  for (; blocks; blocks &= blocks - 1) {
+    const int from_lane = __builtin_ctzll(blocks);
+    const float fc = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), from_lane));
+    uint8_t* all = (from_lane / DG & 1 ? a.c.vc : a.c.kc) +
+                   ((int64_t)__builtin_amdgcn_readlane(block, from_lane) * a.c.KV + h) * (64 * D);
     for (int q = lane; q < 4 * D; q += 64) {
       uint4 w = make_uint4(0, 0, 0, 0);
       if (fc != 0.0f) {
-        w = *reinterpret_cast<const uint4*>(codes + q * 16);
+        w = *reinterpret_cast<const uint4*>(all + q * 16);
         w = make_uint4(rescale4(w.x, fc), rescale4(w.y, fc), rescale4(w.z, fc), rescale4(w.w, fc));
       }
-      *reinterpret_cast<uint4*>(codes + q * 16) = w;
+      *reinterpret_cast<uint4*>(all + q * 16) = w;
     }
   }
-  if (whole) __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the entry's own codes come after them
+  if (any) __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the entries' own codes come after them
   if (!mine) return;
   if (dg == 0) *scale = bad || lost ? __builtin_nanf("") : pow2f(e);
   if (!isv) {
-    *reinterpret_cast<uint2*>(kc + k_offset(D, t, dg * 8)) = make_uint2(lo, hi);
+    *reinterpret_cast<uint2*>(codes + k_offset(D, t, dg * 8)) = make_uint2(lo, hi);
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) vc[v_offset(t, dg * 8 + j)] = (uint8_t)((j < 4 ? lo : hi) >> (8 * (j & 3)));
+    for (int j = 0; j < 8; ++j) codes[v_offset(t, dg * 8 + j)] = (uint8_t)((j < 4 ? lo : hi) >> (8 * (j & 3)));
   }
 }
 

@@ -292,7 +292,7 @@ struct NewCodes {
   StoreArgs st;
   __device__ inline void operator()(const SelectArgs& a, int b) const {
     if (!st.k) return;
-    for (int h = threadIdx.x >> 6; h < a.KV; h += kThreads / 64) store_token<128>(st, b, h);
+    for (int h = threadIdx.x >> 6; h < a.KV; h += kThreads / 64) store_tokens<128>(st, b, (threadIdx.x & 63) < 32, h);
   }
 };
 
