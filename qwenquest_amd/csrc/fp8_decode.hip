@@ -28,7 +28,7 @@
 // (16 significand bits), three for fp32 (all 24).  fp32 queries go in as three bf16 pieces, too.
 // Bound: HBM, the codes once, when they are many: 16 requests of 131072 tokens, 4 heads of 128,
 // 378 us (5.7 TB/s).  A small batch is bound by its chain of memory round trips (slice, table
-// words, scales and codes, partials, count, merge, ~1 us each): one request of 2000 tokens 10.6 us
+// words, scales and codes, partials, count, merge, ~1 us each): one request of 2000 tokens 10.8 us
 // a layer, 15.2 in two launches; the plan 4.4 us a step.  16 requests' 31 pages and window of
 // 131072 tokens 17.6 us with the selection, 14.7 behind a begin launch of 5.3.
 #include "qq_fp8_plan.h"

@@ -25,7 +25,7 @@
 //
 // Bound: the matrix cores and, beside them, the softmax's vector instructions.  Measured, 32 query
 // heads on 4 of 128: 8192 tokens behind 8192 1494 us (1.10 PFLOP/s of the formula's operations;
-// with bf16 scores 1639, with vector lookups 1797), 3440 tokens of 6 prompts 157 us, where the
+// with bf16 scores 1639, with vector lookups 1797), 3440 tokens of 6 prompts 160 us, where the
 // longest tile chain is as long as the rest.
 #include "qq_extend_dev.h"
 #include "qq_fp8.h"
