@@ -65,9 +65,12 @@ class DenseBackend(AttentionBackend):
         dim = pool.head_dim
         q3 = q.reshape(bs, -1, dim)
         if self.fp8:
+            plan = getattr(batch, "decode_plan", None)
+            if plan is not None and plan.bs != bs:  # a part of the batch that was divided
+                plan = None
             return fp8_decode_attention(q3, pool, layer.layer_id, self.req_to_token_pool.block_table,
                                         batch.req_pool_indices, batch.seq_lens, layer.scaling,
-                                        new=(batch.out_cache_loc, k, v), plan=getattr(batch, "decode_plan", None))
+                                        new=(batch.out_cache_loc, k, v), plan=plan)
         heads = q3.shape[1]
         rpi = batch.req_pool_indices.to(device=q3.device, dtype=torch.int64).contiguous()
         seq = batch.seq_lens.to(device=q3.device, dtype=torch.int64).contiguous()

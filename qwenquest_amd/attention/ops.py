@@ -9,12 +9,13 @@ device, in float32.
 
 from __future__ import annotations
 
-from typing import TYPE_CHECKING, NamedTuple
+from typing import TYPE_CHECKING
 
 import torch
 import torch.nn.functional as F
 
 from qwenquest_amd import _lib
+from qwenquest_amd.batch import DecodePlan
 
 if TYPE_CHECKING:
     from qwenquest_amd.paged import Fp8TokenToKVPool
@@ -244,15 +245,8 @@ def _queries(q: torch.Tensor, pool: Fp8TokenToKVPool) -> torch.Tensor:
     return q.clone() if q.data_ptr() % 16 else q
 
 
-class Fp8DecodePlan(NamedTuple):
-    """A decode batch of ``bs`` requests divided for the chip (``fp8_decode_plan``)."""
-
-    bs: int
-    workspace: torch.Tensor
-
-
 def fp8_decode_plan(pool: Fp8TokenToKVPool, block_table: torch.Tensor, req_pool_indices: torch.Tensor,
-                    seq_lens: torch.Tensor) -> Fp8DecodePlan:
+                    seq_lens: torch.Tensor) -> DecodePlan:
     """What ``fp8_decode_attention`` over whole contexts makes of a step's lengths, once for the step's
     layers, on the current stream."""
     dev = pool.device
@@ -262,10 +256,11 @@ def fp8_decode_plan(pool: Fp8TokenToKVPool, block_table: torch.Tensor, req_pool_
     seq = _lengths(seq_lens, bs, dev, "seq_lens")
     need = int(_lib.load().qq_fp8_decode_workspace_bytes(bs, pool.kv_heads, pool.kv_heads, pool.head_dim))
     ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+    stream = _lib.stream(dev)
     with _lib.on(dev):
         _lib.call("qq_fp8_decode_plan", pool.num_blocks, pool.kv_heads, pool.head_dim, bt.shape[0], bt.shape[1],
-                  _lib.ptr(rpi), _lib.ptr(seq), bs, _lib.ptr(ws), need, _lib.stream(dev))
-    return Fp8DecodePlan(bs, ws)
+                  _lib.ptr(rpi), _lib.ptr(seq), bs, _lib.ptr(ws), need, stream)
+    return DecodePlan(bs, ws, stream, torch.cuda.is_current_stream_capturing())
 
 
 def fp8_decode_attention(
@@ -280,7 +275,7 @@ def fp8_decode_attention(
     positions: torch.Tensor | None = None,
     top_k: int = 0,
     new: tuple[torch.Tensor, torch.Tensor, torch.Tensor] | None = None,
-    plan: Fp8DecodePlan | None = None,
+    plan: DecodePlan | None = None,
 ) -> torch.Tensor:
     """Decode over an 8-bit pool: request ``i`` attends ``q[i] [H, D]`` over its first ``seq_lens[i]``
     tokens in the blocks ``block_table[req_pool_indices[i]]``, or, with ``positions [bs, >= top_k]``
@@ -289,7 +284,8 @@ def fp8_decode_attention(
     ``plan``: this step's ``fp8_decode_plan`` (of the same pool, table, requests and lengths, on the
     same stream; not with ``positions``): up to 16 query heads per KV head then run as one launch,
     for which each new token lies in the last block of its own request's context and no two in one
-    block (rows of block 0, the padding, aside).
+    block (rows of block 0, the padding, aside); on another stream, or where one of the two calls is
+    in a graph capture and the other is not, they run as without it.
     Returns ``[bs, H*D]`` in q's dtype (bf16 or fp32): zeros for an empty context, NaN for a request
     outside the table or a context past its blocks."""
     dev = pool.device
@@ -310,7 +306,8 @@ def fp8_decode_attention(
     if plan is not None and positions is not None:
         raise ValueError("a plan is of whole contexts, not of selected pages")
     need = int(_lib.load().qq_fp8_decode_workspace_bytes(bs, heads, pool.kv_heads, dim))
-    if plan is not None and heads <= 16 * pool.kv_heads:
+    stream = _lib.stream(dev)
+    if plan is not None and heads <= 16 * pool.kv_heads and plan.usable(stream):
         ws = plan.workspace
         if plan.bs != bs or ws.device != dev or ws.numel() != max(need, 1):
             raise ValueError("plan is not fp8_decode_plan's of this batch and pool")
@@ -324,7 +321,7 @@ def fp8_decode_attention(
             _lib.ptr(vn), _lib.DTYPE_BF16 if kn is None else _lib.dtype_code(kn.dtype), _lib.ptr(loc),
             *pool.layer_args(layer_id), *_table_args(bt), _lib.ptr(rpi), _lib.ptr(seq), bs, _lib.ptr(positions),
             0 if positions is None else max(positions.stride(0), positions.shape[1]), int(top_k), float(scaling),
-            _lib.ptr(out), _lib.ptr(ws), need, int(plan is not None), _lib.stream(dev),
+            _lib.ptr(out), _lib.ptr(ws), need, int(plan is not None), stream,
         )
     return out
 
@@ -346,7 +343,8 @@ def fp8_quest_step(
     """One layer of Quest decode over an 8-bit pool, after ``quest.decode_step_blocks``: the new tokens
     ``k``/``v`` go to rows ``loc``, the page scores select (``positions [>= bs, top_k]`` int32 is
     written, as ``QuestAlgorithm.retrieve_topk`` writes it), and ``q [bs, H, D]`` attends the selected
-    pages.  On the stream of ``decode_step_blocks``; each new token lies in the last block of its own
+    pages.  On the stream of ``decode_step_blocks``, both in the same graph capture or in none, the
+    step's division of the work saves a launch; each new token lies in the last block of its own
     request's context and no two in one block (rows of block 0 aside).  ``phase``: 1 = scoring and selection, 2 = store and attention after phase 1, 3 = both.
     Returns ``[bs, H*D]`` (complete after phase 2)."""
     dev, step = pool.device, quest._step
@@ -371,8 +369,9 @@ def fp8_quest_step(
     kn, vn = pool.new_rows(k, v, bs)
     out = torch.empty((bs, heads * dim), dtype=q.dtype, device=dev)
     need = int(_lib.load().qq_fp8_decode_workspace_bytes(bs, heads, pool.kv_heads, dim))
-    planned = step.plan is not None and heads <= 16 * pool.kv_heads and step.top_k == quest.top_k
-    ws = step.plan if planned else torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+    stream = _lib.stream(dev)
+    planned = step.plan is not None and heads <= 16 * pool.kv_heads and step.plan.usable(stream)
+    ws = step.plan.workspace if planned else torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
     with _lib.on(dev):
         _lib.call(
             "qq_fp8_quest_step", _lib.ptr(q), _lib.dtype_code(q.dtype), q.stride(0), heads, _lib.ptr(kn), _lib.ptr(vn),
@@ -380,7 +379,7 @@ def fp8_quest_step(
             _lib.ptr(quest.page_k_bounds), layer_id - quest.start_layer, _lib.ptr(rpi), _lib.ptr(step.seq_lens),
             _lib.ptr(step.candidate_limit_i32), bs, quest.max_reqs, quest.max_pages_per_req, quest.top_k, float(scaling),
             _lib.ptr(quest._scores_ws), _lib.ptr(positions), _lib.ptr(out), _lib.ptr(ws), need, int(phase), int(planned),
-            _lib.stream(dev),
+            stream,
         )
     return out
 

@@ -4,14 +4,14 @@ from __future__ import annotations
 
 import enum
 from dataclasses import dataclass
-from typing import TYPE_CHECKING, Any
+from typing import TYPE_CHECKING, Any, NamedTuple
 
 import torch
 
 if TYPE_CHECKING:
     from qwenquest_amd.memory import MHATokenToKVPool, ReqToTokenPool
 
-__all__ = ["ForwardBatch", "ForwardMode"]
+__all__ = ["DecodePlan", "ForwardBatch", "ForwardMode"]
 
 
 class ForwardMode(enum.Enum):
@@ -23,6 +23,20 @@ class ForwardMode(enum.Enum):
 
     def is_decode(self) -> bool:
         return self is ForwardMode.DECODE
+
+
+class DecodePlan(NamedTuple):
+    """A decode batch of ``bs`` requests over an 8-bit pool, divided for the chip once for a step's
+    layers.  It holds for the stream that made it, and inside a graph capture for what that capture
+    records: elsewhere its memory may not be written yet, or no longer be its own."""
+
+    bs: int
+    workspace: torch.Tensor
+    stream: int
+    captured: bool
+
+    def usable(self, stream: int) -> bool:
+        return self.stream == stream and self.captured == torch.cuda.is_current_stream_capturing()
 
 
 @dataclass
@@ -41,7 +55,7 @@ class ForwardBatch:
     extend_prefix_lens: torch.Tensor | None = None
     extend_seq_lens: torch.Tensor | None = None
     #: set by a backend's init_forward_metadata: a decode step's work, divided once for its layers
-    decode_plan: Any = None
+    decode_plan: DecodePlan | None = None
 
     @property
     def batch_size(self) -> int:

@@ -27,6 +27,7 @@ from typing import TYPE_CHECKING
 import torch
 
 from qwenquest_amd import _lib
+from qwenquest_amd.batch import DecodePlan
 
 if TYPE_CHECKING:
     from qwenquest_amd.paged import Fp8TokenToKVPool
@@ -50,8 +51,8 @@ class StepLayout:
     candidate_limit_i32: torch.Tensor  # [bs] int32  pages >= this are never candidates
     page_size: int
     top_k: int
-    #: over an 8-bit pool: the workspace into which the step's attention is divided
-    plan: torch.Tensor | None = None
+    #: over an 8-bit pool: the division of the step's attention
+    plan: DecodePlan | None = None
 
     @property
     def candidate_limit(self) -> torch.Tensor:
@@ -380,22 +381,26 @@ class QuestAlgorithm:
         if any(t is not None and t.numel() != bs for t in lens):
             raise ValueError("req_indices, seq_lens and prefix_lens differ in length")
         codes, _, scale, _, *geometry = pool.layer_args(self.start_layer)
-        actual = limit = plan = None
+        actual = limit = ws = None
         if decode:
             actual, limit = torch.empty((2, bs), dtype=torch.int32, device=self.device).unbind(0)
             need = int(_lib.load().qq_fp8_decode_workspace_bytes(bs, self.kv_heads, self.kv_heads, self.head_dim))
             # of this step alone: a graph's replay must not find another step's division in it
-            plan = torch.empty(max(need, 1), dtype=torch.uint8, device=self.device)
+            ws = torch.empty(max(need, 1), dtype=torch.uint8, device=self.device)
+        stream = _lib.stream(self.device)
         with _lib.on(self.device):
             _lib.call(
                 "qq_fp8_page_bounds", codes, pool.k_codes.stride(0), scale, pool.k_scale.stride(0), *geometry,
                 _lib.ptr(block_table), max(block_table.stride(0), block_table.shape[1]), block_table.shape[0],
                 block_table.shape[1], *(_lib.ptr(t) for t in lens), bs, int(decode), int(max_new), self.num_layers,
                 _lib.ptr(self.page_k_bounds), self.max_reqs, self.max_pages_per_req, self.top_k,
-                int(self.avoid_recent_overlap), _lib.ptr(actual), _lib.ptr(limit), _lib.ptr(plan),
-                0 if plan is None else plan.numel(), _lib.stream(self.device),
+                int(self.avoid_recent_overlap), _lib.ptr(actual), _lib.ptr(limit), _lib.ptr(ws),
+                0 if ws is None else ws.numel(), stream,
             )
-        return StepLayout(lens[1], actual, limit, self.page_size, self.top_k, plan) if decode else None
+        if not decode:
+            return None
+        plan = DecodePlan(bs, ws, stream, torch.cuda.is_current_stream_capturing())
+        return StepLayout(lens[1], actual, limit, self.page_size, self.top_k, plan)
 
     def update_prefill_representations_blocks(
         self,

@@ -186,6 +186,73 @@ def test_decode_steps_in_a_replayed_graph(cuda):
     e.rtp.poll_errors()
 
 
+@pytest.mark.parametrize("backend", ["dense", "quest"])
+def test_a_step_s_division_stays_with_its_stream_and_capture(cuda, backend):
+    """Layers on another stream, layers captured without their init_forward_metadata and replayed as
+    lengths grow (dense), eager layers behind a capture that never ran, a part of the batch."""
+    from dataclasses import replace
+
+    e, w = (Engine(cuda, backend, 1, 32, 4, 128, torch.bfloat16, 3, 5000, 100, top_k=512, seed=5) for _ in range(2))
+    for x in (e, w):
+        if backend == "quest":
+            x.be.quest.trace = None
+        x.prefill([0, 1, 2], [700, 63, 2000])
+    rpi, seq = torch.arange(3, device=cuda), i64([701, 64, 2001], cuda)
+    q, k, v = (torch.zeros(3, h, 128, device=cuda, dtype=torch.bfloat16) for h in (32, 4, 4))
+
+    def begin(x):
+        loc, pos = x.rtp.assign_decode(rpi, seq)
+        batch = ForwardBatch(ForwardMode.DECODE, None, pos, rpi, seq, loc, x.rtp, x.kvp, x.be)
+        x.be.init_forward_metadata(batch)
+        return batch
+
+    def layer(x, batch):
+        return x.be.forward(q, k, v, x.mods[0], batch)
+
+    def same(out):
+        want = layer(w, begin(w))
+        assert not want.isnan().any() and torch.allclose(out.float(), want.float(), rtol=2**-7, atol=2**-9)
+        assert torch.equal(e.kvp.k_codes, w.kvp.k_codes) and torch.equal(e.kvp.v_scale, w.kvp.v_scale)
+
+    def more():
+        seq.add_(1)
+        for t in (q, k, v):
+            t.normal_(generator=e.gen)
+
+    more()
+    side, batch = torch.cuda.Stream(), begin(e)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = layer(e, batch)
+    torch.cuda.current_stream().wait_stream(side)
+    same(out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layer(e, batch)
+    for _ in range(3 if backend == "dense" else 0):
+        more()
+        loc, _ = e.rtp.assign_decode(rpi, seq)
+        batch.out_cache_loc.copy_(loc)
+        e.be.init_forward_metadata(batch)
+        graph.replay()
+        same(out)
+    more()
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        captured = begin(e)
+        layer(e, captured)
+    e.rtp.assign_decode(rpi, seq)
+    eager = begin(e)
+    if backend == "dense":  # (Quest's layout of the capture has no values yet)
+        eager.decode_plan = captured.decode_plan
+        part = replace(eager, decode_plan=begin(e).decode_plan, req_pool_indices=rpi[:2], seq_lens=seq[:2],
+                       out_cache_loc=eager.out_cache_loc[:2])
+        whole = layer(e, eager)
+        assert torch.allclose(e.be.forward(q[:2], k[:2], v[:2], e.mods[0], part).float(), whole[:2].float(), rtol=2**-7, atol=2**-9)
+    else:
+        e.be.quest._step.plan = e.be.quest._step.plan._replace(captured=True)
+    same(layer(e, eager))
+
+
 def test_padded_entries_of_a_decode_batch(cuda):
     """seq_lens 0: no row, no token stored, an output of zeros."""
     e = Engine(cuda, "dense", 1, 4, 2, 128, torch.bfloat16, 3, 300, 20)
