@@ -723,7 +723,8 @@ void launch(const DecArgs& a, const StoreArgs& st, const SelectArgs& sel, bool p
 // Whether a planned step of Quest runs as two launches: the scores with the new tokens, and an
 // attention that selects by itself.  A slice must not be longer than a request's selection (at
 // most as many requests as the grid has slices, and 8 units, fp8_slice_len's least), so that a block
-// selects for two requests at most.
+// selects for two requests at most.  (A layer of one request of 32768 tokens 17.2 us against 19.3 in
+// three launches, of 16 of 131072 36.8 against 38.8.)
 bool selects_itself(const DecArgs& a, const SelectArgs& sel, int q_dtype) {
   return q_dtype == QQ_DTYPE_BF16 && a.c.D == 128 && a.tiles == 1 && a.bs <= a.max_slices && sel.top_k >= 8 * 64 &&
          sel.k_sel <= 64 && sel.MP > 0 && max(sel.MP, sel.k_sel) <= 16 * 64 * kDecWaves &&
