@@ -486,10 +486,15 @@ int qq_fp8_decode_attention(const void* q, int q_dtype, int64_t q_batch_stride, 
                             int planned, void* stream);
 int64_t qq_fp8_decode_workspace_bytes(int bs, int num_q_heads, int kv_heads, int head_dim);
 
+/* The graph capture that `stream` is in: a number of that capture's own, 0 outside of any, -1 where
+ * the runtime does not say.  What a capture records fills its memory when the graph runs, so a
+ * plan made in one serves the calls of that same one. */
+int64_t qq_stream_capture_id(void* stream);
+
 /* The part of qq_fp8_decode_attention that depends on a step's lengths alone, once for its layers:
  * divides the batch into `workspace` (>= qq_fp8_decode_workspace_bytes(bs, kv_heads, kv_heads,
  * head_dim)), with which calls for the same requests, lengths, table and cache geometry, without
- * positions, on the same stream pass planned != 0 and run as one launch each, at up to 16 query
+ * positions, on the same stream and in the same graph capture or in none pass planned != 0 and run as one launch each, at up to 16 query
  * heads per KV head (others as without a plan, with a workspace of their own size).  In a planned
  * call each new token lies in the last block of its own request's context, no two in one block,
  * or in no block (rows of block 0).  A plan of another bs or top_k writes nothing; requests whose
@@ -504,7 +509,7 @@ int qq_fp8_decode_plan(int num_blocks, int kv_heads, int head_dim, int block_tab
  * and the attention over the selected pages (as qq_fp8_decode_attention).  Three launches: the
  * scores; the selection with the store; the attention.  planned != 0: workspace is the plan that
  * this step's qq_fp8_page_bounds made (same requests, lengths, table, geometry and top_k, on the same
- * stream; up to 16 query heads per KV head, others as without), for which the new tokens lie as
+ * stream and in the same graph capture or in none; up to 16 query heads per KV head, others as without), for which the new tokens lie as
  * in a planned qq_fp8_decode_attention.  bf16 at 4 KV heads x 128 with 2 to 8 query heads each,
  * top_k of 512 to 4160, up to 8192 pages and 64 requests then takes two launches: the scores with the
  * store; the selection with the attention.  phase 1 = scores and selection, 2 = store

@@ -119,6 +119,7 @@ SIGNATURES: dict[str, tuple] = {
         [_P, _I, _L, _I, _P, _P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _P, _L, _I, _I, _P, _P, _I, _P, _L, _I, _F,
          _P, _P, _L, _I, _P],
     ),
+    "qq_stream_capture_id": (_L, [_P]),
     "qq_fp8_decode_plan": (_I, [_I, _I, _I, _I, _I, _P, _P, _I, _P, _L, _P]),
     "qq_fp8_decode_workspace_bytes": (_L, [_I, _I, _I, _I]),
     "qq_fp8_quest_step": (
@@ -212,6 +213,14 @@ def stream(device: torch.device | None = None) -> int:
     index = device.index if device is not None else None
     # the handle alone: a Stream object for it costs a call 2 us
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
+
+
+def capture_id(device: torch.device, stream: int) -> int:
+    """The graph capture that ``stream`` of ``device`` is in, as a number of its own: 0 for none, -1 where
+    the runtime does not say.  (``torch.cuda.graph`` captures on one stream, which does not
+    tell its captures apart.)"""
+    with on(device):
+        return load().qq_stream_capture_id(stream)
 
 
 class _Same:

@@ -260,7 +260,7 @@ def fp8_decode_plan(pool: Fp8TokenToKVPool, block_table: torch.Tensor, req_pool_
     with _lib.on(dev):
         _lib.call("qq_fp8_decode_plan", pool.num_blocks, pool.kv_heads, pool.head_dim, bt.shape[0], bt.shape[1],
                   _lib.ptr(rpi), _lib.ptr(seq), bs, _lib.ptr(ws), need, stream)
-    return DecodePlan(bs, ws, stream, torch.cuda.is_current_stream_capturing())
+    return DecodePlan(bs, ws, stream, _lib.capture_id(dev, stream))
 
 
 def fp8_decode_attention(
@@ -284,8 +284,8 @@ def fp8_decode_attention(
     ``plan``: this step's ``fp8_decode_plan`` (of the same pool, table, requests and lengths, on the
     same stream; not with ``positions``): up to 16 query heads per KV head then run as one launch,
     for which each new token lies in the last block of its own request's context and no two in one
-    block (rows of block 0, the padding, aside); on another stream, or where one of the two calls is
-    in a graph capture and the other is not, they run as without it.
+    block (rows of block 0, the padding, aside); on another stream, or where the two calls are not in
+    the same graph capture or both in none, they run as without it.
     Returns ``[bs, H*D]`` in q's dtype (bf16 or fp32): zeros for an empty context, NaN for a request
     outside the table or a context past its blocks."""
     dev = pool.device

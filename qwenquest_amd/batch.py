@@ -8,6 +8,8 @@ from typing import TYPE_CHECKING, Any, NamedTuple
 
 import torch
 
+from qwenquest_amd import _lib
+
 if TYPE_CHECKING:
     from qwenquest_amd.memory import MHATokenToKVPool, ReqToTokenPool
 
@@ -27,16 +29,17 @@ class ForwardMode(enum.Enum):
 
 class DecodePlan(NamedTuple):
     """A decode batch of ``bs`` requests over an 8-bit pool, divided for the chip once for a step's
-    layers.  It holds for the stream that made it, and inside a graph capture for what that capture
-    records: elsewhere its memory may not be written yet, or no longer be its own."""
+    layers.  It holds for the stream that made it, and inside a graph capture for what that same
+    capture records: elsewhere its memory may not be written yet, or no longer be its own."""
 
     bs: int
     workspace: torch.Tensor
     stream: int
-    captured: bool
+    #: the capture's number (``_lib.capture_id``), 0 outside of any
+    captured: int
 
     def usable(self, stream: int) -> bool:
-        return self.stream == stream and self.captured == torch.cuda.is_current_stream_capturing()
+        return self.stream == stream and self.captured == _lib.capture_id(self.workspace.device, stream) >= 0
 
 
 @dataclass

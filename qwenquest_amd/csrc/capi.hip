@@ -1,4 +1,4 @@
-// Library-level entry points: version and error reporting.
+// Library-level entry points: version, error reporting, a stream's capture.
 #include <stdarg.h>
 #include <string.h>
 
@@ -28,3 +28,14 @@ int check_launch(const char* what) {
 extern "C" int qq_version(void) { return 100; }
 
 extern "C" const char* qq_last_error(void) { return qq::g_last_error; }
+
+extern "C" int64_t qq_stream_capture_id(void* stream) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (hipStreamGetCaptureInfo(static_cast<hipStream_t>(stream), &status, &id) != hipSuccess) {
+    (void)hipGetLastError();
+    return -1;
+  }
+  if (status == hipStreamCaptureStatusNone) return 0;
+  return status == hipStreamCaptureStatusActive ? (int64_t)(id + 1) : -1;
+}

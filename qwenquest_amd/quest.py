@@ -399,7 +399,7 @@ class QuestAlgorithm:
             )
         if not decode:
             return None
-        plan = DecodePlan(bs, ws, stream, torch.cuda.is_current_stream_capturing())
+        plan = DecodePlan(bs, ws, stream, _lib.capture_id(self.device, stream))
         return StepLayout(lens[1], actual, limit, self.page_size, self.top_k, plan)
 
     def update_prefill_representations_blocks(

@@ -14,6 +14,7 @@ import torch
 
 from oracle import fp8_cache as of
 from qwenquest_amd import _lib
+from qwenquest_amd.batch import DecodePlan
 from qwenquest_amd.paged import BlockReqToTokenPool, Fp8TokenToKVPool
 from tests.test_launch_shapes import CSRC, shutil
 
@@ -156,6 +157,21 @@ def test_decode_workspace(lib):
     assert lib.qq_fp8_decode_workspace_bytes(2, 30, 4, 128) == 0
     small, large = (lib.qq_fp8_decode_workspace_bytes(bs, 32, 4, 128) for bs in (1, 1000))
     assert 0 < small < large < 32 << 20
+
+
+def test_a_plan_is_its_capture_s(monkeypatch):
+    """A plan made in one graph capture, or in none, is of no use in another."""
+    ids = {11: 0, 12: 5}
+    monkeypatch.setattr(_lib, "capture_id", lambda device, stream: ids[stream])
+    ws = torch.empty(1)
+    eager, captured, unsaid = (DecodePlan(2, ws, s, i) for s, i in ((11, 0), (12, 5), (12, -1)))
+    assert eager.usable(11) and captured.usable(12) and not eager.usable(12) and not captured.usable(11)
+    ids.update({11: 6, 12: 6})  # two other captures on those streams
+    assert not eager.usable(11) and not captured.usable(12)
+    ids[12] = 0
+    assert not captured.usable(12)
+    ids[12] = -1  # the runtime does not say
+    assert not unsaid.usable(12)
 
 
 # ---------------------------------------------------------------- the division of the work

@@ -253,6 +253,51 @@ def test_a_step_s_division_stays_with_its_stream_and_capture(cuda, backend):
     same(layer(e, eager))
 
 
+@pytest.mark.parametrize("backend", ["dense", "quest"])
+def test_a_step_captured_apart_from_its_layers(cuda, backend):
+    """init_forward_metadata in one graph, the layers in another: both are captured on the same stream,
+    and the layers do not rely on memory of the first graph that a plan would lie in."""
+    e, w = (Engine(cuda, backend, 1, 32, 4, 128, torch.bfloat16, 3, 5000, 100, top_k=512, seed=9) for _ in range(2))
+    for x in (e, w):
+        if backend == "quest":
+            x.be.quest.trace = None
+        x.prefill([0, 1, 2], [700, 63, 2000])
+    rpi, seq = torch.arange(3, device=cuda), i64([701, 64, 2001], cuda)
+    loc = torch.zeros(3, dtype=torch.int64, device=cuda)
+    q, k, v = (torch.zeros(3, h, 128, device=cuda, dtype=torch.bfloat16) for h in (32, 4, 4))
+
+    def batch_of(x, rows):
+        return ForwardBatch(ForwardMode.DECODE, None, None, rpi, seq, rows, x.rtp, x.kvp, x.be)
+
+    batch = batch_of(e, loc)
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    with torch.cuda.graph(graphs[0]):
+        e.be.init_forward_metadata(batch)
+    plan = batch.decode_plan if backend == "dense" else e.be.quest._step.plan
+    assert plan.captured > 0 and not plan.usable(plan.stream)
+    with torch.cuda.graph(graphs[1]):
+        stream = torch.cuda.current_stream().cuda_stream
+        assert stream == plan.stream and not plan.usable(stream)
+        out = e.be.forward(q, k, v, e.mods[0], batch)
+    plan.workspace.fill_(255)  # nothing reads it
+    for step in range(4):
+        if step:
+            seq.add_(1)
+        for t in (q, k, v):
+            t.normal_(generator=e.gen)
+        loc.copy_(e.rtp.assign_decode(rpi, seq)[0])
+        if backend == "quest" or step % 2:  # (Quest's layout comes from the first graph)
+            graphs[0].replay()
+            plan.workspace.fill_(255)
+        graphs[1].replay()
+        rows, _ = w.rtp.assign_decode(rpi, seq)
+        other = batch_of(w, rows)
+        w.be.init_forward_metadata(other)
+        want = w.be.forward(q, k, v, w.mods[0], other)
+        assert not want.isnan().any() and torch.equal(out, want)
+        assert torch.equal(e.kvp.k_codes, w.kvp.k_codes) and torch.equal(e.kvp.v_scale, w.kvp.v_scale)
+
+
 def test_padded_entries_of_a_decode_batch(cuda):
     """seq_lens 0: no row, no token stored, an output of zeros."""
     e = Engine(cuda, "dense", 1, 4, 2, 128, torch.bfloat16, 3, 300, 20)
