@@ -497,7 +497,8 @@ int64_t qq_stream_capture_id(void* stream);
  * positions, on the same stream and in the same graph capture or in none pass planned != 0 and run as one launch each, at up to 16 query
  * heads per KV head (others as without a plan, with a workspace of their own size).  In a planned
  * call each new token lies in the last block of its own request's context, no two in one block,
- * or in no block (rows of block 0).  A plan of another bs or top_k writes nothing; requests whose
+ * or in no block (rows of block 0).  With a plan of another bs or top_k every output is NaN and, without
+ * positions, no new token is stored; requests whose
  * lengths or table rows have changed since get NaN, where what changed matters to the plan. */
 int qq_fp8_decode_plan(int num_blocks, int kv_heads, int head_dim, int block_table_rows, int block_table_cols,
                        const int64_t* req_pool_indices, const int64_t* seq_lens, int bs, void* workspace,

@@ -309,7 +309,7 @@ def fp8_decode_attention(
     stream = _lib.stream(dev)
     if plan is not None and heads <= 16 * pool.kv_heads and plan.usable(stream):
         ws = plan.workspace
-        if plan.bs != bs or ws.device != dev or ws.numel() != max(need, 1):
+        if plan.bs != bs or plan.top_k != 0 or ws.device != dev or ws.numel() != max(need, 1):
             raise ValueError("plan is not fp8_decode_plan's of this batch and pool")
     else:
         # of this call alone: it holds the division of the batch, which a graph's replay or a call on
@@ -372,6 +372,8 @@ def fp8_quest_step(
     stream = _lib.stream(dev)
     planned = step.plan is not None and heads <= 16 * pool.kv_heads and step.plan.usable(stream)
     ws = step.plan.workspace if planned else torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+    if planned and (step.plan.bs != bs or step.plan.top_k != quest.top_k or ws.device != dev or ws.numel() != max(need, 1)):
+        raise ValueError("the step's plan is not decode_step_blocks' of this batch and pool")
     with _lib.on(dev):
         _lib.call(
             "qq_fp8_quest_step", _lib.ptr(q), _lib.dtype_code(q.dtype), q.stride(0), heads, _lib.ptr(kn), _lib.ptr(vn),

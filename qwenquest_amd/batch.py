@@ -37,6 +37,8 @@ class DecodePlan(NamedTuple):
     stream: int
     #: the capture's number (``_lib.capture_id``), 0 outside of any
     captured: int
+    #: tokens that a longer context selects (Quest), or 0: contexts are whole
+    top_k: int = 0
 
     def usable(self, stream: int) -> bool:
         return self.stream == stream and self.captured == _lib.capture_id(self.workspace.device, stream) >= 0

@@ -274,12 +274,19 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void fp8_attend_kernel(DecArgs a
   const int head = blockIdx.x % a.heads, slice = blockIdx.x / a.heads;
   const DecPlan plan = *a.plan;
   const DecItem item = a.items[slice];  // both in one round trip; stale past the last slice
-  if (slice >= plan.slices || plan.bs != a.bs || plan.top_k != a.top_k) return;  // another batch's plan answers nothing
   const int h = head / a.tiles, tile = head - h * a.tiles;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int m16 = lane & 15, g = lane >> 4;
   const int rows = min(a.G - tile * kTile, kTile);  // query heads of this tile
   const int q_head = h * a.G + tile * kTile;
+  if (plan.bs != a.bs || plan.top_k != a.top_k) {  // another batch's plan: no answer to any request
+    const float nan = __builtin_nanf("");
+    for (int b = slice; b < a.bs; b += a.max_slices)
+      for (int i = tid; i < rows * (D / 4); i += 64 * kDecWaves)
+        store4(static_cast<T*>(a.out) + ((int64_t)b * a.H + q_head) * D + i * 4, nan, nan, nan, nan);
+    return;
+  }
+  if (slice >= plan.slices) return;
   const int at = slice * plan.len, end = min(at + plan.len, plan.total);
   // this wave's units
   const int s0 = at + (int)((int64_t)(end - at) * wave / kDecWaves), s1 = at + (int)((int64_t)(end - at) * (wave + 1) / kDecWaves);

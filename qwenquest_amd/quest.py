@@ -399,7 +399,7 @@ class QuestAlgorithm:
             )
         if not decode:
             return None
-        plan = DecodePlan(bs, ws, stream, _lib.capture_id(self.device, stream))
+        plan = DecodePlan(bs, ws, stream, _lib.capture_id(self.device, stream), self.top_k)
         return StepLayout(lens[1], actual, limit, self.page_size, self.top_k, plan)
 
     def update_prefill_representations_blocks(

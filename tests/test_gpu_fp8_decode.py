@@ -10,6 +10,7 @@ import torch
 from oracle import fp8_cache as of
 from qwenquest_amd.attention.ops import fp8_decode_attention, fp8_decode_plan
 from qwenquest_amd.paged import Fp8TokenToKVPool
+from qwenquest_amd.quest import QuestAlgorithm
 
 pytestmark = pytest.mark.gpu
 
@@ -295,6 +296,32 @@ def test_a_plan_is_checked(cuda):
                              positions=torch.zeros(2, 64, dtype=torch.int32, device=cuda))
     s.check(fp8_decode_attention(q, s.pool, s.layer, s.table, r, n, 0.1, plan=plan), q, 0.1)
     assert fp8_decode_plan(s.pool, s.table, r[:0], n[:0]).bs == 0
+
+
+@pytest.mark.parametrize("heads, kv, dim, dtype", [(32, 4, 128, torch.bfloat16), (3, 3, 64, torch.float32), (10, 1, 128, torch.bfloat16)])
+def test_a_plan_of_another_batch_answers_nan(cuda, heads, kv, dim, dtype):
+    """Plans of other requests, or of selections, that do not show it: every output written, and NaN; the
+    cache as it was.  Those that show it are refused."""
+    lens = [500, 64, 0, 1300]
+    s = Setup(cuda, lens, kv, dim)
+    q, reqs, n = s.queries(heads, dtype), torch.arange(4, device=cuda), i64(lens, cuda)
+    rows = torch.cat([s.rows(r, [max(m, 1) - 1]) for r, m in enumerate(lens)])
+    new = (rows, *(torch.randn(4, kv, dim, device=cuda, dtype=dtype) for _ in range(2)))
+    few = fp8_decode_plan(s.pool, s.table, reqs[:3], n[:3])
+    quest = QuestAlgorithm(128, 64, cuda)
+    quest.init_storage(0, 2, 4, s.table.shape[1] * 64, kv, dim)
+    sparse = quest.decode_step_blocks(reqs, n, s.pool, s.table).plan
+    before = s.pool.k_codes.clone(), s.pool.v_scale.clone()
+    for plan in (few._replace(bs=4), sparse._replace(top_k=0)):
+        junk = torch.full((4, heads * dim), 7.0, device=cuda, dtype=dtype)  # what the allocator may hand out again
+        del junk
+        out = fp8_decode_attention(q, s.pool, s.layer, s.table, reqs, n, 0.1, new=new, plan=plan)
+        assert out.isnan().all()
+        assert torch.equal(before[0], s.pool.k_codes) and torch.equal(before[1], s.pool.v_scale)
+    for plan in (few, sparse):
+        with pytest.raises(ValueError, match="plan"):
+            fp8_decode_attention(q, s.pool, s.layer, s.table, reqs, n, 0.1, plan=plan)
+    s.check(fp8_decode_attention(q, s.pool, s.layer, s.table, reqs, n, 0.1, plan=fp8_decode_plan(s.pool, s.table, reqs, n)), q, 0.1)
 
 
 def test_arguments_are_checked(cuda):

@@ -298,6 +298,29 @@ def test_a_step_captured_apart_from_its_layers(cuda, backend):
         assert torch.equal(e.kvp.k_codes, w.kvp.k_codes) and torch.equal(e.kvp.v_scale, w.kvp.v_scale)
 
 
+def test_a_quest_step_refuses_another_step_s_plan(cuda):
+    from qwenquest_amd.attention.ops import fp8_decode_plan
+
+    e = Engine(cuda, "quest", 1, 16, 4, 128, torch.bfloat16, 2, 2000, 70, top_k=512)
+    e.be.quest.trace = None
+    e.prefill([0, 1], [700, 63])
+    rpi, seq = i64([0, 1], cuda), i64([701, 64], cuda)
+    loc, pos = e.rtp.assign_decode(rpi, seq)
+    batch = ForwardBatch(ForwardMode.DECODE, None, pos, rpi, seq, loc, e.rtp, e.kvp, e.be)
+    e.be.init_forward_metadata(batch)
+    q, k, v = e.rand(2, 16, 128), e.rand(2, 4, 128), e.rand(2, 4, 128)
+    step = e.be.quest._step
+    plan, dense = step.plan, fp8_decode_plan(e.kvp, e.rtp.block_table, rpi, seq)
+    for bad in (dense, plan._replace(bs=1), plan._replace(top_k=576), plan._replace(workspace=plan.workspace[256:])):
+        step.plan = bad
+        with pytest.raises(ValueError, match="plan"):
+            e.be.forward(q, k, v, e.mods[0], batch)
+    step.plan = dense._replace(top_k=512)  # does not show what it is of: no answer, and all of it written
+    assert e.be.forward(q, k, v, e.mods[0], batch).isnan().all()
+    step.plan = plan
+    assert not e.be.forward(q, k, v, e.mods[0], batch).isnan().any()
+
+
 def test_padded_entries_of_a_decode_batch(cuda):
     """seq_lens 0: no row, no token stored, an output of zeros."""
     e = Engine(cuda, "dense", 1, 4, 2, 128, torch.bfloat16, 3, 300, 20)
