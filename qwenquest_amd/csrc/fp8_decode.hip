@@ -24,8 +24,10 @@
 // looked up together, and a request's first unit is loaded under the one before it.  A wave
 // takes a unit at a time: K and V codes straight from memory to registers in the
 // operands' order (1 KiB runs), converted to bf16 (exact), S^T = K Q^T, the softmax in
-// registers, O^T += V^T P^T, with P's values scaled by vs as bf16 pieces: two for bf16 output
-// (16 significand bits), three for fp32 (all 24).  fp32 queries go in as three bf16 pieces, too.
+// registers, O^T += V^T P^T, with P's values scaled by vs as three bf16 pieces, which hold all 24
+// significand bits (in two pieces, 16 bits, bf16 outputs were off by a step in a few of a hundred places,
+// for 2 us less of 145 in 12 layers of one request of 2000 tokens).  fp32 queries go in as three bf16
+// pieces, too.
 // Bound: HBM, the codes once, when they are many: 16 requests of 131072 tokens, 4 heads of 128,
 // 378 us (5.7 TB/s).  A small batch is bound by its chain of memory round trips (slice, table
 // words, scales and codes, partials, count, merge, ~1 us each): one request of 2000 tokens 10.8 us
@@ -265,7 +267,7 @@ __device__ inline void select_pages(const SelectArgs& sel, int b, RankSelectSmem
 // KPT > 0: the requests' pages are selected here, KPT scores a thread.
 template <int D, typename T, int KPT>
 __global__ __launch_bounds__(64 * kDecWaves, 2) void fp8_attend_kernel(DecArgs a, StoreArgs st, SelectArgs sel) {
-  constexpr int QP = sizeof(T) == 2 ? 1 : 3, PP = sizeof(T) == 2 ? 2 : 3;  // pieces of q and of the weights
+  constexpr int QP = sizeof(T) == 2 ? 1 : 3, PP = 3;  // pieces of q and of the weights
   constexpr int KL = D / 64, VL = D / 16;  // 16-byte loads a lane: per 16 tokens of K, per block of V
   constexpr int RF = dec_row_floats(D);
   extern __shared__ __align__(16) unsigned char smem_raw[];

@@ -107,6 +107,43 @@ def test_any_scale(cuda, scale):
     s.check(out, q, scale)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_weights_keep_their_bits(cuda, dim, dtype):
+    """A sum in which values cancel, so that a weight's lower bits decide: head h's token 0 weighs
+    exp(-a) against 1 of tokens 1 and 2, which hold -exp(-a) to 8 bits in channel h.
+
+    Roundings: the score's one product is exact, its scaling to a power of two and back a few times 2^-24
+    of |t| <= 2, so that a weight is off by under 2^-21 of itself, the exponential's last place included;
+    pieces of 24 bits add 2^-24, sums of three terms as much each.  All of it under 2^-20 of
+    sum p |v|; a weight of 16 bits alone is off by up to 2^-15."""
+    heads = 16
+    a = (0.3 + torch.arange(heads) / 12.0).to(torch.bfloat16).double()
+    pool = Fp8TokenToKVPool(2, 1, 1, dim, cuda)
+    k, v = torch.zeros(3, 1, dim, dtype=torch.float64), torch.zeros(3, 1, dim, dtype=torch.float64)
+    k[0, 0, 0] = -1.0
+    v[0, 0, :heads] = 1.0
+    p = torch.exp(-a)
+    first = torch.from_numpy(of.round_e4m3(p.numpy()))
+    v[1, 0, :heads] = -first
+    v[2, 0, :heads] = -torch.from_numpy(of.round_e4m3((p - first).numpy() * 64) / 64)
+    pool.set_kv_buffer(0, torch.arange(64, 67), k.float().to(cuda), v.float().to(cuda))
+    got = pool.get_rows(0, torch.arange(64, 67), torch.float32)
+    assert torch.equal(got[0].cpu().double(), k) and torch.equal(got[1].cpu().double(), v)  # exact in 8 bits
+    q = torch.zeros(1, heads, dim, dtype=torch.float64)
+    q[0, :, 0] = a
+    table = torch.tensor([[1]], dtype=torch.int32, device=cuda)
+    out = fp8_decode_attention(q.to(cuda, dtype), pool, 0, table, i64([0], cuda), i64([3], cuda), 1.0)
+    got = out.view(heads, dim).double().cpu().diagonal()
+    total = p + 2
+    want = (p + v[1, 0, :heads] + v[2, 0, :heads]) / total
+    spread = (p + v[1:, 0, :heads].abs().sum(0)) / total
+    assert (want.abs() < spread * 2.0**-8).all() and (want.abs() > spread * 2.0**-20).sum() > heads // 2
+    half = 2.0**-8 if dtype == torch.bfloat16 else 2.0**-24
+    err = (got - want).abs()
+    assert (err <= half * want.abs() + 2.0**-20 * spread).all(), (err / (half * want.abs() + 2.0**-20 * spread)).max()
+
+
 def picked(rng, n, top_k, pages=None):
     """A selection as retrieve_topk lays it out: pages in any order, expanded, then the recent window."""
     k = top_k // 64 - 1
