@@ -512,8 +512,8 @@ int qq_fp8_decode_plan(int num_blocks, int kv_heads, int head_dim, int block_tab
  * this step's qq_fp8_page_bounds made (same requests, lengths, table, geometry and top_k, on the same
  * stream and in the same graph capture or in none; up to 16 query heads per KV head, others as without), for which the new tokens lie as
  * in a planned qq_fp8_decode_attention.  bf16 at 4 KV heads x 128 with 2 to 8 query heads each,
- * top_k of 512 to 4160, up to 8192 pages and 64 requests then takes two launches: the scores with the
- * store; the selection with the attention.  phase 1 = scores and selection, 2 = store
+ * top_k of 512 to 2624 (in tables of more than 4096 pages to 4160), up to 8192 pages and 64 requests then
+ * takes two launches: the scores with the store; the selection with the attention.  phase 1 = scores and selection, 2 = store
  * and attention over the positions that phase 1 left, 3 = both. */
 int qq_fp8_quest_step(const void* q, int q_dtype, int64_t q_batch_stride, int num_q_heads, const void* k_new,
                       const void* v_new, int new_dtype, const int64_t* out_cache_loc, uint8_t* k_codes,

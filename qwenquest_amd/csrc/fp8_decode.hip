@@ -16,7 +16,7 @@
 // (fp8_plan_kernel, or beside the page bounds), a dense layer is one launch, in which the wave that
 // has a request's last block stores the request's new token into it first; a layer of Quest stores
 // beside the page scores (a selected page may be the one that is written) and selects here, at
-// shapes where a block does that for two requests at most.
+// shapes where that costs less than a launch (selects_itself).
 //
 // Of its block's slice a wave takes an eighth, units in a row, and goes through their requests on
 // its own; what a request's end finds in one wave is written by that wave, the rest meets in the
@@ -710,6 +710,8 @@ void attend(const DecArgs& a, const StoreArgs& st, const SelectArgs& sel, hipStr
   fp8_attend_kernel<D, T, KPT><<<a.max_slices * a.heads, 64 * kDecWaves, bytes, s>>>(a, st, sel);
 }
 
+constexpr int kBeginPages = 16 * 256;  // pages that a begin launch selects of, at most
+
 // `sel`: with k_sel > 0 the pages are selected first, from scores that are there.  planned: the
 // workspace holds the slices, and nothing of another head tile waits for the new tokens.
 template <int D>
@@ -720,7 +722,7 @@ void launch(const DecArgs& a, const StoreArgs& st, const SelectArgs& sel, bool p
   else if (!sel.positions) begin<D, 0>(a, st, sel, s);
   else if (sel.k_sel <= 64 && n <= 4 * 256) begin<D, 4>(a, st, sel, s);
   else if (sel.k_sel <= 64 && n <= 9 * 256) begin<D, 9>(a, st, sel, s);
-  else if (sel.k_sel <= 64 && n <= 16 * 256) begin<D, 16>(a, st, sel, s);
+  else if (sel.k_sel <= 64 && n <= kBeginPages) begin<D, 16>(a, st, sel, s);
   else {
     launch_select(sel, a.bs, sel.MP, sel.k_sel, s);
     begin<D, 0>(a, st, sel, s);
@@ -732,11 +734,21 @@ void launch(const DecArgs& a, const StoreArgs& st, const SelectArgs& sel, bool p
 // Whether a planned step of Quest runs as two launches: the scores with the new tokens, and an
 // attention that selects by itself.  A slice must not be longer than a request's selection (at
 // most as many requests as the grid has slices, and 8 units, fp8_slice_len's least), so that a block
-// selects for two requests at most.  (A layer of one request of 32768 tokens 17.2 us against 19.3 in
-// three launches, of 16 of 131072 36.8 against 38.8.)
+// selects for two requests at most.
+//
+// Every block of a request repeats its selection, which is dear once more than a wave's 64 pages pass
+// its filter (the k-th largest of 64 groups' maxima: 64 ln(64 / (64 - k)) pages, 64 of them from
+// k = 40 on), where a launch for it does it once: two launches are taken up to that, and past the 4096
+// pages that a begin launch can select of, which takes four.  A layer-step in two launches and in
+// three, us, 32 heads on 4, contexts of 32768 tokens unless said: 1 request, 31 pages 16.6, 18.9; 12:
+// 26.4, 28.1; 40: 43.3, 45.4; 63: 47.7, 51.4; 12 of 131072: 33.7, 35.5; 40 pages, 1 request 17.1, 19.9; 7:
+// 24.9, 26.5; 63: 56.5, 58.9; 42 pages, 7 requests 28.4, 26.6; 63 pages, 1: 24.9, 23.2; 64 pages, 16: 53.9,
+// 46.7.  In tables of 4097 pages: 44 pages, 1 of 262144 tokens 22.9, 52.0; 64 pages, 12: 44.1, 52.5; 63:
+// 107, 104.
 bool selects_itself(const DecArgs& a, const SelectArgs& sel, int q_dtype) {
+  const int n = max(sel.MP, sel.k_sel);
   return q_dtype == QQ_DTYPE_BF16 && a.c.D == 128 && a.tiles == 1 && a.bs <= a.max_slices && sel.top_k >= 8 * 64 &&
-         sel.k_sel <= 64 && sel.MP > 0 && max(sel.MP, sel.k_sel) <= 16 * 64 * kDecWaves &&
+         sel.k_sel <= (n <= kBeginPages ? 40 : 64) && sel.MP > 0 && n <= 16 * 64 * kDecWaves &&
          (int64_t)a.table_cols * kCacheTokens > sel.top_k;
 }
 
