@@ -397,6 +397,60 @@ def test_a_divided_step_of_quest(cuda, lens, top_k, width, heads, avoid):
     rtp.check_errors()
 
 
+@pytest.mark.parametrize("lens, top_k, width, avoid", [
+    ([200000, 700, 1, 164000], 2048, 200000, False),    # 3125 pages: more than 2560, which a block selects of in one form less
+    ([3000, 66, 1500, 900], 1024, 200000, True),        # the same table with few candidates
+    ([262208, 70000], 2624, 262208, True),              # 4097 pages: past what a begin launch selects of
+    ([524288, 300], 2048, 524288, False),               # 8192 pages, the most that a block selects of
+    ([524352, 5000], 512, 524352, False),               # one more
+    ([40000, 3000, 64], 2624, 40001, False), ([40000, 3000, 64], 2688, 40001, True),  # 40 pages and one more
+    ([270000, 5000], 4160, 270000, False), ([5000, 6000], 4160, 180000, False)])  # 64 pages
+def test_selections_in_wide_tables(cuda, lens, top_k, width, avoid):
+    """Selections of every form that a step over many pages takes: the oracle's positions, in two launches
+    and in three, and the same answers; pages with scores of their own, and all alike."""
+    kv, dim, heads, bs = 4, 128, 16, len(lens)
+    gen = torch.Generator(device=cuda).manual_seed(width + top_k)
+    rtp = BlockReqToTokenPool(bs, width, sum(n // 64 + 2 for n in lens) + 1, cuda)
+    kvp = Fp8TokenToKVPool(rtp.num_blocks, 1, kv, dim, cuda)
+    be = QuestOnlyBackend(rtp, kvp, {"algorithm": "quest", "top_k": top_k, "quest_page_size": 64, "avoid_recent_overlap": avoid})
+    reqs, had = torch.arange(bs, device=cuda), [n - 1 for n in lens]
+    for r, n in enumerate(had):  # (a request at a time: the values are made in float32)
+        if n == 0:
+            continue
+        loc, _ = rtp.assign(i64([r], cuda), i64([0], cuda), i64([n], cuda), n)
+        x = torch.randn(n // 64 + 1, kv, dim, device=cuda, generator=gen).repeat_interleave(64, 0)[:n].to(torch.bfloat16)
+        kvp.set_kv_buffer(0, loc, x + torch.randn(n, kv, dim, device=cuda, generator=gen).to(torch.bfloat16),
+                          torch.randn(n, kv, dim, device=cuda, generator=gen).to(torch.bfloat16))
+    be.quest.update_prefill_representations_blocks(reqs, i64(had, cuda), kvp, rtp.block_table)
+    rtp.check_errors()
+    seq = i64(lens, cuda)
+    loc, pos = rtp.assign_decode(reqs, seq)
+    batch = ForwardBatch(ForwardMode.DECODE, None, pos, reqs, seq, loc, rtp, kvp, be)
+    for alike in (False, True):
+        q, k, v = (torch.randn(bs, h, dim, device=cuda, generator=gen).bfloat16() for h in (heads, kv, kv))
+        if alike:
+            q[:] = 0
+        be.init_forward_metadata(batch)
+        outs = []
+        for planned in (True, False):
+            if not planned:
+                be.quest._step.plan = None
+            be._positions.fill_(-7)
+            outs.append((be.forward(q, k, v, Layer(0, dim), batch), be._positions.clone()))
+        assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1]) and not outs[0][0].isnan().any()
+        qbar = oq.group_queries(q.float().cpu().numpy(), kv, dim, True)
+        for i, s in enumerate(lens):
+            if s <= top_k:
+                want = np.arange(s)
+            else:
+                full = (s - 1) // 64
+                words = be.quest.page_k_bounds[0, i, :full].view(torch.int16).cpu().numpy().view(np.uint16)
+                limit = s // 64 - 1 if avoid else s // 64
+                pages = oq.topk_pages(oq.page_scores(qbar[i : i + 1], words[None])[0], min(limit, full), top_k // 64 - 1)
+                want = np.concatenate([(pages[:, None] * 64 + np.arange(64)).reshape(-1), np.arange(s - 64, s)])
+            assert outs[0][1][i, : len(want)].tolist() == want.tolist(), (i, alike)
+
+
 def test_pools_that_do_not_go_together(cuda):
     paged, rows = BlockReqToTokenPool(2, 300, 9, cuda), ReqToTokenPool(2, 300, cuda)
     fp8, plain = Fp8TokenToKVPool(9, 1, 2, 128, cuda), MHATokenToKVPool(600, 1, 2, 128, torch.bfloat16, cuda)
