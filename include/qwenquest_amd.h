@@ -454,7 +454,8 @@ int qq_fp8_rows(const uint8_t* k_codes, const uint8_t* v_codes, const float* k_s
  * (src/qwenquest/quest.py:231-280 and 284-321 in one form: nothing runs along).  Blocks come
  * from block_table; requests outside it are skipped, a block outside the cache gives NaN.
  * actual_lens and candidate_limit (both or neither): qq_quest_prepare_step's outputs for pages
- * of 64, in the same launch.  plan (decode only, or NULL): a workspace of
+ * of 64, in the same launch, but that the page which the token at seq_lens[i] - 1 completes is no
+ * candidate (its bounds come with the next step).  plan (decode only, or NULL): a workspace of
  * qq_fp8_decode_workspace_bytes(bs, kv_heads, kv_heads, head_dim), into which the step's
  * selections of top_k tokens are divided for its qq_fp8_quest_step calls. */
 int qq_fp8_page_bounds(const uint8_t* k_codes, int64_t codes_layer_stride, const float* k_scale,

@@ -133,7 +133,8 @@ __global__ __launch_bounds__(256) void fp8_page_bounds_kernel(PageArgs a) {
   const int64_t req = a.rpi[b], seq = a.seq[b], s = max(seq, (int64_t)0);
   if (a.actual && layer == 0 && blockIdx.x == 0 && threadIdx.x == 0) {
     a.actual[b] = (int32_t)min(seq, (int64_t)a.top_k);  // quest.py:343-352
-    a.limit[b] = (int32_t)(a.avoid ? max(seq / 64 - 1, (int64_t)0) : seq / 64);
+    // the page that the step's own token completes has no bounds yet, whatever lies in its place
+    a.limit[b] = (int32_t)(a.avoid ? max(seq / 64 - 1, (int64_t)0) : max(seq - 1, (int64_t)0) / 64);
   }
   if (req < 0 || req >= a.R || req >= a.table_rows) return;
   int64_t lo, hi;  // pages

@@ -337,6 +337,44 @@ def test_padded_entries_of_a_decode_batch(cuda):
     assert not out[1].any() and not e.kvp.k_codes[0, 0].any()
 
 
+@pytest.mark.parametrize("how", ["rolled back", "slot used again"])
+def test_bounds_left_behind_select_nothing(cuda, how):
+    """A request that is rolled back past a page's end and decodes other tokens, and one in a slot whose
+    blocks went back without on_request_finished: the page that the step completes has no bounds
+    yet, whatever stands in its place, and the selections are those of an engine without a past."""
+    e, w = (Engine(cuda, "quest", 1, 16, 4, 128, torch.bfloat16, 2, 1000, 40, top_k=256, seed=4) for _ in range(2))
+    gen = torch.Generator(device=cuda).manual_seed(8)
+    prompt = [torch.randn(500, h, 128, device=cuda, generator=gen).bfloat16() for h in (16, 4, 4)]
+
+    def run(x, mode, seq, q, k, v):
+        n = q.shape[0]
+        rpi, sl, pre = i64([1], cuda), i64([seq], cuda), i64([seq - n], cuda)
+        ext = i64([n], cuda)
+        loc, pos = x.rtp.assign(rpi, pre, ext, n) if mode is ForwardMode.EXTEND else x.rtp.assign_decode(rpi, sl)
+        batch = ForwardBatch(mode, None, pos, rpi, sl, loc, x.rtp, x.kvp, x.be, extend_prefix_lens=pre, extend_seq_lens=ext)
+        x.be.init_forward_metadata(batch)
+        return x.be.forward(q, k, v, x.mods[0], batch)
+
+    def token(size=1.0):
+        return [torch.randn(1, h, 128, device=cuda, generator=gen).bfloat16() * size for h in (16, 4, 4)]
+
+    run(e, ForwardMode.EXTEND, 500, *prompt)
+    for seq in range(501, 516):  # large keys in page 7, which 513 finds complete
+        run(e, ForwardMode.DECODE, seq, *token(30.0))
+    if how == "slot used again":
+        e.rtp.release(i64([1], cuda))
+        run(e, ForwardMode.EXTEND, 500, *prompt)
+    run(w, ForwardMode.EXTEND, 500, *prompt)
+    # what was rolled back has left page 7 a larger scale, which its bounds show from 513 on
+    for seq in range(501, 513 if how == "rolled back" else 516):
+        q, k, v = token()
+        a, b = (run(x, ForwardMode.DECODE, seq, q, k, v) for x in (e, w))
+        got, want = (x.be.quest.trace.records[-1].positions.tolist() for x in (e, w))
+        assert got == want, seq
+        if how == "slot used again":
+            assert torch.equal(a, b), seq
+
+
 def test_phases_are_the_step_in_two(cuda):
     e = Engine(cuda, "quest", 1, 8, 2, 128, torch.bfloat16, 2, 900, 30)
     e.prefill([0, 1], [500, 70])
