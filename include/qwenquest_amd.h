@@ -397,25 +397,26 @@ int qq_kv_scatter(void* k_layer, void* v_layer, int buf_dtype, int64_t kv_rows, 
  * padding row).  new_lens NULL: a decode batch, one token at position lens[i] - 1 each
  * (total == bs; an entry with lens[i] < 1 is padding and gets row 0).  An entry without new
  * tokens is ignored.  Asked again for the same lengths it takes nothing and answers the same.
- * Refused as a whole, on the device, with every loc and pos 0 and nothing taken: bit 1 of
- * *error_flags (and of error_mirror, device-accessible host memory, or NULL) when the stack
- * has too few blocks, 2 for a request or a length outside its table, 4 for a request listed
- * twice, 8 for more than `total` tokens.  workspace: qq_block_workspace_bytes(bs), this call's
+ * Refused as a whole, on the device, with every loc and pos 0 and nothing taken, and counted: in
+ * error_counts[0] (and error_mirror[0], 4 words of device-accessible host memory, or NULL) when the
+ * stack has too few blocks, [1] for a request or a length outside its table, [2] for a request listed
+ * twice, [3] for more than `total` tokens.  The counts are never set back.  workspace: qq_block_workspace_bytes(bs), this call's
  * alone until its launches are done; a decode batch needs none. */
 int qq_block_assign(const int64_t* req_pool_indices, const int64_t* lens, const int64_t* new_lens, int bs,
                     int64_t total, int32_t* block_table, int64_t block_table_stride, int32_t* req_to_token,
                     int64_t req_to_token_stride, int64_t max_context_len, int max_reqs, int32_t* held,
                     int32_t* free_blocks, int32_t* free_count, int64_t free_cap, int64_t* loc, int64_t* pos,
-                    int32_t* error_flags, int32_t* error_mirror, void* workspace, int64_t workspace_bytes,
+                    int32_t* error_counts, int32_t* error_mirror, void* workspace, int64_t workspace_bytes,
                     void* stream);
 
 /* The listed requests' blocks back on the stack (what assigning them in this order took off
  * it lies there as before), their block_table entries and req_to_token positions cleared,
- * held 0.  Refused as a whole with bits 2, 4 and 8 (more blocks than the stack has room for). */
+ * held 0.  Refused as a whole and counted under [1], [2] and [3] (more blocks than the stack has room
+ * for). */
 int qq_block_release(const int64_t* req_pool_indices, int bs, int32_t* block_table, int64_t block_table_stride,
                      int32_t* req_to_token, int64_t req_to_token_stride, int64_t max_context_len, int max_reqs,
                      int32_t* held, int32_t* free_blocks, int32_t* free_count, int64_t free_cap,
-                     int32_t* error_flags, int32_t* error_mirror, void* workspace, int64_t workspace_bytes,
+                     int32_t* error_counts, int32_t* error_mirror, void* workspace, int64_t workspace_bytes,
                      void* stream);
 int64_t qq_block_workspace_bytes(int bs);
 

@@ -27,7 +27,7 @@ namespace qq {
 namespace {
 
 constexpr int kPlan = 1024;      // threads of the planning block, at most
-constexpr int kErrExhausted = 1, kErrRequest = 2, kErrTwice = 4, kErrTotal = 8;
+constexpr int kErrExhausted = 1, kErrRequest = 2, kErrTwice = 4, kErrTotal = 8, kErrKinds = 4;
 constexpr int kMaxPoolReqs = 1 << 18;  // the planning block's bitmap of requests: 32 KiB
 
 // What the planning block hands to the fill: a header, then a record per request.
@@ -58,8 +58,8 @@ struct BlockArgs {
   int64_t cap;  // entries of the stack
   int64_t* loc;
   int64_t* pos;
-  int32_t* err;
-  int32_t* err_mirror;
+  int32_t* err;         // [kErrKinds] refused calls
+  int32_t* err_mirror;  // the same in host memory, or nullptr
   PlanHead* head;
   PlanRow* rows;
   int here;  // the planning block writes the slots itself
@@ -135,9 +135,15 @@ __device__ inline bool mark(uint32_t* seen, int64_t req) {
   return atomicOr(&seen[req >> 5], bit) & bit;
 }
 
+// Counts a refused call under each of its reasons.  The counts only grow, so that a host that reads
+// them at any time misses no call.
 __device__ inline void report(const BlockArgs& a, int err) {
-  *a.err |= err;
-  if (a.err_mirror) *a.err_mirror |= err;
+  for (int kind = 0; kind < kErrKinds; ++kind)
+    if (err >> kind & 1) {
+      const int32_t n = a.err[kind] + 1;
+      a.err[kind] = n;
+      if (a.err_mirror) a.err_mirror[kind] = n;
+    }
 }
 
 // The last request whose first token (BLK: block) is at or before `at`, among those with any.
@@ -368,12 +374,12 @@ extern "C" int qq_block_assign(const int64_t* req_pool_indices, const int64_t* l
                                int64_t total, int32_t* block_table, int64_t block_table_stride, int32_t* req_to_token,
                                int64_t req_to_token_stride, int64_t max_context_len, int max_reqs, int32_t* held,
                                int32_t* free_blocks, int32_t* free_count, int64_t free_cap, int64_t* loc, int64_t* pos,
-                               int32_t* error_flags, int32_t* error_mirror, void* workspace, int64_t workspace_bytes,
+                               int32_t* error_counts, int32_t* error_mirror, void* workspace, int64_t workspace_bytes,
                                void* stream) {
   const char* what = "qq_block_assign";
   BlockArgs a{req_pool_indices, lens, new_lens, bs, total, block_table, block_table_stride, req_to_token,
               req_to_token_stride, max_context_len, max_reqs, held, free_blocks, free_count, free_cap, loc, pos,
-              error_flags, error_mirror, nullptr, nullptr, 0};
+              error_counts, error_mirror, nullptr, nullptr, 0};
   int st = check_pool(a, what);
   if (st != QQ_OK) return st;
   QQ_REQUIRE(bs == 0 || lens, "%s: null pointer", what);
@@ -395,12 +401,12 @@ extern "C" int qq_block_assign(const int64_t* req_pool_indices, const int64_t* l
 extern "C" int qq_block_release(const int64_t* req_pool_indices, int bs, int32_t* block_table,
                                 int64_t block_table_stride, int32_t* req_to_token, int64_t req_to_token_stride,
                                 int64_t max_context_len, int max_reqs, int32_t* held, int32_t* free_blocks,
-                                int32_t* free_count, int64_t free_cap, int32_t* error_flags, int32_t* error_mirror,
+                                int32_t* free_count, int64_t free_cap, int32_t* error_counts, int32_t* error_mirror,
                                 void* workspace, int64_t workspace_bytes, void* stream) {
   const char* what = "qq_block_release";
   BlockArgs a{req_pool_indices, nullptr, nullptr, bs, 0, block_table, block_table_stride, req_to_token,
               req_to_token_stride, max_context_len, max_reqs, held, free_blocks, free_count, free_cap, nullptr, nullptr,
-              error_flags, error_mirror, nullptr, nullptr, 0};
+              error_counts, error_mirror, nullptr, nullptr, 0};
   int st = check_pool(a, what);
   if (st != QQ_OK) return st;
   if (bs == 0) return QQ_OK;

@@ -19,7 +19,13 @@ __all__ = ["BLOCK_TOKENS", "BlockReqToTokenPool", "Fp8TokenToKVPool"]
 
 BLOCK_TOKENS = 64
 
-_ERR_EXHAUSTED, _ERR_REQUEST, _ERR_TWICE, _ERR_TOTAL = 1, 2, 4, 8
+# what the device counts refused calls by, and what they are raised as
+_REFUSALS = (
+    (RuntimeError, "KV pool out of memory: too few free blocks for the batch"),
+    (ValueError, "a request index or length lies outside the request table"),
+    (ValueError, "a request is listed twice"),
+    (ValueError, "the requests' tokens exceed total, or blocks are released that were not assigned"),
+)
 
 
 def _indexed(device: torch.device | str) -> torch.device:
@@ -66,8 +72,10 @@ class BlockReqToTokenPool(ReqToTokenPool):
         self.held = torch.zeros(size, dtype=torch.int32, device=dev)
         self.free_blocks = torch.arange(num_blocks - 1, 0, -1, dtype=torch.int32, device=dev)
         self.free_count = torch.full((1,), num_blocks - 1, dtype=torch.int32, device=dev)
-        self._err = torch.zeros(1, dtype=torch.int32, device=dev)
-        self._err_host = pinned_zeros((1,), torch.int32)
+        # refused calls by reason, never set back; what has been raised of them
+        self._err = torch.zeros(len(_REFUSALS), dtype=torch.int32, device=dev)
+        self._err_host = pinned_zeros((len(_REFUSALS),), torch.int32)
+        self._raised = [0] * len(_REFUSALS)
         self._err_host_dev = HiSparseCoordinator._device_address(self._err_host)
         # the C entries' view of the pool, whose tensors stay where they are
         r2t, bt = self.req_to_token, self.block_table
@@ -133,22 +141,20 @@ class BlockReqToTokenPool(ReqToTokenPool):
         super().free(req_pool_idx)
 
     def check_errors(self, sync: bool = True) -> None:
-        """Raise what a call refused on the device: RuntimeError when the blocks ran out, ValueError
-        for lengths, requests or totals that do not fit.  ``sync``: read the device word (a
-        synchronisation); otherwise its mirror in pinned host memory, which shows the calls whose
-        kernels have finished."""
-        err = int(self._err.item() if sync else self._err_host[0])
-        if not err:
-            return
-        self._err.zero_()
-        self._err_host.zero_()
-        if err & _ERR_TWICE:
-            raise ValueError("a request is listed twice")
-        if err & _ERR_REQUEST:
-            raise ValueError("a request index or length lies outside the request table")
-        if err & _ERR_TOTAL:
-            raise ValueError("the requests' tokens exceed total, or blocks are released that were not assigned")
-        raise RuntimeError("KV pool out of memory: too few free blocks for the batch")
+        """Raise what calls since the last error were refused for on the device: ValueError for lengths,
+        requests or totals that do not fit, RuntimeError when only the blocks ran out.  ``sync``:
+        read the device's counts (a synchronisation with the current stream); otherwise their mirror in
+        pinned host memory, which shows the calls whose kernels have finished.  A call that is
+        refused meanwhile is raised by the next check."""
+        counts = (self._err if sync else self._err_host).tolist()
+        new = []
+        for i, n in enumerate(counts):
+            if 0 < (n - self._raised[i]) % (1 << 32) < 1 << 31:
+                self._raised[i] = n
+                new.append(_REFUSALS[i])
+        if new:
+            kind = ValueError if any(k is ValueError for k, _ in new) else RuntimeError
+            raise kind("; ".join(said for _, said in new))
 
     def poll_errors(self) -> None:
         """``check_errors`` without a synchronisation, as a caller of replayed graphs needs it."""

@@ -137,6 +137,40 @@ def test_a_refused_batch_takes_nothing(cuda, rpi, prefix, new, total, error):
     pool.check_errors()
 
 
+@pytest.mark.parametrize("poll", [True, False])
+def test_a_refusal_behind_another_is_raised_as_well(cuda, poll):
+    """A call that is refused while an earlier refusal is looked at: each of them is raised, once,
+    whether its kernel had run by then or not."""
+    pool = BlockReqToTokenPool(2, 500, 10, cuda)
+    work = torch.randn(4096, 4096, device=cuda)
+    for _ in range(3):
+        said = []
+        pool.assign(i64([0, 1], cuda), i64([0, 0], cuda), i64([300, 300], cuda), 600)  # 10 blocks of 9
+        torch.cuda.synchronize()
+        twice = i64([0, 0], cuda), i64([0, 0], cuda), i64([10, 10], cuda)
+        for _ in range(20):
+            work = work @ work * 1e-2
+        pool.assign(*twice, 20)
+        for check in (pool.poll_errors if poll else pool.check_errors, pool.check_errors):
+            try:
+                check()
+            except (RuntimeError, ValueError) as e:
+                said.append(str(e))
+        assert sum("out of memory" in s for s in said) == 1 and sum("twice" in s for s in said) == 1, said
+        torch.cuda.synchronize()
+        pool.poll_errors()
+        pool.check_errors()
+
+
+def test_a_call_refused_for_two_reasons(cuda):
+    pool = BlockReqToTokenPool(2, 500, 3, cuda)
+    pool.assign(i64([0, 0], cuda), i64([0, 0], cuda), i64([300, 300], cuda), 500)
+    with pytest.raises(ValueError, match="out of memory.*twice.*total"):
+        pool.check_errors()
+    torch.cuda.synchronize()
+    pool.poll_errors()
+
+
 def test_refused_decode_and_release(cuda):
     pool = BlockReqToTokenPool(3, 200, 3, cuda)
     loc, pos = pool.assign_decode(i64([0, 1, 2], cuda), i64([1, 1, 1], cuda))  # 3 blocks of 2
