@@ -201,6 +201,19 @@ def ptr(t: torch.Tensor | None) -> int | None:
     return t.data_ptr()
 
 
+def table_args(block_table: torch.Tensor, device: torch.device) -> tuple:
+    """A block table as the C entries read it, int32 rows one after the other on ``device``: pointer, row
+    stride, rows, columns."""
+    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.stride(1) != 1:
+        raise ValueError("block_table must be a 2-D int32 tensor with unit column stride")
+    if block_table.device != device:
+        raise ValueError(f"block_table lies on {block_table.device}, the pool on {device}")
+    rows, cols = block_table.shape
+    if rows > 1 and block_table.stride(0) < cols:
+        raise ValueError("block_table's rows must not overlap")
+    return ptr(block_table), max(block_table.stride(0), cols), rows, cols
+
+
 def dtype_code(dt: torch.dtype) -> int:
     if dt == torch.bfloat16:
         return DTYPE_BF16

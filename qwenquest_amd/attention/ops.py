@@ -206,20 +206,6 @@ def extend_attention_batch_checked(
     return out if tokens >= out.shape[0] else out[:tokens]
 
 
-def _block_table(block_table: torch.Tensor, device: torch.device) -> torch.Tensor:
-    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.stride(1) != 1:
-        raise ValueError("block_table must be a 2-D int32 tensor with unit column stride")
-    if block_table.device != device:
-        raise ValueError(f"block_table lies on {block_table.device}, the pool on {device}")
-    if block_table.shape[0] > 1 and block_table.stride(0) < block_table.shape[1]:
-        raise ValueError("block_table's rows must not overlap")
-    return block_table
-
-
-def _table_args(bt: torch.Tensor) -> tuple:
-    return _lib.ptr(bt), max(bt.stride(0), bt.shape[1]), bt.shape[0], bt.shape[1]
-
-
 def _lengths(t: torch.Tensor, n: int, device: torch.device, what: str) -> torch.Tensor:
     if t.dim() != 1 or t.shape[0] != n:
         raise ValueError(f"{what} must have {n} entries, got {tuple(t.shape)}")
@@ -251,14 +237,14 @@ def fp8_decode_plan(pool: Fp8TokenToKVPool, block_table: torch.Tensor, req_pool_
     layers, on the current stream."""
     dev = pool.device
     bs = int(req_pool_indices.shape[0])
-    bt = _block_table(block_table, dev)
+    table = _lib.table_args(block_table, dev)
     rpi = _lengths(req_pool_indices, bs, dev, "req_pool_indices")
     seq = _lengths(seq_lens, bs, dev, "seq_lens")
     need = int(_lib.load().qq_fp8_decode_workspace_bytes(bs, pool.kv_heads, pool.kv_heads, pool.head_dim))
     ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
     stream = _lib.stream(dev)
     with _lib.on(dev):
-        _lib.call("qq_fp8_decode_plan", pool.num_blocks, pool.kv_heads, pool.head_dim, bt.shape[0], bt.shape[1],
+        _lib.call("qq_fp8_decode_plan", pool.num_blocks, pool.kv_heads, pool.head_dim, table[2], table[3],
                   _lib.ptr(rpi), _lib.ptr(seq), bs, _lib.ptr(ws), need, stream)
     return DecodePlan(bs, ws, stream, _lib.capture_id(dev, stream))
 
@@ -291,7 +277,7 @@ def fp8_decode_attention(
     dev = pool.device
     q = _queries(q, pool)
     bs, heads, dim = q.shape
-    bt = _block_table(block_table, dev)
+    table = _lib.table_args(block_table, dev)
     rpi = _lengths(req_pool_indices, bs, dev, "req_pool_indices")
     seq = _lengths(seq_lens, bs, dev, "seq_lens")
     if positions is not None:
@@ -319,7 +305,7 @@ def fp8_decode_attention(
         _lib.call(
             "qq_fp8_decode_attention", _lib.ptr(q), _lib.dtype_code(q.dtype), q.stride(0), heads, _lib.ptr(kn),
             _lib.ptr(vn), _lib.DTYPE_BF16 if kn is None else _lib.dtype_code(kn.dtype), _lib.ptr(loc),
-            *pool.layer_args(layer_id), *_table_args(bt), _lib.ptr(rpi), _lib.ptr(seq), bs, _lib.ptr(positions),
+            *pool.layer_args(layer_id), *table, _lib.ptr(rpi), _lib.ptr(seq), bs, _lib.ptr(positions),
             0 if positions is None else max(positions.stride(0), positions.shape[1]), int(top_k), float(scaling),
             _lib.ptr(out), _lib.ptr(ws), need, int(plan is not None), stream,
         )
@@ -356,14 +342,15 @@ def fp8_quest_step(
         raise ValueError("batch size differs from the one given to decode_step_blocks()")
     if bs > quest.max_reqs:
         raise ValueError(f"batch {bs} exceeds max_reqs {quest.max_reqs}")
-    if quest.page_size != 64 or quest.kv_heads != pool.kv_heads or quest.head_dim != dim:
+    if (quest.page_size != 64 or quest.kv_heads != pool.kv_heads or quest.head_dim != dim
+            or quest.page_k_bounds.device != dev):
         raise ValueError("the Quest state is not of this pool's pages and heads")
     if not quest.start_layer <= layer_id < quest.end_layer:
         raise IndexError(f"layer {layer_id} is no Quest layer ({quest.start_layer} .. {quest.end_layer - 1})")
     if (positions.dtype != torch.int32 or positions.device != dev or not positions.is_contiguous()
             or positions.dim() != 2 or positions.shape[0] < bs or positions.shape[1] != quest.top_k):
         raise ValueError(f"positions must be a contiguous int32 tensor [>= {bs}, {quest.top_k}] on {dev}")
-    bt = _block_table(block_table, dev)
+    table = _lib.table_args(block_table, dev)
     rpi = _lengths(req_pool_indices, bs, dev, "req_pool_indices")
     loc = _lengths(loc, bs, dev, "out_cache_loc")
     kn, vn = pool.new_rows(k, v, bs)
@@ -377,7 +364,7 @@ def fp8_quest_step(
     with _lib.on(dev):
         _lib.call(
             "qq_fp8_quest_step", _lib.ptr(q), _lib.dtype_code(q.dtype), q.stride(0), heads, _lib.ptr(kn), _lib.ptr(vn),
-            _lib.dtype_code(kn.dtype), _lib.ptr(loc), *pool.layer_args(layer_id), *_table_args(bt),
+            _lib.dtype_code(kn.dtype), _lib.ptr(loc), *pool.layer_args(layer_id), *table,
             _lib.ptr(quest.page_k_bounds), layer_id - quest.start_layer, _lib.ptr(rpi), _lib.ptr(step.seq_lens),
             _lib.ptr(step.candidate_limit_i32), bs, quest.max_reqs, quest.max_pages_per_req, quest.top_k, float(scaling),
             _lib.ptr(quest._scores_ws), _lib.ptr(positions), _lib.ptr(out), _lib.ptr(ws), need, int(phase), int(planned),
@@ -407,19 +394,19 @@ def fp8_extend_attention(
         raise ValueError(f"unsupported dtype {q.dtype}; the prefill kernel takes bfloat16")
     q = _queries(q, pool)
     n, heads, dim = q.shape
-    bt = _block_table(block_table, dev)
+    table = _lib.table_args(block_table, dev)
     bs = int(req_pool_indices.shape[0])
     rpi, seq, prefix, ext = (_lengths(t, bs, dev, what) for t, what in (
         (req_pool_indices, "req_pool_indices"), (seq_lens, "seq_lens"), (prefix_lens, "prefix_lens"),
         (extend_lens, "extend_lens")))
     if bs == 0 and n:
         raise ValueError(f"{n} tokens of no request")
-    need = int(_lib.load().qq_fp8_extend_workspace_bytes(n, bs, heads, pool.kv_heads, dim, bt.shape[1]))
+    need = int(_lib.load().qq_fp8_extend_workspace_bytes(n, bs, heads, pool.kv_heads, dim, table[3]))
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     out = torch.empty((n, heads * dim), dtype=q.dtype, device=dev)
     with _lib.on(dev):
         _lib.call(
-            "qq_fp8_extend_attention", _lib.ptr(q), heads, *pool.layer_args(layer_id), *_table_args(bt), _lib.ptr(rpi),
+            "qq_fp8_extend_attention", _lib.ptr(q), heads, *pool.layer_args(layer_id), *table, _lib.ptr(rpi),
             _lib.ptr(seq), _lib.ptr(prefix), _lib.ptr(ext), bs, n, float(scaling), _lib.ptr(out), _lib.ptr(ws), need,
             _lib.stream(dev),
         )

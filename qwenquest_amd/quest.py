@@ -373,9 +373,10 @@ class QuestAlgorithm:
         if pool.kv_heads != self.kv_heads or pool.head_dim != self.head_dim or pool.num_layers < self.end_layer:
             raise ValueError(f"the pool ({pool.num_layers} layers, {pool.kv_heads} x {pool.head_dim}) does not hold the "
                              f"Quest layers' keys ({self.end_layer} layers, {self.kv_heads} x {self.head_dim})")
-        if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.stride(1) != 1:
-            raise ValueError("block_table must be a 2-D int32 tensor with unit column stride")
-        lens = [t if t is None else t.to(device=self.device, dtype=torch.int64).contiguous()
+        if self.page_k_bounds.device != pool.device:
+            raise ValueError(f"the page bounds lie on {self.page_k_bounds.device}, the pool on {pool.device}")
+        dev, table = pool.device, _lib.table_args(block_table, pool.device)
+        lens = [t if t is None else t.to(device=dev, dtype=torch.int64).contiguous()
                 for t in (reqs, seq_lens, prefix_lens)]
         bs = int(lens[0].numel())
         if any(t is not None and t.numel() != bs for t in lens):
@@ -383,23 +384,22 @@ class QuestAlgorithm:
         codes, _, scale, _, *geometry = pool.layer_args(self.start_layer)
         actual = limit = ws = None
         if decode:
-            actual, limit = torch.empty((2, bs), dtype=torch.int32, device=self.device).unbind(0)
+            actual, limit = torch.empty((2, bs), dtype=torch.int32, device=dev).unbind(0)
             need = int(_lib.load().qq_fp8_decode_workspace_bytes(bs, self.kv_heads, self.kv_heads, self.head_dim))
             # of this step alone: a graph's replay must not find another step's division in it
-            ws = torch.empty(max(need, 1), dtype=torch.uint8, device=self.device)
-        stream = _lib.stream(self.device)
-        with _lib.on(self.device):
+            ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+        stream = _lib.stream(dev)
+        with _lib.on(dev):
             _lib.call(
                 "qq_fp8_page_bounds", codes, pool.k_codes.stride(0), scale, pool.k_scale.stride(0), *geometry,
-                _lib.ptr(block_table), max(block_table.stride(0), block_table.shape[1]), block_table.shape[0],
-                block_table.shape[1], *(_lib.ptr(t) for t in lens), bs, int(decode), int(max_new), self.num_layers,
+                *table, *(_lib.ptr(t) for t in lens), bs, int(decode), int(max_new), self.num_layers,
                 _lib.ptr(self.page_k_bounds), self.max_reqs, self.max_pages_per_req, self.top_k,
                 int(self.avoid_recent_overlap), _lib.ptr(actual), _lib.ptr(limit), _lib.ptr(ws),
                 0 if ws is None else ws.numel(), stream,
             )
         if not decode:
             return None
-        plan = DecodePlan(bs, ws, stream, _lib.capture_id(self.device, stream), self.top_k)
+        plan = DecodePlan(bs, ws, stream, _lib.capture_id(dev, stream), self.top_k)
         return StepLayout(lens[1], actual, limit, self.page_size, self.top_k, plan)
 
     def update_prefill_representations_blocks(

@@ -319,6 +319,21 @@ def test_bounds_of_spoilt_and_missing_blocks(cuda):
         other.decode_step_blocks(i64([0], cuda), i64([1], cuda), pool, table)
 
 
+def test_bounds_refuse_tables_that_are_no_rows(cuda):
+    """One row shown as several, whose stride is not the table's width: the kernel would read past it."""
+    pool = Fp8TokenToKVPool(6, 1, 2, 128, cuda)
+    quest = QuestAlgorithm(128, 64, cuda)
+    quest.init_storage(0, 1, 3, 300, 2, 128)
+    row = table_of([[1, 2, 3, 4]], cuda, 5)
+    lens = i64([0, 1], cuda), i64([65, 65], cuda)
+    for bad, said in ((row.expand(3, -1), "overlap"), (row.cpu(), "lies on"), (row[0], "2-D"), (row.t(), "stride")):
+        for call in (quest.decode_step_blocks, quest.update_prefill_representations_blocks):
+            with pytest.raises(ValueError, match=said):
+                call(*lens, pool, bad)
+    step = quest.decode_step_blocks(i64([0], cuda), i64([65], cuda), pool, row.expand(1, -1))
+    assert step.actual_lens.tolist() == [65] and (quest.page_k_bounds[0, 0, 0] == 0).all()
+
+
 def test_rescaling_is_exact_down_to_subnormals(cuda):
     """A power of two: growing the scale by 2^m keeps every code whose value stays a multiple of the
     least step."""
