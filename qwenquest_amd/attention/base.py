@@ -7,6 +7,7 @@ with ``layer_id`` and ``scaling`` (the reference's ``RadixAttention``).
 
 from __future__ import annotations
 
+import math
 from abc import ABC, abstractmethod
 from typing import TYPE_CHECKING, Any
 
@@ -106,10 +107,10 @@ class AttentionBackend(ABC):
         """forward_extend over an 8-bit pool, which holds the new K/V: every token attends the
         pool's values, its own included.  bf16 queries with a positive scale run the whole batch in
         one launch that reads the lengths on the device (NaN where the loop would refuse a request
-        index, and for rows of q past the requests' tokens); others go request by request over the
-        values."""
+        index); others go request by request over the values.  Either way the output has q's rows,
+        and NaN in those past the requests' tokens."""
         pool = self.token_to_kv_pool
-        q = q.reshape(q.shape[0], -1, pool.head_dim)
+        q = q.reshape(q.shape[0], math.prod(q.shape[1:]) // pool.head_dim, pool.head_dim)
         if (q.dtype == torch.bfloat16 and 0.0 < float(layer.scaling) < float("inf") and _plain(q)
                 and batch.extend_seq_lens is not None):
             return fp8_extend_attention(q, pool, layer.layer_id, self.req_to_token_pool.block_table,
@@ -122,6 +123,8 @@ class AttentionBackend(ABC):
             k, v = pool.get_rows(layer.layer_id, locs, torch.float32)
             outputs.append(extend_attention(q[offsets[i] : offsets[i + 1]], k, v,
                                             prefix_len=int(batch.extend_prefix_lens[i]), scaling=layer.scaling))
+        if offsets[-1] < q.shape[0]:
+            outputs.append(q.new_full((q.shape[0] - offsets[-1], q.shape[1] * q.shape[2]), float("nan")))
         return torch.cat(outputs, dim=0)
 
     def _extend_fast(self, q: torch.Tensor, k_buf: torch.Tensor, v_buf: torch.Tensor, scaling: float,

@@ -12,6 +12,7 @@ attention over the explicit row list ``req_to_token[req, :seq_len]``.  Over an 8
 
 from __future__ import annotations
 
+import math
 from typing import TYPE_CHECKING
 
 import torch
@@ -63,14 +64,15 @@ class DenseBackend(AttentionBackend):
         pool = self.token_to_kv_pool
         bs = batch.batch_size
         dim = pool.head_dim
-        q3 = q.reshape(bs, -1, dim)
         if self.fp8:
+            q3 = q.reshape(bs, math.prod(q.shape[1:]) // dim, dim)
             plan = getattr(batch, "decode_plan", None)
             if plan is not None and plan.bs != bs:  # a part of the batch that was divided
                 plan = None
             return fp8_decode_attention(q3, pool, layer.layer_id, self.req_to_token_pool.block_table,
                                         batch.req_pool_indices, batch.seq_lens, layer.scaling,
                                         new=(batch.out_cache_loc, k, v), plan=plan)
+        q3 = q.reshape(bs, -1, dim)
         heads = q3.shape[1]
         rpi = batch.req_pool_indices.to(device=q3.device, dtype=torch.int64).contiguous()
         seq = batch.seq_lens.to(device=q3.device, dtype=torch.int64).contiguous()

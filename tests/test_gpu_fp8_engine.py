@@ -375,6 +375,34 @@ def test_bounds_left_behind_select_nothing(cuda, how):
             assert torch.equal(a, b), seq
 
 
+def prefill_batch(e, reqs, prefix, new):
+    rpi, pre, ext = i64(reqs, e.dev), i64(prefix, e.dev), i64(new, e.dev)
+    loc, pos = e.rtp.assign(rpi, pre, ext, sum(new))
+    return ForwardBatch(ForwardMode.EXTEND, None, pos, rpi, pre + ext, loc, e.rtp, e.kvp, e.be, extend_prefix_lens=pre,
+                        extend_seq_lens=ext)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("backend", ["dense", "quest"])
+def test_prefills_without_tokens_and_with_rows_past_them(cuda, backend, dtype):
+    """Both query types answer alike: as many rows as q has, NaN past the requests' tokens; a batch, and a
+    decode batch, of nothing."""
+    e = Engine(cuda, backend, 1, 4, 2, 64, dtype, 3, 300, 20, top_k=128)
+    b = prefill_batch(e, [0, 1], [0, 0], [70, 5])
+    q, k, v = e.rand(80, 4, 64), e.rand(75, 2, 64), e.rand(75, 2, 64)
+    out = e.be.forward(q, k, v, e.mods[0], b)
+    assert out.shape == (80, 256) and out.dtype == dtype and out[75:].isnan().all() and not out[:75].isnan().any()
+    assert torch.equal(out[:75], e.be.forward(q[:75], k, v, e.mods[0], b))
+    for shape in ((0, 4, 64), (0, 256)):
+        b = prefill_batch(e, [0, 1], [70, 5], [0, 0])
+        assert e.be.forward(e.rand(*shape), k[:0], v[:0], e.mods[0], b).shape == (0, 256)
+        none = i64([], cuda)
+        b = ForwardBatch(ForwardMode.DECODE, None, none, none, none, none, e.rtp, e.kvp, e.be)
+        e.be.init_forward_metadata(b)
+        assert e.be.forward(e.rand(*shape), k[:0], v[:0], e.mods[0], b).shape == (0, 256)
+    e.rtp.check_errors()
+
+
 def test_phases_are_the_step_in_two(cuda):
     e = Engine(cuda, "quest", 1, 8, 2, 128, torch.bfloat16, 2, 900, 30)
     e.prefill([0, 1], [500, 70])
