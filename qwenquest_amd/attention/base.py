@@ -80,6 +80,9 @@ class AttentionBackend(ABC):
         """
         assert batch.out_cache_loc is not None and batch.extend_prefix_lens is not None
         pool = self.token_to_kv_pool
+        if self.fp8 and torch._C._get_tracing_state() is not None:
+            # neither the store nor the rows read back are torch operations
+            raise RuntimeError("a prefill over an 8-bit pool cannot be traced: a trace would keep its values, not its work")
         pool.set_kv_buffer(layer.layer_id, batch.out_cache_loc, k, v)
         if self.fp8:
             return self._forward_extend_fp8(q, layer, batch)

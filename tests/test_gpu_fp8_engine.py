@@ -403,6 +403,16 @@ def test_prefills_without_tokens_and_with_rows_past_them(cuda, backend, dtype):
     e.rtp.check_errors()
 
 
+def test_a_prefill_cannot_be_traced(cuda):
+    e = Engine(cuda, "dense", 1, 4, 2, 128, torch.bfloat16, 1, 300, 10)
+    b = prefill_batch(e, [0], [0], [20])
+    q, k, v = e.rand(20, 4, 128), e.rand(20, 2, 128), e.rand(20, 2, 128)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(lambda x: e.be.forward(x, k, v, e.mods[0], b), q, check_trace=False)
+    assert not e.kvp.k_codes.any()  # nothing stored
+    assert not e.be.forward(q, k, v, e.mods[0], b).isnan().any()
+
+
 def test_phases_are_the_step_in_two(cuda):
     e = Engine(cuda, "quest", 1, 8, 2, 128, torch.bfloat16, 2, 900, 30)
     e.prefill([0, 1], [500, 70])
