@@ -7,10 +7,10 @@
 // go to the LDS as they lie (two buffers, one barrier a tile; 32 KiB).  The codes are in operand
 // order, so a lane's 16-byte LDS reads, one after the other in every quarter wave, are 16 codes of
 // its token (K) or channel (V): no bank conflicts and nothing transposed.
-//   S^T = K Q^T  v_mfma_f32_32x32x64_f8f6f4, K's codes as they are and a query as the sum of two
-//   e4m3 pieces, the second at 2^-4 of the first's scale: 4 + 4 significand bits hold a bf16
-//   value exactly down to 2^-15 of the row's largest and to 2^-22 of that below.  At twice bf16's
-//   rate the two products take the same time as one in bf16, and K needs no conversion.
+//   S^T = K Q^T  v_mfma_f32_32x32x16_bf16, K's codes to bf16 (exact).  (The 8-bit matrix instructions
+//   take the codes as they are and a query in two pieces, in the same matrix time: 8192 tokens behind
+//   8192 1521 us against 1622.  But they do not add in 32 bits: where one of 64 products carries the sum,
+//   it comes out off by 2^-11 of itself, bf16's by 2^-22, and keys have channels like that.)
 //   O^T += V^T W^T  v_mfma_f32_32x32x16_f16, V's codes to f16 (exact)
 // With t = scale log2(e) ks (q . kc), M a running maximum of t that is let lag by 8 (the sums are
 // rescaled once it lags more), and R the largest exponent of a V scale so far (one number per
@@ -24,9 +24,9 @@
 // is 2^-8 of it; the weights' sum stays in fp32.
 //
 // Bound: the matrix cores and, beside them, the softmax's vector instructions.  Measured, 32 query
-// heads on 4 of 128: 8192 tokens behind 8192 1494 us (1.10 PFLOP/s of the formula's operations;
-// with bf16 scores 1639, with vector lookups 1797), 3440 tokens of 6 prompts 160 us, where the
-// longest tile chain is as long as the rest.
+// heads on 4 of 128: 8192 tokens behind 8192 1622 us (1.02 PFLOP/s of the formula's operations; with
+// vector lookups 10 % more), 3440 tokens of 6 prompts 186 us with their store, where the longest tile chain is
+// as long as the rest.
 #include "qq_extend_dev.h"
 #include "qq_fp8.h"
 
@@ -59,13 +59,18 @@ struct Fp8ExtendArgs {
   float* part_ml;  // [splits, KV, tiles, 128 rows, 2]
 };
 
-typedef int i32x8_t __attribute__((ext_vector_type(8)));
-constexpr int kOne = 0x7F7F7F7F, kSecond = 0x7B7B7B7B;  // scales of the products: 2^0, 2^-4
-
-__device__ inline i32x8_t operand32(uint4 a, uint4 b) {
-  return {(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
+// Sixteen codes as the operands of two steps.
+__device__ inline void codes16(uint4 w, bf16x8_t& a, bf16x8_t& b) {
+  const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+  u32x4_t y[2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    y[i >> 1][(i & 1) * 2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[i], 1.0f, false));
+    y[i >> 1][(i & 1) * 2 + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[i], 1.0f, true));
+  }
+  a = __builtin_bit_cast(bf16x8_t, y[0]);
+  b = __builtin_bit_cast(bf16x8_t, y[1]);
 }
-
 __device__ inline f16x8_t codes_f16(uint32_t a, uint32_t b) {
   u32x4_t w;
   w.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, false));
@@ -133,53 +138,11 @@ __global__ __launch_bounds__(64 * kExtWaves, 2) void fp8_extend_kernel(Fp8Extend
   const int j_begin = split * chunk, j_end = min(nt_all, j_begin + chunk);
   if (j_begin >= j_end && split != 0) return;
 
-  // This row's query over 2^qe, of step i channels (4 i + hf) * 16 .. + 15 and (4 i + 2 + hf) * 16 ..
-  // + 15, in two pieces; both halves of the wave agree on the row's largest value.
-  i32x8_t qb[KI / 2][2];
-  float q_scale;
-  bool q_bad = false;
-  {
-    uint4 raw[KI][2];
-    float qm = 0.0f;
+  // channels of step (i, p): (2 i + hf) * 16 + 8 p .. + 7
+  bf16x8_t qb[2 * KI];
 #pragma unroll
-    for (int i = 0; i < KI; ++i)
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        raw[i][x] = *reinterpret_cast<const uint4*>(qp + (2 * i + hf) * 16 + x * 8);
-        const uint32_t w[4] = {raw[i][x].x, raw[i][x].y, raw[i][x].z, raw[i][x].w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float f0 = __uint_as_float(w[e] << 16), f1 = __uint_as_float(w[e] & 0xFFFF0000u);
-          q_bad |= !(fabsf(f0) < INFINITY) || !(fabsf(f1) < INFINITY);
-          qm = fmaxf(qm, fmaxf(fabsf(f0), fabsf(f1)));
-        }
-      }
-    qm = fmaxf(qm, lane_xor32(qm, lane));
-    q_bad |= lane_xor32(q_bad ? 1.0f : 0.0f, lane) != 0.0f;
-    const int qe = q_bad ? 0 : scale_exponent(qm);
-    const float inv = q_bad ? 0.0f : pow2f(-qe);  // a row that is not finite has no answer
-    q_scale = pow2f(qe);
-#pragma unroll
-    for (int i = 0; i < KI; ++i)
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const uint32_t w[4] = {raw[i][x].x, raw[i][x].y, raw[i][x].z, raw[i][x].w};
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float f[4];
-#pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            f[2 * y] = q_bad ? 0.0f : __uint_as_float(w[2 * e + y] << 16) * inv;
-            f[2 * y + 1] = q_bad ? 0.0f : __uint_as_float(w[2 * e + y] & 0xFFFF0000u) * inv;
-          }
-          const uint32_t hi = encode4(f[0], f[1], f[2], f[3]);
-          const float4 d = decode4(hi);
-          qb[i >> 1][0][(i & 1) * 4 + x * 2 + e] = (int)hi;
-          qb[i >> 1][1][(i & 1) * 4 + x * 2 + e] =
-              (int)encode4((f[0] - d.x) * 16.0f, (f[1] - d.y) * 16.0f, (f[2] - d.z) * 16.0f, (f[3] - d.w) * 16.0f);
-        }
-      }
-  }
+  for (int i = 0; i < 2 * KI; ++i)
+    qb[i] = *reinterpret_cast<const bf16x8_t*>(qp + ((i >> 1) * 2 + hf) * 16 + (i & 1) * 8);
 
   const scalar_words_t bt = (scalar_words_t)(uintptr_t)(a.table + (int64_t)max(et.req, 0) * a.table_stride);
   const scalar_floats_t ksp = (scalar_floats_t)(uintptr_t)(a.c.ks + h), vsp = (scalar_floats_t)(uintptr_t)(a.c.vs + h);
@@ -248,13 +211,15 @@ __global__ __launch_bounds__(64 * kExtWaves, 2) void fp8_extend_kernel(Fp8Extend
     }
     // (independent accumulators one after the other)
 #pragma unroll
-    for (int i = 0; i < KI / 2; ++i)
+    for (int i = 0; i < KI; ++i) {
+      bf16x8_t k0[2], k1[2];
 #pragma unroll
-      for (int p = 0; p < 2; ++p)
+      for (int t = 0; t < 2; ++t) codes16(kw[t][i], k0[t], k1[t]);
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-          s[t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand32(kw[t][2 * i], kw[t][2 * i + 1]), qb[i][p], s[t],
-                                                                 0, 0, 0, kOne, 0, p ? kSecond : kOne);
+      for (int t = 0; t < 2; ++t) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k0[t], qb[2 * i], s[t], 0, 0, 0);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k1[t], qb[2 * i + 1], s[t], 0, 0, 0);
+    }
     // the values' codes arrive under the softmax
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -272,7 +237,7 @@ __global__ __launch_bounds__(64 * kExtWaves, 2) void fp8_extend_kernel(Fp8Extend
         for (int i = 0; i < 16; ++i) s[t][i] = (t * 32 + 8 * (i / 4) + i % 4) < left ? s[t][i] : -INFINITY;
     }
     // a positive factor, also where the scale underflows; NaN stays
-    float c = ks * (a.sl2 * q_scale);
+    float c = ks * a.sl2;
     c = c < 1.2e-38f ? 1.2e-38f : c;
     float mx = s[0][0];
 #pragma unroll
@@ -331,8 +296,7 @@ __global__ __launch_bounds__(64 * kExtWaves, 2) void fp8_extend_kernel(Fp8Extend
     }
   }
   L += lane_xor32(L, lane);
-  // a block that is not there, a query that is not finite: no answer
-  if (__syncthreads_or(bad) || q_bad) L = __builtin_nanf("");
+  if (__syncthreads_or(bad)) L = __builtin_nanf("");  // a block that is not there: no answer
   const bool mine = r0 + wave * 32 + lo < rows_n;
   const float unit = pow2f(R - kLift);
   if (whole) {

@@ -86,6 +86,22 @@ def test_values_of_very_different_size(cuda):
     check(s, fp8_extend_attention(q, s.pool, s.layer, s.table, *lens, 0.1), q, prefix, new, 0.1)
 
 
+@pytest.mark.parametrize("prefix, new", [([0], [200]), ([2000], [3])])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("large", [1.0, 4.0, 16.0, 64.0])
+def test_a_channel_that_carries_the_scores(cuda, large, dim, prefix, new):
+    """One channel in which every key is large: what tells tokens apart are the others' products, next to one
+    that is up to 2^16 times theirs.  The tolerance is that of sums in float32."""
+    s, q, lens = batch(cuda, prefix, new, 1, dim, 4, seed=6)
+    gen = torch.Generator(device=cuda).manual_seed(3)
+    n = prefix[0] + new[0]
+    k = torch.empty((n, 1, dim), device=cuda).normal_(generator=gen) * 0.5
+    k[..., 0] = large
+    s.pool.set_kv_buffer(s.layer, s.rows(0, np.arange(n)), k, torch.empty((n, 1, dim), device=cuda).normal_(generator=gen))
+    q[..., 0] = large
+    check(s, fp8_extend_attention(q, s.pool, s.layer, s.table, *lens, 0.25), q, prefix, new, 0.25)
+
+
 def test_extreme_key_scales(cuda):
     s, q, lens = batch(cuda, [0], [200], 1, 64, 2)
     for b, size in enumerate((1e-33, 1.0, 0.0)):
