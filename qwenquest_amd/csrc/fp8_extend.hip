@@ -12,12 +12,13 @@
 //   8192 1521 us against 1622.  But they do not add in 32 bits: where one of 64 products carries the sum,
 //   it comes out off by 2^-11 of itself, bf16's by 2^-22, and keys have channels like that.)
 //   O^T += V^T W^T  v_mfma_f32_32x32x16_f16, V's codes to f16 (exact)
-// With t = scale log2(e) ks (q . kc), M a running maximum of t that is let lag by 8 (the sums are
-// rescaled once it lags more), and R the largest exponent of a V scale so far (one number per
-// wave), a weight goes into the product as
-//   w = 2^(t - M + lv - R + 7),  vs = 2^lv,
-// so V's scale costs nothing per element, w fills f16's range from the top (7 + 8) and what
-// another block's far larger values leave of it is lost only under 2^-32 of those.  w goes to f16's
+// With t = scale log2(e) ks (q . kc), vs = 2^lv, M a row's running maximum of t that is let lag by 8 (the
+// sums are rescaled once it lags more), and R that of t - M + lv, a whole number that likewise lags by
+// 8 and falls where M rises, a weight goes into the product as
+//   w = 2^(t - M + lv - R + 7),
+// so V's scale costs nothing per element, w fills f16's range from the top (7 + 8), and a token is
+// lost only where its weight times its block's V scale is under 2^-31 of the row's largest such product
+// (larger V scales of tokens that weigh next to nothing take nothing from the others).  w goes to f16's
 // 11 bits by truncation (one instruction for two weights) of w (1 + 0.72 * 2^-11): truncation takes
 // half a step on average, 2^-10 / 2 over the significand's 1 .. 2, in the mean 0.72 * 2^-11.
 // A weight is off by 0.64 * 2^-10 at most, an output by that of sum p |v|, where its own rounding
@@ -37,7 +38,7 @@ typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 
 constexpr int kLift = 7, kSlack = 8;  // w <= 2^(7 + 8) * kRound < f16's 65504
 constexpr float kRound = 1.0003516f, kRoundLog2 = 5.0713e-4f;  // 1 + 0.72 * 2^-11
-constexpr int kExpFloor = -60;      // of lv - R: f16 has nothing left of such weights, their fp32 sum has
+constexpr float kExpFloor = -60.0f;  // of lv - R: f16 has nothing left of such weights, their fp32 sum has
 
 struct Fp8ExtendArgs {
   const uint16_t* q;  // [n, H, D]
@@ -167,8 +168,7 @@ __global__ __launch_bounds__(64 * kExtWaves, 2) void fp8_extend_kernel(Fp8Extend
   for (int c = 0; c < NC; ++c)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[c][i] = 0.0f;
-  float M = -INFINITY, L = 0.0f;
-  int R = kScaleMin;
+  float M = -INFINITY, R = 0.0f, L = 0.0f;
   // LDS addresses of this lane's pieces: K token lo of a half, pieces 2 i + hf; V channel lo of a
   // tile of 32, token groups hf and hf + 2
   const int k_off = (lo >> 4) * 16 * D + (lo & 15) * 16 + hf * 256;
@@ -245,12 +245,14 @@ __global__ __launch_bounds__(64 * kExtWaves, 2) void fp8_extend_kernel(Fp8Extend
 #pragma unroll
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[t][i]);
     mx = fmaxf(mx, lane_xor32(mx, lane)) * c;
-    const int lv = vs != vs ? R : exponent_of(vs);
-    if (__any(mx > M + kSlack) || lv > R) {
+    const float lv = vs != vs ? 0.0f : (float)exponent_of(vs);
+    if (__any(mx > M + kSlack || mx + lv > M + R + kSlack)) {
       const float Mn = fmaxf(M, mx);
+      const float was = M == -INFINITY ? -INFINITY : R + (M - Mn);
+      // (at least kScaleMin, but for scores that are not finite and a row without any so far)
+      const float Rn = Mn == -INFINITY ? R : fmaxf(ceilf(fmaxf(lv + (mx - Mn), was)), -126.0f);
       const float am = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - Mn);
-      const int Rn = max(R, lv);
-      const float ao = am * __builtin_amdgcn_exp2f((float)max(R - Rn, -126));
+      const float ao = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(fmaxf(was - Rn, -126.0f));
       L *= am;
 #pragma unroll
       for (int x = 0; x < NC; ++x)
@@ -259,9 +261,9 @@ __global__ __launch_bounds__(64 * kExtWaves, 2) void fp8_extend_kernel(Fp8Extend
       M = Mn;
       R = Rn;
     }
-    const int lift = max(lv - R, kExpFloor) + kLift;
+    const float lift = fmaxf(lv - R, kExpFloor) + (float)kLift;
     // NaN where the block's V scale is
-    float bias = (float)lift + kRoundLog2 + (vs != vs ? vs : 0.0f);
+    float bias = lift + kRoundLog2 + (vs != vs ? vs : 0.0f);
     bias = M == -INFINITY ? bias : bias - M;
     float sum = 0.0f;
 #pragma unroll
@@ -278,7 +280,7 @@ __global__ __launch_bounds__(64 * kExtWaves, 2) void fp8_extend_kernel(Fp8Extend
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int i = 0; i < 16; ++i) sum += s[t][i];
-    L = __builtin_fmaf(sum, pow2f(-lift) * (1.0f / kRound), L);
+    L += __builtin_amdgcn_ldexpf(sum * (1.0f / kRound), -(int)lift);
     // O^T += V^T W^T, 16 tokens at a time
     u32x4_t wv[4];
 #pragma unroll
@@ -298,7 +300,7 @@ __global__ __launch_bounds__(64 * kExtWaves, 2) void fp8_extend_kernel(Fp8Extend
   L += lane_xor32(L, lane);
   if (__syncthreads_or(bad)) L = __builtin_nanf("");  // a block that is not there: no answer
   const bool mine = r0 + wave * 32 + lo < rows_n;
-  const float unit = pow2f(R - kLift);
+  const float unit = __builtin_amdgcn_exp2f(R - (float)kLift);
   if (whole) {
     if (!mine) return;
     uint16_t* op = a.out + (qp - a.q) + 4 * hf;

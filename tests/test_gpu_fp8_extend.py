@@ -102,6 +102,28 @@ def test_a_channel_that_carries_the_scores(cuda, large, dim, prefix, new):
     check(s, fp8_extend_attention(q, s.pool, s.layer, s.table, *lens, 0.25), q, prefix, new, 0.25)
 
 
+@pytest.mark.parametrize("prefix, new", [([0], [330]), ([2000], [3]), ([60, 0], [270, 200])])
+@pytest.mark.parametrize("size", [2.0**20, 2.0**40, 2.0**-40])
+@pytest.mark.parametrize("at", [0, 2, -1])
+def test_values_of_very_different_size_and_weight(cuda, prefix, new, size, at):
+    """One block whose values are far larger (or smaller) than the others' and whose tokens weigh next to
+    nothing, 2^-90: the others' values come back as without it."""
+    dim, scale = 64, 0.5
+    s, q, lens = batch(cuda, prefix, new, 1, dim, 4, seed=5)
+    gen = torch.Generator(device=cuda).manual_seed(2)
+    q.mul_(0.25)
+    q[..., 0] = 8.0
+    for r, (p, n) in enumerate(zip(prefix, new)):
+        blocks = -(-(p + n) // 64)
+        for b in range(blocks):
+            k = torch.empty((64, 1, dim), device=cuda).normal_(generator=gen) * 0.25
+            v = torch.empty((64, 1, dim), device=cuda).normal_(generator=gen)
+            odd = b == at % blocks
+            k[..., 0] = -8.0 if odd else 8.0
+            s.pool.set_kv_buffer(s.layer, s.rows(r, np.arange(b * 64, b * 64 + 64)), k, v * (size if odd else 1.0))
+    check(s, fp8_extend_attention(q, s.pool, s.layer, s.table, *lens, scale), q, prefix, new, scale)
+
+
 def test_extreme_key_scales(cuda):
     s, q, lens = batch(cuda, [0], [200], 1, 64, 2)
     for b, size in enumerate((1e-33, 1.0, 0.0)):
