@@ -128,7 +128,7 @@ class QuestOnlyBackend(AttentionBackend):
 
     def _update_quest_for_extend(self, batch: ForwardBatch) -> None:
         """[Q2] Per request: bounds of positions ``0 .. seq_len-1`` at every layer (quest_only.py:115-128)."""
-        if self.fp8:
+        if self.fp8:  # from page 0 in every chunk: a prefix may be in the pool without this backend's prefill
             self.quest.update_prefill_representations_blocks(batch.req_pool_indices, batch.seq_lens,
                                                              self.token_to_kv_pool, self.req_to_token_pool.block_table)
             return

@@ -25,14 +25,15 @@
 // takes a unit at a time: K and V codes straight from memory to registers in the
 // operands' order (1 KiB runs), converted to bf16 (exact), S^T = K Q^T, the softmax in
 // registers, O^T += V^T P^T, with P's values scaled by vs as three bf16 pieces, which hold all 24
-// significand bits (in two pieces, 16 bits, bf16 outputs were off by a step in a few of a hundred places,
+// significand bits (in two pieces, 16 bits, bf16 outputs were off by a step in a few of a thousand places,
 // for 2 us less of 145 in 12 layers of one request of 2000 tokens).  fp32 queries go in as three bf16
 // pieces, too.
 // Bound: HBM, the codes once, when they are many: 16 requests of 131072 tokens, 4 heads of 128,
-// 378 us (5.7 TB/s).  A small batch is bound by its chain of memory round trips (slice, table
-// words, scales and codes, partials, count, merge, ~1 us each): one request of 2000 tokens 10.8 us
-// a layer, 15.2 in two launches; the plan 4.4 us a step.  16 requests' 31 pages and window of
-// 131072 tokens 17.6 us with the selection, 14.7 behind a begin launch of 5.3.
+// 379 us (5.7 TB/s; matrix pipes 18 % busy, vector units 44 %).  A small batch is bound by its chain
+// of memory round trips (slice, table words, scales and codes, partials, count, merge, ~1 us each):
+// one request of 2000 tokens 11.4 us a layer, of which its waves wait 80 %; 15.8 in two launches; the
+// plan 4.6 us a step.  16 requests' 31 pages and window of 131072 tokens 18.1 us with the selection
+// (waiting 54 %), 16.1 behind a begin launch of 5.4.
 #include "qq_fp8_plan.h"
 #include "qq_fp8_store.h"
 #include "qq_quest_dev.h"

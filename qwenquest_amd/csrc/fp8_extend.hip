@@ -22,12 +22,17 @@
 // 11 bits by truncation (one instruction for two weights) of w (1 + 0.72 * 2^-11): truncation takes
 // half a step on average, 2^-10 / 2 over the significand's 1 .. 2, in the mean 0.72 * 2^-11.
 // A weight is off by 0.64 * 2^-10 at most, an output by that of sum p |v|, where its own rounding
-// is 2^-8 of it; the weights' sum stays in fp32.
+// is 2^-8 of it; the weights' sum stays in fp32.  (Against 64 bits the output of 8192 tokens behind 8192
+// is off by 0.001672 of its size, of which the bf16 rounding alone is 0.001658.  A second f16 piece of
+// the weights, 22 bits, leaves that alone, and costs another value product: 1601 -> 2167 us, 3440
+// tokens of 6 prompts 182 -> 232.)
 //
-// Bound: the matrix cores and, beside them, the softmax's vector instructions.  Measured, 32 query
-// heads on 4 of 128: 8192 tokens behind 8192 1622 us (1.02 PFLOP/s of the formula's operations; with
-// vector lookups 10 % more), 3440 tokens of 6 prompts 186 us with their store, where the longest tile chain is
-// as long as the rest.
+// Bound: the matrix cores and, beside them, the softmax's vector instructions: by the counters
+// the matrix pipes are busy for 49 % of the time and the vector units for 65 % (4 cycles for each of
+// their other instructions), waves wait for memory for 14 % of theirs, and no LDS access meets a bank
+// conflict.  Measured, 32 query heads on 4 of 128: 8192 tokens behind 8192 1618 us (1.02 PFLOP/s of the
+// formula's operations; 1598 to 1624 by box), 3440 tokens of 6 prompts 173 to 187 with their store, where
+// the longest tile chain is as long as the rest.
 #include "qq_extend_dev.h"
 #include "qq_fp8.h"
 
