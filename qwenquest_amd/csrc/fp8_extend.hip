@@ -31,7 +31,7 @@
 // the matrix pipes are busy for 49 % of the time and the vector units for 65 % (4 cycles for each of
 // their other instructions), waves wait for memory for 14 % of theirs, and no LDS access meets a bank
 // conflict.  Measured, 32 query heads on 4 of 128: 8192 tokens behind 8192 1618 us (1.02 PFLOP/s of the
-// formula's operations; 1598 to 1624 by box), 3440 tokens of 6 prompts 173 to 187 with their store, where
+// formula's operations; 1598 to 1635 by box), 3440 tokens of 6 prompts 173 to 187 with their store, where
 // the longest tile chain is as long as the rest.
 #include "qq_extend_dev.h"
 #include "qq_fp8.h"
