@@ -488,8 +488,6 @@ def _plain_cache(blocks: int, layers: int, kv: int, D: int) -> dict:
 def _quantised(x: torch.Tensor, group: int) -> torch.Tensor:
     """[n, KV, D] as the cache keeps it, one scale for `group` channels."""
     y = x.float().unflatten(-1, (-1, group))
-    good = torch.isfinite(y).all(-1, keepdim=True)
-    y = torch.where(good, y, 0.0)
     frac, e = torch.frexp(y.abs().amax(-1, keepdim=True))  # amax <= 7 * 2 ** e: 7 = 0.875 * 2 ** 3
     e = torch.where(frac <= 0.875, e - 3, e - 2)
     e = torch.where(frac == 0, E_LO, e).clamp(E_LO, E_HI)
@@ -497,15 +495,17 @@ def _quantised(x: torch.Tensor, group: int) -> torch.Tensor:
     y = y * half[0] * half[1]
     _, ye = torch.frexp(y)
     step = _pow2((ye - 1).clamp(min=0) - 1)
-    y = (torch.round(y / step) * step).clamp(-TOP, TOP) * _pow2(e)
-    return torch.where(good, y, math.nan).flatten(-2).to(torch.bfloat16)
+    return ((torch.round(y / step) * step).clamp(-TOP, TOP) * _pow2(e)).flatten(-2).to(torch.bfloat16)
 
 
 def _plain_store(st: dict, layer: int, loc: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
-    for values, x, group in ((st["kc"], k, GROUP), (st["vc"], v, v.shape[-1])):
-        rows = values[layer].view(-1, *x.shape[1:])
-        for a in range(0, loc.numel(), 1 << 17):  # a long prompt's in 32 bits are large
-            rows[loc[a : a + (1 << 17)]] = _quantised(x[a : a + (1 << 17)], group)
+    for a in range(0, loc.numel(), 1 << 17):  # a long prompt's in 32 bits are large
+        at, x, y = (t[a : a + (1 << 17)] for t in (loc, k, v))
+        # of a token and head that holds what is not finite nothing is kept
+        good = torch.isfinite(x).all(-1, keepdim=True) & torch.isfinite(y).all(-1, keepdim=True)
+        for values, z, group in ((st["kc"], x, GROUP), (st["vc"], y, y.shape[-1])):
+            z = _quantised(torch.where(good, z, 0.0), group)
+            values[layer].view(-1, *z.shape[1:])[at] = torch.where(good, z, math.nan)
 
 
 def _plain_rows(st: dict, layer: int, loc: torch.Tensor):
