@@ -27,7 +27,7 @@ own = False
 
 BLOCK = 64  # tokens of a block, and of a Quest page
 GROUP = 32  # channels of a key that share a scale
-E_LO, E_HI = -96, 125  # exponents of a scale
+K_EXP, V_EXP = (-96, 125), (-50, 59)  # exponents of a scale
 TOP = 6.0  # largest e2m1 value
 EPS = 1e-6
 DEV = torch.device("cuda", 0)
@@ -485,12 +485,12 @@ def _plain_cache(blocks: int, layers: int, kv: int, D: int) -> dict:
     return {c: torch.zeros((layers, blocks, BLOCK, kv, D), dtype=torch.bfloat16, device=DEV) for c in ("kc", "vc")}
 
 
-def _quantised(x: torch.Tensor, group: int) -> torch.Tensor:
+def _quantised(x: torch.Tensor, group: int, span: tuple[int, int]) -> torch.Tensor:
     """[n, KV, D] as the cache keeps it, one scale for `group` channels."""
     y = x.float().unflatten(-1, (-1, group))
     frac, e = torch.frexp(y.abs().amax(-1, keepdim=True))  # amax <= 7 * 2 ** e: 7 = 0.875 * 2 ** 3
     e = torch.where(frac <= 0.875, e - 3, e - 2)
-    e = torch.where(frac == 0, E_LO, e).clamp(E_LO, E_HI)
+    e = torch.where(frac == 0, span[0], e).clamp(*span)
     half = _pow2(-(e // 2)), _pow2(-(e - e // 2))
     y = y * half[0] * half[1]
     _, ye = torch.frexp(y)
@@ -501,10 +501,10 @@ def _quantised(x: torch.Tensor, group: int) -> torch.Tensor:
 def _plain_store(st: dict, layer: int, loc: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
     for a in range(0, loc.numel(), 1 << 17):  # a long prompt's in 32 bits are large
         at, x, y = (t[a : a + (1 << 17)] for t in (loc, k, v))
-        # of a token and head that holds what is not finite nothing is kept
-        good = torch.isfinite(x).all(-1, keepdim=True) & torch.isfinite(y).all(-1, keepdim=True)
-        for values, z, group in ((st["kc"], x, GROUP), (st["vc"], y, y.shape[-1])):
-            z = _quantised(torch.where(good, z, 0.0), group)
+        # of a token and head that holds what is not finite, or too large in V, nothing is kept
+        good = torch.isfinite(x).all(-1, keepdim=True) & (y.abs() <= 7 * 2.0 ** V_EXP[1]).all(-1, keepdim=True)
+        for values, z, group, span in ((st["kc"], x, GROUP, K_EXP), (st["vc"], y, y.shape[-1], V_EXP)):
+            z = _quantised(torch.where(good, z, 0.0), group, span)
             values[layer].view(-1, *z.shape[1:])[at] = torch.where(good, z, math.nan)
 
 
@@ -622,7 +622,7 @@ def run(state: dict):
 # ---------------------------------------------------------------- the same in 64 bits
 
 
-def _exact_values(x: torch.Tensor, group: int) -> torch.Tensor:
+def _exact_values(x: torch.Tensor, group: int, span: tuple[int, int]) -> torch.Tensor:
     """The nearest of +-{0, 1/2, 1, 3/2, 2, 3, 4, 6} times the group's scale, ties to the even code."""
     grid = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], dtype=torch.float64, device=x.device)
     border = (grid[1:] + grid[:-1]) / 2
@@ -630,11 +630,11 @@ def _exact_values(x: torch.Tensor, group: int) -> torch.Tensor:
     for part in x.split(1 << 16):
         y = part.double().unflatten(-1, (-1, group))
         high = y.abs().amax(-1, keepdim=True)
-        e = torch.full_like(high, E_LO)
+        e = torch.full_like(high, span[0])
         e = torch.where(high > 0, torch.ceil(torch.log2(high.clamp(min=1e-300) / 7.0)), e)
         # a logarithm may be off next to a power of two
         e = torch.where(high > 7.0 * torch.exp2(e), e + 1, e)
-        e = torch.where(high <= 7.0 * torch.exp2(e - 1), e - 1, e).clamp(E_LO, E_HI)
+        e = torch.where(high <= 7.0 * torch.exp2(e - 1), e - 1, e).clamp(*span)
         y = y / torch.exp2(e)
         code = torch.bucketize(y.abs(), border)  # the lower neighbour at a border
         on_border = (code < 7) & (y.abs() == border[code.clamp(max=6)])
@@ -687,7 +687,7 @@ def exact(case: dict, seed: int):
 
     def values(layer: int, i: int):
         k, v = kv_of(layer, i)
-        return _exact_values(k, GROUP), _exact_values(v, D)
+        return _exact_values(k, GROUP, K_EXP), _exact_values(v, D, V_EXP)
 
     if kind == "store":
         rows = [], []
