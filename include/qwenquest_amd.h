@@ -547,6 +547,99 @@ int qq_fp8_extend_attention(const void* q, int num_q_heads, const uint8_t* k_cod
 int64_t qq_fp8_extend_workspace_bytes(int64_t n, int bs, int num_q_heads, int kv_heads, int head_dim,
                                       int block_table_cols);
 
+/* ---------------------------------------------------------- 4-bit K/V cache
+ * A cache of num_blocks blocks of 64 tokens (block 0 is padding: never written): of each layer
+ * k_codes / v_codes [num_blocks, kv_heads, 32 * head_dim] bytes of e2m1 codes in the kernels'
+ * order (csrc/qq_fp4.h), and scales, each the byte of a power of two's exponent: k_scale
+ * [num_blocks, kv_heads, 2 * head_dim], one for each token and 32 channels, v_scale
+ * [num_blocks, kv_heads, 64], one for each token; a value is code * 2^(scale - 127).  head_dim 64
+ * or 128.  Pool row r is token r % 64 of block r / 64.  What is not said here is as in the 8-bit
+ * cache's entry of the same name. */
+
+/* k[i], v[i] ([n, kv_heads, head_dim] bf16 or fp32, 16-byte aligned) go to row loc[i].  The scale
+ * of values with largest magnitude m is 2^e, e the least with m <= 7 * 2^e, of K -96 to 125, of V -50 to
+ * 59; codes are rounded to nearest even, 6 at most.  Of a token and head whose K or V holds a value that
+ * is not finite, or whose V one above 7 * 2^59, nothing is kept: K and V read as NaN.  Rows of block 0 and
+ * outside the cache are skipped.  The entries of one block stand next to each other in loc (of a
+ * row listed in two runs either entry's value, or parts of both, may stay); of a row listed twice in a
+ * run the last entry counts.  No other row is touched. */
+int qq_fp4_store(uint8_t* k_codes, uint8_t* v_codes, uint8_t* k_scale, uint8_t* v_scale, int num_blocks,
+                 int kv_heads, int head_dim, const void* k, const void* v, int src_dtype, const int64_t* loc,
+                 int64_t n, void* stream);
+
+/* k[i], v[i] = the values of row loc[i] ([n, kv_heads, head_dim]; exact in bf16 as in fp32);
+ * NaN for a row outside the cache. */
+int qq_fp4_rows(const uint8_t* k_codes, const uint8_t* v_codes, const uint8_t* k_scale, const uint8_t* v_scale,
+                int num_blocks, int kv_heads, int head_dim, const int64_t* loc, int64_t n, void* k, void* v,
+                int dst_dtype, void* stream);
+
+/* qq_fp8_page_bounds over the 4-bit cache (layer strides in bytes); a page that holds a lost token has
+ * NaN bounds for that head.  plan: a workspace of qq_fp4_decode_workspace_bytes. */
+int qq_fp4_page_bounds(const uint8_t* k_codes, int64_t codes_layer_stride, const uint8_t* k_scale,
+                       int64_t scale_layer_stride, int num_blocks, int kv_heads, int head_dim,
+                       const int32_t* block_table, int64_t block_table_stride, int block_table_rows,
+                       int block_table_cols, const int64_t* req_pool_indices, const int64_t* seq_lens,
+                       const int64_t* prefix_lens, int bs, int decode, int64_t max_new, int n_layers,
+                       uint16_t* page_k_bounds, int max_reqs, int max_pages, int top_k,
+                       int avoid_recent_overlap, int32_t* actual_lens, int32_t* candidate_limit, void* plan,
+                       int64_t plan_bytes, void* stream);
+
+/* qq_fp8_decode_attention over the 4-bit cache. */
+int qq_fp4_decode_attention(const void* q, int q_dtype, int64_t q_batch_stride, int num_q_heads,
+                            const void* k_new, const void* v_new, int new_dtype, const int64_t* out_cache_loc,
+                            uint8_t* k_codes, uint8_t* v_codes, uint8_t* k_scale, uint8_t* v_scale, int num_blocks,
+                            int kv_heads, int head_dim, const int32_t* block_table, int64_t block_table_stride,
+                            int block_table_rows, int block_table_cols, const int64_t* req_pool_indices,
+                            const int64_t* seq_lens, int bs, const int32_t* positions, int64_t positions_stride,
+                            int top_k, float scale, void* out, void* workspace, int64_t workspace_bytes,
+                            int planned, void* stream);
+int64_t qq_fp4_decode_workspace_bytes(int bs, int num_q_heads, int kv_heads, int head_dim);
+
+/* qq_fp8_decode_plan for calls of qq_fp4_decode_attention. */
+int qq_fp4_decode_plan(int num_blocks, int kv_heads, int head_dim, int block_table_rows, int block_table_cols,
+                       const int64_t* req_pool_indices, const int64_t* seq_lens, int bs, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+
+/* qq_fp8_quest_step over the 4-bit cache.  Planned (by qq_fp4_page_bounds), bf16 queries of 128 channels,
+ * up to 16 query heads per KV head, top_k of 512 to 2624 (in tables of more than 4096 pages to 4160), up to 8192 pages
+ * and as many requests as the chip's blocks hold per head (256 / kv_heads) take two launches: the scores; the
+ * selection with the store and the attention.  Others take three or four, as there. */
+int qq_fp4_quest_step(const void* q, int q_dtype, int64_t q_batch_stride, int num_q_heads, const void* k_new,
+                      const void* v_new, int new_dtype, const int64_t* out_cache_loc, uint8_t* k_codes,
+                      uint8_t* v_codes, uint8_t* k_scale, uint8_t* v_scale, int num_blocks, int kv_heads, int head_dim,
+                      const int32_t* block_table, int64_t block_table_stride, int block_table_rows,
+                      int block_table_cols, const uint16_t* page_k_bounds, int layer,
+                      const int64_t* req_pool_indices, const int64_t* seq_lens, const int32_t* candidate_limit,
+                      int bs, int max_reqs, int max_pages, int top_k, float scale, float* scores_ws,
+                      int32_t* positions, void* out, void* workspace, int64_t workspace_bytes, int phase,
+                      int planned, void* stream);
+
+/* qq_fp8_extend_attention over the 4-bit cache. */
+int qq_fp4_extend_attention(const void* q, int num_q_heads, const uint8_t* k_codes, const uint8_t* v_codes,
+                            const uint8_t* k_scale, const uint8_t* v_scale, int num_blocks, int kv_heads,
+                            int head_dim, const int32_t* block_table, int64_t block_table_stride,
+                            int block_table_rows, int block_table_cols, const int64_t* req_pool_indices,
+                            const int64_t* seq_lens, const int64_t* prefix_lens, const int64_t* extend_lens,
+                            int bs, int64_t n, float scale, void* out, void* workspace,
+                            int64_t workspace_bytes, void* stream);
+int64_t qq_fp4_extend_workspace_bytes(int64_t n, int bs, int num_q_heads, int kv_heads, int head_dim,
+                                      int block_table_cols);
+
+/* ------------------------------------------------- norms and rotation of heads
+ * Of n tokens the query heads q[i] ([H, head_dim], rows q_stride elements apart) and key heads k[i]
+ * become y = x / sqrt(mean x^2 + eps) * weight per head (q_weight, k_weight [head_dim] fp32; NULL: no norm),
+ * then pair j of the first 2 * pairs channels (a, b) becomes (a cos t - b sin t, b cos t + a sin t) with t =
+ * positions[pair_axis[j] * positions_stride + i] * quarter_turns[j] quarter turns; b is channel j + pairs of a = j, with
+ * neighbours != 0 channel 2 j + 1 of 2 j.  fp32, rounded once to dtype (bf16 or fp32); q_out [n, H, head_dim] and k_out dense.
+ * v (or NULL) is copied to v_out as it is.  A token at a position of 2^31 or beyond, either way, gets NaN where it would
+ * turn.  head_dim a multiple of 8 up to 512; pairs a multiple of 8 (neighbours: 4), 0: no rotation; every row
+ * 16-byte aligned.  pair_axis [pairs] holds 0 .. axes - 1.  The outputs must not overlap the inputs. */
+int qq_qk_norm_rotary(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                      int dtype, int num_q_heads, int kv_heads, int head_dim, int64_t n, const float* q_weight,
+                      const float* k_weight, float eps, const double* quarter_turns, const int32_t* pair_axis, int pairs,
+                      int neighbours, const int64_t* positions, int64_t positions_stride, int axes, void* q_out, void* k_out,
+                      void* v_out, void* stream);
+
 /* ------------------------------------------------------------- HiSparse tier
  * Layouts of the reference HiSparseCoordinator (src/qwenquest/hisparse/coordinator.py:103-131):
  * device_k/v[layer] [R*(buf+1), KV, D] (request r owns rows r*(buf+1) + slot,

@@ -10,8 +10,9 @@ runs in hand-written gfx950 HIP kernels of ``libqwenquest_amd.so`` behind a C AB
 from qwenquest_amd.batch import ForwardBatch, ForwardMode
 from qwenquest_amd.config import SparseConfig, parse_hisparse_config
 from qwenquest_amd.memory import MHATokenToKVPool, ReqToTokenPool, TokenToKVPoolAllocator
-from qwenquest_amd.paged import BlockReqToTokenPool, Fp8TokenToKVPool
+from qwenquest_amd.paged import BlockReqToTokenPool, Fp4TokenToKVPool, Fp8TokenToKVPool
 from qwenquest_amd.quest import QuestAlgorithm, QuestSelection, QuestTrace, StepLayout
+from qwenquest_amd.rotary import QKNormRotary
 
 __version__ = "0.1.0"
 
@@ -19,8 +20,10 @@ __all__ = [
     "BlockReqToTokenPool",
     "ForwardBatch",
     "ForwardMode",
+    "Fp4TokenToKVPool",
     "Fp8TokenToKVPool",
     "MHATokenToKVPool",
+    "QKNormRotary",
     "QuestAlgorithm",
     "QuestSelection",
     "QuestTrace",

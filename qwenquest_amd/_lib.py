@@ -132,6 +132,34 @@ SIGNATURES: dict[str, tuple] = {
         [_P, _I, _P, _P, _P, _P, _I, _I, _I, _P, _L, _I, _I, _P, _P, _P, _P, _I, _L, _F, _P, _P, _L, _P],
     ),
     "qq_fp8_extend_workspace_bytes": (_L, [_L, _I, _I, _I, _I, _I]),
+    "qq_fp4_store": (_I, [_P, _P, _P, _P, _I, _I, _I, _P, _P, _I, _P, _L, _P]),
+    "qq_fp4_rows": (_I, [_P, _P, _P, _P, _I, _I, _I, _P, _L, _P, _P, _I, _P]),
+    "qq_fp4_page_bounds": (
+        _I,
+        [_P, _L, _P, _L, _I, _I, _I, _P, _L, _I, _I, _P, _P, _P, _I, _I, _L, _I, _P, _I, _I, _I, _I, _P, _P, _P,
+         _L, _P],
+    ),
+    "qq_fp4_decode_attention": (
+        _I,
+        [_P, _I, _L, _I, _P, _P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _P, _L, _I, _I, _P, _P, _I, _P, _L, _I, _F,
+         _P, _P, _L, _I, _P],
+    ),
+    "qq_fp4_decode_plan": (_I, [_I, _I, _I, _I, _I, _P, _P, _I, _P, _L, _P]),
+    "qq_fp4_decode_workspace_bytes": (_L, [_I, _I, _I, _I]),
+    "qq_fp4_quest_step": (
+        _I,
+        [_P, _I, _L, _I, _P, _P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _P, _L, _I, _I, _P, _I, _P, _P, _P, _I, _I, _I,
+         _I, _F, _P, _P, _P, _P, _L, _I, _I, _P],
+    ),
+    "qq_fp4_extend_attention": (
+        _I,
+        [_P, _I, _P, _P, _P, _P, _I, _I, _I, _P, _L, _I, _I, _P, _P, _P, _P, _I, _L, _F, _P, _P, _L, _P],
+    ),
+    "qq_fp4_extend_workspace_bytes": (_L, [_L, _I, _I, _I, _I, _I]),
+    "qq_qk_norm_rotary": (
+        _I,
+        [_P, _L, _P, _L, _P, _L, _I, _I, _I, _I, _L, _P, _P, _F, _P, _P, _I, _I, _P, _L, _I, _P, _P, _P, _P],
+    ),
     "qq_hisparse_swap_in": (
         _I,
         [_P, _L, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _L, _P, _P, _P, _P, _L, _L, _P, _P, _P,

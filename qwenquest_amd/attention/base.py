@@ -15,12 +15,12 @@ import torch
 from torch.autograd import forward_ad
 
 from qwenquest_amd.attention.ops import (
+    coded_extend_attention,
     extend_attention,
     extend_attention_batch,
     extend_attention_batch_checked,
-    fp8_extend_attention,
 )
-from qwenquest_amd.paged import BlockReqToTokenPool, Fp8TokenToKVPool
+from qwenquest_amd.paged import BlockReqToTokenPool, CodedTokenToKVPool, Fp8TokenToKVPool
 
 if TYPE_CHECKING:
     from qwenquest_amd.batch import ForwardBatch
@@ -47,11 +47,12 @@ class AttentionBackend(ABC):
     def __init__(self, req_to_token_pool: ReqToTokenPool, token_to_kv_pool: MHATokenToKVPool):
         self.req_to_token_pool = req_to_token_pool
         self.token_to_kv_pool = token_to_kv_pool
-        #: whether the pool holds 8-bit blocks
+        #: whether the pool holds blocks of codes, in 8 or 4 bits; whether in 8
+        self.coded = isinstance(token_to_kv_pool, CodedTokenToKVPool)
         self.fp8 = isinstance(token_to_kv_pool, Fp8TokenToKVPool)
-        if self.fp8:
+        if self.coded:
             if not isinstance(req_to_token_pool, BlockReqToTokenPool):
-                raise ValueError("an Fp8TokenToKVPool needs a BlockReqToTokenPool")
+                raise ValueError(f"an {type(token_to_kv_pool).__name__} needs a BlockReqToTokenPool")
             if req_to_token_pool.num_blocks > token_to_kv_pool.num_blocks:
                 raise ValueError(f"the request pool hands out {req_to_token_pool.num_blocks} blocks, the K/V pool has "
                                  f"{token_to_kv_pool.num_blocks}")
@@ -68,6 +69,14 @@ class AttentionBackend(ABC):
             return self.forward_decode(q, k, v, layer, batch)
         return self.forward_extend(q, k, v, layer, batch)
 
+    def forward_qkv(self, qkv: torch.Tensor, layer: Any, batch: ForwardBatch) -> torch.Tensor:
+        """``forward`` from the layer's QKV product ``[n, (heads + 2 kv_heads) * head_dim]``: the norms of its heads and
+        their rotation at ``batch.positions`` by ``layer.rotary`` (``QKNormRotary``), then the attention."""
+        rotary = getattr(layer, "rotary", None)
+        if rotary is None or batch.positions is None:
+            raise ValueError("forward_qkv needs layer.rotary (a QKNormRotary) and batch.positions")
+        return self.forward(*rotary(qkv, batch.positions), layer, batch)
+
     def forward_extend(self, q, k, v, layer, batch: ForwardBatch) -> torch.Tensor:
         """Dense causal prefill: save the new K/V, then attend per request (base.py:65-93).
 
@@ -80,12 +89,12 @@ class AttentionBackend(ABC):
         """
         assert batch.out_cache_loc is not None and batch.extend_prefix_lens is not None
         pool = self.token_to_kv_pool
-        if self.fp8 and torch._C._get_tracing_state() is not None:
+        if self.coded and torch._C._get_tracing_state() is not None:
             # neither the store nor the rows read back are torch operations
-            raise RuntimeError("a prefill over an 8-bit pool cannot be traced: a trace would keep its values, not its work")
+            raise RuntimeError("a prefill over a pool of codes cannot be traced: a trace would keep its values, not its work")
         pool.set_kv_buffer(layer.layer_id, batch.out_cache_loc, k, v)
-        if self.fp8:
-            return self._forward_extend_fp8(q, layer, batch)
+        if self.coded:
+            return self._forward_extend_coded(q, layer, batch)
         k_buf, v_buf = pool.get_kv_buffer(layer.layer_id)
         if self._extend_fast(q, k_buf, v_buf, layer.scaling, batch):
             attend = (extend_attention_batch if torch.cuda.is_current_stream_capturing()
@@ -106,8 +115,8 @@ class AttentionBackend(ABC):
             )
         return torch.cat(outputs, dim=0)
 
-    def _forward_extend_fp8(self, q: torch.Tensor, layer: Any, batch: ForwardBatch) -> torch.Tensor:
-        """forward_extend over an 8-bit pool, which holds the new K/V: every token attends the
+    def _forward_extend_coded(self, q: torch.Tensor, layer: Any, batch: ForwardBatch) -> torch.Tensor:
+        """forward_extend over an 8- or 4-bit pool, which holds the new K/V: every token attends the
         pool's values, its own included.  bf16 queries with a positive scale run the whole batch in
         one launch that reads the lengths on the device (NaN where the loop would refuse a request
         index); others go request by request over the values.  Either way the output has q's rows,
@@ -116,9 +125,9 @@ class AttentionBackend(ABC):
         q = q.reshape(q.shape[0], math.prod(q.shape[1:]) // pool.head_dim, pool.head_dim)
         if (q.dtype == torch.bfloat16 and 0.0 < float(layer.scaling) < float("inf") and _plain(q)
                 and batch.extend_seq_lens is not None):
-            return fp8_extend_attention(q, pool, layer.layer_id, self.req_to_token_pool.block_table,
-                                        batch.req_pool_indices, batch.seq_lens, batch.extend_prefix_lens,
-                                        batch.extend_seq_lens, float(layer.scaling))
+            return coded_extend_attention(q, pool, layer.layer_id, self.req_to_token_pool.block_table,
+                                          batch.req_pool_indices, batch.seq_lens, batch.extend_prefix_lens,
+                                          batch.extend_seq_lens, float(layer.scaling))
         offsets = batch.extend_token_offsets()
         outputs = []
         for i in range(batch.batch_size):

@@ -5,9 +5,9 @@ Every decode step attends each request's whole KV history in the device token
 pool.  bf16 with 4 KV heads x 128 runs one C call (``qq_dense_forward_decode``:
 the new K/V store, then the attention kernel of the Quest layer step over all
 of a request's rows); other shapes store the new K/V and run the split-K
-attention over the explicit row list ``req_to_token[req, :seq_len]``.  Over an 8-bit pool
-(``Fp8TokenToKVPool``) one C call does both for every shape the pool takes
-(``qq_fp8_decode_attention``), after ``init_forward_metadata`` as one launch.
+attention over the explicit row list ``req_to_token[req, :seq_len]``.  Over an 8- or 4-bit
+pool (``Fp8TokenToKVPool``, ``Fp4TokenToKVPool``) one C call does both for every shape the pool takes
+(``qq_fp8_decode_attention``, ``qq_fp4_decode_attention``), after ``init_forward_metadata`` as one launch.
 """
 
 from __future__ import annotations
@@ -21,9 +21,9 @@ from qwenquest_amd import _lib
 from qwenquest_amd.attention.base import AttentionBackend
 from qwenquest_amd.attention.ops import (
     AttentionWorkspace,
+    coded_decode_attention,
+    coded_decode_plan,
     decode_attention_rows,
-    fp8_decode_attention,
-    fp8_decode_plan,
 )
 
 if TYPE_CHECKING:
@@ -52,11 +52,11 @@ class DenseBackend(AttentionBackend):
                 and pool.head_dim == 128 and heads % 4 == 0 and heads // 4 <= 16)
 
     def init_forward_metadata(self, batch: ForwardBatch) -> None:
-        """Over an 8-bit pool: the step's division of the decode batch, for all of its layers.  It stays
+        """Over an 8- or 4-bit pool: the step's division of the decode batch, for all of its layers.  It stays
         with the batch, whose requests and lengths it is of."""
-        if self.fp8 and batch.forward_mode.is_decode():
-            batch.decode_plan = fp8_decode_plan(self.token_to_kv_pool, self.req_to_token_pool.block_table,
-                                                batch.req_pool_indices, batch.seq_lens)
+        if self.coded and batch.forward_mode.is_decode():
+            batch.decode_plan = coded_decode_plan(self.token_to_kv_pool, self.req_to_token_pool.block_table,
+                                                  batch.req_pool_indices, batch.seq_lens)
 
     def forward_decode(self, q, k, v, layer, batch: ForwardBatch) -> torch.Tensor:
         """dense.py:26-42: set_kv_buffer, then attention over req_to_token[req, :seq_len]."""
@@ -64,14 +64,14 @@ class DenseBackend(AttentionBackend):
         pool = self.token_to_kv_pool
         bs = batch.batch_size
         dim = pool.head_dim
-        if self.fp8:
+        if self.coded:
             q3 = q.reshape(bs, math.prod(q.shape[1:]) // dim, dim)
             plan = getattr(batch, "decode_plan", None)
             if plan is not None and plan.bs != bs:  # a part of the batch that was divided
                 plan = None
-            return fp8_decode_attention(q3, pool, layer.layer_id, self.req_to_token_pool.block_table,
-                                        batch.req_pool_indices, batch.seq_lens, layer.scaling,
-                                        new=(batch.out_cache_loc, k, v), plan=plan)
+            return coded_decode_attention(q3, pool, layer.layer_id, self.req_to_token_pool.block_table,
+                                          batch.req_pool_indices, batch.seq_lens, layer.scaling,
+                                          new=(batch.out_cache_loc, k, v), plan=plan)
         q3 = q.reshape(bs, -1, dim)
         heads = q3.shape[1]
         rpi = batch.req_pool_indices.to(device=q3.device, dtype=torch.int64).contiguous()

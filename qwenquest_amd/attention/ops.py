@@ -1,7 +1,8 @@
 """Attention math (reference ``src/qwenquest/attention/ops.py``).
 
 ``decode_attention`` runs the HIP split-K kernel over an explicit row list;
-``fp8_decode_attention`` and ``fp8_extend_attention`` run the HIP kernels over an 8-bit block cache;
+``fp8_decode_attention`` and ``fp8_extend_attention`` run the HIP kernels over an 8-bit block cache,
+``fp4_decode_attention`` and ``fp4_extend_attention`` over a 4-bit one (``coded_*`` over either);
 ``extend_attention_batch`` runs a whole prefill batch (bf16, head_dim 128) in the HIP
 prefill kernel; ``extend_attention``, one request of any shape, uses torch's SDPA on the
 device, in float32.
@@ -18,11 +19,13 @@ from qwenquest_amd import _lib
 from qwenquest_amd.batch import DecodePlan
 
 if TYPE_CHECKING:
-    from qwenquest_amd.paged import Fp8TokenToKVPool
+    from qwenquest_amd.paged import CodedTokenToKVPool, Fp4TokenToKVPool, Fp8TokenToKVPool
     from qwenquest_amd.quest import QuestAlgorithm
 
-__all__ = ["decode_attention", "extend_attention", "extend_attention_batch", "fp8_decode_attention",
-           "fp8_extend_attention", "fp8_quest_step", "AttentionWorkspace"]
+__all__ = ["decode_attention", "extend_attention", "extend_attention_batch", "coded_decode_attention", "coded_decode_plan",
+           "coded_extend_attention", "coded_quest_step", "fp4_decode_attention", "fp4_decode_plan", "fp4_extend_attention",
+           "fp4_quest_step", "fp8_decode_attention", "fp8_decode_plan", "fp8_extend_attention", "fp8_quest_step",
+           "AttentionWorkspace"]
 
 
 class AttentionWorkspace:
@@ -214,7 +217,7 @@ def _lengths(t: torch.Tensor, n: int, device: torch.device, what: str) -> torch.
     return t.to(device=device, dtype=torch.int64).contiguous()
 
 
-def _queries(q: torch.Tensor, pool: Fp8TokenToKVPool) -> torch.Tensor:
+def _queries(q: torch.Tensor, pool: CodedTokenToKVPool) -> torch.Tensor:
     """``q [n, H, D]`` (or ``[n, H*D]``) dense and 16-byte aligned."""
     dim = pool.head_dim
     if q.device != pool.device:
@@ -231,27 +234,37 @@ def _queries(q: torch.Tensor, pool: Fp8TokenToKVPool) -> torch.Tensor:
     return q.clone() if q.data_ptr() % 16 else q
 
 
-def fp8_decode_plan(pool: Fp8TokenToKVPool, block_table: torch.Tensor, req_pool_indices: torch.Tensor,
-                    seq_lens: torch.Tensor) -> DecodePlan:
-    """What ``fp8_decode_attention`` over whole contexts makes of a step's lengths, once for the step's
+def _entry(pool: CodedTokenToKVPool, name: str):
+    return getattr(_lib.load(), f"qq_{pool.kind}_{name}")
+
+
+def _of_kind(pool: CodedTokenToKVPool, kind: str) -> CodedTokenToKVPool:
+    if pool.kind != kind:
+        raise ValueError(f"expected an {kind.capitalize()}TokenToKVPool, got an {type(pool).__name__}")
+    return pool
+
+
+def coded_decode_plan(pool: CodedTokenToKVPool, block_table: torch.Tensor, req_pool_indices: torch.Tensor,
+                      seq_lens: torch.Tensor) -> DecodePlan:
+    """What ``coded_decode_attention`` over whole contexts makes of a step's lengths, once for the step's
     layers, on the current stream."""
     dev = pool.device
     bs = int(req_pool_indices.shape[0])
     table = _lib.table_args(block_table, dev)
     rpi = _lengths(req_pool_indices, bs, dev, "req_pool_indices")
     seq = _lengths(seq_lens, bs, dev, "seq_lens")
-    need = int(_lib.load().qq_fp8_decode_workspace_bytes(bs, pool.kv_heads, pool.kv_heads, pool.head_dim))
+    need = int(_entry(pool, "decode_workspace_bytes")(bs, pool.kv_heads, pool.kv_heads, pool.head_dim))
     ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
     stream = _lib.stream(dev)
     with _lib.on(dev):
-        _lib.call("qq_fp8_decode_plan", pool.num_blocks, pool.kv_heads, pool.head_dim, table[2], table[3],
+        _lib.call(f"qq_{pool.kind}_decode_plan", pool.num_blocks, pool.kv_heads, pool.head_dim, table[2], table[3],
                   _lib.ptr(rpi), _lib.ptr(seq), bs, _lib.ptr(ws), need, stream)
     return DecodePlan(bs, ws, stream, _lib.capture_id(dev, stream))
 
 
-def fp8_decode_attention(
+def coded_decode_attention(
     q: torch.Tensor,
-    pool: Fp8TokenToKVPool,
+    pool: CodedTokenToKVPool,
     layer_id: int,
     block_table: torch.Tensor,
     req_pool_indices: torch.Tensor,
@@ -263,11 +276,11 @@ def fp8_decode_attention(
     new: tuple[torch.Tensor, torch.Tensor, torch.Tensor] | None = None,
     plan: DecodePlan | None = None,
 ) -> torch.Tensor:
-    """Decode over an 8-bit pool: request ``i`` attends ``q[i] [H, D]`` over its first ``seq_lens[i]``
+    """Decode over an 8- or 4-bit pool: request ``i`` attends ``q[i] [H, D]`` over its first ``seq_lens[i]``
     tokens in the blocks ``block_table[req_pool_indices[i]]``, or, with ``positions [bs, >= top_k]``
     (``QuestAlgorithm.retrieve_topk``) and a longer context than ``top_k``, over the pages listed
     there and the last 64 tokens.  ``new``: ``(loc, k, v)`` of the batch's new tokens, stored first.
-    ``plan``: this step's ``fp8_decode_plan`` (of the same pool, table, requests and lengths, on the
+    ``plan``: this step's ``coded_decode_plan`` (of the same pool, table, requests and lengths, on the
     same stream; not with ``positions``): up to 16 query heads per KV head then run as one launch,
     for which each new token lies in the last block of its own request's context and no two in one
     block (rows of block 0, the padding, aside); on another stream, or where the two calls are not in
@@ -291,19 +304,19 @@ def fp8_decode_attention(
     out = torch.empty((bs, heads * dim), dtype=q.dtype, device=dev)
     if plan is not None and positions is not None:
         raise ValueError("a plan is of whole contexts, not of selected pages")
-    need = int(_lib.load().qq_fp8_decode_workspace_bytes(bs, heads, pool.kv_heads, dim))
+    need = int(_entry(pool, "decode_workspace_bytes")(bs, heads, pool.kv_heads, dim))
     stream = _lib.stream(dev)
     if plan is not None and heads <= 16 * pool.kv_heads and plan.usable(stream):
         ws = plan.workspace
         if plan.bs != bs or plan.top_k != 0 or ws.device != dev or ws.numel() != max(need, 1):
-            raise ValueError("plan is not fp8_decode_plan's of this batch and pool")
+            raise ValueError("plan is not coded_decode_plan's of this batch and pool")
     else:
         # of this call alone: it holds the division of the batch, which a graph's replay or a call on
         # another stream must not find replaced
         ws, plan = torch.empty(max(need, 1), dtype=torch.uint8, device=dev), None
     with _lib.on(dev):
         _lib.call(
-            "qq_fp8_decode_attention", _lib.ptr(q), _lib.dtype_code(q.dtype), q.stride(0), heads, _lib.ptr(kn),
+            f"qq_{pool.kind}_decode_attention", _lib.ptr(q), _lib.dtype_code(q.dtype), q.stride(0), heads, _lib.ptr(kn),
             _lib.ptr(vn), _lib.DTYPE_BF16 if kn is None else _lib.dtype_code(kn.dtype), _lib.ptr(loc),
             *pool.layer_args(layer_id), *table, _lib.ptr(rpi), _lib.ptr(seq), bs, _lib.ptr(positions),
             0 if positions is None else max(positions.stride(0), positions.shape[1]), int(top_k), float(scaling),
@@ -312,12 +325,12 @@ def fp8_decode_attention(
     return out
 
 
-def fp8_quest_step(
+def coded_quest_step(
     q: torch.Tensor,
     k: torch.Tensor,
     v: torch.Tensor,
     loc: torch.Tensor,
-    pool: Fp8TokenToKVPool,
+    pool: CodedTokenToKVPool,
     layer_id: int,
     block_table: torch.Tensor,
     quest: QuestAlgorithm,
@@ -326,7 +339,7 @@ def fp8_quest_step(
     scaling: float,
     phase: int = 3,
 ) -> torch.Tensor:
-    """One layer of Quest decode over an 8-bit pool, after ``quest.decode_step_blocks``: the new tokens
+    """One layer of Quest decode over an 8- or 4-bit pool, after ``quest.decode_step_blocks``: the new tokens
     ``k``/``v`` go to rows ``loc``, the page scores select (``positions [>= bs, top_k]`` int32 is
     written, as ``QuestAlgorithm.retrieve_topk`` writes it), and ``q [bs, H, D]`` attends the selected
     pages.  On the stream of ``decode_step_blocks``, both in the same graph capture or in none, the
@@ -355,7 +368,7 @@ def fp8_quest_step(
     loc = _lengths(loc, bs, dev, "out_cache_loc")
     kn, vn = pool.new_rows(k, v, bs)
     out = torch.empty((bs, heads * dim), dtype=q.dtype, device=dev)
-    need = int(_lib.load().qq_fp8_decode_workspace_bytes(bs, heads, pool.kv_heads, dim))
+    need = int(_entry(pool, "decode_workspace_bytes")(bs, heads, pool.kv_heads, dim))
     stream = _lib.stream(dev)
     planned = step.plan is not None and heads <= 16 * pool.kv_heads and step.plan.usable(stream)
     ws = step.plan.workspace if planned else torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
@@ -363,7 +376,7 @@ def fp8_quest_step(
         raise ValueError("the step's plan is not decode_step_blocks' of this batch and pool")
     with _lib.on(dev):
         _lib.call(
-            "qq_fp8_quest_step", _lib.ptr(q), _lib.dtype_code(q.dtype), q.stride(0), heads, _lib.ptr(kn), _lib.ptr(vn),
+            f"qq_{pool.kind}_quest_step", _lib.ptr(q), _lib.dtype_code(q.dtype), q.stride(0), heads, _lib.ptr(kn), _lib.ptr(vn),
             _lib.dtype_code(kn.dtype), _lib.ptr(loc), *pool.layer_args(layer_id), *table,
             _lib.ptr(quest.page_k_bounds), layer_id - quest.start_layer, _lib.ptr(rpi), _lib.ptr(step.seq_lens),
             _lib.ptr(step.candidate_limit_i32), bs, quest.max_reqs, quest.max_pages_per_req, quest.top_k, float(scaling),
@@ -373,9 +386,9 @@ def fp8_quest_step(
     return out
 
 
-def fp8_extend_attention(
+def coded_extend_attention(
     q: torch.Tensor,
-    pool: Fp8TokenToKVPool,
+    pool: CodedTokenToKVPool,
     layer_id: int,
     block_table: torch.Tensor,
     req_pool_indices: torch.Tensor,
@@ -384,7 +397,7 @@ def fp8_extend_attention(
     extend_lens: torch.Tensor,
     scaling: float,
 ) -> torch.Tensor:
-    """Causal prefill of a batch over an 8-bit pool that holds the new K/V: ``q [n, H, D]`` (bf16)
+    """Causal prefill of a batch over an 8- or 4-bit pool that holds the new K/V: ``q [n, H, D]`` (bf16)
     holds the requests' new tokens one request after the other; token ``t`` of request ``i`` attends
     positions ``0 .. prefix_lens[i] + t``.  Returns ``[n, H*D]``; the lengths are read on the device
     only.  NaN: a request outside the table, a query tile that attends a block which is not there,
@@ -401,13 +414,133 @@ def fp8_extend_attention(
         (extend_lens, "extend_lens")))
     if bs == 0 and n:
         raise ValueError(f"{n} tokens of no request")
-    need = int(_lib.load().qq_fp8_extend_workspace_bytes(n, bs, heads, pool.kv_heads, dim, table[3]))
+    need = int(_entry(pool, "extend_workspace_bytes")(n, bs, heads, pool.kv_heads, dim, table[3]))
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     out = torch.empty((n, heads * dim), dtype=q.dtype, device=dev)
     with _lib.on(dev):
         _lib.call(
-            "qq_fp8_extend_attention", _lib.ptr(q), heads, *pool.layer_args(layer_id), *table, _lib.ptr(rpi),
+            f"qq_{pool.kind}_extend_attention", _lib.ptr(q), heads, *pool.layer_args(layer_id), *table, _lib.ptr(rpi),
             _lib.ptr(seq), _lib.ptr(prefix), _lib.ptr(ext), bs, n, float(scaling), _lib.ptr(out), _lib.ptr(ws), need,
             _lib.stream(dev),
         )
     return out
+
+
+def fp8_decode_plan(pool: Fp8TokenToKVPool, block_table: torch.Tensor, req_pool_indices: torch.Tensor,
+                    seq_lens: torch.Tensor) -> DecodePlan:
+    """``coded_decode_plan`` of an 8-bit pool."""
+    return coded_decode_plan(_of_kind(pool, "fp8"), block_table, req_pool_indices, seq_lens)
+
+
+def fp8_decode_attention(
+    q: torch.Tensor,
+    pool: Fp8TokenToKVPool,
+    layer_id: int,
+    block_table: torch.Tensor,
+    req_pool_indices: torch.Tensor,
+    seq_lens: torch.Tensor,
+    scaling: float,
+    *,
+    positions: torch.Tensor | None = None,
+    top_k: int = 0,
+    new: tuple[torch.Tensor, torch.Tensor, torch.Tensor] | None = None,
+    plan: DecodePlan | None = None,
+) -> torch.Tensor:
+    """``coded_decode_attention`` over an 8-bit pool."""
+    return coded_decode_attention(q, _of_kind(pool, "fp8"), layer_id, block_table, req_pool_indices, seq_lens, scaling,
+                                  positions=positions, top_k=top_k, new=new, plan=plan)
+
+
+def fp8_quest_step(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    loc: torch.Tensor,
+    pool: Fp8TokenToKVPool,
+    layer_id: int,
+    block_table: torch.Tensor,
+    quest: QuestAlgorithm,
+    req_pool_indices: torch.Tensor,
+    positions: torch.Tensor,
+    scaling: float,
+    phase: int = 3,
+) -> torch.Tensor:
+    """``coded_quest_step`` over an 8-bit pool."""
+    return coded_quest_step(q, k, v, loc, _of_kind(pool, "fp8"), layer_id, block_table, quest, req_pool_indices, positions,
+                            scaling, phase)
+
+
+def fp8_extend_attention(
+    q: torch.Tensor,
+    pool: Fp8TokenToKVPool,
+    layer_id: int,
+    block_table: torch.Tensor,
+    req_pool_indices: torch.Tensor,
+    seq_lens: torch.Tensor,
+    prefix_lens: torch.Tensor,
+    extend_lens: torch.Tensor,
+    scaling: float,
+) -> torch.Tensor:
+    """``coded_extend_attention`` over an 8-bit pool."""
+    return coded_extend_attention(q, _of_kind(pool, "fp8"), layer_id, block_table, req_pool_indices, seq_lens, prefix_lens,
+                                  extend_lens, scaling)
+
+
+def fp4_decode_plan(pool: Fp4TokenToKVPool, block_table: torch.Tensor, req_pool_indices: torch.Tensor,
+                    seq_lens: torch.Tensor) -> DecodePlan:
+    """``coded_decode_plan`` of a 4-bit pool."""
+    return coded_decode_plan(_of_kind(pool, "fp4"), block_table, req_pool_indices, seq_lens)
+
+
+def fp4_decode_attention(
+    q: torch.Tensor,
+    pool: Fp4TokenToKVPool,
+    layer_id: int,
+    block_table: torch.Tensor,
+    req_pool_indices: torch.Tensor,
+    seq_lens: torch.Tensor,
+    scaling: float,
+    *,
+    positions: torch.Tensor | None = None,
+    top_k: int = 0,
+    new: tuple[torch.Tensor, torch.Tensor, torch.Tensor] | None = None,
+    plan: DecodePlan | None = None,
+) -> torch.Tensor:
+    """``coded_decode_attention`` over a 4-bit pool."""
+    return coded_decode_attention(q, _of_kind(pool, "fp4"), layer_id, block_table, req_pool_indices, seq_lens, scaling,
+                                  positions=positions, top_k=top_k, new=new, plan=plan)
+
+
+def fp4_quest_step(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    loc: torch.Tensor,
+    pool: Fp4TokenToKVPool,
+    layer_id: int,
+    block_table: torch.Tensor,
+    quest: QuestAlgorithm,
+    req_pool_indices: torch.Tensor,
+    positions: torch.Tensor,
+    scaling: float,
+    phase: int = 3,
+) -> torch.Tensor:
+    """``coded_quest_step`` over a 4-bit pool."""
+    return coded_quest_step(q, k, v, loc, _of_kind(pool, "fp4"), layer_id, block_table, quest, req_pool_indices, positions,
+                            scaling, phase)
+
+
+def fp4_extend_attention(
+    q: torch.Tensor,
+    pool: Fp4TokenToKVPool,
+    layer_id: int,
+    block_table: torch.Tensor,
+    req_pool_indices: torch.Tensor,
+    seq_lens: torch.Tensor,
+    prefix_lens: torch.Tensor,
+    extend_lens: torch.Tensor,
+    scaling: float,
+) -> torch.Tensor:
+    """``coded_extend_attention`` over a 4-bit pool."""
+    return coded_extend_attention(q, _of_kind(pool, "fp4"), layer_id, block_table, req_pool_indices, seq_lens, prefix_lens,
+                                  extend_lens, scaling)

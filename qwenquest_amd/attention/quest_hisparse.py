@@ -50,7 +50,7 @@ class QuestHiSparseBackend(AttentionBackend):
         async_admission: bool = False,
     ):
         super().__init__(req_to_token_pool, token_to_kv_pool)
-        if self.fp8:
+        if self.coded:
             raise ValueError("QuestHiSparseBackend keeps rows, not blocks: it takes an MHATokenToKVPool")
         cfg = parse_hisparse_config(sparse_config)
         if cfg.algorithm != "quest" or cfg.quest_page_size is None:

@@ -10,7 +10,7 @@ Per decode step::
     forward_decode (x L):   save new K/V -> [Q6] retrieve_topk (score + select + layout)
                             -> [Q7] req_to_token gather + split-K attention
 
-Over an 8-bit pool (``Fp8TokenToKVPool``) pages are the pool's blocks: a page's bounds are taken
+Over an 8- or 4-bit pool (``Fp8TokenToKVPool``, ``Fp4TokenToKVPool``) pages are the pool's blocks: a page's bounds are taken
 from its codes when its last token is in (no running bounds), and the attention takes the
 selected pages by block.
 """
@@ -24,7 +24,7 @@ import torch
 
 from qwenquest_amd import _lib
 from qwenquest_amd.attention.base import AttentionBackend
-from qwenquest_amd.attention.ops import AttentionWorkspace, fp8_quest_step
+from qwenquest_amd.attention.ops import AttentionWorkspace, coded_quest_step
 from qwenquest_amd.config import SparseConfig, parse_hisparse_config
 from qwenquest_amd.paged import BLOCK_TOKENS
 from qwenquest_amd.quest import QuestAlgorithm
@@ -52,8 +52,8 @@ class QuestOnlyBackend(AttentionBackend):
         cfg = parse_hisparse_config(sparse_config)
         if cfg.algorithm != "quest" or cfg.quest_page_size is None:
             raise ValueError("Quest backends require hisparse_config with algorithm='quest'")
-        if self.fp8 and cfg.quest_page_size != BLOCK_TOKENS:
-            raise ValueError(f"an Fp8TokenToKVPool's pages are its blocks of {BLOCK_TOKENS} tokens: "
+        if self.coded and cfg.quest_page_size != BLOCK_TOKENS:
+            raise ValueError(f"an {type(token_to_kv_pool).__name__}'s pages are its blocks of {BLOCK_TOKENS} tokens: "
                              f"quest_page_size must be {BLOCK_TOKENS}, got {cfg.quest_page_size}")
         self.sparse_config = cfg
         device = token_to_kv_pool.device
@@ -90,7 +90,7 @@ class QuestOnlyBackend(AttentionBackend):
             bs = int(batch.req_pool_indices.numel())
             if bs > self._step_locs.numel():
                 raise ValueError(f"batch {bs} exceeds the request pool ({self._step_locs.numel()})")
-            if self.fp8:
+            if self.coded:
                 self.quest.decode_step_blocks(batch.req_pool_indices, batch.seq_lens, self.token_to_kv_pool,
                                               self.req_to_token_pool.block_table)
                 return
@@ -128,7 +128,7 @@ class QuestOnlyBackend(AttentionBackend):
 
     def _update_quest_for_extend(self, batch: ForwardBatch) -> None:
         """[Q2] Per request: bounds of positions ``0 .. seq_len-1`` at every layer (quest_only.py:115-128)."""
-        if self.fp8:  # from page 0 in every chunk: a prefix may be in the pool without this backend's prefill
+        if self.coded:  # from page 0 in every chunk: a prefix may be in the pool without this backend's prefill
             self.quest.update_prefill_representations_blocks(batch.req_pool_indices, batch.seq_lens,
                                                              self.token_to_kv_pool, self.req_to_token_pool.block_table)
             return
@@ -158,8 +158,8 @@ class QuestOnlyBackend(AttentionBackend):
         heads, dim = q3.shape[1], pool.head_dim
         if step.seq_lens.shape[0] != bs:
             raise ValueError("batch size differs from the one given to prepare_step()")
-        if self.fp8:
-            return self._forward_decode_fp8(q3, k, v, layer, batch, phase)
+        if self.coded:
+            return self._forward_decode_coded(q3, k, v, layer, batch, phase)
         kn = k.reshape(bs, pool.kv_heads * dim)
         vn = v.reshape(bs, pool.kv_heads * dim)
         if kn.dtype != vn.dtype or kn.dtype not in (torch.bfloat16, torch.float32):
@@ -191,12 +191,12 @@ class QuestOnlyBackend(AttentionBackend):
             quest._record(layer.layer_id, rpi, step, self._positions[:bs])
         return out
 
-    def _forward_decode_fp8(self, q3, k, v, layer, batch: ForwardBatch, phase: int) -> torch.Tensor:
-        """forward_decode_phase over an 8-bit pool in one C call: 1 = scoring and selection, 2 = new-token
+    def _forward_decode_coded(self, q3, k, v, layer, batch: ForwardBatch, phase: int) -> torch.Tensor:
+        """forward_decode_phase over an 8- or 4-bit pool in one C call: 1 = scoring and selection, 2 = new-token
         store and attention."""
         quest, rpi = self.quest, batch.req_pool_indices
-        out = fp8_quest_step(q3, k, v, batch.out_cache_loc, self.token_to_kv_pool, layer.layer_id,
-                             self.req_to_token_pool.block_table, quest, rpi, self._positions, layer.scaling, phase)
+        out = coded_quest_step(q3, k, v, batch.out_cache_loc, self.token_to_kv_pool, layer.layer_id,
+                               self.req_to_token_pool.block_table, quest, rpi, self._positions, layer.scaling, phase)
         if quest.trace is not None and phase & 1:
             quest._record(layer.layer_id, rpi, quest._step, self._positions[: batch.batch_size])
         return out
@@ -205,8 +205,9 @@ class QuestOnlyBackend(AttentionBackend):
         """[Q7] rows = req_to_token[req, positions[:n]] -> attention over exactly those rows."""
         heads = q.shape[1] if q.dim() == 3 else q.shape[1] // self.token_to_kv_pool.head_dim
         dim = self.token_to_kv_pool.head_dim
-        if self.fp8:
-            raise ValueError("an Fp8TokenToKVPool is attended by block: fp8_decode_attention takes the positions")
+        if self.coded:
+            pool = self.token_to_kv_pool
+            raise ValueError(f"an {type(pool).__name__} is attended by block: {pool.kind}_decode_attention takes the positions")
         q3 = q.reshape(bs, heads, dim).contiguous()
         k_buf, v_buf = self.token_to_kv_pool.get_kv_buffer(layer.layer_id)
         rpi = req_pool_indices

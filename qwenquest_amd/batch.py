@@ -28,7 +28,7 @@ class ForwardMode(enum.Enum):
 
 
 class DecodePlan(NamedTuple):
-    """A decode batch of ``bs`` requests over an 8-bit pool, divided for the chip once for a step's
+    """A decode batch of ``bs`` requests over an 8- or 4-bit pool, divided for the chip once for a step's
     layers.  It holds for the stream that made it, and inside a graph capture for what that same
     capture records: elsewhere its memory may not be written yet, or no longer be its own."""
 

@@ -1,0 +1,268 @@
+// The 4-bit K/V cache's writes and reads (layout: qq_fp4.h): the form of
+// MHATokenToKVPool.set_kv_buffer (reference src/qwenquest/memory.py:114-120) for blocks of e2m1
+// codes with scales of their own for every token, the rows back as values, and the page bounds of
+// QuestAlgorithm (src/qwenquest/quest.py:231-321) from the codes.
+#include "qq_fp4_store.h"
+#include "qq_fp8_plan.h"
+#include "qq_quest_dev.h"
+
+namespace qq {
+namespace {
+
+template <int D, typename SRC>
+__global__ __launch_bounds__(256) void fp4_store_kernel(Fp4StoreArgs a) {
+  const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / (D / 4);
+  const int64_t i = item / a.c.KV;
+  fp4_store_group<D, SRC>(a, i, i < a.n, (int)(item - i * a.c.KV));
+}
+
+__device__ inline void fp4_write8(uint16_t* out, uint32_t w, float s) {
+  u32x4_t y;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = s != s ? 0x7FC07FC0u : __builtin_bit_cast(uint32_t, fp4_pair(w, s, i));
+  *reinterpret_cast<u32x4_t*>(out) = y;
+}
+__device__ inline void fp4_write8(float* out, uint32_t w, float s) {
+  float y[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t p = __builtin_bit_cast(uint32_t, fp4_pair(w, s, i));
+    y[2 * i] = s != s ? s : __uint_as_float(p << 16);
+    y[2 * i + 1] = s != s ? s : __uint_as_float(p & 0xFFFF0000u);
+  }
+  *reinterpret_cast<float4*>(out) = make_float4(y[0], y[1], y[2], y[3]);
+  *reinterpret_cast<float4*>(out + 4) = make_float4(y[4], y[5], y[6], y[7]);
+}
+
+// Values of listed rows: a thread 8 channels of K and of V of one row and head.
+template <int D, typename DST>
+__global__ __launch_bounds__(256) void fp4_rows_kernel(Fp4Cache c, const int64_t* loc, int64_t n, DST* k, DST* v) {
+  constexpr int DG = D / 8;
+  const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / DG;
+  const int dg = threadIdx.x % DG;
+  const int64_t i = item / c.KV;
+  if (i >= n) return;
+  const int h = (int)(item - i * c.KV);
+  const int64_t row = loc[i];
+  const bool in = row >= 0 && (row >> 6) < c.blocks;
+  const int64_t at = (in ? row >> 6 : 0) * c.KV + h;
+  const int t = (int)(row & 63);
+  auto factor = [&](uint32_t e) { return in && e != kFp4Lost ? __uint_as_float(e << 23) : __builtin_nanf(""); };
+  const float ks = factor(c.ks[at * (2 * D) + fp4_ks_offset(t, dg * 8)]), vs = factor(c.vs[at * 64 + fp4_vs_offset(t)]);
+  fp4_write8(k + item * D + dg * 8, *reinterpret_cast<const uint32_t*>(c.kc + at * (32 * D) + fp4_k_offset(D, t, dg * 8)), ks);
+  uint32_t w = 0;
+  const uint8_t* codes = c.vc + at * (32 * D) + fp4_v_offset(t, dg * 8);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) w |= ((codes[j * 16] >> (dg & 4 ? 4 : 0)) & 15u) << (4 * j);
+  fp4_write8(v + item * D + dg * 8, w, vs);
+}
+
+struct Fp4PageArgs {
+  const uint8_t* kc;  // first layer
+  const uint8_t* ks;
+  int64_t kc_stride, ks_stride;  // of a layer, bytes
+  int blocks, KV;
+  const int32_t* table;
+  int64_t table_stride;
+  int table_rows, table_cols;
+  const int64_t* rpi;
+  const int64_t* seq;
+  const int64_t* prefix;  // nullptr: from page 0 (prefill)
+  int decode;
+  uint32_t* bounds;  // [layers, R, MP, KV * D] (min, max) words
+  int R, MP;
+  int top_k, avoid;
+  int32_t* actual;  // nullptr, or the step's layout: actual_lens, candidate_limit
+  int32_t* limit;
+  int layers;
+  PlanArgs plan;  // cu nullptr, or the step's division of the attention's work, by a block past the layers
+};
+
+// Min and max of a page's keys per channel, a wave per (page, head, layer): lane m + 16 g has 8
+// channels (those of byte 4 (g % 4) of each 16 bytes) of the tokens 16 T + m for every group of 32.
+template <int D>
+__global__ __launch_bounds__(256) void fp4_page_bounds_kernel(Fp4PageArgs a) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int b = blockIdx.y, layer = blockIdx.z;
+  if (layer == a.layers) {
+    if (b == 0 && blockIdx.x == 0) plan_slices(a.plan);
+    return;
+  }
+  const int64_t req = a.rpi[b], seq = a.seq[b], s = max(seq, (int64_t)0);
+  if (a.actual && layer == 0 && blockIdx.x == 0 && threadIdx.x == 0) {
+    a.actual[b] = (int32_t)min(seq, (int64_t)a.top_k);  // quest.py:343-352
+    // the page that the step's own token completes has no bounds yet, whatever lies in its place
+    a.limit[b] = (int32_t)(a.avoid ? max(seq / 64 - 1, (int64_t)0) : max(seq - 1, (int64_t)0) / 64);
+  }
+  if (req < 0 || req >= a.R || req >= a.table_rows) return;
+  int64_t lo, hi;  // pages
+  if (a.decode) {  // the page that the token before the newest completes
+    hi = s >= 2 && (s - 1) % 64 == 0 ? (s - 1) / 64 : 0;
+    lo = max(hi - 1, (int64_t)0);
+  } else {
+    hi = s / 64;
+    lo = a.prefix ? max(a.prefix[b], (int64_t)0) / 64 : 0;
+  }
+  hi = min(hi, (int64_t)min(a.MP, a.table_cols));
+  const int64_t units = (hi - lo) * a.KV;
+  const int m = lane & 15, g = lane >> 4;
+  for (int64_t u = blockIdx.x * 4 + wave; u < units; u += gridDim.x * 4) {
+    const int64_t page = lo + u / a.KV;
+    const int h = (int)(u % a.KV);
+    const int32_t blk = a.table[req * a.table_stride + page];
+    const bool in = blk >= 0 && blk < a.blocks;
+    const int64_t at = (int64_t)(in ? blk : 0) * a.KV + h;
+    const uint8_t* kp = a.kc + layer * a.kc_stride + at * (32 * D) + m * 16 + g * 4;
+    const uint8_t* sp = a.ks + layer * a.ks_stride + at * (2 * D) + m * 4;
+    uint32_t w[4][D / 32], e[D / 32];
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) {
+      e[c] = *reinterpret_cast<const uint32_t*>(sp + c * 64);
+#pragma unroll
+      for (int T = 0; T < 4; ++T) w[T][c] = *reinterpret_cast<const uint32_t*>(kp + (T * (D / 32) + c) * 256);
+    }
+    uint32_t* out = a.bounds + (((int64_t)layer * a.R + req) * a.MP + page) * (a.KV * D) + h * D;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) {
+      float mn[8], mx[8];
+      bool lost = !in;
+#pragma unroll
+      for (int T = 0; T < 4; ++T) {
+        lost |= ((e[c] >> (8 * T)) & 255u) == kFp4Lost;
+        const float f = fp4_factor(e[c], T);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t p = __builtin_bit_cast(uint32_t, fp4_pair(w[T][c], f, i));
+          const float x = __uint_as_float(p << 16), y = __uint_as_float(p & 0xFFFF0000u);
+          mn[2 * i] = T ? fminf(mn[2 * i], x) : x;
+          mx[2 * i] = T ? fmaxf(mx[2 * i], x) : x;
+          mn[2 * i + 1] = T ? fminf(mn[2 * i + 1], y) : y;
+          mx[2 * i + 1] = T ? fmaxf(mx[2 * i + 1], y) : y;
+        }
+      }
+      // over the 16 tokens of a row of lanes, in halves, each lane keeping half of its channels
+#pragma unroll
+      for (int half = 4; half >= 1; half >>= 1) {  // partner lane ^ 2 * half
+        const bool up = lane & (2 * half);
+#pragma unroll
+        for (int j = 0; j < half; ++j) {
+          const float rn = __shfl_xor(up ? mn[j] : mn[j + half], 2 * half, 64), rx = __shfl_xor(up ? mx[j] : mx[j + half], 2 * half, 64);
+          mn[j] = fminf(up ? mn[j + half] : mn[j], rn);
+          mx[j] = fmaxf(up ? mx[j + half] : mx[j], rx);
+        }
+      }
+      const float n = fminf(mn[0], __shfl_xor(mn[0], 1, 64)), x = fmaxf(mx[0], __shfl_xor(mx[0], 1, 64));
+      lost = __any(lost);
+      // lane pair (m, m ^ 1) has channel 8 g + (m / 2 with its bits in the order of the halves)
+      const uint32_t word = lost ? 0x7FC07FC0u : (uint32_t)f2bf(n) | ((uint32_t)f2bf(x) << 16);
+      if ((lane & 1) == 0) out[c * 32 + g * 8 + (lane & 8 ? 4 : 0) + (lane & 4 ? 2 : 0) + (lane & 2 ? 1 : 0)] = word;
+    }
+  }
+}
+
+}  // namespace
+
+int check_cache(const Fp4Cache& c, const char* what) {
+  QQ_REQUIRE(c.kc && c.vc && c.ks && c.vs, "%s: null cache pointer", what);
+  QQ_REQUIRE(c.blocks > 0 && c.blocks <= kMaxPoolBlocks, "%s: %d blocks, at most %d", what, c.blocks, kMaxPoolBlocks);
+  QQ_REQUIRE(c.KV > 0 && c.KV <= 1024, "%s: %d KV heads", what, c.KV);
+  QQ_REQUIRE(fp8_dim_ok(c.D), "%s: head_dim %d is not 64 or 128", what, c.D);
+  return QQ_OK;
+}
+
+}  // namespace qq
+
+using namespace qq;
+
+extern "C" int qq_fp4_store(uint8_t* k_codes, uint8_t* v_codes, uint8_t* k_scale, uint8_t* v_scale, int num_blocks,
+                            int kv_heads, int head_dim, const void* k, const void* v, int src_dtype, const int64_t* loc,
+                            int64_t n, void* stream) {
+  const char* what = "qq_fp4_store";
+  const Fp4StoreArgs a{{k_codes, v_codes, k_scale, v_scale, num_blocks, kv_heads, head_dim}, k, v, src_dtype, loc, n, 1};
+  const int st = check_cache(a.c, what);
+  if (st != QQ_OK) return st;
+  QQ_REQUIRE(dtype_ok(src_dtype), "%s: bad dtype", what);
+  QQ_REQUIRE(n >= 0 && n < (int64_t)1 << 31, "%s: bad sizes", what);
+  if (n == 0) return QQ_OK;
+  QQ_REQUIRE(k && v && loc, "%s: null pointer", what);
+  QQ_REQUIRE(((uintptr_t)k | (uintptr_t)v) % 16 == 0, "%s: k and v must be 16-byte aligned", what);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int64_t grid = (n * kv_heads * (head_dim / 4) + 255) / 256;
+  QQ_REQUIRE(grid < (int64_t)1 << 31, "%s: bad sizes", what);
+  const bool bf = src_dtype == QQ_DTYPE_BF16;
+  if (head_dim == 128) {
+    if (bf) fp4_store_kernel<128, uint16_t><<<(unsigned)grid, 256, 0, s>>>(a);
+    else fp4_store_kernel<128, float><<<(unsigned)grid, 256, 0, s>>>(a);
+  } else {
+    if (bf) fp4_store_kernel<64, uint16_t><<<(unsigned)grid, 256, 0, s>>>(a);
+    else fp4_store_kernel<64, float><<<(unsigned)grid, 256, 0, s>>>(a);
+  }
+  return check_launch(what);
+}
+
+extern "C" int qq_fp4_rows(const uint8_t* k_codes, const uint8_t* v_codes, const uint8_t* k_scale, const uint8_t* v_scale,
+                           int num_blocks, int kv_heads, int head_dim, const int64_t* loc, int64_t n, void* k, void* v,
+                           int dst_dtype, void* stream) {
+  const char* what = "qq_fp4_rows";
+  const Fp4Cache c{const_cast<uint8_t*>(k_codes), const_cast<uint8_t*>(v_codes), const_cast<uint8_t*>(k_scale),
+                   const_cast<uint8_t*>(v_scale), num_blocks, kv_heads, head_dim};
+  const int st = check_cache(c, what);
+  if (st != QQ_OK) return st;
+  QQ_REQUIRE(dtype_ok(dst_dtype), "%s: bad dtype", what);
+  QQ_REQUIRE(n >= 0 && n < (int64_t)1 << 31, "%s: bad sizes", what);
+  if (n == 0) return QQ_OK;
+  QQ_REQUIRE(loc && k && v, "%s: null pointer", what);
+  const int64_t grid = (n * kv_heads * (head_dim / 8) + 255) / 256;
+  QQ_REQUIRE(grid < (int64_t)1 << 31, "%s: bad sizes", what);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  uint16_t *kb = static_cast<uint16_t*>(k), *vb = static_cast<uint16_t*>(v);
+  float *kf = static_cast<float*>(k), *vf = static_cast<float*>(v);
+  const bool bf = dst_dtype == QQ_DTYPE_BF16;
+  if (head_dim == 128) {
+    if (bf) fp4_rows_kernel<128><<<(unsigned)grid, 256, 0, s>>>(c, loc, n, kb, vb);
+    else fp4_rows_kernel<128><<<(unsigned)grid, 256, 0, s>>>(c, loc, n, kf, vf);
+  } else {
+    if (bf) fp4_rows_kernel<64><<<(unsigned)grid, 256, 0, s>>>(c, loc, n, kb, vb);
+    else fp4_rows_kernel<64><<<(unsigned)grid, 256, 0, s>>>(c, loc, n, kf, vf);
+  }
+  return check_launch(what);
+}
+
+extern "C" int qq_fp4_page_bounds(const uint8_t* k_codes, int64_t codes_layer_stride, const uint8_t* k_scale,
+                                  int64_t scale_layer_stride, int num_blocks, int kv_heads, int head_dim,
+                                  const int32_t* block_table, int64_t block_table_stride, int block_table_rows,
+                                  int block_table_cols, const int64_t* req_pool_indices, const int64_t* seq_lens,
+                                  const int64_t* prefix_lens, int bs, int decode, int64_t max_new, int n_layers,
+                                  uint16_t* page_k_bounds, int max_reqs, int max_pages, int top_k,
+                                  int avoid_recent_overlap, int32_t* actual_lens, int32_t* candidate_limit, void* plan,
+                                  int64_t plan_bytes, void* stream) {
+  const char* what = "qq_fp4_page_bounds";
+  uint8_t *codes = const_cast<uint8_t*>(k_codes), *scales = const_cast<uint8_t*>(k_scale);
+  const int st = check_cache(Fp4Cache{codes, codes, scales, scales, num_blocks, kv_heads, head_dim}, what);
+  if (st != QQ_OK) return st;
+  QQ_REQUIRE(bs >= 0 && bs < 65536 && n_layers > 0 && n_layers < 65535 && max_reqs > 0 && max_pages > 0 && max_new >= 0 &&
+                 block_table_cols > 0 && block_table_stride >= block_table_cols && block_table_rows > 0,
+             "%s: bad sizes", what);
+  QQ_REQUIRE(!actual_lens == !candidate_limit, "%s: one of the layout's outputs is missing", what);
+  if (bs == 0) return QQ_OK;
+  QQ_REQUIRE(block_table && req_pool_indices && seq_lens && page_k_bounds, "%s: null pointer", what);
+  Fp4PageArgs a{k_codes, k_scale, codes_layer_stride, scale_layer_stride, num_blocks, kv_heads, block_table, block_table_stride,
+                block_table_rows, block_table_cols, req_pool_indices, seq_lens, prefix_lens, decode,
+                reinterpret_cast<uint32_t*>(page_k_bounds), max_reqs, max_pages, top_k, avoid_recent_overlap, actual_lens,
+                candidate_limit, n_layers, {}};
+  if (plan) {
+    QQ_REQUIRE(decode && top_k > 0 && top_k % 64 == 0, "%s: a plan is of a decode step's selections of whole pages", what);
+    QQ_REQUIRE((int64_t)block_table_cols * bs < (int64_t)1 << 30, "%s: too many units of work", what);
+    const DecSpace sp = decode_space(bs, kv_heads, kv_heads, head_dim);
+    QQ_REQUIRE(plan_bytes >= sp.bytes, "%s: workspace %lld bytes < %lld needed", what, (long long)plan_bytes, (long long)sp.bytes);
+    set_plan(a.plan, sp, plan, req_pool_indices, seq_lens, bs, block_table_rows, block_table_cols, top_k, kv_heads);
+  }
+  // pages of a request, at most: those its new tokens can complete
+  const int64_t pages = decode ? 1 : min((int64_t)max_pages, max_new > 0 && prefix_lens ? max_new / 64 + 1 : (int64_t)max_pages);
+  const int64_t need = (pages * kv_heads + 3) / 4, fill = max((int64_t)1, (int64_t)16384 / ((int64_t)bs * n_layers));
+  const dim3 grid((unsigned)min(need, fill), bs, n_layers + (plan ? 1 : 0));
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (head_dim == 128) fp4_page_bounds_kernel<128><<<grid, 256, 0, s>>>(a);
+  else fp4_page_bounds_kernel<64><<<grid, 256, 0, s>>>(a);
+  return check_launch(what);
+}

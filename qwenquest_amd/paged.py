@@ -1,5 +1,5 @@
-"""Pools whose rows come in blocks of 64 tokens: request tables built on the GPU, and a K/V pool
-held in 8 bits.
+"""Pools whose rows come in blocks of 64 tokens: request tables built on the GPU, and K/V pools
+held in 8 or 4 bits.
 
 ``BlockReqToTokenPool`` is ``ReqToTokenPool`` with a device allocator: it hands out whole blocks
 from the requests' lengths and writes the block table, ``req_to_token`` and the slot map of a
@@ -15,7 +15,7 @@ from qwenquest_amd import _lib
 from qwenquest_amd.hisparse.coordinator import HiSparseCoordinator, pinned_zeros
 from qwenquest_amd.memory import ReqToTokenPool
 
-__all__ = ["BLOCK_TOKENS", "BlockReqToTokenPool", "Fp8TokenToKVPool"]
+__all__ = ["BLOCK_TOKENS", "BlockReqToTokenPool", "CodedTokenToKVPool", "Fp4TokenToKVPool", "Fp8TokenToKVPool"]
 
 BLOCK_TOKENS = 64
 
@@ -161,26 +161,19 @@ class BlockReqToTokenPool(ReqToTokenPool):
         self.check_errors(sync=False)
 
 
-class Fp8TokenToKVPool:
-    """A K/V pool in 8 bits: per layer ``num_blocks`` blocks of 64 tokens (block 0 is padding) of
-    e4m3 codes, with one power-of-two float scale for each block and KV head, K and V apart
-    (``k_scale``, ``v_scale`` ``[num_layers, num_blocks, kv_heads]``).  ``head_dim`` 64 or 128.
+class CodedTokenToKVPool:
+    """What the pools of coded blocks share: per layer ``num_blocks`` blocks of 64 tokens (block 0 is padding)
+    of codes (``k_codes``, ``v_codes [num_layers, num_blocks, kv_heads, ...]``, in the order that the attention
+    kernels take them) and scales (``k_scale``, ``v_scale``).  ``set_kv_buffer`` writes values and
+    ``get_rows`` reads them, by pool row.  ``head_dim`` 64 or 128."""
 
-    The codes (``k_codes``, ``v_codes``) lie in the order that the attention kernels take them;
-    ``set_kv_buffer`` writes values and ``get_rows`` reads them, by pool row.  Of a block's values
-    the scale is the least power of two (not under 2^-110) that keeps them within the codes' 448;
-    a later token with a larger value raises it, and the block's earlier codes are rounded again.
-    Writing a block's first row begins the block: what it held is gone.  Values that are not finite
-    make the scale of their (block, head) NaN until the block is begun again, and whoever attends
-    it gets NaN.
-    """
-
-    dtype = torch.float8_e4m3fn
+    #: the C entries' prefix
+    kind: str = ""
 
     def __init__(self, num_blocks: int, num_layers: int, kv_heads: int, head_dim: int, device: torch.device | str):
         self.device = _indexed(device)
         if self.device.type != "cuda":
-            raise RuntimeError("qwenquest_amd.Fp8TokenToKVPool needs a GPU device (no CPU path)")
+            raise RuntimeError(f"qwenquest_amd.{type(self).__name__} needs a GPU device (no CPU path)")
         if head_dim not in (64, 128):
             raise ValueError(f"head_dim must be 64 or 128, got {head_dim}")
         if not 1 <= num_blocks <= 1 << 24 or num_layers < 1 or not 1 <= kv_heads <= 1024:
@@ -191,24 +184,21 @@ class Fp8TokenToKVPool:
         self.kv_heads = kv_heads
         self.head_dim = head_dim
         self.size = num_blocks * BLOCK_TOKENS - 1
-        codes = (num_layers, num_blocks, kv_heads, BLOCK_TOKENS * head_dim)
-        self.k_codes = torch.zeros(codes, dtype=torch.uint8, device=self.device)
-        self.v_codes = torch.zeros(codes, dtype=torch.uint8, device=self.device)
-        self.k_scale = torch.full(codes[:3], 2.0**-110, dtype=torch.float32, device=self.device)
-        self.v_scale = torch.full(codes[:3], 2.0**-110, dtype=torch.float32, device=self.device)
+        self._allocate((num_layers, num_blocks, kv_heads))
         # one layer's codes and scales with the geometry, as the C entries take them; the tensors
         # stay where they are
-        code_step, scale_step = self.k_codes.stride(0), self.k_scale.stride(0) * 4
-        base = [_lib.ptr(t) for t in (self.k_codes, self.v_codes, self.k_scale, self.v_scale)]
-        self._layers = [(base[0] + i * code_step, base[1] + i * code_step, base[2] + i * scale_step,
-                         base[3] + i * scale_step, num_blocks, kv_heads, head_dim) for i in range(num_layers)]
+        steps = [(_lib.ptr(t), t.stride(0) * t.element_size()) for t in (self.k_codes, self.v_codes, self.k_scale, self.v_scale)]
+        self._layers = [(*(base + i * step for base, step in steps), num_blocks, kv_heads, head_dim) for i in range(num_layers)]
+
+    def _allocate(self, shape: tuple[int, int, int]) -> None:
+        raise NotImplementedError
 
     @property
     def rows(self) -> int:
         return self.num_blocks * BLOCK_TOKENS
 
     def storage_bytes(self) -> int:
-        return 2 * (self.k_codes.numel() + 4 * self.k_scale.numel())
+        return sum(t.numel() * t.element_size() for t in (self.k_codes, self.v_codes, self.k_scale, self.v_scale))
 
     def layer_args(self, layer_id: int) -> tuple:
         """One layer's codes and scales with the geometry, as the C entries take them."""
@@ -242,7 +232,7 @@ class Fp8TokenToKVPool:
             return
         k, v = self.new_rows(k, v, n)
         with _lib.on(self.device):
-            _lib.call("qq_fp8_store", *self.layer_args(layer_id), _lib.ptr(k), _lib.ptr(v), _lib.dtype_code(k.dtype),
+            _lib.call(f"qq_{self.kind}_store", *self.layer_args(layer_id), _lib.ptr(k), _lib.ptr(v), _lib.dtype_code(k.dtype),
                       _lib.ptr(loc), n, _lib.stream(self.device))
 
     def get_rows(self, layer_id: int, loc: torch.Tensor,
@@ -255,6 +245,58 @@ class Fp8TokenToKVPool:
         k, v = torch.empty((2, n, self.kv_heads, self.head_dim), dtype=dtype, device=self.device).unbind(0)
         if n:
             with _lib.on(self.device):
-                _lib.call("qq_fp8_rows", *self.layer_args(layer_id), _lib.ptr(loc), n, _lib.ptr(k), _lib.ptr(v), code,
+                _lib.call(f"qq_{self.kind}_rows", *self.layer_args(layer_id), _lib.ptr(loc), n, _lib.ptr(k), _lib.ptr(v), code,
                           _lib.stream(self.device))
         return k, v
+
+
+class Fp8TokenToKVPool(CodedTokenToKVPool):
+    """A K/V pool in 8 bits: per layer ``num_blocks`` blocks of 64 tokens (block 0 is padding) of
+    e4m3 codes, with one power-of-two float scale for each block and KV head, K and V apart
+    (``k_scale``, ``v_scale`` ``[num_layers, num_blocks, kv_heads]``).  ``head_dim`` 64 or 128.
+
+    The codes (``k_codes``, ``v_codes``) lie in the order that the attention kernels take them;
+    ``set_kv_buffer`` writes values and ``get_rows`` reads them, by pool row.  Of a block's values
+    the scale is the least power of two (not under 2^-110) that keeps them within the codes' 448;
+    a later token with a larger value raises it, and the block's earlier codes are rounded again.
+    Writing a block's first row begins the block: what it held is gone.  Values that are not finite
+    make the scale of their (block, head) NaN until the block is begun again, and whoever attends
+    it gets NaN.
+    """
+
+    dtype = torch.float8_e4m3fn
+
+    kind = "fp8"
+
+    def _allocate(self, shape):
+        codes = (*shape, BLOCK_TOKENS * self.head_dim)
+        self.k_codes = torch.zeros(codes, dtype=torch.uint8, device=self.device)
+        self.v_codes = torch.zeros(codes, dtype=torch.uint8, device=self.device)
+        self.k_scale = torch.full(shape, 2.0**-110, dtype=torch.float32, device=self.device)
+        self.v_scale = torch.full(shape, 2.0**-110, dtype=torch.float32, device=self.device)
+
+
+class Fp4TokenToKVPool(CodedTokenToKVPool):
+    """A K/V pool in 4 bits: per layer ``num_blocks`` blocks of 64 tokens (block 0 is padding) of e2m1
+    codes with power-of-two scales, each the byte of its exponent: of K one for each token, KV head and 32
+    channels (``k_scale [num_layers, num_blocks, kv_heads, 2 * head_dim]``), of V one for each token and KV head
+    (``v_scale [num_layers, num_blocks, kv_heads, 64]``).  ``head_dim`` 64 or 128.  133 bytes for a token's K and V of
+    128 channels, where bf16 takes 512.
+
+    Of the values that share a scale it is the least power of two that keeps them within 7 times itself
+    (values between 6 and 7 times it become 6 times it, the largest code), for K 2^-96 at least (and 2^125 at
+    most), for V 2^-50.  Tokens are independent of each other: a row may be written at any time and over and
+    over.  Of a token and KV head whose K or V holds a value that is not finite, or whose V one above 7 * 2^59,
+    nothing is kept: K and V read back as NaN, and whoever attends it gets NaN.
+    """
+
+    kind = "fp4"
+    #: two e2m1 codes a byte
+    dtype = torch.uint8
+
+    def _allocate(self, shape):
+        codes = (*shape, BLOCK_TOKENS * self.head_dim // 2)
+        self.k_codes = torch.zeros(codes, dtype=torch.uint8, device=self.device)
+        self.v_codes = torch.zeros(codes, dtype=torch.uint8, device=self.device)
+        self.k_scale = torch.full((*shape, 2 * self.head_dim), 127, dtype=torch.uint8, device=self.device)
+        self.v_scale = torch.full((*shape, BLOCK_TOKENS), 127, dtype=torch.uint8, device=self.device)

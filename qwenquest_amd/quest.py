@@ -30,7 +30,7 @@ from qwenquest_amd import _lib
 from qwenquest_amd.batch import DecodePlan
 
 if TYPE_CHECKING:
-    from qwenquest_amd.paged import Fp8TokenToKVPool
+    from qwenquest_amd.paged import CodedTokenToKVPool
 
 __all__ = ["QuestAlgorithm", "QuestSelection", "QuestTrace", "StepLayout"]
 
@@ -51,7 +51,7 @@ class StepLayout:
     candidate_limit_i32: torch.Tensor  # [bs] int32  pages >= this are never candidates
     page_size: int
     top_k: int
-    #: over an 8-bit pool: the division of the step's attention
+    #: over an 8- or 4-bit pool: the division of the step's attention
     plan: DecodePlan | None = None
 
     @property
@@ -364,12 +364,12 @@ class QuestAlgorithm:
         self._step = StepLayout(seq, actual, limit, self.page_size, self.top_k)
         return self._step
 
-    # -------------------------------------------- pages of an 8-bit block pool
+    # --------------------------------------- pages of an 8- or 4-bit block pool
 
-    def _page_bounds(self, pool: Fp8TokenToKVPool, block_table, reqs, seq_lens, prefix_lens, decode: bool,
+    def _page_bounds(self, pool: CodedTokenToKVPool, block_table, reqs, seq_lens, prefix_lens, decode: bool,
                      max_new: int) -> StepLayout | None:
         if self.page_size != 64:
-            raise ValueError(f"an 8-bit pool's pages are its blocks of 64 tokens, not of {self.page_size}")
+            raise ValueError(f"an 8- or 4-bit pool's pages are its blocks of 64 tokens, not of {self.page_size}")
         if pool.kv_heads != self.kv_heads or pool.head_dim != self.head_dim or pool.num_layers < self.end_layer:
             raise ValueError(f"the pool ({pool.num_layers} layers, {pool.kv_heads} x {pool.head_dim}) does not hold the "
                              f"Quest layers' keys ({self.end_layer} layers, {self.kv_heads} x {self.head_dim})")
@@ -385,13 +385,13 @@ class QuestAlgorithm:
         actual = limit = ws = None
         if decode:
             actual, limit = torch.empty((2, bs), dtype=torch.int32, device=dev).unbind(0)
-            need = int(_lib.load().qq_fp8_decode_workspace_bytes(bs, self.kv_heads, self.kv_heads, self.head_dim))
+            need = int(getattr(_lib.load(), f"qq_{pool.kind}_decode_workspace_bytes")(bs, self.kv_heads, self.kv_heads, self.head_dim))
             # of this step alone: a graph's replay must not find another step's division in it
             ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
         stream = _lib.stream(dev)
         with _lib.on(dev):
             _lib.call(
-                "qq_fp8_page_bounds", codes, pool.k_codes.stride(0), scale, pool.k_scale.stride(0), *geometry,
+                f"qq_{pool.kind}_page_bounds", codes, pool.k_codes.stride(0), scale, pool.k_scale.stride(0), *geometry,
                 *table, *(_lib.ptr(t) for t in lens), bs, int(decode), int(max_new), self.num_layers,
                 _lib.ptr(self.page_k_bounds), self.max_reqs, self.max_pages_per_req, self.top_k,
                 int(self.avoid_recent_overlap), _lib.ptr(actual), _lib.ptr(limit), _lib.ptr(ws),
@@ -406,21 +406,21 @@ class QuestAlgorithm:
         self,
         req_indices: torch.Tensor,
         seq_lens: torch.Tensor,
-        pool: Fp8TokenToKVPool,
+        pool: CodedTokenToKVPool,
         block_table: torch.Tensor,
         *,
         prefix_lens: torch.Tensor | None = None,
         max_new: int = 0,
     ) -> None:
-        """[Q2] for a batch over an 8-bit pool, every Quest layer in one launch: bounds of the pages
+        """[Q2] for a batch over an 8- or 4-bit pool, every Quest layer in one launch: bounds of the pages
         that the first ``seq_lens[i]`` tokens of each request complete, from ``prefix_lens[i]``'s
         page on if given (``max_new``: the most new tokens of a request, where the caller knows it,
         sizes the launch).  A page is complete or has no bounds: nothing is kept for the tail."""
         self._page_bounds(pool, block_table, req_indices, seq_lens, prefix_lens, False, max_new)
 
-    def decode_step_blocks(self, req_indices: torch.Tensor, seq_lens: torch.Tensor, pool: Fp8TokenToKVPool,
+    def decode_step_blocks(self, req_indices: torch.Tensor, seq_lens: torch.Tensor, pool: CodedTokenToKVPool,
                            block_table: torch.Tensor) -> StepLayout:
-        """[Q3] + [Q4] over an 8-bit pool in one launch: bounds of the pages that the previous step's
+        """[Q3] + [Q4] over an 8- or 4-bit pool in one launch: bounds of the pages that the previous step's
         tokens completed, at every layer, the step layout, and the division of the step's attention."""
         self._step = self._page_bounds(pool, block_table, req_indices, seq_lens, None, True, 0)
         return self._step

@@ -1,0 +1,164 @@
+"""What stands between a layer's QKV product and its attention: RMS norms of each query and key head
+and the rotation by position, in one launch (``qq_qk_norm_rotary``).
+
+``AttentionBackend.forward_qkv`` calls it for layers that carry one.
+"""
+
+from __future__ import annotations
+
+import math
+from collections.abc import Sequence
+
+import torch
+
+from qwenquest_amd import _lib
+from qwenquest_amd.paged import _indexed
+
+__all__ = ["QKNormRotary"]
+
+_ORDERS = ("blocks", "cycled")
+_PAIRS = ("halves", "neighbours")
+
+
+class QKNormRotary:
+    """Norms and rotation of one layer's queries and keys.
+
+    A head x becomes ``y = x / sqrt(mean(x^2) + eps) * weight`` (``q_weight`` / ``k_weight [head_dim]``, copied;
+    None: no norm), then of the first ``rotary_dim`` channels pair j turns by ``position * inv_freq[j]``:
+    ``(a, b) -> (a cos - b sin, b cos + a sin)``.  In float32, angles exact to its last places at any position
+    under 2^31, rounded once to the input's type (bfloat16 or float32).
+
+    ``inv_freq [rotary_dim / 2]``: by default ``base ** (-2 j / rotary_dim)``.  ``pairs``: "halves" (channel j with
+    j + rotary_dim / 2) or "neighbours" (2 j with 2 j + 1).  ``sections``: the number of pairs that turn by each of several
+    position axes (time, height, width), in ``section_order`` "blocks" (the first axis's pairs, then the second's) or
+    "cycled" (dealt to the axes in turn, as long as each has pairs left).
+    """
+
+    def __init__(
+        self,
+        num_heads: int,
+        kv_heads: int,
+        head_dim: int,
+        *,
+        q_weight: torch.Tensor | None = None,
+        k_weight: torch.Tensor | None = None,
+        eps: float = 1e-6,
+        base: float = 10000.0,
+        rotary_dim: int | None = None,
+        inv_freq: Sequence[float] | torch.Tensor | None = None,
+        sections: Sequence[int] | None = None,
+        section_order: str = "blocks",
+        pairs: str = "halves",
+        device: torch.device | str,
+    ):
+        self.device = _indexed(device)
+        if self.device.type != "cuda":
+            raise RuntimeError("qwenquest_amd.QKNormRotary needs a GPU device (no CPU path)")
+        if not 0 < num_heads < 1 << 16 or not 0 < kv_heads < 1 << 16:
+            raise ValueError(f"num_heads and kv_heads must be 1 .. 65535, got {num_heads} and {kv_heads}")
+        if head_dim % 8 or not 8 <= head_dim <= 512:
+            raise ValueError(f"head_dim must be a multiple of 8 up to 512, got {head_dim}")
+        if pairs not in _PAIRS or section_order not in _ORDERS:
+            raise ValueError(f"pairs must be one of {_PAIRS} and section_order of {_ORDERS}, got {pairs!r} and {section_order!r}")
+        rotary_dim = head_dim if rotary_dim is None else rotary_dim
+        step = 8 if pairs == "neighbours" else 16
+        if not 0 <= rotary_dim <= head_dim or rotary_dim % step:
+            raise ValueError(f"rotary_dim must be a multiple of {step} up to head_dim for pairs={pairs!r}, got {rotary_dim}")
+        if not 0.0 <= eps < math.inf:
+            raise ValueError(f"eps must be finite and not negative, got {eps}")
+        count = rotary_dim // 2
+        if inv_freq is None:
+            if not 0.0 < base < math.inf:
+                raise ValueError(f"base must be positive, got {base}")
+            freq = torch.tensor([float(base) ** (-2.0 * j / rotary_dim) for j in range(count)], dtype=torch.float64)
+        else:
+            freq = torch.as_tensor(inv_freq, dtype=torch.float64, device="cpu").flatten()
+            if freq.numel() != count or not bool(torch.isfinite(freq).all()):
+                raise ValueError(f"inv_freq must hold {count} finite frequencies, one for each pair")
+        left = [count] if sections is None else [int(s) for s in sections]
+        if not left or min(left) < 0 or sum(left) != count:
+            raise ValueError(f"sections {tuple(left)} must add up to the {count} pairs")
+        self.num_heads, self.kv_heads, self.head_dim, self.rotary_dim = num_heads, kv_heads, head_dim, rotary_dim
+        self.eps, self.axes, self.neighbours = float(eps), len(left), pairs == "neighbours"
+        # in quarter turns, as the kernel takes angles
+        self._quarters = (freq * (2.0 / math.pi)).to(self.device)
+        self._axis = torch.tensor(_deal(left, section_order == "cycled"), dtype=torch.int32, device=self.device)
+        self._weights = [self._weight(w, what) for w, what in ((q_weight, "q_weight"), (k_weight, "k_weight"))]
+
+    def _weight(self, w: torch.Tensor | None, what: str) -> torch.Tensor | None:
+        if w is None:
+            return None
+        if w.shape != (self.head_dim,) or not w.dtype.is_floating_point:
+            raise ValueError(f"{what} must hold {self.head_dim} floating-point values, got {tuple(w.shape)} {w.dtype}")
+        return w.detach().to(device=self.device, dtype=torch.float32, copy=True).contiguous()
+
+    def __call__(self, qkv: torch.Tensor, positions: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """``qkv [n, (num_heads + 2 kv_heads) * head_dim]``, a token's query heads, key heads and value heads in a
+        row, at ``positions`` -> ``q [n, num_heads, head_dim]``, ``k`` and ``v [n, kv_heads, head_dim]``, dense (v as it
+        was)."""
+        h, kv, dim = self.num_heads, self.kv_heads, self.head_dim
+        if qkv.dim() != 2 or qkv.shape[1] != (h + 2 * kv) * dim:
+            raise ValueError(f"qkv must be [n, ({h} + 2 * {kv}) * {dim}], got {tuple(qkv.shape)}")
+        return self._run(qkv[:, : h * dim], qkv[:, h * dim : (h + kv) * dim], qkv[:, (h + kv) * dim :], positions)
+
+    def apply(self, q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """``q [n, num_heads, head_dim]`` and ``k [n, kv_heads, head_dim]`` (or with the heads in a row) at
+        ``positions``, as new dense tensors."""
+        out = []
+        for x, heads, what in ((q, self.num_heads, "q"), (k, self.kv_heads, "k")):
+            if x.dim() == 3 and x.shape[1:] == (heads, self.head_dim):
+                # a view wherever a token's heads lie in a row
+                x = x.reshape(x.shape[0], heads * self.head_dim)
+            if x.dim() != 2 or x.shape[1] != heads * self.head_dim:
+                raise ValueError(f"{what} must be [n, {heads}, {self.head_dim}], got {tuple(x.shape)}")
+            out.append(x)
+        return self._run(out[0], out[1], None, positions)[:2]
+
+    def _run(self, q, k, v, positions):
+        n, dev, dt = q.shape[0], self.device, q.dtype
+        code = _lib.dtype_code(dt)
+        rows = []
+        for x in (q, k, v):
+            if x is None:
+                rows.append((None, 0))
+                continue
+            if x.device != dev:
+                raise ValueError(f"the heads lie on {x.device}, the weights and frequencies on {dev}")
+            if x.shape[0] != n or x.dtype != dt:
+                raise ValueError("q and k differ in tokens or type")
+            if x.requires_grad and torch.is_grad_enabled():
+                raise RuntimeError("QKNormRotary computes no gradients: detach its inputs or call it under torch.no_grad()")
+            step = 16 // x.element_size()
+            if x.stride(1) != 1 or x.data_ptr() % 16 or (n > 1 and (x.stride(0) % step or x.stride(0) < 0)):
+                x = x.clone(memory_format=torch.contiguous_format)
+            rows.append((x, x.stride(0) if n > 1 else x.shape[1]))
+        pos = positions
+        if pos.dtype.is_floating_point or pos.dtype == torch.bool:
+            raise ValueError(f"positions must hold whole numbers, got {pos.dtype}")
+        if pos.shape != ((n,) if self.axes == 1 and pos.dim() == 1 else (self.axes, n)):
+            raise ValueError(f"positions must be [{self.axes}, {n}]{f' or [{n}]' if self.axes == 1 else ''}, got {tuple(pos.shape)}")
+        pos = pos.to(device=dev, dtype=torch.int64).contiguous()
+        outs = [torch.empty((n, heads, self.head_dim), dtype=dt, device=dev)
+                for heads in (self.num_heads, self.kv_heads, self.kv_heads)[: 2 if v is None else 3]]
+        wq, wk = self._weights
+        with _lib.on(dev):
+            _lib.call(
+                "qq_qk_norm_rotary", *(y for x, stride in rows for y in (_lib.ptr(x), stride)), code, self.num_heads,
+                self.kv_heads, self.head_dim, n, _lib.ptr(wq), _lib.ptr(wk), self.eps, _lib.ptr(self._quarters),
+                _lib.ptr(self._axis), self._axis.numel(), int(self.neighbours), _lib.ptr(pos), n, self.axes,
+                *(_lib.ptr(o) for o in outs), *([None] if v is None else []), _lib.stream(dev),
+            )
+        return outs if v is None else tuple(outs)
+
+
+def _deal(left: list[int], cycled: bool) -> list[int]:
+    """The axis of each pair."""
+    if not cycled:
+        return [axis for axis, count in enumerate(left) for _ in range(count)]
+    left, out, axis = list(left), [], 0
+    while sum(left):
+        if left[axis]:
+            out.append(axis)
+            left[axis] -= 1
+        axis = (axis + 1) % len(left)
+    return out
