@@ -16,6 +16,35 @@ __global__ __launch_bounds__(256) void fp4_store_kernel(Fp4StoreArgs a) {
   fp4_store_group<D, SRC>(a, i, i < a.n, (int)(item - i * a.c.KV));
 }
 
+// Runs of entries of one block, a segment of 64 entries and a head a thread block; where more than 8 runs begin in
+// the segment, they go entry by entry.
+template <int D, typename SRC>
+__global__ __launch_bounds__(2 * D) void fp4_store_runs_kernel(Fp4StoreArgs a) {
+  __shared__ int from[64];
+  const int lane = threadIdx.x & 63;
+  const int64_t e0 = (int64_t)blockIdx.x * 64;
+  auto block_at = [&](int64_t i) { return i >= 0 && i < a.n ? block_of(a.loc[i], a.c.blocks) : 0; };
+  const int mine = block_at(e0 + lane), before = block_at(e0 + lane - 1);
+  const uint64_t starts = __ballot(mine > 0 && mine != before);
+  if (__popcll(starts) > 8) {
+    int64_t end = e0 + 64;  // of the last run
+    for (const int last = __builtin_amdgcn_readlane(mine, 63); last > 0;) {
+      const uint64_t past = __ballot(block_at(end + lane) != last);
+      end += past ? __builtin_ctzll(past) : 64;
+      if (past) break;
+    }
+    constexpr int kGroups = 2 * D / (D / 4);
+    for (int64_t i0 = e0 + __builtin_ctzll(starts); i0 < end; i0 += kGroups) {
+      const int64_t i = i0 + threadIdx.x / (D / 4);
+      fp4_store_group<D, SRC>(a, i, i < end && i < a.n, blockIdx.y);
+    }
+    return;
+  }
+  each_run(a.loc, a.n, a.c.blocks, 64, blockIdx.x, from, [&](int block, int) {
+    if (block) fp4_store_block<D, SRC>(a, from, block, blockIdx.y);
+  });
+}
+
 __device__ inline void fp4_write8(uint16_t* out, uint32_t w, float s) {
   u32x4_t y;
 #pragma unroll
@@ -55,6 +84,67 @@ __global__ __launch_bounds__(256) void fp4_rows_kernel(Fp4Cache c, const int64_t
 #pragma unroll
   for (int j = 0; j < 8; ++j) w |= ((codes[j * 16] >> (dg & 4 ? 4 : 0)) & 15u) << (4 * j);
   fp4_write8(v + item * D + dg * 8, w, vs);
+}
+
+// The same for many rows: a thread block 64 entries of one head.  A run of one block reads its V as it lies, which
+// the threads turn to a token's channels side by side, and goes on through the LDS; where more than 8 runs
+// meet, as above.
+template <int D, typename DST>
+__global__ __launch_bounds__(2 * D) void fp4_rows_runs_kernel(Fp4Cache c, const int64_t* loc, int64_t n, DST* k, DST* v) {
+  constexpr int DG = D / 8;
+  __shared__ uint32_t codes[64 * DG];  // [token][8 channels]
+  const int lane = threadIdx.x & 63, tt = threadIdx.x / DG, dg = lane % DG, g = tt >> 2, u = tt & 3, h = blockIdx.y;
+  const int64_t e0 = (int64_t)blockIdx.x * 64;
+  const int count = (int)min((int64_t)64, n - e0);
+  const int64_t row = lane < count ? loc[e0 + lane] : -1;
+  const bool in = row >= 0 && (row >> 6) < c.blocks;
+  const int blk = in ? (int)(row >> 6) : -1, slot = (int)(row & 63);
+  const int prev = __shfl_up(blk, 1, 64);
+  const uint64_t starts = __ballot(lane < count && (lane == 0 || blk != prev));
+  const bool apart = __popcll(starts) > 8;
+  auto factor = [](uint32_t e, bool ok) { return ok && e != kFp4Lost ? __uint_as_float(e << 23) : __builtin_nanf(""); };
+  auto entry = [&](int e, bool staged) {
+    const int b = __shfl(blk, e, 64), t = __shfl(slot, e, 64);
+    if (e >= count) return;
+    const int64_t at = (int64_t)max(b, 0) * c.KV + h, to = ((e0 + e) * c.KV + h) * D + dg * 8;
+    const uint32_t kw = *reinterpret_cast<const uint32_t*>(c.kc + at * (32 * D) + fp4_k_offset(D, t, dg * 8));
+    const float ks = factor(c.ks[at * (2 * D) + fp4_ks_offset(t, dg * 8)], b >= 0), vs = factor(c.vs[at * 64 + fp4_vs_offset(t)], b >= 0);
+    uint32_t vw = 0;
+    if (staged) {
+      vw = codes[t * DG + dg];
+    } else {
+      const uint8_t* p = c.vc + at * (32 * D) + fp4_v_offset(t, dg * 8);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) vw |= ((p[j * 16] >> (dg & 4 ? 4 : 0)) & 15u) << (4 * j);
+    }
+    fp4_write8(k + to, kw, ks);
+    fp4_write8(v + to, vw, vs);
+  };
+  if (apart) {
+    for (int i = 0; i < 4; ++i) entry(tt + 16 * i, false);
+    return;
+  }
+  for (uint64_t left = starts; left;) {
+    const int first = __builtin_ctzll(left);
+    left &= left - 1;
+    const int end = left ? __builtin_ctzll(left) : count;
+    const int64_t at = (int64_t)max(__builtin_amdgcn_readlane(blk, first), 0) * c.KV + h;
+    const uint4 w = *reinterpret_cast<const uint4*>(c.vc + at * (32 * D) + fp4_v_offset(4 * g, (dg & ~4) * 8 + (dg & 4) + u));
+    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+    __syncthreads();  // the run before is done with the LDS
+#pragma unroll
+    for (int T = 0; T < 4; ++T) {
+      const uint32_t pairs = turn_bytes<DG>(words[T], u);  // of token 16 T + 4 g + u four channel pairs
+      const uint32_t other = __shfl_xor(pairs, 4, 64);
+      codes[(16 * T + tt) * DG + dg] = dg & 4 ? gather_nibbles(other >> 4) | (gather_nibbles(pairs >> 4) << 16)
+                                              : gather_nibbles(pairs) | (gather_nibbles(other) << 16);
+    }
+    __syncthreads();
+    for (int e0r = first & ~15; e0r < end; e0r += 16) {
+      const int e = e0r + tt;
+      entry(e >= first && e < end ? e : 64, true);
+    }
+  }
 }
 
 struct Fp4PageArgs {
@@ -174,6 +264,8 @@ int check_cache(const Fp4Cache& c, const char* what) {
 
 using namespace qq;
 
+constexpr int64_t kRunEntries = 16384;  // entries times heads from which runs are stored and read together
+
 extern "C" int qq_fp4_store(uint8_t* k_codes, uint8_t* v_codes, uint8_t* k_scale, uint8_t* v_scale, int num_blocks,
                             int kv_heads, int head_dim, const void* k, const void* v, int src_dtype, const int64_t* loc,
                             int64_t n, void* stream) {
@@ -187,15 +279,25 @@ extern "C" int qq_fp4_store(uint8_t* k_codes, uint8_t* v_codes, uint8_t* k_scale
   QQ_REQUIRE(k && v && loc, "%s: null pointer", what);
   QQ_REQUIRE(((uintptr_t)k | (uintptr_t)v) % 16 == 0, "%s: k and v must be 16-byte aligned", what);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const int64_t grid = (n * kv_heads * (head_dim / 4) + 255) / 256;
-  QQ_REQUIRE(grid < (int64_t)1 << 31, "%s: bad sizes", what);
   const bool bf = src_dtype == QQ_DTYPE_BF16;
+  if (n * kv_heads >= kRunEntries) {
+    const dim3 grid((unsigned)((n + 63) / 64), kv_heads);
+    if (head_dim == 128) {
+      if (bf) fp4_store_runs_kernel<128, uint16_t><<<grid, 256, 0, s>>>(a);
+      else fp4_store_runs_kernel<128, float><<<grid, 256, 0, s>>>(a);
+    } else {
+      if (bf) fp4_store_runs_kernel<64, uint16_t><<<grid, 128, 0, s>>>(a);
+      else fp4_store_runs_kernel<64, float><<<grid, 128, 0, s>>>(a);
+    }
+    return check_launch(what);
+  }
+  const unsigned grid = (unsigned)((n * kv_heads * (head_dim / 4) + 255) / 256);
   if (head_dim == 128) {
-    if (bf) fp4_store_kernel<128, uint16_t><<<(unsigned)grid, 256, 0, s>>>(a);
-    else fp4_store_kernel<128, float><<<(unsigned)grid, 256, 0, s>>>(a);
+    if (bf) fp4_store_kernel<128, uint16_t><<<grid, 256, 0, s>>>(a);
+    else fp4_store_kernel<128, float><<<grid, 256, 0, s>>>(a);
   } else {
-    if (bf) fp4_store_kernel<64, uint16_t><<<(unsigned)grid, 256, 0, s>>>(a);
-    else fp4_store_kernel<64, float><<<(unsigned)grid, 256, 0, s>>>(a);
+    if (bf) fp4_store_kernel<64, uint16_t><<<grid, 256, 0, s>>>(a);
+    else fp4_store_kernel<64, float><<<grid, 256, 0, s>>>(a);
   }
   return check_launch(what);
 }
@@ -212,18 +314,28 @@ extern "C" int qq_fp4_rows(const uint8_t* k_codes, const uint8_t* v_codes, const
   QQ_REQUIRE(n >= 0 && n < (int64_t)1 << 31, "%s: bad sizes", what);
   if (n == 0) return QQ_OK;
   QQ_REQUIRE(loc && k && v, "%s: null pointer", what);
-  const int64_t grid = (n * kv_heads * (head_dim / 8) + 255) / 256;
-  QQ_REQUIRE(grid < (int64_t)1 << 31, "%s: bad sizes", what);
   hipStream_t s = static_cast<hipStream_t>(stream);
   uint16_t *kb = static_cast<uint16_t*>(k), *vb = static_cast<uint16_t*>(v);
   float *kf = static_cast<float*>(k), *vf = static_cast<float*>(v);
   const bool bf = dst_dtype == QQ_DTYPE_BF16;
+  if (n * kv_heads >= kRunEntries) {
+    const dim3 grid((unsigned)((n + 63) / 64), kv_heads);
+    if (head_dim == 128) {
+      if (bf) fp4_rows_runs_kernel<128><<<grid, 256, 0, s>>>(c, loc, n, kb, vb);
+      else fp4_rows_runs_kernel<128><<<grid, 256, 0, s>>>(c, loc, n, kf, vf);
+    } else {
+      if (bf) fp4_rows_runs_kernel<64><<<grid, 128, 0, s>>>(c, loc, n, kb, vb);
+      else fp4_rows_runs_kernel<64><<<grid, 128, 0, s>>>(c, loc, n, kf, vf);
+    }
+    return check_launch(what);
+  }
+  const unsigned grid = (unsigned)((n * kv_heads * (head_dim / 8) + 255) / 256);
   if (head_dim == 128) {
-    if (bf) fp4_rows_kernel<128><<<(unsigned)grid, 256, 0, s>>>(c, loc, n, kb, vb);
-    else fp4_rows_kernel<128><<<(unsigned)grid, 256, 0, s>>>(c, loc, n, kf, vf);
+    if (bf) fp4_rows_kernel<128><<<grid, 256, 0, s>>>(c, loc, n, kb, vb);
+    else fp4_rows_kernel<128><<<grid, 256, 0, s>>>(c, loc, n, kf, vf);
   } else {
-    if (bf) fp4_rows_kernel<64><<<(unsigned)grid, 256, 0, s>>>(c, loc, n, kb, vb);
-    else fp4_rows_kernel<64><<<(unsigned)grid, 256, 0, s>>>(c, loc, n, kf, vf);
+    if (bf) fp4_rows_kernel<64><<<grid, 256, 0, s>>>(c, loc, n, kb, vb);
+    else fp4_rows_kernel<64><<<grid, 256, 0, s>>>(c, loc, n, kf, vf);
   }
   return check_launch(what);
 }

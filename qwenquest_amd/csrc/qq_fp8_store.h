@@ -192,50 +192,60 @@ __device__ inline void store_block(const StoreArgs& a, StoreSmem<D>& sm, int blo
   }
 }
 
-// K or V of the runs of loc that begin in segment `segment`, head h.  Entries of one block stand next
-// to each other in loc; the thread block in whose segment such a run begins writes its (block,
-// head) alone, so nothing is shared between thread blocks and the result does not depend on
+// The runs of loc that begin in segment `segment`, seg entries each (at most 64): f(0, lane) by the first wave,
+// then f(block, lane) by all with from[64], the entry that writes each token of the block or -1, in the LDS.
+// Entries of one block stand next to each other in loc; the thread block in whose segment such a run begins writes its block
+// alone, so nothing is shared between thread blocks and the result does not depend on
 // their order.  Of a row listed twice in a run the last entry counts.
-template <int D, typename SRC, bool V>
-__device__ inline void store_segment(const StoreArgs& a, StoreSmem<D>& sm, int64_t segment, int h) {
+template <typename F>
+__device__ inline void each_run(const int64_t* loc, int64_t n, int blocks, int seg, int64_t segment, int (&from)[64], F f) {
   const int tid = threadIdx.x, lane = tid & 63;
-  const int64_t e0 = segment * a.seg;
+  const int64_t e0 = segment * seg;
   // every wave for itself: the rows of the segment's entries and of as many after them, and
   // where its runs begin
-  auto row_at = [&](int64_t i) { return i >= 0 && i < a.n ? a.loc[i] : (int64_t)-1; };
+  auto row_at = [&](int64_t i) { return i >= 0 && i < n ? loc[i] : (int64_t)-1; };
   const int64_t row0 = row_at(e0 + lane), row1 = row_at(e0 + 64 + lane), row_before = row_at(e0 - 1);
-  const int b0 = block_of(row0, a.c.blocks), b1 = block_of(row1, a.c.blocks);
+  const int b0 = block_of(row0, blocks), b1 = block_of(row1, blocks);
   int prev = __shfl_up(b0, 1, 64);
-  if (lane == 0) prev = block_of(row_before, a.c.blocks);
-  uint64_t starts = __ballot(lane < a.seg && b0 > 0 && b0 != prev);
+  if (lane == 0) prev = block_of(row_before, blocks);
+  uint64_t starts = __ballot(lane < seg && b0 > 0 && b0 != prev);
   while (starts) {
     const int at = __builtin_ctzll(starts);
     starts &= starts - 1;
     const int block = __builtin_amdgcn_readlane(b0, at);
-    __syncthreads();  // the run before is done with sm
+    __syncthreads();  // the run before is done with the LDS
     if (tid < 64) {
-      sm.from[lane] = -1;
-      if (lane == 0) sm.bad = 0;
+      from[lane] = -1;
+      f(0, lane);
       // (one wave's LDS operations stay in order)
       const uint64_t other = __ballot(b0 != block && lane >= at);
       const int end0 = other ? __builtin_ctzll(other) : 64;
-      if (lane >= at && lane < end0) atomicMax(&sm.from[row0 & 63], (int)(e0 + lane));
+      if (lane >= at && lane < end0) atomicMax(&from[row0 & 63], (int)(e0 + lane));
       if (end0 == 64) {
         const uint64_t other1 = __ballot(b1 != block);
         const int end1 = other1 ? __builtin_ctzll(other1) : 64;
-        if (lane < end1) atomicMax(&sm.from[row1 & 63], (int)(e0 + 64 + lane));
+        if (lane < end1) atomicMax(&from[row1 & 63], (int)(e0 + 64 + lane));
         for (int64_t i0 = e0 + 128; end1 == 64; i0 += 64) {  // rows listed twice
           const int64_t row = row_at(i0 + lane);
-          const uint64_t more = __ballot(block_of(row, a.c.blocks) != block);
+          const uint64_t more = __ballot(block_of(row, blocks) != block);
           const int len = more ? __builtin_ctzll(more) : 64;
-          if (lane < len) atomicMax(&sm.from[row & 63], (int)(i0 + lane));
+          if (lane < len) atomicMax(&from[row & 63], (int)(i0 + lane));
           if (len < 64) break;
         }
       }
     }
     __syncthreads();
-    store_block<D, SRC, V>(a, sm, block, h);
+    f(block, lane);
   }
+}
+
+// K or V of those runs, head h.
+template <int D, typename SRC, bool V>
+__device__ inline void store_segment(const StoreArgs& a, StoreSmem<D>& sm, int64_t segment, int h) {
+  each_run(a.loc, a.n, a.c.blocks, a.seg, segment, sm.from, [&](int block, int lane) {
+    if (block) store_block<D, SRC, V>(a, sm, block, h);
+    else if (lane == 0) sm.bad = 0;  // before a run, by the first wave
+  });
 }
 
 // Single entries by one wave, each by a group of D / 4 lanes, K in the group's first half and V in the

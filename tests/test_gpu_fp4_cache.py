@@ -36,8 +36,8 @@ def same(pool, cache, layer=0, rows=None):
 def test_rows_written_and_read(cuda, kv, dim, dtype):
     """Runs that begin and end inside blocks, whole blocks, single rows, over and over."""
     rng = np.random.default_rng(kv * dim)
-    pool, cache = Fp4TokenToKVPool(12, 2, kv, dim, cuda), o4.Cache(12, kv, dim)
-    for lo, hi in ((64, 65), (70, 300), (128, 192), (64, 128), (301, 302), (300, 301), (200, 768), (64, 767), (767, 768)):
+    pool, cache = Fp4TokenToKVPool(64, 2, kv, dim, cuda), o4.Cache(64, kv, dim)
+    for lo, hi in ((64, 65), (70, 300), (128, 192), (64, 128), (301, 302), (300, 301), (200, 768), (64, 767), (767, 768), (70, 2500), (2000, 2563), (65, 4095)):
         rows = np.arange(lo, hi)
         k, v = values(rng, len(rows), kv, dim, dtype), values(rng, len(rows), kv, dim, dtype)
         pool.set_kv_buffer(1, i64(rows, cuda), k.to(cuda), v.to(cuda))
@@ -47,15 +47,16 @@ def test_rows_written_and_read(cuda, kv, dim, dtype):
     assert not pool.k_codes[1, 0].any() and not pool.v_codes[1, 0].any()  # the padding block
 
 
-@pytest.mark.parametrize("n", [1, 2, 31, 64, 65, 700])
+@pytest.mark.parametrize("n", [1, 2, 31, 64, 65, 700, 3900])
 def test_scattered_blocks(cuda, n):
     """Entries of many blocks in any order, one and several of a block at a time."""
     rng = np.random.default_rng(n)
-    pool, cache = Fp4TokenToKVPool(800, 1, 2, 64, cuda), o4.Cache(800, 2, 64)
+    total = 800 if n < 800 else 4000
+    pool, cache = Fp4TokenToKVPool(total, 1, 4, 64, cuda), o4.Cache(total, 4, 64)
     for step in range(3):
-        blocks = rng.permutation(np.arange(1, 800))[:n]
-        rows = np.concatenate([b * 64 + rng.permutation(64)[: 1 + (step and rng.integers(0, 5))] for b in blocks])
-        k, v = values(rng, len(rows), 2, 64, torch.bfloat16), values(rng, len(rows), 2, 64, torch.bfloat16)
+        blocks = rng.permutation(np.arange(1, total))[:n]
+        rows = np.concatenate([b * 64 + rng.permutation(64)[: 1 + (step and rng.integers(0, (5, 64)[step == 2 and n < 800]))] for b in blocks])
+        k, v = values(rng, len(rows), 4, 64, torch.bfloat16), values(rng, len(rows), 4, 64, torch.bfloat16)
         pool.set_kv_buffer(0, i64(rows, cuda), k.to(cuda), v.to(cuda))
         cache.write(rows, k.double().numpy(), v.double().numpy())
         same(pool, cache, rows=np.concatenate([np.arange(b * 64, b * 64 + 64) for b in blocks]))
