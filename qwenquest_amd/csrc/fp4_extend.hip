@@ -8,11 +8,12 @@
 // tile ahead.
 //   S^T = K Q^T  v_mfma_f32_32x32x16_bf16, K's codes times their scales as bf16 (exact)
 //   O^T += V^T W^T  v_mfma_f32_32x32x16_f16, V's codes as f16 (exact)
-// With t = scale log2(e) (q . k), 2^E a token's V scale (E biased by 127, as it is stored) and N a row's
+// With t = scale log2(e) (q . k), 2^E a token's V scale and N a row's
 // running maximum of t + E, which is let lag by 8 (the sums are rescaled once it lags more), a weight goes
 // into the product as
 //   w = 2^(t + E - N + 7),
-// which fills f16's range from the top (7 + 8); the weights' sum adds w 2^(128 - E), in fp32.  V's exponents
+// which fills f16's range from the top (7 + 8); the weights' sum adds w 2^(1 - E), in fp32.  E and 2^(1 - E) of a lane's 32 tokens
+// come by matrix instructions, a step of K Q^T that holds them as channels.  V's exponents
 // span 109, so a token whose w underflows weighs less than 2^-24 of another one.  w goes to f16's
 // 11 bits by truncation (one instruction for two weights) of w (1 + 0.72 * 2^-11): truncation takes
 // half a step on average, 2^-10 / 2 over the significand's 1 .. 2, in the mean 0.72 * 2^-11.
@@ -43,7 +44,8 @@ struct Fp4ExtendArgs {
   int bs, n;
   int tiles;   // query tiles the grid holds (an upper bound of the requests' tiles), one more at its end
   int splits;  // K/V splits the grid holds
-  float sl2;   // scale * log2(e)
+  float sl2;   // scale * log2(e) / q_factor
+  float q_factor;  // a power of two, 1 but for scales far from 1: sl2 within 2^+-100
   uint16_t* out;
   float* part_o;   // [splits, KV, tiles, 128 rows, D]
   float* part_ml;  // [splits, KV, tiles, 128 rows, 2]
@@ -63,6 +65,11 @@ __device__ inline f16x8_t fp4_f16(uint32_t w) {
   y.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 2));
   y.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 3));
   return __builtin_bit_cast(f16x8_t, y);
+}
+
+__device__ inline float trunc_bf16(float x) { return __uint_as_float(__float_as_uint(x) & 0xFFFF0000u); }
+__device__ inline uint32_t pack_trunc(float even, float odd) {
+  return __builtin_amdgcn_perm(__float_as_uint(odd), __float_as_uint(even), 0x07060302u);
 }
 
 // find_tile's answer is the same in every lane; in scalar registers it makes the K/V loop's control
@@ -127,11 +134,31 @@ __global__ __launch_bounds__(64 * kExtWaves, 2) void fp4_extend_kernel(Fp4Extend
 #pragma unroll
   for (int i = 0; i < 4 * KI; ++i)
     qb[i] = *reinterpret_cast<const bf16x8_t*>(qp + ((i >> 2) * 2 + hf) * 32 + (i & 3) * 8);
+  if (a.q_factor != 1.0f) {
+#pragma unroll
+    for (int i = 0; i < 4 * KI; ++i)
+#pragma unroll
+      for (int x = 0; x < 8; ++x) qb[i][x] = (__bf16)((float)qb[i][x] * a.q_factor);
+  }
+  // A further step over channels of which K's side holds (E, E, E, 2^(1 - E)) of a token: against 1 / sl2 in three bf16
+  // pieces it adds E / sl2 to every product; against (0, 0, 0, 1) it spreads 2^(1 - E) as the products lie
+  bf16x8_t q_add, q_spread;
+  {
+    const float r = 1.0f / a.sl2, r1 = r - trunc_bf16(r), r2 = r1 - trunc_bf16(r1);
+    u32x4_t w = {0, 0, 0, 0}, v = {0, 0, 0, 0};
+    if (hf == 0) {
+      w.x = pack_trunc(r, r1);
+      w.y = __float_as_uint(r2) >> 16;
+      v.y = 0x3F800000u;
+    }
+    q_add = __builtin_bit_cast(bf16x8_t, w);
+    q_spread = __builtin_bit_cast(bf16x8_t, v);
+  }
 
   const scalar_words_t bt = (scalar_words_t)(uintptr_t)(a.table + (int64_t)max(et.req, 0) * a.table_stride);
-  // this lane's scales: of tokens 16 T + lo % 16 for pieces 2 i + hf, of tokens 16 T + 4 hf + r and 8 more
+  // this lane's scales: of K pieces 2 i + hf and of V, of tokens lo of both halves (of K's 16 T + lo % 16, a word)
   const uint8_t* ksp = a.c.ks + (int64_t)h * (2 * D) + (hf * 16 + (lo & 15)) * 4;
-  const uint8_t* vsp = a.c.vs + (int64_t)h * 64 + hf * 16;
+  const uint8_t* vsp = a.c.vs + (int64_t)h * 64 + ((lo & 15) >> 2) * 16 + (lo >> 4) * 4 + (lo & 3);
   bool bad = et.req < 0;
   // a tile's block; padding and ids outside the cache are read as padding, and spoil the answer
   auto block_of_word = [&](int word) {
@@ -150,14 +177,13 @@ __global__ __launch_bounds__(64 * kExtWaves, 2) void fp4_extend_kernel(Fp4Extend
       load_lds16((wave < 2 ? a.c.kc : a.c.vc) + at + (wave & 1) * 1024, base + wave * 1024);
     }
   };
-  uint32_t ks[KI], ks_next[KI];
-  u32x4_t vs[2], vs_next[2];
+  uint32_t ks[KI], ks_next[KI], vs[2], vs_next[2];
   auto load_scales = [&](int blk) {
     const int64_t at = (int64_t)blk * a.KV;
 #pragma unroll
     for (int i = 0; i < KI; ++i) ks_next[i] = *reinterpret_cast<const uint32_t*>(ksp + at * (2 * D) + i * 128);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) vs_next[i] = *reinterpret_cast<const u32x4_t*>(vsp + at * 64 + i * 32);
+    for (int t = 0; t < 2; ++t) vs_next[t] = vsp[at * 64 + t * 8];
   };
   float16_t o[NC];
 #pragma unroll
@@ -181,7 +207,7 @@ __global__ __launch_bounds__(64 * kExtWaves, 2) void fp4_extend_kernel(Fp4Extend
 #pragma unroll
     for (int i = 0; i < KI; ++i) ks[i] = ks_next[i] >> (8 * (lo >> 4));  // bytes 0 and 2: the lane's tokens of the halves
 #pragma unroll
-    for (int i = 0; i < 2; ++i) vs[i] = vs_next[i];
+    for (int t = 0; t < 2; ++t) vs[t] = vs_next[t];
     if (j + 1 < j_end) {
       const int blk = block_of_word(word);
       load_tile(buf ^ 1, blk);
@@ -215,6 +241,17 @@ __global__ __launch_bounds__(64 * kExtWaves, 2) void fp4_extend_kernel(Fp4Extend
 #pragma unroll
         for (int t = 0; t < 2; ++t) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kb[t], qb[4 * i + p], s[t], 0, 0, 0);
       }
+    float16_t spread[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const uint32_t e = __float_as_uint((float)vs[t] - 127.0f);
+      const u32x4_t w = {__builtin_amdgcn_perm(e, e, 0x07060706u), (e >> 16) | ((255u - vs[t]) << 23), 0, 0};
+      const bf16x8_t ext = __builtin_bit_cast(bf16x8_t, w);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) spread[t][i] = 0.0f;
+      s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ext, q_add, s[t], 0, 0, 0);
+      spread[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ext, q_spread, spread[t], 0, 0, 0);
+    }
     // the values' codes arrive under the softmax
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -225,18 +262,20 @@ __global__ __launch_bounds__(64 * kExtWaves, 2) void fp4_extend_kernel(Fp4Extend
     __builtin_amdgcn_sched_barrier(0);
     const bool edge = (j + 1) * kExtTile > lim_full;  // block-uniform: some row's limit is inside this tile
     const int left = lim - j * kExtTile - 4 * hf;
-    // scale bytes of tokens 32 t + 8 q + 4 hf + 0 .. 3
-    auto vs_word = [&](int t, int q) { return vs[q & 1][2 * t + (q >> 1)]; };
-    float mx = -INFINITY;
+    if (edge) {
+      int last = left;
+      __asm__ volatile("" : "+v"(last));  // a branch, not 64 selects in every tile
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[t][i] = (t * 32 + 8 * (i / 4) + i % 4) < last ? s[t][i] : -INFINITY;
+    }
+    float mx = s[0][0];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[t][i] = __builtin_fmaf(s[t][i], a.sl2, (float)((vs_word(t, i >> 2) >> (8 * (i & 3))) & 255u));
-        if (edge) s[t][i] = (t * 32 + 8 * (i / 4) + i % 4) < left ? s[t][i] : -INFINITY;
-        mx = fmaxf(mx, s[t][i]);
-      }
-    mx = fmaxf(mx, lane_xor32(mx, lane));
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[t][i]);
+    mx = fmaxf(mx, lane_xor32(mx, lane)) * a.sl2;
     if (__any(mx > N + kSlack)) {
       const float Nn = fmaxf(N, mx), am = N == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(N - Nn);
       L *= am;
@@ -248,31 +287,28 @@ __global__ __launch_bounds__(64 * kExtWaves, 2) void fp4_extend_kernel(Fp4Extend
     }
     const float bias = (float)kLift + kRoundLog2 - (N == -INFINITY ? 0.0f : N);
     float sum = 0.0f;
+    // O^T += V^T W^T, 16 tokens at a time, the products of some under the weights of the next
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int u = 0; u < 4; ++u) {
+      float w[8];
+      u32x4_t wv;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[t][i] = __builtin_amdgcn_exp2f(s[t][i] + bias);
-        // 2^(255 - byte) next to a weight that holds 2^byte
-        sum = __builtin_fmaf(s[t][i], fp4_factor(~vs_word(t, i >> 2), i & 3), sum);
+      for (int x = 0; x < 8; ++x) {
+        float& e = w[x];
+        e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u >> 1][(u & 1) * 8 + x], a.sl2, bias));
+        sum = __builtin_fmaf(e, spread[u >> 1][(u & 1) * 8 + x], sum);
       }
-    L += sum;
-    // O^T += V^T W^T, 16 tokens at a time
-    u32x4_t wv[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+      for (int x = 0; x < 4; ++x) wv[x] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(w[x], w[4 + x]));
+      const f16x8_t wf = __builtin_bit_cast(f16x8_t, wv);
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
-        wv[u][x] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(s[u >> 1][(u & 1) * 8 + x], s[u >> 1][(u & 1) * 8 + 4 + x]));
-#pragma unroll
-    for (int x = 0; x < KI; ++x)
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int x = 0; x < KI; ++x) {
         const uint32_t va = vw[x][0][u], vb = vw[x][1][u];
-        const f16x8_t w = __builtin_bit_cast(f16x8_t, wv[u]);
-        o[2 * x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp4_f16(fp4_lower(va, vb)), w, o[2 * x], 0, 0, 0);
-        o[2 * x + 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp4_f16(fp4_upper(va, vb)), w, o[2 * x + 1], 0, 0, 0);
+        o[2 * x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp4_f16(fp4_lower(va, vb)), wf, o[2 * x], 0, 0, 0);
+        o[2 * x + 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp4_f16(fp4_upper(va, vb)), wf, o[2 * x + 1], 0, 0, 0);
       }
+    }
+    L += sum;
   }
   L += lane_xor32(L, lane);
   if (__syncthreads_or(bad)) L = __builtin_nanf("");  // a block that is not there: no answer
@@ -368,7 +404,8 @@ extern "C" int qq_fp4_extend_attention(const void* q, int num_q_heads, const uin
   const int64_t grid = (tiles * a.splits + 1) * kv_heads;
   QQ_REQUIRE(grid < (int64_t)1 << 31, "%s: too many query rows", what);
   a.tiles = (int)tiles;
-  a.sl2 = scale * kLog2e;
+  a.q_factor = scale < 0x1p-60f ? 0x1p-64f : scale > 0x1p60f ? 0x1p64f : 1.0f;
+  a.sl2 = scale / a.q_factor * kLog2e;
   a.out = static_cast<uint16_t*>(out);
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = a.part_o ? a.part_o + a.splits * kv_heads * tiles * kExtRows * head_dim : nullptr;
