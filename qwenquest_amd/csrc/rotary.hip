@@ -11,6 +11,11 @@
 // A wave works on a token: a lane per pair for the angles, which meet the heads in the LDS, then D / 8 lanes
 // (to the next power of two) per head, 8 channels a lane, whose cosines and sines stay in registers over the
 // token's heads; where tokens are few, more waves share a token's heads.
+// Bound: HBM at prompts: 16384 tokens, 32 + 4 + 4 heads of 128 in bf16, 74 us (4.5 TB/s, a copy 4.7; 104 with the heads'
+// values asked for one after the other, exchanged through the LDS and rounded by hand). 16 tokens 4.4, a launch and
+// two memory round trips.
+#include <type_traits>
+
 #include "qq_quest_dev.h"
 
 namespace qq {
@@ -41,6 +46,8 @@ struct RotaryArgs {
   int per, parts;  // heads of a wave, waves of a token
 };
 
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+
 template <typename T>
 struct Row8;  // eight values as they lie
 template <>
@@ -56,7 +63,10 @@ struct Row8<uint16_t> {
   __device__ inline void set(const float (&x)[8]) {
     uint32_t u[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) u[i] = (uint32_t)f2bf(x[2 * i]) | ((uint32_t)f2bf(x[2 * i + 1]) << 16);
+    for (int i = 0; i < 4; ++i) {
+      const bf16x2_t b = {(__bf16)x[2 * i], (__bf16)x[2 * i + 1]};  // to nearest even
+      u[i] = __builtin_bit_cast(uint32_t, b);
+    }
     w = make_uint4(u[0], u[1], u[2], u[3]);
   }
 };
@@ -82,17 +92,52 @@ struct Row8<float> {
   }
 };
 
+// The sum over L lanes next to each other, in each of them.
+template <int L>
+__device__ inline float lanes_sum(float v, int lane) {
+  auto add = [&](auto j) { v += __uint_as_float(lane_xor_u32<decltype(j)::value>(__float_as_uint(v), lane)); };
+  if constexpr (L >= 2) add(std::integral_constant<int, 1>{});
+  if constexpr (L >= 4) add(std::integral_constant<int, 2>{});
+  if constexpr (L >= 8) add(std::integral_constant<int, 4>{});
+  if constexpr (L >= 16) add(std::integral_constant<int, 8>{});
+  if constexpr (L >= 32) add(std::integral_constant<int, 16>{});
+  if constexpr (L >= 64) add(std::integral_constant<int, 32>{});
+  return v;
+}
+
+// Where a channel's partner lies: in the lane itself, L / 2 lanes off (D = 8 L, all of it turning), or elsewhere.
+enum Partner { kOwn, kAcross, kAway };
+
 // L lanes a head.
-template <typename T, int L>
+template <typename T, int L, Partner P>
 __global__ __launch_bounds__(64 * kRotWaves) void rotary_kernel(RotaryArgs a) {
   extern __shared__ float turned[];  // [waves][cosines, sines][pairs]
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t item = (int64_t)blockIdx.x * kRotWaves + wave;
-  const int64_t token = item / a.parts;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int64_t token = (int64_t)blockIdx.x * kRotWaves + wave;
   if (token >= a.n) return;  // (no block barrier below)
+  const int sub = lane / L, dl = lane % L;
+  const bool in = dl * 8 < a.D;
+  const int d = in ? dl * 8 : 0;
+  const int heads = a.H + a.KV + (a.v ? a.KV : 0);
+  const int h0 = blockIdx.y * a.per, h1 = min(h0 + a.per, heads);
+  constexpr int kStep = 64 / L;
+  // lanes past the last head do it once more, and write nothing
+  auto load = [&](Row8<T>& r, int hb) {
+    const int h = min(hb + sub, h1 - 1);
+    const T* p = static_cast<const T*>(a.q) + token * a.q_stride + (int64_t)h * a.D;
+    if (h >= a.H) p = static_cast<const T*>(a.k) + token * a.k_stride + (int64_t)(h - a.H) * a.D;
+    if (h >= a.H + a.KV) p = static_cast<const T*>(a.v) + token * a.v_stride + (int64_t)(h - a.H - a.KV) * a.D;
+    r.load(p + d);
+  };
+  // the heads' values are under way while the angles are taken
+  constexpr int kAhead = 3;
+  Row8<T> rows[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i)
+    if (h0 + i * kStep < h1) load(rows[i], h0 + i * kStep);
   float *cs = turned + wave * 2 * a.pairs, *sn = cs + a.pairs;
   for (int j = lane; j < a.pairs; j += 64) {
-    const int64_t at = a.pos[min(a.axis[j], a.axes - 1) * a.pos_stride + token];
+    const int64_t at = a.pos[(a.axes == 1 ? 0 : min(a.axis[j], a.axes - 1)) * a.pos_stride + token];
     const double t = (double)at * a.quarters[j], whole = rint(t);
     const int quarter = (int)(whole - 4.0 * floor(whole * 0.25));  // 0 .. 3
     float s, c;
@@ -103,47 +148,30 @@ __global__ __launch_bounds__(64 * kRotWaves) void rotary_kernel(RotaryArgs a) {
   }
   __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // a wave's own LDS words
   __builtin_amdgcn_wave_barrier();
-  const int sub = lane / L, dl = lane % L;
-  const bool in = dl * 8 < a.D;
-  const int d = in ? dl * 8 : 0;
   // the lane's pairs: its 8 channels are all first or all second ones, or four whole pairs
-  const bool turns = in && d < 2 * a.pairs, second = !a.neighbours && d >= a.pairs;
-  const int hop = a.neighbours ? 0 : second ? -(a.pairs / 8) : a.pairs / 8;  // lanes to the partner
+  const bool turns = in && d < 2 * a.pairs, second = P != kOwn && d >= a.pairs;
+  const int hop = second ? -(a.pairs / 8) : a.pairs / 8;  // lanes to the partner
   float c[8], s[8], wq[8], wk[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int j = a.neighbours ? (d + i) / 2 : d + i - (second ? a.pairs : 0);
+    const int j = P == kOwn ? (d + i) / 2 : d + i - (second ? a.pairs : 0);
     c[i] = turns ? cs[j] : 1.0f;
     s[i] = turns ? sn[j] : 0.0f;
-    if (a.neighbours ? !(i & 1) : !second) s[i] = -s[i];
+    if (P == kOwn ? !(i & 1) : !second) s[i] = -s[i];
     wq[i] = a.wq ? a.wq[d + i] : 1.0f;
     wk[i] = a.wk ? a.wk[d + i] : 1.0f;
   }
-  const int heads = a.H + a.KV + (a.v ? a.KV : 0);
-  const int h0 = (int)(item - token * a.parts) * a.per, h1 = min(h0 + a.per, heads);
-  auto from = [&](int h) -> const T* {
-    if (h < a.H) return static_cast<const T*>(a.q) + token * a.q_stride + (int64_t)h * a.D;
-    if (h < a.H + a.KV) return static_cast<const T*>(a.k) + token * a.k_stride + (int64_t)(h - a.H) * a.D;
-    return static_cast<const T*>(a.v) + token * a.v_stride + (int64_t)(h - a.H - a.KV) * a.D;
-  };
-  auto to = [&](int h) -> T* {
-    if (h < a.H) return static_cast<T*>(a.q_out) + (token * a.H + h) * a.D;
-    if (h < a.H + a.KV) return static_cast<T*>(a.k_out) + (token * a.KV + h - a.H) * a.D;
-    return static_cast<T*>(a.v_out) + (token * a.KV + h - a.H - a.KV) * a.D;
-  };
-  for (int hb = h0; hb < h1; hb += 64 / L) {
-    const int h = min(hb + sub, h1 - 1);  // lanes past the last head do it once more, and write nothing
-    Row8<T> r;
-    r.load(from(h) + d);
+  const float share = 1.0f / (float)a.D;
+  auto work = [&](Row8<T> r, int hb) {
+    const int h = min(hb + sub, h1 - 1);
     float x[8], y[8];
     r.get(x);
     float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum += in ? x[i] * x[i] : 0.0f;
-#pragma unroll
-    for (int m = L / 2; m >= 1; m >>= 1) sum += __shfl_xor(sum, m, 64);
+    for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(x[i], x[i], sum);
+    sum = lanes_sum<L>(in ? sum : 0.0f, lane);
     const bool key = h >= a.H;
-    const float mean = sum / (float)a.D + a.eps;
+    const float mean = __builtin_fmaf(sum, share, a.eps);
     float f = __builtin_amdgcn_rsqf(mean);
     // a Newton step: the instruction is off by up to 2^-23
     f = mean < INFINITY && mean > 1e-37f ? f + 0.5f * f * __builtin_fmaf(-mean * f, f, 1.0f) : f;
@@ -151,7 +179,10 @@ __global__ __launch_bounds__(64 * kRotWaves) void rotary_kernel(RotaryArgs a) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = normed ? x[i] * f * (key ? wk[i] : wq[i]) : x[i];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = a.neighbours ? x[i ^ 1] : __shfl(x[i], lane + hop, 64);
+    for (int i = 0; i < 8; ++i)
+      y[i] = P == kOwn      ? x[i ^ 1]
+             : P == kAcross ? __uint_as_float(lane_xor_u32<L / 2>(__float_as_uint(x[i]), lane))
+                            : __shfl(x[i], lane + hop, 64);
     if (h < a.H + a.KV) {
       if (turns) {
 #pragma unroll
@@ -159,18 +190,38 @@ __global__ __launch_bounds__(64 * kRotWaves) void rotary_kernel(RotaryArgs a) {
       }
       r.set(x);
     }
-    if (in && hb + sub < h1) r.store(to(h) + d);
+    if (!in || hb + sub >= h1) return;
+    T* p = static_cast<T*>(a.q_out) + (token * a.H + h) * a.D;
+    if (h >= a.H) p = static_cast<T*>(a.k_out) + (token * a.KV + h - a.H) * a.D;
+    if (h >= a.H + a.KV) p = static_cast<T*>(a.v_out) + (token * a.KV + h - a.H - a.KV) * a.D;
+    r.store(p + d);
+  };
+  for (int hb = h0; hb < h1; hb += kAhead * kStep) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (hb + i * kStep >= h1) break;  // wave-uniform
+      const Row8<T> r = rows[i];
+      if (hb + (i + kAhead) * kStep < h1) load(rows[i], hb + (i + kAhead) * kStep);
+      work(r, hb + i * kStep);
+    }
   }
+}
+
+template <typename T, int L>
+void launch_lanes(const RotaryArgs& a, dim3 blocks, size_t lds, hipStream_t s) {
+  if (a.neighbours) rotary_kernel<T, L, kOwn><<<blocks, 64 * kRotWaves, lds, s>>>(a);
+  else if (a.D == 8 * L && 2 * a.pairs == a.D) rotary_kernel<T, L, kAcross><<<blocks, 64 * kRotWaves, lds, s>>>(a);
+  else rotary_kernel<T, L, kAway><<<blocks, 64 * kRotWaves, lds, s>>>(a);
 }
 
 template <typename T>
 void launch(const RotaryArgs& a, hipStream_t s) {
-  const unsigned blocks = (unsigned)((a.n * a.parts + kRotWaves - 1) / kRotWaves);
+  const dim3 blocks((unsigned)((a.n + kRotWaves - 1) / kRotWaves), a.parts);
   const size_t lds = (size_t)kRotWaves * 2 * a.pairs * sizeof(float);
-  if (a.D <= 64) rotary_kernel<T, 8><<<blocks, 64 * kRotWaves, lds, s>>>(a);
-  else if (a.D <= 128) rotary_kernel<T, 16><<<blocks, 64 * kRotWaves, lds, s>>>(a);
-  else if (a.D <= 256) rotary_kernel<T, 32><<<blocks, 64 * kRotWaves, lds, s>>>(a);
-  else rotary_kernel<T, 64><<<blocks, 64 * kRotWaves, lds, s>>>(a);
+  if (a.D <= 64) launch_lanes<T, 8>(a, blocks, lds, s);
+  else if (a.D <= 128) launch_lanes<T, 16>(a, blocks, lds, s);
+  else if (a.D <= 256) launch_lanes<T, 32>(a, blocks, lds, s);
+  else launch_lanes<T, 64>(a, blocks, lds, s);
 }
 
 }  // namespace
@@ -205,7 +256,9 @@ extern "C" int qq_qk_norm_rotary(const void* q, int64_t q_stride, const void* k,
   const int heads = num_q_heads + (v ? 2 : 1) * kv_heads;
   const int step = 64 / (head_dim <= 64 ? 8 : head_dim <= 128 ? 16 : head_dim <= 256 ? 32 : 64);  // heads a wave has at once
   const int rounds = (heads + step - 1) / step;
-  a.parts = (int)min((int64_t)rounds, max((int64_t)1, 4096 / n));
+  // as many waves as the chip has SIMDs, where there are fewer tokens (512 tokens of 32 + 8 heads in 2 parts 6.9 us, in 1
+  // 9.2, in 8 9.1; 128 in 8 parts 5.0, in 2 or 10 6.3)
+  a.parts = (int)min((int64_t)rounds, max((int64_t)1, 1024 / n));
   a.per = (rounds + a.parts - 1) / a.parts * step;
   a.parts = (heads + a.per - 1) / a.per;
   hipStream_t s = static_cast<hipStream_t>(stream);

@@ -84,6 +84,9 @@ class QKNormRotary:
         self._quarters = (freq * (2.0 / math.pi)).to(self.device)
         self._axis = torch.tensor(_deal(left, section_order == "cycled"), dtype=torch.int32, device=self.device)
         self._weights = [self._weight(w, what) for w, what in ((q_weight, "q_weight"), (k_weight, "k_weight"))]
+        # what every call passes, of tensors that stay where they are
+        self._args = (*(_lib.ptr(w) for w in self._weights), self.eps, _lib.ptr(self._quarters), _lib.ptr(self._axis), count,
+                      int(self.neighbours))
 
     def _weight(self, w: torch.Tensor | None, what: str) -> torch.Tensor | None:
         if w is None:
@@ -94,61 +97,59 @@ class QKNormRotary:
 
     def __call__(self, qkv: torch.Tensor, positions: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """``qkv [n, (num_heads + 2 kv_heads) * head_dim]``, a token's query heads, key heads and value heads in a
-        row, at ``positions`` -> ``q [n, num_heads, head_dim]``, ``k`` and ``v [n, kv_heads, head_dim]``, dense (v as it
-        was)."""
+        row, at ``positions`` (``[n]``, or ``[axes, n]``) -> ``q [n, num_heads, head_dim]``, ``k`` and ``v [n, kv_heads,
+        head_dim]``, dense (v as it was)."""
         h, kv, dim = self.num_heads, self.kv_heads, self.head_dim
         if qkv.dim() != 2 or qkv.shape[1] != (h + 2 * kv) * dim:
             raise ValueError(f"qkv must be [n, ({h} + 2 * {kv}) * {dim}], got {tuple(qkv.shape)}")
-        return self._run(qkv[:, : h * dim], qkv[:, h * dim : (h + kv) * dim], qkv[:, (h + kv) * dim :], positions)
+        qkv, ptr, stride, size = self._rows(qkv)
+        n, step = qkv.shape[0], dim * size
+        return self._launch((ptr, stride, ptr + h * step, stride, ptr + (h + kv) * step, stride), qkv.dtype, n, positions, 3)
 
     def apply(self, q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """``q [n, num_heads, head_dim]`` and ``k [n, kv_heads, head_dim]`` (or with the heads in a row) at
         ``positions``, as new dense tensors."""
-        out = []
+        rows, args = [], []
         for x, heads, what in ((q, self.num_heads, "q"), (k, self.kv_heads, "k")):
             if x.dim() == 3 and x.shape[1:] == (heads, self.head_dim):
                 # a view wherever a token's heads lie in a row
                 x = x.reshape(x.shape[0], heads * self.head_dim)
             if x.dim() != 2 or x.shape[1] != heads * self.head_dim:
                 raise ValueError(f"{what} must be [n, {heads}, {self.head_dim}], got {tuple(x.shape)}")
-            out.append(x)
-        return self._run(out[0], out[1], None, positions)[:2]
+            x, ptr, stride, _ = self._rows(x)
+            rows.append(x)
+            args += [ptr, stride]
+        if rows[0].shape[0] != rows[1].shape[0] or rows[0].dtype != rows[1].dtype:
+            raise ValueError("q and k differ in tokens or type")
+        return self._launch((*args, None, 0), rows[0].dtype, rows[0].shape[0], positions, 2)
 
-    def _run(self, q, k, v, positions):
-        n, dev, dt = q.shape[0], self.device, q.dtype
-        code = _lib.dtype_code(dt)
-        rows = []
-        for x in (q, k, v):
-            if x is None:
-                rows.append((None, 0))
-                continue
-            if x.device != dev:
-                raise ValueError(f"the heads lie on {x.device}, the weights and frequencies on {dev}")
-            if x.shape[0] != n or x.dtype != dt:
-                raise ValueError("q and k differ in tokens or type")
-            if x.requires_grad and torch.is_grad_enabled():
-                raise RuntimeError("QKNormRotary computes no gradients: detach its inputs or call it under torch.no_grad()")
-            step = 16 // x.element_size()
-            if x.stride(1) != 1 or x.data_ptr() % 16 or (n > 1 and (x.stride(0) % step or x.stride(0) < 0)):
-                x = x.clone(memory_format=torch.contiguous_format)
-            rows.append((x, x.stride(0) if n > 1 else x.shape[1]))
-        pos = positions
+    def _rows(self, x: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
+        """``x [n, width]`` with rows that the kernel takes: itself or a copy; its address, row stride and element size."""
+        if x.device != self.device:
+            raise ValueError(f"the heads lie on {x.device}, the weights and frequencies on {self.device}")
+        if x.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("QKNormRotary computes no gradients: detach its inputs or call it under torch.no_grad()")
+        size, (n, width), (stride, unit) = x.element_size(), x.shape, x.stride()
+        if n <= 1:
+            stride = width
+        if unit != 1 or x.data_ptr() % 16 or stride * size % 16 or stride < 0:
+            x, stride = x.clone(memory_format=torch.contiguous_format), width
+        return x, x.data_ptr(), stride, size
+
+    def _launch(self, rows: tuple, dtype: torch.dtype, n: int, pos: torch.Tensor, outputs: int) -> tuple[torch.Tensor, ...]:
+        dev, code = self.device, _lib.dtype_code(dtype)
         if pos.dtype.is_floating_point or pos.dtype == torch.bool:
             raise ValueError(f"positions must hold whole numbers, got {pos.dtype}")
         if pos.shape != ((n,) if self.axes == 1 and pos.dim() == 1 else (self.axes, n)):
             raise ValueError(f"positions must be [{self.axes}, {n}]{f' or [{n}]' if self.axes == 1 else ''}, got {tuple(pos.shape)}")
-        pos = pos.to(device=dev, dtype=torch.int64).contiguous()
-        outs = [torch.empty((n, heads, self.head_dim), dtype=dt, device=dev)
-                for heads in (self.num_heads, self.kv_heads, self.kv_heads)[: 2 if v is None else 3]]
-        wq, wk = self._weights
+        if pos.dtype != torch.int64 or pos.device != dev or not pos.is_contiguous():
+            pos = pos.to(device=dev, dtype=torch.int64).contiguous()
+        outs = tuple(torch.empty((n, heads, self.head_dim), dtype=dtype, device=dev)
+                     for heads in (self.num_heads, self.kv_heads, self.kv_heads)[:outputs])
         with _lib.on(dev):
-            _lib.call(
-                "qq_qk_norm_rotary", *(y for x, stride in rows for y in (_lib.ptr(x), stride)), code, self.num_heads,
-                self.kv_heads, self.head_dim, n, _lib.ptr(wq), _lib.ptr(wk), self.eps, _lib.ptr(self._quarters),
-                _lib.ptr(self._axis), self._axis.numel(), int(self.neighbours), _lib.ptr(pos), n, self.axes,
-                *(_lib.ptr(o) for o in outs), *([None] if v is None else []), _lib.stream(dev),
-            )
-        return outs if v is None else tuple(outs)
+            _lib.call("qq_qk_norm_rotary", *rows, code, self.num_heads, self.kv_heads, self.head_dim, n, *self._args,
+                      pos.data_ptr(), n, self.axes, *(o.data_ptr() for o in outs), *([None] * (3 - outputs)), _lib.stream(dev))
+        return outs
 
 
 def _deal(left: list[int], cycled: bool) -> list[int]:
