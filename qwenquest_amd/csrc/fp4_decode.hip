@@ -29,13 +29,13 @@ struct Fp4Unit {
   using Store = Fp4StoreArgs;
   struct BeginSmem {};
   static constexpr int kDim = D;
+  static constexpr bool kOneFactor = true;
   static constexpr int KW = D / 32, VL = D / 32;  // words a lane: of a token of K; 16-byte loads: of a block of V
   typedef uint32_t words_t __attribute__((ext_vector_type(KW)));
   words_t kr[4];
   uint32_t ks;         // scales of this lane's tokens 16 T + m
   u32x4_t vr[VL], vs;  // ... and of 16 T + 4 g + u
   u32x4_t v2[VL], vs2; // of a window's second block
-  float sl2;
 
   // lane group g's channels: of 128 a scale's 32, of 64 half of that
   static __device__ inline int channel(int i, int g) { return g * (D / 4) + i * 8; }
@@ -66,13 +66,12 @@ struct Fp4Unit {
   }
   __device__ inline void load_v(const Fp4Cache& c, int h, int lane, int blk) { load_values(c, h, lane, blk, vr, vs); }
   __device__ inline void load_window_v(const Fp4Cache& c, int h, int lane, int blk2) { load_values(c, h, lane, blk2, v2, vs2); }
-  __device__ inline void begin(int, bool, float scale) { sl2 = scale; }
+  __device__ inline void begin(int, bool, float) {}
   __device__ inline void keys(int t, int i, bf16x8_t& k0, bf16x8_t& k1) const {
     const float s = fp4_factor(ks, t);
     k0 = fp4_operand(kr[t][2 * i], s);
     k1 = fp4_operand(kr[t][2 * i + 1], s);
   }
-  __device__ inline float score(int, int) const { return sl2; }
   __device__ inline float weight(int t, int i, int, int) const { return fp4_factor(vs[t], i); }
   // bytes of word t whose tokens come from a window's second block
   static __device__ inline uint32_t window_mask(int t, int from2, int g) {

@@ -38,6 +38,7 @@ struct Fp8Unit {
   using Store = StoreArgs;
   using BeginSmem = StoreSmem<D>;
   static constexpr int kDim = D;
+  static constexpr bool kOneFactor = false;  // a block's scale is one
   static constexpr int KL = D / 64, VL = D / 16;  // 16-byte loads a lane: per 16 tokens of K, per block of V
   float ks = 0.0f, vs = 0.0f, ks2 = 0.0f, vs2 = 0.0f;  // of this lane's unit
   float kscale, vscale, kscale2, vscale2;              // of the unit at hand
@@ -82,7 +83,6 @@ struct Fp8Unit {
   }
   __device__ inline float score(int tok, int from2) const { return tok < from2 ? kscale2 : kscale; }
   __device__ inline float weight(int, int, int tok, int from2) const { return tok < from2 ? vscale2 : vscale; }
-  __device__ inline void merge_window_scales(int, int) {}  // weight tells them apart
   __device__ inline void merge_window(int from2, int g) {
 #pragma unroll
     for (int t = 0; t < 4; ++t) {

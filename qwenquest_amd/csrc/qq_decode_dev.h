@@ -32,10 +32,11 @@
 //   load_k(c, h, lane, blk, blk2, from2), load_v(c, h, lane, blk)
 //                                 codes of one unit; K's of tokens before from2 from blk2
 //   load_window_v(c, h, lane, blk2)   a window's second V, over K's registers
+//   kOneFactor                    whether all products take the factor sl2, and weights what weight(t, i, ..) says
 //   begin(j, win, sl2)            the factors of lane j's unit
 //   keys(t, i, k0, k1)            operands of steps 2 i and 2 i + 1 for tokens 16 t ..
-//   score(tok, from2), weight(t, i, tok, from2)   factors of a product and of a weight
-//   merge_window_scales(from2, g), merge_window(from2, g)   both V of a window in one, before weight and values
+//   score(tok, from2), weight(t, i, tok, from2)   factors of a product (without kOneFactor) and of a weight
+//   merge_window_scales(from2, g) (with kOneFactor, before weight), merge_window(from2, g)   both V of a window in one
 //   tile_of(st, x, y), place_of(x, y)   where the weight of element 2 x + y of step st lies in S^T
 //   values(i, st)                 operand of channels 16 i .. and step st
 //   store_tokens(st, i, on, h), BeginSmem, begin_blocks(st), begin_store<SRC>(st, smem, block)
@@ -421,6 +422,10 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attend_kernel(DecArgs<typen
     for (int i = 0; i < 2 * KS; ++i) {
       const int d = U::channel(i, g);
       load_query<QP>(a.q, (int64_t)b * a.q_bstride + (int64_t)(q_head + min(m16, rows - 1)) * D + d, m16 < rows, qf[i]);
+      if (U::kOneFactor && a.sl2 < 0.0f) {
+#pragma unroll
+        for (int p = 0; p < QP; ++p) qf[i][p] = -qf[i][p];
+      }
     }
   };
   // loads come back in order: the queries before the keys, the keys before the values
@@ -467,37 +472,94 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attend_kernel(DecArgs<typen
     if (win) unit.load_window_v(a.c, h, lane, __builtin_amdgcn_readlane(blk2, j));
     else if (!last && !next_set) load_k(j + 1);
     float mx = -INFINITY;
+    auto fold = [&](float alpha) {
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+      for (int i = 0; i < VL; ++i)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int tok = t * 16 + g * 4 + i;
-        s[t][i] = tok < hi ? s[t][i] * unit.score(tok, seq & 63) : -INFINITY;
-        mx = fmaxf(mx, s[t][i]);
+        for (int x = 0; x < 4; ++x) o[i][x] *= alpha;
+    };
+    if constexpr (U::kOneFactor) {
+      // every product takes the same factor, not negative here: the maximum is the products', and may lag by 8
+      const float sl2 = fabsf(a.sl2);
+      int left = hi - g * 4;  // a token 16 t + i is masked from here on
+      if (hi < 64) {
+        __asm__ volatile("" : "+v"(left));  // a branch, not selects in every unit
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[t][i] = t * 16 + i < left ? s[t][i] : -INFINITY;
       }
-    mx = fmaxf(mx, lane_xor16(mx, lane));
-    mx = fmaxf(mx, lane_xor32(mx, lane));
-    const float Mn = fmaxf(M, mx);
-    if (win) unit.merge_window_scales(seq & 63, g);
-    const float mb = Mn == -INFINITY ? 0.0f : Mn;
-    const float alpha = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - mb);
-    M = Mn;
-    float sum = 0.0f;
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float p = __builtin_amdgcn_exp2f(s[t][i] - mb);
-        sum += p;
-        // a masked token weighs nothing whatever its block's scale is
-        s[t][i] = s[t][i] == -INFINITY ? 0.0f : p * unit.weight(t, i, t * 16 + g * 4 + i, seq & 63);
+        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[t][i]);
+      mx = fmaxf(mx, lane_xor16(mx, lane));
+      mx = fmaxf(mx, lane_xor32(mx, lane)) * sl2;
+      if (__any(mx > M + 8.0f)) {
+        const float Mn = fmaxf(M, mx), alpha = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - Mn);
+        M = Mn;
+        L *= alpha;
+        fold(alpha);
       }
-    if (win) unit.merge_window(seq & 63, g);
-    L = L * alpha + sum;
+      if (win) unit.merge_window_scales(seq & 63, g);
+      const float mb = M == -INFINITY ? 0.0f : M;
 #pragma unroll
-    for (int i = 0; i < VL; ++i)
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) o[i][x] *= alpha;
+        for (int i = 0; i < 4; ++i) s[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], sl2, -mb));
+      if (hi < 64) {  // (a factor of 0 makes NaN of what is masked)
+        __asm__ volatile("" : "+v"(left));
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[t][i] = t * 16 + i < left ? s[t][i] : 0.0f;
+      }
+      float sum = 0.0f;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          sum += s[t][i];
+          s[t][i] *= unit.weight(t, i, 0, 0);
+        }
+      L += sum;
+      if (hi < 64) {  // a masked token weighs nothing whatever its scale is
+        __asm__ volatile("" : "+v"(left));
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[t][i] = t * 16 + i < left ? s[t][i] : 0.0f;
+      }
+      if (win) unit.merge_window(seq & 63, g);
+    } else {
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int tok = t * 16 + g * 4 + i;
+          s[t][i] = tok < hi ? s[t][i] * unit.score(tok, seq & 63) : -INFINITY;
+          mx = fmaxf(mx, s[t][i]);
+        }
+      mx = fmaxf(mx, lane_xor16(mx, lane));
+      mx = fmaxf(mx, lane_xor32(mx, lane));
+      const float Mn = fmaxf(M, mx);
+      const float mb = Mn == -INFINITY ? 0.0f : Mn;
+      const float alpha = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - mb);
+      M = Mn;
+      float sum = 0.0f;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float p = __builtin_amdgcn_exp2f(s[t][i] - mb);
+          sum += p;
+          // a masked token weighs nothing whatever its block's scale is
+          s[t][i] = s[t][i] == -INFINITY ? 0.0f : p * unit.weight(t, i, t * 16 + g * 4 + i, seq & 63);
+        }
+      if (win) unit.merge_window(seq & 63, g);
+      L = L * alpha + sum;
+      fold(alpha);
+    }
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
       bf16x8_t pw[PP];
