@@ -422,10 +422,6 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attend_kernel(DecArgs<typen
     for (int i = 0; i < 2 * KS; ++i) {
       const int d = U::channel(i, g);
       load_query<QP>(a.q, (int64_t)b * a.q_bstride + (int64_t)(q_head + min(m16, rows - 1)) * D + d, m16 < rows, qf[i]);
-      if (U::kOneFactor && a.sl2 < 0.0f) {
-#pragma unroll
-        for (int p = 0; p < QP; ++p) qf[i][p] = -qf[i][p];
-      }
     }
   };
   // loads come back in order: the queries before the keys, the keys before the values
@@ -479,22 +475,32 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attend_kernel(DecArgs<typen
         for (int x = 0; x < 4; ++x) o[i][x] *= alpha;
     };
     if constexpr (U::kOneFactor) {
-      // every product takes the same factor, not negative here: the maximum is the products', and may lag by 8
-      const float sl2 = fabsf(a.sl2);
+      // every product takes the same factor: the largest score is the largest product's or the smallest's, and the
+      // maximum may lag by 8
+      const float none = a.sl2 < 0.0f ? INFINITY : -INFINITY;
       int left = hi - g * 4;  // a token 16 t + i is masked from here on
       if (hi < 64) {
         __asm__ volatile("" : "+v"(left));  // a branch, not selects in every unit
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[t][i] = t * 16 + i < left ? s[t][i] : -INFINITY;
+          for (int i = 0; i < 4; ++i) s[t][i] = t * 16 + i < left ? s[t][i] : none;
       }
+      mx = none;
+      if (a.sl2 < 0.0f) {
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[t][i]);
+          for (int i = 0; i < 4; ++i) mx = fminf(mx, s[t][i]);
+      } else {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[t][i]);
+      }
+      mx *= a.sl2;
       mx = fmaxf(mx, lane_xor16(mx, lane));
-      mx = fmaxf(mx, lane_xor32(mx, lane)) * sl2;
+      mx = fmaxf(mx, lane_xor32(mx, lane));
       if (__any(mx > M + 8.0f)) {
         const float Mn = fmaxf(M, mx), alpha = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - Mn);
         M = Mn;
@@ -506,7 +512,7 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attend_kernel(DecArgs<typen
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], sl2, -mb));
+        for (int i = 0; i < 4; ++i) s[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], a.sl2, -mb));
       if (hi < 64) {  // (a factor of 0 makes NaN of what is masked)
         __asm__ volatile("" : "+v"(left));
 #pragma unroll
