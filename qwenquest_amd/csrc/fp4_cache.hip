@@ -2,6 +2,8 @@
 // MHATokenToKVPool.set_kv_buffer (reference src/qwenquest/memory.py:114-120) for blocks of e2m1
 // codes with scales of their own for every token, the rows back as values, and the page bounds of
 // QuestAlgorithm (src/qwenquest/quest.py:231-321) from the codes.
+#include <type_traits>
+
 #include "qq_fp4_store.h"
 #include "qq_fp8_plan.h"
 #include "qq_quest_dev.h"
@@ -168,8 +170,63 @@ struct Fp4PageArgs {
   PlanArgs plan;  // cu nullptr, or the step's division of the attention's work, by a block past the layers
 };
 
-// Min and max of a page's keys per channel, a wave per (page, head, layer): lane m + 16 g has 8
-// channels (those of byte 4 (g % 4) of each 16 bytes) of the tokens 16 T + m for every group of 32.
+// Pairs of channels as the page bounds compare them: in f16, the values relative to the largest scale (exact where the
+// scales lie within 2^22), or in fp32.
+__device__ inline f16x2_t fp4_two(uint32_t w, float s, int i, f16x2_t) {
+  switch (i) {
+    case 0: return __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 0);
+    case 1: return __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 1);
+    case 2: return __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 2);
+    default: return __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 3);
+  }
+}
+__device__ inline f32x2_t fp4_two(uint32_t w, float s, int i, f32x2_t) {
+  const uint32_t p = __builtin_bit_cast(uint32_t, fp4_pair(w, s, i));
+  return f32x2_t{__uint_as_float(p << 16), __uint_as_float(p & 0xFFFF0000u)};
+}
+template <int J>
+__device__ inline f16x2_t lane_xor_pair(f16x2_t v, int lane) {
+  return __builtin_bit_cast(f16x2_t, lane_xor_u32<J>(__builtin_bit_cast(uint32_t, v), lane));
+}
+template <int J>
+__device__ inline f32x2_t lane_xor_pair(f32x2_t v, int lane) {
+  return f32x2_t{__uint_as_float(lane_xor_u32<J>(__float_as_uint(v.x), lane)), __uint_as_float(lane_xor_u32<J>(__float_as_uint(v.y), lane))};
+}
+
+// Least and largest of 32 channels over the T tokens of each lane and the 16 lanes of a row: lane m ends with pair m.
+template <typename V, int T>
+__device__ inline void fp4_extremes(const u32x4_t (&w)[T], const float (&s)[T], int lane, V& least, V& largest) {
+  V mn[16], mx[16];
+#pragma unroll
+  for (int t = 0; t < T; ++t)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const V x = fp4_two(w[t][j >> 2], s[t], j & 3, V{});
+      mn[j] = t ? __builtin_elementwise_min(mn[j], x) : x;
+      mx[j] = t ? __builtin_elementwise_max(mx[j], x) : x;
+    }
+  auto fold = [&](auto step) {  // partner lane ^ J, each lane keeping half of its pairs
+    constexpr int J = decltype(step)::value;
+    const bool up = lane & J;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const V rn = lane_xor_pair<J>(up ? mn[j] : mn[j + J], lane), rx = lane_xor_pair<J>(up ? mx[j] : mx[j + J], lane);
+      mn[j] = __builtin_elementwise_min(up ? mn[j + J] : mn[j], rn);
+      mx[j] = __builtin_elementwise_max(up ? mx[j + J] : mx[j], rx);
+    }
+  };
+  fold(std::integral_constant<int, 8>{});
+  fold(std::integral_constant<int, 4>{});
+  fold(std::integral_constant<int, 2>{});
+  fold(std::integral_constant<int, 1>{});
+  least = mn[0];
+  largest = mx[0];
+}
+
+// Min and max of a page's keys per channel, a wave per (page, head, layer).  A lane reads 16 bytes, 32 channels that share
+// a scale, of tokens 16 T + m.  Codes times scales are compared two channels at a time in f16, as multiples of
+// the page's largest scale, or where scales lie further apart than f16 holds in fp32; the 16 tokens of a row of lanes are
+// folded in halves, each lane keeping half of its channels.
 template <int D>
 __global__ __launch_bounds__(256) void fp4_page_bounds_kernel(Fp4PageArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -195,58 +252,61 @@ __global__ __launch_bounds__(256) void fp4_page_bounds_kernel(Fp4PageArgs a) {
   }
   hi = min(hi, (int64_t)min(a.MP, a.table_cols));
   const int64_t units = (hi - lo) * a.KV;
-  const int m = lane & 15, g = lane >> 4;
+  // lane (m, g): of 128 channels group g, of 64 group g % 2 and half of the tokens
+  constexpr int T = D / 32;
+  const int m = lane & 15, g = lane >> 4, c = g % (D / 32), t0 = D == 128 ? 0 : (g >> 1) * 2;
   for (int64_t u = blockIdx.x * 4 + wave; u < units; u += gridDim.x * 4) {
     const int64_t page = lo + u / a.KV;
     const int h = (int)(u % a.KV);
     const int32_t blk = a.table[req * a.table_stride + page];
     const bool in = blk >= 0 && blk < a.blocks;
     const int64_t at = (int64_t)(in ? blk : 0) * a.KV + h;
-    const uint8_t* kp = a.kc + layer * a.kc_stride + at * (32 * D) + m * 16 + g * 4;
-    const uint8_t* sp = a.ks + layer * a.ks_stride + at * (2 * D) + m * 4;
-    uint32_t w[4][D / 32], e[D / 32];
+    const uint8_t* kp = a.kc + layer * a.kc_stride + at * (32 * D) + ((t0 * (D / 32) + c) * 16 + m) * 16;
+    const uint32_t e = *reinterpret_cast<const uint32_t*>(a.ks + layer * a.ks_stride + at * (2 * D) + (c * 16 + m) * 4) >> (8 * t0);
+    u32x4_t w[T];
 #pragma unroll
-    for (int c = 0; c < D / 32; ++c) {
-      e[c] = *reinterpret_cast<const uint32_t*>(sp + c * 64);
+    for (int t = 0; t < T; ++t) w[t] = *reinterpret_cast<const u32x4_t*>(kp + t * (D / 32) * 256);
+    uint32_t top = 0, low = 255;  // scales of the page's channels here
 #pragma unroll
-      for (int T = 0; T < 4; ++T) w[T][c] = *reinterpret_cast<const uint32_t*>(kp + (T * (D / 32) + c) * 256);
+    for (int t = 0; t < T; ++t) {
+      top = max(top, e >> (8 * t) & 255u);
+      low = min(low, e >> (8 * t) & 255u);
     }
-    uint32_t* out = a.bounds + (((int64_t)layer * a.R + req) * a.MP + page) * (a.KV * D) + h * D;
+    auto over = [&](auto step) {
+      constexpr int J = decltype(step)::value;
+      top = max(top, lane_xor_u32<J>(top, lane));
+      low = min(low, lane_xor_u32<J>(low, lane));
+    };
+    over(std::integral_constant<int, 1>{});
+    over(std::integral_constant<int, 2>{});
+    over(std::integral_constant<int, 4>{});
+    over(std::integral_constant<int, 8>{});
+    if (D == 64) over(std::integral_constant<int, 32>{});
+    float s[T];
+    f32x2_t least, largest;
+    if (__any(top != kFp4Lost && top - low > 22)) {
 #pragma unroll
-    for (int c = 0; c < D / 32; ++c) {
-      float mn[8], mx[8];
-      bool lost = !in;
+      for (int t = 0; t < T; ++t) s[t] = fp4_factor(e, t);
+      fp4_extremes<f32x2_t, T>(w, s, lane, least, largest);
+    } else {
 #pragma unroll
-      for (int T = 0; T < 4; ++T) {
-        lost |= ((e[c] >> (8 * T)) & 255u) == kFp4Lost;
-        const float f = fp4_factor(e[c], T);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t p = __builtin_bit_cast(uint32_t, fp4_pair(w[T][c], f, i));
-          const float x = __uint_as_float(p << 16), y = __uint_as_float(p & 0xFFFF0000u);
-          mn[2 * i] = T ? fminf(mn[2 * i], x) : x;
-          mx[2 * i] = T ? fmaxf(mx[2 * i], x) : x;
-          mn[2 * i + 1] = T ? fminf(mn[2 * i + 1], y) : y;
-          mx[2 * i + 1] = T ? fmaxf(mx[2 * i + 1], y) : y;
-        }
-      }
-      // over the 16 tokens of a row of lanes, in halves, each lane keeping half of its channels
-#pragma unroll
-      for (int half = 4; half >= 1; half >>= 1) {  // partner lane ^ 2 * half
-        const bool up = lane & (2 * half);
-#pragma unroll
-        for (int j = 0; j < half; ++j) {
-          const float rn = __shfl_xor(up ? mn[j] : mn[j + half], 2 * half, 64), rx = __shfl_xor(up ? mx[j] : mx[j + half], 2 * half, 64);
-          mn[j] = fminf(up ? mn[j + half] : mn[j], rn);
-          mx[j] = fmaxf(up ? mx[j + half] : mx[j], rx);
-        }
-      }
-      const float n = fminf(mn[0], __shfl_xor(mn[0], 1, 64)), x = fmaxf(mx[0], __shfl_xor(mx[0], 1, 64));
-      lost = __any(lost);
-      // lane pair (m, m ^ 1) has channel 8 g + (m / 2 with its bits in the order of the halves)
-      const uint32_t word = lost ? 0x7FC07FC0u : (uint32_t)f2bf(n) | ((uint32_t)f2bf(x) << 16);
-      if ((lane & 1) == 0) out[c * 32 + g * 8 + (lane & 8 ? 4 : 0) + (lane & 4 ? 2 : 0) + (lane & 2 ? 1 : 0)] = word;
+      for (int t = 0; t < T; ++t) s[t] = __uint_as_float(((e >> (8 * t) & 255u) + 127u - top) << 23);
+      f16x2_t n, x;
+      fp4_extremes<f16x2_t, T>(w, s, lane, n, x);
+      const float f = __uint_as_float(top << 23);
+      least = f32x2_t{(float)n.x * f, (float)n.y * f};
+      largest = f32x2_t{(float)x.x * f, (float)x.y * f};
     }
+    if (D == 64) {
+      least = __builtin_elementwise_min(least, lane_xor_pair<32>(least, lane));
+      largest = __builtin_elementwise_max(largest, lane_xor_pair<32>(largest, lane));
+      if (lane >= 32) continue;
+    }
+    const bool lost = !in || top == kFp4Lost;
+    const uint2 words = make_uint2((uint32_t)f2bf(least.x) | ((uint32_t)f2bf(largest.x) << 16),
+                                   (uint32_t)f2bf(least.y) | ((uint32_t)f2bf(largest.y) << 16));
+    *reinterpret_cast<uint2*>(a.bounds + (((int64_t)layer * a.R + req) * a.MP + page) * (a.KV * D) + h * D + c * 32 + m * 2) =
+        lost ? make_uint2(0x7FC07FC0u, 0x7FC07FC0u) : words;
   }
 }
 
