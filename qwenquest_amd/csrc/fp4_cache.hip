@@ -324,6 +324,7 @@ int check_cache(const Fp4Cache& c, const char* what) {
 
 using namespace qq;
 
+constexpr int64_t kMaxEntries = ((int64_t)1 << 30) - 64;  // a launch holds fewer than 2^32 threads, 256 for 64 entries
 constexpr int64_t kRunEntries = 16384;  // entries times heads from which runs are stored and read together
 
 extern "C" int qq_fp4_store(uint8_t* k_codes, uint8_t* v_codes, uint8_t* k_scale, uint8_t* v_scale, int num_blocks,
@@ -334,7 +335,7 @@ extern "C" int qq_fp4_store(uint8_t* k_codes, uint8_t* v_codes, uint8_t* k_scale
   const int st = check_cache(a.c, what);
   if (st != QQ_OK) return st;
   QQ_REQUIRE(dtype_ok(src_dtype), "%s: bad dtype", what);
-  QQ_REQUIRE(n >= 0 && n < (int64_t)1 << 30, "%s: bad sizes", what);
+  QQ_REQUIRE(n >= 0 && n <= kMaxEntries, "%s: bad sizes", what);
   if (n == 0) return QQ_OK;
   QQ_REQUIRE(k && v && loc, "%s: null pointer", what);
   QQ_REQUIRE(((uintptr_t)k | (uintptr_t)v) % 16 == 0, "%s: k and v must be 16-byte aligned", what);
@@ -371,7 +372,7 @@ extern "C" int qq_fp4_rows(const uint8_t* k_codes, const uint8_t* v_codes, const
   const int st = check_cache(c, what);
   if (st != QQ_OK) return st;
   QQ_REQUIRE(dtype_ok(dst_dtype), "%s: bad dtype", what);
-  QQ_REQUIRE(n >= 0 && n < (int64_t)1 << 30, "%s: bad sizes", what);
+  QQ_REQUIRE(n >= 0 && n <= kMaxEntries, "%s: bad sizes", what);
   if (n == 0) return QQ_OK;
   QQ_REQUIRE(loc && k && v, "%s: null pointer", what);
   hipStream_t s = static_cast<hipStream_t>(stream);

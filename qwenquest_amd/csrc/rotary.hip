@@ -242,7 +242,8 @@ extern "C" int qq_qk_norm_rotary(const void* q, int64_t q_stride, const void* k,
              kv_heads);
   QQ_REQUIRE(pairs >= 0 && 2 * pairs <= head_dim && pairs % (neighbours ? 4 : 8) == 0,
              "%s: %d pairs of %d channels, in multiples of %d", what, pairs, head_dim, neighbours ? 4 : 8);
-  QQ_REQUIRE(n >= 0 && n < (int64_t)1 << 28 && axes > 0, "%s: bad sizes", what);
+  // (a launch holds fewer than 2^32 threads, 64 a token)
+  QQ_REQUIRE(n >= 0 && n < ((int64_t)1 << 26) - kRotWaves && axes > 0, "%s: bad sizes", what);
   if (n == 0) return QQ_OK;
   QQ_REQUIRE(q && k && q_out && k_out && (!v || v_out) && (pairs == 0 || (quarter_turns && pair_axis && positions)),
              "%s: null pointer", what);

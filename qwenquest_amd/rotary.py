@@ -10,6 +10,7 @@ import math
 from collections.abc import Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from qwenquest_amd import _lib
 from qwenquest_amd.paged import _indexed
@@ -127,7 +128,7 @@ class QKNormRotary:
         """``x [n, width]`` with rows that the kernel takes: itself or a copy; its address, row stride and element size."""
         if x.device != self.device:
             raise ValueError(f"the heads lie on {x.device}, the weights and frequencies on {self.device}")
-        if x.requires_grad and torch.is_grad_enabled():
+        if (x.requires_grad and torch.is_grad_enabled()) or forward_ad.unpack_dual(x).tangent is not None:
             raise RuntimeError("QKNormRotary computes no gradients: detach its inputs or call it under torch.no_grad()")
         size, (n, width), (stride, unit) = x.element_size(), x.shape, x.stride()
         if n <= 1:

@@ -119,6 +119,15 @@ def test_rotary_refuses(lib, kw, said):  # noqa: F811
     refused(lib.qq_qk_norm_rotary(*a.values(), None), lib, said)
 
 
+def test_no_launch_past_2_32_threads(lib):  # noqa: F811
+    n = (1 << 30) - 63  # 2^24 blocks of 256
+    refused(lib.qq_fp4_store(*{**CACHE, **dict(k=FAKE, v=FAKE, dtype=0, loc=FAKE, n=n)}.values(), None), lib, b"bad sizes")
+    refused(lib.qq_fp4_rows(*{**CACHE, **dict(loc=FAKE, n=n, k=FAKE, v=FAKE, dtype=0)}.values(), None), lib, b"bad sizes")
+    a = dict(q=FAKE, qs=8, k=FAKE, ks=8, v=None, vs=0, dtype=0, H=1, KV=1, dim=8, n=(1 << 26) - 4, wq=None, wk=None, eps=1e-6, turns=None,
+             axis=None, pairs=0, neighbours=0, pos=None, ps=0, axes=1, qo=FAKE, ko=FAKE, vo=None)
+    refused(lib.qq_qk_norm_rotary(*a.values(), None), lib, b"bad sizes")
+
+
 def test_nothing_to_do(lib):  # noqa: F811
     assert lib.qq_fp4_store(*{**CACHE, **dict(k=None, v=None, dtype=0, loc=None, n=0)}.values(), None) == _lib.QQ_OK
     assert lib.qq_fp4_decode_workspace_bytes(0, 32, 4, 128) == 0 == lib.qq_fp4_decode_workspace_bytes(2, 30, 4, 128)

@@ -207,6 +207,18 @@ def test_what_is_refused(cuda):
         op(x.clone().requires_grad_(), pos)
 
 
+def test_a_tangent_is_refused(cuda):
+    op = QKNormRotary(2, 1, 64, device=cuda)
+    x, pos = torch.zeros(3, 256, device=cuda), torch.zeros(3, dtype=torch.int64, device=cuda)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(RuntimeError, match="no gradients"):
+            op(dual, pos)
+        with pytest.raises(RuntimeError, match="no gradients"):
+            op.apply(dual[:, :128], x[:, 128:192], pos)
+        op(x, pos)
+
+
 def test_captured_and_on_another_stream(cuda):
     w = torch.rand(128, device=cuda) + 0.5
     op = QKNormRotary(8, 2, 128, q_weight=w, k_weight=w, base=1e6, device=cuda)
