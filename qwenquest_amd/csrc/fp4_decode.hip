@@ -111,6 +111,13 @@ struct Fp4Unit {
   }
 };
 
+// Where a layer selects in its attention (selects_itself).  Of several requests a slice may select twice, and the reading
+// behind a selection is half of the 8-bit cache's: a layer-step in two launches and in three, us, contexts of 32768
+// tokens, 32 heads on 4 (64 on 8; 8 on 1): 1 request, 31 pages 17.6, 18.3 (19.5, 20.3; 18.0, 18.7); 40 pages 17.3, 18.9 (19.5,
+// 21.0; 17.1, 19.1); 63 pages 26.1, 22.2.  16 requests, 31 pages 26.4, 27.2 (33.4, 34.4; 22.9, 23.0); 36 pages 34.2, 33.2 (39.3,
+// 39.3; 27.8, 26.7); 40 pages 37.1, 33.3.  4 and 40 requests: 31 pages 0.4 less to 0.8 more, 40 pages 0.1 to 3.8 more.
+inline int self_pages(int bs) { return bs == 1 ? 40 : 32; }
+
 }  // namespace
 }  // namespace qq
 
@@ -212,7 +219,7 @@ extern "C" int qq_fp4_quest_step(const void* q, int q_dtype, int64_t q_batch_str
   hipStream_t s = static_cast<hipStream_t>(stream);
   // the new tokens may go in with the attention: pages that are selected are complete, a new token's is not
   const bool one = planned && phase != 1 && a.tiles == 1;
-  if (one && phase == 3 && selects_itself(a, sel, q_dtype)) {
+  if (one && phase == 3 && selects_itself(a, sel, q_dtype, self_pages(bs))) {
     const int scored = launch_score(sel, bs, false, s);
     if (scored != QQ_OK) return scored;
     launch_selecting<Fp4Unit<128>>(a, st, sel, s);

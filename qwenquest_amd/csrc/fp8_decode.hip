@@ -113,6 +113,14 @@ struct Fp8Unit {
   }
 };
 
+// Where a layer selects in its attention (selects_itself): a layer-step in two launches and in
+// three, us, 32 heads on 4, contexts of 32768 tokens unless said: 1 request, 31 pages 16.6, 18.9; 12:
+// 26.4, 28.1; 40: 43.3, 45.4; 63: 47.7, 51.4; 12 of 131072: 33.7, 35.5; 40 pages, 1 request 17.1, 19.9; 7:
+// 24.9, 26.5; 63: 56.5, 58.9; 42 pages, 7 requests 28.4, 26.6; 63 pages, 1: 24.9, 23.2; 64 pages, 16: 53.9,
+// 46.7.  In tables of 4097 pages: 44 pages, 1 of 262144 tokens 22.9, 52.0; 64 pages, 12: 44.1, 52.5; 63:
+// 107, 104.
+constexpr int kSelfPages = 40;
+
 }  // namespace
 }  // namespace qq
 
@@ -213,7 +221,7 @@ extern "C" int qq_fp8_quest_step(const void* q, int q_dtype, int64_t q_batch_str
   sel.scores = scores_ws;
   sel.positions = positions;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (planned && phase == 3 && selects_itself(a, sel, q_dtype)) {
+  if (planned && phase == 3 && selects_itself(a, sel, q_dtype, kSelfPages)) {
     const int scored = launch_score_codes(sel, bs, a.c, k_new, v_new, new_dtype, out_cache_loc, s);
     if (scored < 0) return scored;
     if (scored == QQ_OK) {

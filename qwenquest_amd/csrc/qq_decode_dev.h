@@ -771,18 +771,14 @@ void launch_decode(const DecArgs<typename U::Cache>& a, const typename U::Store&
 //
 // Every block of a request repeats its selection, which is dear once more than a wave's 64 pages pass
 // its filter (the k-th largest of 64 groups' maxima: 64 ln(64 / (64 - k)) pages, 64 of them from
-// k = 40 on), where a launch for it does it once: two launches are taken up to that, and past the 4096
-// pages that a begin launch can select of, which takes four.  A layer-step in two launches and in
-// three, us, 32 heads on 4, contexts of 32768 tokens unless said: 1 request, 31 pages 16.6, 18.9; 12:
-// 26.4, 28.1; 40: 43.3, 45.4; 63: 47.7, 51.4; 12 of 131072: 33.7, 35.5; 40 pages, 1 request 17.1, 19.9; 7:
-// 24.9, 26.5; 63: 56.5, 58.9; 42 pages, 7 requests 28.4, 26.6; 63 pages, 1: 24.9, 23.2; 64 pages, 16: 53.9,
-// 46.7.  In tables of 4097 pages: 44 pages, 1 of 262144 tokens 22.9, 52.0; 64 pages, 12: 44.1, 52.5; 63:
-// 107, 104.
+// k = 40 on), where a launch for it does it once: two launches are taken up to `most` pages, which
+// depends on what the attention costs besides, and to 64 past the 4096 pages that a begin launch can
+// select of, which takes four.
 template <typename Args>
-bool selects_itself(const Args& a, const SelectArgs& sel, int q_dtype) {
+bool selects_itself(const Args& a, const SelectArgs& sel, int q_dtype, int most) {
   const int n = max(sel.MP, sel.k_sel);
   return q_dtype == QQ_DTYPE_BF16 && a.c.D == 128 && a.tiles == 1 && a.bs <= a.max_slices && sel.top_k >= 8 * 64 &&
-         sel.k_sel <= (n <= kBeginPages ? 40 : 64) && sel.MP > 0 && n <= 16 * 64 * kDecWaves &&
+         sel.k_sel <= (n <= kBeginPages ? most : 64) && sel.MP > 0 && n <= 16 * 64 * kDecWaves &&
          (int64_t)a.table_cols * kCacheTokens > sel.top_k;
 }
 
