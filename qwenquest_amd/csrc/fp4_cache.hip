@@ -325,7 +325,13 @@ int check_cache(const Fp4Cache& c, const char* what) {
 using namespace qq;
 
 constexpr int64_t kMaxEntries = ((int64_t)1 << 30) - 64;  // a launch holds fewer than 2^32 threads, 256 for 64 entries
-constexpr int64_t kRunEntries = 16384;  // entries times heads from which runs are stored and read together
+// Values (of K, entries x heads x channels) from which runs of entries are stored, and read, together.  Entries one by one
+// and in runs, us, 128 channels, a prompt's run that begins inside a block (six such; a block for every entry): stored,
+// 8192 entries and heads 6.9 (6.9; 7.9) and 7.7 (8.1; 14); 13760 9.9 (9.8; 11) and 8.2 (8.6; 18); 131072 59 (57; 25)
+// and 22 (23; 31): prompts come in runs, and a decode step's entries go in with its attention.  Of 64 channels, 16384 6.9 (7.3)
+// and 7.6 (10.7); 24576 9.1 (8.9) and 8.7 (12.3); 32768 11.1 (11.1) and 9.5 (9.8).  Read, six runs, 32768 8.4 and 8.4 to 10; 49152 12 and 10; 131072 24 and 18;
+// of 64 channels 65536 8.6 and 9.3, 131072 14.3 and 11.7.
+constexpr int64_t kStoreValues = (int64_t)3 << 19, kRowValues = (int64_t)6 << 20;
 
 extern "C" int qq_fp4_store(uint8_t* k_codes, uint8_t* v_codes, uint8_t* k_scale, uint8_t* v_scale, int num_blocks,
                             int kv_heads, int head_dim, const void* k, const void* v, int src_dtype, const int64_t* loc,
@@ -341,7 +347,7 @@ extern "C" int qq_fp4_store(uint8_t* k_codes, uint8_t* v_codes, uint8_t* k_scale
   QQ_REQUIRE(((uintptr_t)k | (uintptr_t)v) % 16 == 0, "%s: k and v must be 16-byte aligned", what);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool bf = src_dtype == QQ_DTYPE_BF16;
-  if (n * kv_heads >= kRunEntries) {
+  if (n * kv_heads * head_dim >= kStoreValues) {
     const dim3 grid((unsigned)((n + 63) / 64), kv_heads);
     if (head_dim == 128) {
       if (bf) fp4_store_runs_kernel<128, uint16_t><<<grid, 256, 0, s>>>(a);
@@ -379,7 +385,7 @@ extern "C" int qq_fp4_rows(const uint8_t* k_codes, const uint8_t* v_codes, const
   uint16_t *kb = static_cast<uint16_t*>(k), *vb = static_cast<uint16_t*>(v);
   float *kf = static_cast<float*>(k), *vf = static_cast<float*>(v);
   const bool bf = dst_dtype == QQ_DTYPE_BF16;
-  if (n * kv_heads >= kRunEntries) {
+  if (n * kv_heads * head_dim >= kRowValues) {
     const dim3 grid((unsigned)((n + 63) / 64), kv_heads);
     if (head_dim == 128) {
       if (bf) fp4_rows_runs_kernel<128><<<grid, 256, 0, s>>>(c, loc, n, kb, vb);

@@ -63,6 +63,34 @@ def test_scattered_blocks(cuda, n):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("kv, dim, blocks", [(4, 128, 400), (8, 64, 400), (1, 128, 1200), (3, 64, 800)])
+def test_many_entries_at_once(cuda, kv, dim, blocks, dtype):
+    """Over a pool, all at once: whole blocks, pieces of them, single rows and rows that are not there, in any order."""
+    rng = np.random.default_rng(blocks + dim)
+    pool, cache = Fp4TokenToKVPool(blocks, 1, kv, dim, cuda), o4.Cache(blocks, kv, dim)
+    for step in range(2):
+        pieces = []
+        for b in rng.permutation(np.arange(1, blocks)):
+            lo, hi = sorted(rng.integers(0, 65, 2)) if rng.random() < 0.3 else (0, 64)
+            one = b * 64 + np.arange(lo, hi)
+            pieces.append(one if rng.random() < 0.7 else rng.permutation(one)[: rng.integers(1, 65)])
+            if rng.random() < 0.1:
+                pieces.append(np.array([-1, blocks * 64, 5, 1 << 40]))  # outside the pool, and padding
+        rows = np.concatenate(pieces)
+        assert len(rows) * kv * dim > 1 << 21
+        k, v = values(rng, len(rows), kv, dim, dtype), values(rng, len(rows), kv, dim, dtype)
+        pool.set_kv_buffer(0, i64(rows, cuda), k.to(cuda), v.to(cuda))
+        cache.write(rows, k.double().numpy(), v.double().numpy())
+        everything = np.arange(pool.rows)
+        while len(everything) * kv * dim < 7 << 20:
+            everything = np.concatenate([everything, everything])
+        same(pool, cache, rows=everything)
+        same(pool, cache, rows=rng.permutation(everything))
+        same(pool, cache, rows=everything[13:-29])
+    assert not pool.k_codes[0, 0].any() and not pool.v_codes[0, 0].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_every_border_and_size(cuda, dtype):
     """Values at and next to the borders between codes, at every exponent, the largest and the least."""
     steps = torch.tensor([0.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 6.5, 7.0, 0.5, 1.0, 1.5, 2.0, 3.0], dtype=torch.float64)
