@@ -2,6 +2,12 @@
 // MHATokenToKVPool.set_kv_buffer (reference src/qwenquest/memory.py:114-120) for blocks of e2m1
 // codes with scales of their own for every token, the rows back as values, and the page bounds of
 // QuestAlgorithm (src/qwenquest/quest.py:231-321) from the codes.
+//
+// Bound: HBM where entries are many: 47921 tokens, 8 heads of 128 in bf16, stored in 51 to 67 us (196 MB read and 51
+// written, of which half is in the caches; 456 entry by entry, whose V writes are single bytes), 47971 rows back in 43 us (248 MB, 5.8 TB/s);
+// page bounds of two prompts of 16384 tokens, 4 heads of 128, 48 layers 113 us (4.2 TB/s), where the vector
+// units have the rest (343 with 4-byte loads and comparisons in fp32).  Few entries are a chain of two round trips behind a launch: 32 tokens
+// stored in 3.7 us, 1181 rows in 4.1.
 #include <type_traits>
 
 #include "qq_fp4_store.h"
@@ -18,8 +24,8 @@ __global__ __launch_bounds__(256) void fp4_store_kernel(Fp4StoreArgs a) {
   fp4_store_group<D, SRC>(a, i, i < a.n, (int)(item - i * a.c.KV));
 }
 
-// Runs of entries of one block, a segment of 64 entries and a head a thread block; where more than 8 runs begin in
-// the segment, they go entry by entry.
+// Runs of entries of one block, a segment of 64 entries and a head a thread block.  Runs go one after the other, a round trip
+// each; where more than 8 begin in the segment, they go entry by entry, 8 at a time.
 template <int D, typename SRC>
 __global__ __launch_bounds__(2 * D) void fp4_store_runs_kernel(Fp4StoreArgs a) {
   __shared__ int from[64];
@@ -328,9 +334,9 @@ constexpr int64_t kMaxEntries = ((int64_t)1 << 30) - 64;  // a launch holds fewe
 // Values (of K, entries x heads x channels) from which runs of entries are stored, and read, together.  Entries one by one
 // and in runs, us, 128 channels, a prompt's run that begins inside a block (six such; a block for every entry): stored,
 // 8192 entries and heads 6.9 (6.9; 7.9) and 7.7 (8.1; 14); 13760 9.9 (9.8; 11) and 8.2 (8.6; 18); 131072 59 (57; 25)
-// and 22 (23; 31): prompts come in runs, and a decode step's entries go in with its attention.  Of 64 channels, 16384 6.9 (7.3)
-// and 7.6 (10.7); 24576 9.1 (8.9) and 8.7 (12.3); 32768 11.1 (11.1) and 9.5 (9.8).  Read, six runs, 32768 8.4 and 8.4 to 10; 49152 12 and 10; 131072 24 and 18;
-// of 64 channels 65536 8.6 and 9.3, 131072 14.3 and 11.7.
+// and 22 (23; 31): prompts come in runs, and a decode step's entries go in with its attention.  Of 64 channels, 16384
+// 6.9 (7.3) and 7.6 (10.7); 24576 9.1 (8.9) and 8.7 (12.3); 32768 11.1 (11.1) and 9.5 (9.8).  Read, six runs, 32768 8.4
+// and 8.4 to 10; 49152 12 and 10; 131072 24 and 18; of 64 channels 65536 8.6 and 9.3, 131072 14.3 and 11.7.
 constexpr int64_t kStoreValues = (int64_t)3 << 19, kRowValues = (int64_t)6 << 20;
 
 extern "C" int qq_fp4_store(uint8_t* k_codes, uint8_t* v_codes, uint8_t* k_scale, uint8_t* v_scale, int num_blocks,

@@ -19,6 +19,13 @@
 // half a step on average, 2^-10 / 2 over the significand's 1 .. 2, in the mean 0.72 * 2^-11.
 // A weight is off by 0.64 * 2^-10 at most, an output by that of sum p |v|, where its own rounding
 // is 2^-8 of it.
+//
+// Bound: the matrix cores, near the clock that they hold: 8192 tokens behind 8192, 32 heads on 4 of 128, 1555 to 1615 us (by
+// card): 36 matrix instructions a tile and wave are 1.19 PFLOP/s, where a plain product of 8192^3 reaches 1.225; of the
+// formula's 1.02 to 1.06.  E and 2^(1 - E) by lane exchanges instead of matrix instructions 1953; weights and products one
+// after the other 1690.  Not taken: the next tile's scores between this one's products (256 registers, 1693), three
+// blocks a CU with the queries in the LDS (1635), wave priorities (no change).  A short batch by its longest request's
+// tiles: 3440 new of 8330 tokens 174 us with the store.
 #include "qq_extend_dev.h"
 #include "qq_fp4.h"
 

@@ -26,7 +26,6 @@
 //
 // The policy U of a cache, one object a lane:
 //   kDim, Cache, Store            head size, the cache's and a store's arguments
-//   kKRegs, kVRegs ... in flight  its own registers
 //   channel(i, g)                 first of the 8 channels that step i's operands hold in lane group g
 //   look_up(c, h, blk, blk2, w)   of this lane's unit what there is one word of (w: also of blk2)
 //   load_k(c, h, lane, blk, blk2, from2), load_v(c, h, lane, blk)

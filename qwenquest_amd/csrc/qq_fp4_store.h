@@ -2,6 +2,10 @@
 // whole
 //   e = least with max |x| <= 7 * 2^e, of K's -96 .. 125, of V's -50 .. 59,  code = e2m1(x / 2^e),
 // to nearest even, 6 at most.  Of a row listed twice in a run of one block the last entry counts.
+//
+// A token's V is half bytes of D / 2 places (its byte at each holds two channels), a token's K 16 bytes at D / 32 places: a
+// token alone writes them so (fp4_store_group), the tokens of a run turn theirs between the lanes until 16 tokens of
+// two channels are a lane's 16 bytes (fp4_store_block; times: fp4_cache.hip).
 #pragma once
 
 #include "qq_fp4.h"
