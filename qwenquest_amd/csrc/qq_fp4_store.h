@@ -27,14 +27,14 @@ struct Fp4StoreArgs {
 };
 
 // Whether an entry after i in its run of one block has the same row, which is the one that counts then; by the
-// W lanes of i's group, as many entries at a time.
+// W lanes of i's group, as many entries at a time.  `next`: the row of this lane's first, i + 1 + its place in the group.
 template <int W>
-__device__ inline bool written_again(const Fp4StoreArgs& a, int64_t i, int64_t row, bool on) {
+__device__ inline bool written_again(const Fp4StoreArgs& a, int64_t i, int64_t row, int64_t next, bool on) {
   const int lane = threadIdx.x & 63, first = lane / W * W;
   constexpr uint64_t kGroup = (1ull << W) - 1ull;
   bool again = false;
   for (int64_t j = i + 1 + lane - first; __any(on); j += W) {
-    const int64_t other = on && j < a.n ? a.loc[j] : (int64_t)-1;
+    const int64_t other = on && j < a.n ? (j < i + 1 + W ? next : a.loc[j]) : (int64_t)-1;
     const uint64_t ends = __ballot(other >> 6 != row >> 6) >> first & kGroup;
     const uint64_t same = __ballot(other == row) >> first & kGroup;
     again |= on && (ends ? same & ((ends & -ends) - 1) : same) != 0;
@@ -52,11 +52,11 @@ __device__ inline void fp4_store_group(const Fp4StoreArgs& a, int64_t i, bool on
   const int lane = threadIdx.x & 63, dg = lane % DG;
   const bool isv = lane / DG & 1;
   if (!on) i = 0;
-  const int64_t row = a.loc[i];
+  const int64_t row = a.loc[i], next = a.loc[min(i + 1 + lane % (2 * DG), a.n - 1)];  // (in one round trip)
   Values8<SRC> in;
   in.load(isv ? a.v : a.k, (i * a.c.KV + h) * D + dg * 8);
   const int block = on ? block_of(row, a.c.blocks) : 0, t = (int)(row & 63);
-  const bool again = written_again<2 * DG>(a, i, row, block > 0), mine = block > 0 && !again;
+  const bool again = written_again<2 * DG>(a, i, row, next, block > 0), mine = block > 0 && !again;
   float x[8], m = 0.0f;
   bool bad = false;
 #pragma unroll
