@@ -175,3 +175,49 @@ def test_a_layer_from_its_qkv_product_on(cuda, backend):
         lens = [a + b for a, b in zip(lens, new)]
     assert max(lens) > 512
     rtp.check_errors()
+
+
+@pytest.mark.parametrize("kv, group, lens, top_k", [
+    (1, 8, [700 + 13 * i for i in range(256)], 512), (1, 16, [700] * 257, 512), (1, 1, [3000], 2112), (1, 5, [2600, 1, 2112, 2113, 64] * 20, 2112),
+    (2, 7, [600 + 5 * i for i in range(128)], 512), (2, 16, [5000, 100], 2112), (3, 4, [900 + 50 * i for i in range(85)], 832),
+    (8, 8, [1300, 40, 1024, 1025] * 8, 1024), (8, 2, [4000] * 3, 2176), (8, 4, [9000], 2624), (4, 8, [9000], 2688), (16, 4, [800] * 16, 576),
+    (64, 1, [700, 650, 600, 30], 512)])
+def test_a_divided_step_of_quest_with_any_number_of_kv_heads(cuda, kv, group, lens, top_k):
+    """As many requests as a slice may meet, selections up to the most that the attention makes itself and past it:
+    positions, cache and answers, to the bit, of the step whose selection is a launch of its own."""
+    dim, bs, width = 128, len(lens), max(lens) + 3
+    gen = torch.Generator(device=cuda).manual_seed(kv * bs)
+    rtp = BlockReqToTokenPool(bs, width, sum(n // 64 + 2 for n in lens) + 2, cuda)
+    kvp = Fp4TokenToKVPool(rtp.num_blocks, 1, kv, dim, cuda)
+    be = QuestOnlyBackend(rtp, kvp, {"algorithm": "quest", "top_k": top_k, "quest_page_size": 64})
+    reqs, had = torch.arange(bs, device=cuda), [n - 1 for n in lens]
+    total = sum(had)
+    loc, _ = rtp.assign(reqs, i64([0] * bs, cuda), i64(had, cuda), total)
+    pages = torch.randn(total // 64 + 1, kv, dim, device=cuda, generator=gen).repeat_interleave(64, 0)[:total]
+    kvp.set_kv_buffer(0, loc, pages + torch.randn(total, kv, dim, device=cuda, generator=gen),
+                      torch.randn(total, kv, dim, device=cuda, generator=gen))
+    be.quest.update_prefill_representations_blocks(reqs, i64(had, cuda), kvp, rtp.block_table)
+    seq = i64(lens, cuda)
+    for step in range(2):
+        loc, pos = rtp.assign_decode(reqs, seq)
+        batch = ForwardBatch(ForwardMode.DECODE, None, pos, reqs, seq, loc, rtp, kvp, be)
+        q, k, v = (torch.randn(bs, h, dim, device=cuda, generator=gen).bfloat16() for h in (group * kv, kv, kv))
+        if kv * dim > 1024:  # more channels than page scores are taken of
+            be.init_forward_metadata(batch)
+            with pytest.raises(ValueError, match="exceeds 1024"):
+                be.forward(q, k, v, engine.Layer(0, dim), batch)
+            return
+        if step:
+            q[:] = 0  # every page scores alike
+        be.init_forward_metadata(batch)
+        got = []
+        for planned in (True, False):
+            if not planned:
+                be.quest._step.plan = None
+            be._positions.fill_(-7)
+            out = be.forward(q, k, v, engine.Layer(0, dim), batch)
+            got.append([t.clone() for t in (out, be._positions, kvp.k_codes, kvp.v_codes, kvp.k_scale, kvp.v_scale)])
+        assert not got[0][0].isnan().any()
+        assert all(torch.equal(a, b) for a, b in zip(*got))
+        seq = seq + 1
+    rtp.check_errors()
