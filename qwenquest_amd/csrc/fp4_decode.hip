@@ -11,7 +11,7 @@
 // and waves waiting 40 %; 228 with the masks and rescalings in every unit.  A small batch by the chain of round trips, as
 // over the 8-bit cache: one request of 2000 tokens 11.1 us a layer (waiting 80 %), 48 of up to 20000 in fp32 23.0.
 // Quest, 16 requests' 31 pages and window of 131072 tokens 16.8 us with the selection.  Not taken: the next two
-// units in flight instead of one (registers spilt), rescaling in every unit without the branch (slower), the sign of a
+// units in flight instead of one (226 us where this took 214; fp32 spills), rescaling in every unit without the branch (slower), the sign of a
 // negative factor on the queries (3 % at one request: another step before the first product).
 #include "qq_decode_dev.h"
 #include "qq_fp4_store.h"
