@@ -13,12 +13,16 @@
 // into the product as
 //   w = 2^(t + E - N + 7),
 // which fills f16's range from the top (7 + 8); the weights' sum adds w 2^(1 - E), in fp32.  E and 2^(1 - E) of a lane's 32 tokens
-// come by matrix instructions, a step of K Q^T that holds them as channels.  V's exponents
-// span 109, so a token whose w underflows weighs less than 2^-24 of another one.  w goes to f16's
+// come by matrix instructions, a step of K Q^T that holds them as channels.  w goes to f16's
 // 11 bits by truncation (one instruction for two weights) of w (1 + 0.72 * 2^-11): truncation takes
 // half a step on average, 2^-10 / 2 over the significand's 1 .. 2, in the mean 0.72 * 2^-11.
-// A weight is off by 0.64 * 2^-10 at most, an output by that of sum p |v|, where its own rounding
-// is 2^-8 of it.
+// A weight from 2^-14 on is off by 0.64 * 2^-10 at most, an output by that of sum p |v|, where its own rounding
+// is 2^-8 of it; smaller ones are whole steps of 2^-24: each token is off by 2^-31 of the row's largest p 2^E at most, times a code
+// of up to 6, which shows in channels where the tokens that weigh most hold 0.  (A second f16 piece of the weights is another value
+// product: a third more time over the 8-bit cache, and the same error against 64 bits.)
+// The sum has no such end.  V's exponents span 109, so tokens that count in it by their number may lie below 2^-126 in w and in the
+// rescaling: that goes in two halves, and a tile with an E below kLowE, values under 2^-27, adds weights of their own, 2^kUp times as
+// large (then a token is missing only under 2^-88 of another one; above kLowE under 2^-44).
 //
 // Bound: the matrix cores, near the clock that they hold: 8192 tokens behind 8192, 32 heads on 4 of 128, 1555 to 1615 us (by
 // card): 36 matrix instructions a tile and wave are 1.19 PFLOP/s, where a plain product of 8192^3 reaches 1.225; of the
@@ -34,7 +38,8 @@ namespace {
 
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 
-constexpr int kLift = 7, kSlack = 8;  // w <= 2^(7 + 8) * kRound < f16's 65504
+constexpr int kLift = 7, kSlack = 8, kLowE = -30, kUp = 64;  // w <= 2^(7 + 8) * kRound < f16's 65504
+constexpr float kDown = 0x1p-64f;  // 2^-kUp
 constexpr float kRound = 1.0003516f, kRoundLog2 = 5.0713e-4f;  // 1 + 0.72 * 2^-11
 
 struct Fp4ExtendArgs {
@@ -283,14 +288,27 @@ __global__ __launch_bounds__(64 * kExtWaves, 2) void fp4_extend_kernel(Fp4Extend
 #pragma unroll
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[t][i]);
     mx = fmaxf(mx, lane_xor32(mx, lane)) * a.sl2;
-    if (__any(mx > N + kSlack)) {
+    const bool small = min(vs[0], vs[1]) < (uint32_t)(127 + kLowE);
+    if (__any(mx > N + kSlack || small)) {
       const float Nn = fmaxf(N, mx), am = N == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(N - Nn);
-      L *= am;
+      L = scaled_sum(L, N, Nn, am);
 #pragma unroll
       for (int x = 0; x < NC; ++x)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[x][i] *= am;
       N = Nn;
+      if (__any(small)) {  // the tile's part of the sum here, none below
+        const float up = (float)(kLift + kUp) + kRoundLog2 - (N == -INFINITY ? 0.0f : N);
+        float part = 0.0f;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            part = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], a.sl2, up)), spread[t][i] * kDown, part);
+            spread[t][i] = 0.0f;
+          }
+        L += part;
+      }
     }
     const float bias = (float)kLift + kRoundLog2 - (N == -INFINITY ? 0.0f : N);
     float sum = 0.0f;

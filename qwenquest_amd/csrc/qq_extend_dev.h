@@ -103,6 +103,14 @@ __device__ inline void tile_barrier() {
   __asm__ volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
+// A sum of weights relative to 2^from, brought to the maximum `to` of what the output sums, w = 2^(from - to): where V's
+// scales are in those maxima, tokens may count in the weights' sum that far below it.
+__device__ inline float scaled_sum(float sum, float from, float to, float w) {
+  if (w > 0.0f || from == -INFINITY) return w * sum;
+  const float half = __builtin_amdgcn_exp2f(0.5f * (from - to));
+  return half * (half * sum);
+}
+
 // Adds up a tile's splits: one block per (tile, KV head, 8 rows), 32 threads a row (of 64
 // channels the upper 16 write nothing).
 template <int D, typename Args>
@@ -131,7 +139,7 @@ __global__ __launch_bounds__(256) void extend_merge_kernel(Args a) {
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) Mx = fmaxf(Mx, __shfl_xor(Mx, d, 32));
   const float w = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - Mx);
-  float Ls = w * ml.y;
+  float Ls = scaled_sum(ml.y, ml.x, Mx, w);
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) Ls += __shfl_xor(Ls, d, 32);
   float4 Os = make_float4(0.f, 0.f, 0.f, 0.f);

@@ -1,0 +1,63 @@
+"""Prefill over the 4-bit block cache at the ends of what the cache holds: values at both ends of V's range.
+References and tolerances: tests/test_gpu_fp4_extend.py."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from tests.test_gpu_fp4_extend import batch, check, run
+
+pytestmark = pytest.mark.gpu
+
+
+def two_kinds(cuda, prefix, new, dim, heads, gap, at, low):
+    """One token (position `at`) of values near 7 * 2^59 that weighs 2^gap of each other one, whose values are `low` in size."""
+    s, q, lens = batch(cuda, [prefix], [new], 1, dim, heads, seed=dim)
+    n = prefix + new
+    gen = torch.Generator(device=cuda).manual_seed(n)
+    k = torch.empty((n, 1, dim), device=cuda).normal_(generator=gen) * 2.0**-6
+    v = torch.empty((n, 1, dim), device=cuda).normal_(generator=gen).clamp_(-6, 6) * low
+    one = torch.empty(dim, device=cuda).uniform_(2.0, 6.5, generator=gen)
+    k[..., 0] = -4.0
+    k[at, 0, 0] = 4.0
+    v[at, 0] = one * torch.where(torch.arange(dim, device=cuda) % 3 == 0, -1.0, 1.0) * 2.0**59
+    s.pool.set_kv_buffer(s.layer, s.rows(0, np.arange(n)), k, v)
+    q.mul_(2.0**-6)
+    q[..., 0] = gap / 8 * 0.6931  # at a scale of 1: 2^gap between the two
+    return s, q, lens
+
+
+@pytest.mark.parametrize("low", [2.0**-51, 0.0])
+@pytest.mark.parametrize("gap", [17.0, 18.5, 20.0])
+@pytest.mark.parametrize("prefix, new, heads, dim", [(8192, 600, 32, 64), (8192, 300, 64, 128), (8192, 3, 4, 128), (20000, 5, 2, 64)])
+def test_the_sum_over_the_whole_range_of_values(cuda, prefix, new, heads, dim, gap, low):
+    """Thousands of tokens at the low end of V's range before one at its high end: whole query tiles and splits.  In the
+    weights' sum all of them count: 8192 times 2^-17 is a sixteenth of it."""
+    s, q, lens = two_kinds(cuda, prefix, new, dim, heads, gap, prefix - 1, low)
+    check(s, run(s, q, lens, 1.0), q, [prefix], [new], 1.0)
+
+
+@pytest.mark.parametrize("first", [True, False])
+@pytest.mark.parametrize("new, heads", [(3, 2), (280, 64)])
+def test_the_sum_where_weights_of_the_products_underflow(cuda, new, heads, first):
+    """2^18 tokens without values that weigh 2^-24.5 of one with the largest: 2^(-24.5 - 50 - 59 + 7) is no normal float32,
+    and still they are a ninetieth of the sum.  All terms are positive: what sums in float32 lose is, of each
+    term, half a step for each of a chain of 32 in a tile, one for each tile, and those of the splits."""
+    prefix, gap = (1 << 18), 24.5
+    s, q, lens = two_kinds(cuda, prefix, new, 64, heads, gap, 0 if first else prefix - 1, 0.0)
+    out = run(s, q, lens, 1.0).double().view(q.shape)
+    n = prefix + new
+    k, v = (x.double()[:, 0] for x in s.pool.get_rows(s.layer, s.rows(0, np.arange(n)), torch.float32))
+    pick = list(range(0, new, 93)) + [new - 1]
+    qh = q[pick].double()
+    t = (qh.reshape(-1, 64) @ k.T.contiguous()).view(len(pick), heads, n)
+    seen = torch.arange(n, device=cuda)[None] <= prefix + torch.tensor(pick, device=cuda)[:, None]
+    w = torch.softmax(t.masked_fill(~seen[:, None], -np.inf), -1)
+    want, spread = (w.view(-1, n) @ v).view(out[pick].shape), (w.view(-1, n) @ v.abs()).view(out[pick].shape)
+    size = (qh.abs().reshape(-1, 64) @ k.abs().T.contiguous()).amax(-1).view(len(pick), heads, 1)
+    tol = 2.0**-8 * want.abs() + (2.0**-10 + 2 * 68 * 2.0**-23 * size + (32 + n / 64 + 32) * 2.0**-24) * spread
+    assert float(1 - w.amax(-1).max()) > 0.008
+    err = (out[pick] - want).abs()
+    assert (err <= tol).all(), f"off by {(err / tol).max().item():.2f} tolerances"
