@@ -219,7 +219,11 @@ __global__ __launch_bounds__(64 * kExtWaves, 2) void fp4_extend_kernel(Fp4Extend
 #pragma unroll
     for (int i = 0; i < KI; ++i) ks[i] = ks_next[i] >> (8 * (lo >> 4));  // bytes 0 and 2: the lane's tokens of the halves
 #pragma unroll
-    for (int t = 0; t < 2; ++t) vs[t] = vs_next[t];
+    for (int t = 0; t < 2; ++t) vs[t] = max(vs_next[t], 1u);  // (of a byte 0 2^(1 - E) would be infinite)
+    if ((j + 1) * kExtTile > lim_blk) {  // behind what the block attends the bytes may be any, and count for 127
+#pragma unroll
+      for (int t = 0; t < 2; ++t) vs[t] = j * kExtTile + t * 32 + lo < lim_blk ? vs[t] : 127u;
+    }
     if (j + 1 < j_end) {
       const int blk = block_of_word(word);
       load_tile(buf ^ 1, blk);

@@ -1,5 +1,5 @@
-"""Prefill over the 4-bit block cache at the ends of what the cache holds: values at both ends of V's range.
-References and tolerances: tests/test_gpu_fp4_extend.py."""
+"""Prefill over the 4-bit block cache at the ends of what the cache holds: values at both ends of V's range, bytes
+behind a context that nobody wrote.  References and tolerances: tests/test_gpu_fp4_extend.py."""
 
 from __future__ import annotations
 
@@ -61,3 +61,21 @@ def test_the_sum_where_weights_of_the_products_underflow(cuda, new, heads, first
     assert float(1 - w.amax(-1).max()) > 0.008
     err = (out[pick] - want).abs()
     assert (err <= tol).all(), f"off by {(err / tol).max().item():.2f} tolerances"
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("prefix, new, heads", [([0, 63, 100], [1, 70, 130], 4), ([3000], [7], 2), ([700], [600], 64)])
+def test_bytes_that_nobody_wrote(cuda, prefix, new, heads, dim):
+    """Whatever the cache's bytes are behind a context, in the block in which it ends: the same answers, to the bit."""
+    s, q, lens = batch(cuda, prefix, new, 1, dim, heads, seed=dim)
+    kept = [s.pool.get_rows(s.layer, s.rows(i, np.arange(n)), torch.float32) for i, n in enumerate(s.lens)]
+    ref = run(s, q, lens, 0.1)
+    check(s, ref, q, prefix, new, 0.1)
+    for codes, scale in ((0, 0), (0x77, 0), (0xFF, 255), (0x91, 254), (0x2F, 1), (0x77, 200)):
+        for t in (s.pool.k_codes, s.pool.v_codes):
+            t.fill_(codes)
+        for t in (s.pool.k_scale, s.pool.v_scale):
+            t.fill_(scale)
+        for i, (k, v) in enumerate(kept):  # exact: the cache's own values
+            s.pool.set_kv_buffer(s.layer, s.rows(i, np.arange(s.lens[i])), k, v)
+        assert torch.equal(run(s, q, lens, 0.1), ref), (codes, scale)
