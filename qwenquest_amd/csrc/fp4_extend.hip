@@ -40,6 +40,7 @@ typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 
 constexpr int kLift = 7, kSlack = 8, kLowE = -30, kUp = 64;  // w <= 2^(7 + 8) * kRound < f16's 65504
 constexpr float kDown = 0x1p-64f;  // 2^-kUp
+constexpr float kFar = 0x1p22f;    // from there on t + E - N is off by more than 1/2 where the product is not rounded before: w would pass f16's end
 constexpr float kRound = 1.0003516f, kRoundLog2 = 5.0713e-4f;  // 1 + 0.72 * 2^-11
 
 struct Fp4ExtendArgs {
@@ -202,7 +203,8 @@ __global__ __launch_bounds__(64 * kExtWaves, 2) void fp4_extend_kernel(Fp4Extend
   for (int c = 0; c < NC; ++c)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[c][i] = 0.0f;
-  float N = -INFINITY, L = 0.0f;
+  float N = -INFINITY, L = 0.0f, bias = (float)kLift + kRoundLog2;
+  bool far = false;  // this row's N is past kFar
   // LDS addresses of this lane's pieces: K token lo of a half, piece 2 i + hf; V channel lo of 64 and the
   // one 32 further on, token groups hf and hf + 2
   const int k_off = (lo >> 4) * 8 * D + (lo & 15) * 16 + hf * 256;
@@ -293,28 +295,38 @@ __global__ __launch_bounds__(64 * kExtWaves, 2) void fp4_extend_kernel(Fp4Extend
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[t][i]);
     mx = fmaxf(mx, lane_xor32(mx, lane)) * a.sl2;
     const bool small = min(vs[0], vs[1]) < (uint32_t)(127 + kLowE);
-    if (__any(mx > N + kSlack || small)) {
-      const float Nn = fmaxf(N, mx), am = N == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(N - Nn);
+    const bool lags = mx - N > kSlack;
+    if (__any(lags || small || far)) {
+      // (each row by its own maximum, whatever brought its wave here)
+      const float Nn = lags ? mx : N, am = N == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(N - Nn);
       L = scaled_sum(L, N, Nn, am);
 #pragma unroll
       for (int x = 0; x < NC; ++x)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[x][i] *= am;
       N = Nn;
+      const float base = N == -INFINITY ? 0.0f : N;
+      far = fabsf(base) > kFar;
+      bias = (float)kLift + kRoundLog2 - (far ? 0.0f : base);
+      if (__any(far)) {  // differences first, of rounded products: 0 where the maximum is
+        const float inv = 1.0f / a.sl2;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[t][i] = far ? (s[t][i] * a.sl2 - base) * inv : s[t][i];
+      }
       if (__any(small)) {  // the tile's part of the sum here, none below
-        const float up = (float)(kLift + kUp) + kRoundLog2 - (N == -INFINITY ? 0.0f : N);
         float part = 0.0f;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            part = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], a.sl2, up)), spread[t][i] * kDown, part);
+            part = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], a.sl2, bias + kUp)), spread[t][i] * kDown, part);
             spread[t][i] = 0.0f;
           }
         L += part;
       }
     }
-    const float bias = (float)kLift + kRoundLog2 - (N == -INFINITY ? 0.0f : N);
     float sum = 0.0f;
     // O^T += V^T W^T, 16 tokens at a time, the products of some under the weights of the next
 #pragma unroll

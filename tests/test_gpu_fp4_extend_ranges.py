@@ -1,5 +1,5 @@
 """Prefill over the 4-bit block cache at the ends of what the cache holds: values at both ends of V's range, bytes
-behind a context that nobody wrote.  References and tolerances: tests/test_gpu_fp4_extend.py."""
+behind a context that nobody wrote, scores far past 2^24.  References and tolerances: tests/test_gpu_fp4_extend.py."""
 
 from __future__ import annotations
 
@@ -79,3 +79,40 @@ def test_bytes_that_nobody_wrote(cuda, prefix, new, heads, dim):
         for i, (k, v) in enumerate(kept):  # exact: the cache's own values
             s.pool.set_kv_buffer(s.layer, s.rows(i, np.arange(s.lens[i])), k, v)
         assert torch.equal(run(s, q, lens, 0.1), ref), (codes, scale)
+
+
+@pytest.mark.parametrize("dim, prefix, new, pad_heads", [(64, 0, 120, 2), (128, 0, 120, 2), (64, 90, 30, 2), (128, 117, 3, 64)])
+def test_scores_far_past_2_24(cuda, dim, prefix, new, pad_heads):
+    """Scores that grow from 2^7 to 2^66 (and fall to -2^66 for the other sign): a row's output is the value of its largest
+    score, every other one being a power of two of e below it."""
+    n = prefix + new
+    s, q, lens = batch(cuda, [prefix], [new], 1, dim, pad_heads, seed=1)
+    j = torch.arange(n, device=cuda)
+    k = torch.zeros((n, 1, dim), device=cuda)
+    k[:, 0, 0] = (1 + (j % 2) / 2) * torch.exp2((7 + j // 2).float())
+    v = torch.randn((n, 1, dim), device=cuda)
+    s.pool.set_kv_buffer(s.layer, s.rows(0, np.arange(n)), k, v)
+    q.zero_()
+    q[:, 0::2, 0], q[:, 1::2, 0] = 1.0, -1.0
+    out = run(s, q, lens, 1.0).view(new, pad_heads, dim)
+    vals = s.pool.get_rows(s.layer, s.rows(0, np.arange(n)), torch.bfloat16)[1][:, 0]
+    assert torch.equal(out[:, 0::2], vals[prefix:][:, None].expand(-1, pad_heads // 2, -1))
+    assert torch.equal(out[:, 1::2], vals[:1][:, None].expand(new, pad_heads // 2, -1))
+
+
+@pytest.mark.parametrize("exponent", [10, 23, 24, 26, 27, 28, 33, 60, 100])
+def test_equal_scores_of_any_size_weigh_the_same(cuda, exponent):
+    """A mean over the context, whatever the score that all tokens share.  Weights alike, their common rounding (2^-10 at
+    most) cancels against the sum's but for what truncation keeps of it; half a step of bf16."""
+    s, q, lens = batch(cuda, [70], [30], 1, 64, 4, seed=2)
+    k, v = torch.zeros((100, 1, 64), device=cuda), torch.randn((100, 1, 64), device=cuda)
+    k[..., 0] = 1.5 * 2.0**exponent
+    v[..., 0] = 6.0  # one scale for all
+    s.pool.set_kv_buffer(s.layer, s.rows(0, np.arange(100)), k, v.clamp_(-6, 6))
+    q.zero_()
+    q[:, :2, 0], q[:, 2:, 0] = 1.0, -1.0
+    out = run(s, q, lens, 1.0).view(30, 4, 64).double()
+    vals = s.pool.get_rows(s.layer, s.rows(0, np.arange(100)), torch.float32)[1][:, 0].double()
+    for t in range(30):
+        want, spread = vals[: 71 + t].mean(0), vals[: 71 + t].abs().mean(0)
+        assert ((out[t] - want).abs() <= 2.0**-8 * want.abs() + (2.0**-10 + 100 * 2.0**-23) * spread).all(), t
