@@ -203,8 +203,8 @@ __global__ __launch_bounds__(64 * kExtWaves, 2) void fp4_extend_kernel(Fp4Extend
   for (int c = 0; c < NC; ++c)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[c][i] = 0.0f;
-  float N = -INFINITY, L = 0.0f, bias = (float)kLift + kRoundLog2;
-  bool far = false;  // this row's N is past kFar
+  float N = -INFINITY, L = 0.0f;
+  float bias = (float)kLift + kRoundLog2, bar = -INFINITY;  // what goes to every exponent, the score that brings another
   // LDS addresses of this lane's pieces: K token lo of a half, piece 2 i + hf; V channel lo of 64 and the
   // one 32 further on, token groups hf and hf + 2
   const int k_off = (lo >> 4) * 8 * D + (lo & 15) * 16 + hf * 256;
@@ -295,10 +295,9 @@ __global__ __launch_bounds__(64 * kExtWaves, 2) void fp4_extend_kernel(Fp4Extend
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[t][i]);
     mx = fmaxf(mx, lane_xor32(mx, lane)) * a.sl2;
     const bool small = min(vs[0], vs[1]) < (uint32_t)(127 + kLowE);
-    const bool lags = mx - N > kSlack;
-    if (__any(lags || small || far)) {
+    if (__any(mx > bar || small)) {
       // (each row by its own maximum, whatever brought its wave here)
-      const float Nn = lags ? mx : N, am = N == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(N - Nn);
+      const float Nn = mx - N > kSlack ? mx : N, am = N == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(N - Nn);
       L = scaled_sum(L, N, Nn, am);
 #pragma unroll
       for (int x = 0; x < NC; ++x)
@@ -306,7 +305,8 @@ __global__ __launch_bounds__(64 * kExtWaves, 2) void fp4_extend_kernel(Fp4Extend
         for (int i = 0; i < 16; ++i) o[x][i] *= am;
       N = Nn;
       const float base = N == -INFINITY ? 0.0f : N;
-      far = fabsf(base) > kFar;
+      const bool far = fabsf(base) > kFar;
+      bar = far ? -INFINITY : N + kSlack;
       bias = (float)kLift + kRoundLog2 - (far ? 0.0f : base);
       if (__any(far)) {  // differences first, of rounded products: 0 where the maximum is
         const float inv = 1.0f / a.sl2;
