@@ -414,6 +414,7 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attend_kernel(DecArgs<typen
   bf16x8_t qf[2 * KS][QP];
   float4_t o[VL];
   float M = -INFINITY, L = 0.0f;
+  float mb = 0.0f;  // (kOneFactor) M, or 0 before there is one
   bool bad = false;
   int first = s0;  // this request's first unit here
   auto load_q = [&](int b) {
@@ -440,6 +441,7 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attend_kernel(DecArgs<typen
       for (int i = 0; i < VL; ++i) o[i] = float4_t{0.f, 0.f, 0.f, 0.f};
       M = -INFINITY;
       L = 0.0f;
+      mb = 0.0f;
       bad = false;
     }
     const bool sparse = is_sparse(a, seq), win = sparse && u - c0 == picked;
@@ -505,13 +507,24 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attend_kernel(DecArgs<typen
         M = Mn;
         L *= alpha;
         fold(alpha);
+        mb = M == -INFINITY ? 0.0f : M;
       }
       if (win) unit.merge_window_scales(seq & 63, g);
-      const float mb = M == -INFINITY ? 0.0f : M;
+      // A product that is not rounded before the maximum (of rounded ones) is taken off it differs by up to 2^-24 of the
+      // maximum: from 2^31 on exponentials would leave float32's range
+      const bool far = fabsf(mb) > 0x1p22f;
+      if (__builtin_expect(__any(far), 0)) {
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], a.sl2, -mb));
+          for (int i = 0; i < 4; ++i)
+            s[t][i] = __builtin_amdgcn_exp2f(far ? s[t][i] * a.sl2 - mb : __builtin_fmaf(s[t][i], a.sl2, -mb));
+      } else {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], a.sl2, -mb));
+      }
       if (hi < 64) {  // (a factor of 0 makes NaN of what is masked)
         __asm__ volatile("" : "+v"(left));
 #pragma unroll
@@ -548,15 +561,15 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attend_kernel(DecArgs<typen
       mx = fmaxf(mx, lane_xor16(mx, lane));
       mx = fmaxf(mx, lane_xor32(mx, lane));
       const float Mn = fmaxf(M, mx);
-      const float mb = Mn == -INFINITY ? 0.0f : Mn;
-      const float alpha = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - mb);
+      const float mn = Mn == -INFINITY ? 0.0f : Mn;
+      const float alpha = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - mn);
       M = Mn;
       float sum = 0.0f;
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float p = __builtin_amdgcn_exp2f(s[t][i] - mb);
+          const float p = __builtin_amdgcn_exp2f(s[t][i] - mn);
           sum += p;
           // a masked token weighs nothing whatever its block's scale is
           s[t][i] = s[t][i] == -INFINITY ? 0.0f : p * unit.weight(t, i, t * 16 + g * 4 + i, seq & 63);
