@@ -218,6 +218,13 @@ def call(name: str, *args) -> None:
     check(getattr(load(), name)(*args))
 
 
+def refuse_tracing(what: str) -> None:
+    """For operators whose outputs the C entries fill: ``torch.jit.trace`` sees their allocation alone, and a trace's replay
+    would answer with what lies in that memory."""
+    if torch._C._get_tracing_state() is not None:
+        raise RuntimeError(f"{what} cannot be traced: a trace would keep its values, not its work")
+
+
 def ptr(t: torch.Tensor | None) -> int | None:
     """Device pointer of a CUDA (HIP) tensor; the product path never takes CPU tensors."""
     if t is None:

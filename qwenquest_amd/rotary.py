@@ -100,6 +100,7 @@ class QKNormRotary:
         """``qkv [n, (num_heads + 2 kv_heads) * head_dim]``, a token's query heads, key heads and value heads in a
         row, at ``positions`` (``[n]``, or ``[axes, n]``) -> ``q [n, num_heads, head_dim]``, ``k`` and ``v [n, kv_heads,
         head_dim]``, dense (v as it was)."""
+        _lib.refuse_tracing("QKNormRotary")
         h, kv, dim = self.num_heads, self.kv_heads, self.head_dim
         if qkv.dim() != 2 or qkv.shape[1] != (h + 2 * kv) * dim:
             raise ValueError(f"qkv must be [n, ({h} + 2 * {kv}) * {dim}], got {tuple(qkv.shape)}")
@@ -110,6 +111,7 @@ class QKNormRotary:
     def apply(self, q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """``q [n, num_heads, head_dim]`` and ``k [n, kv_heads, head_dim]`` (or with the heads in a row) at
         ``positions``, as new dense tensors."""
+        _lib.refuse_tracing("QKNormRotary")
         rows, args = [], []
         for x, heads, what in ((q, self.num_heads, "q"), (k, self.kv_heads, "k")):
             if x.dim() == 3 and x.shape[1:] == (heads, self.head_dim):
