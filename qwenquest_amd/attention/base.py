@@ -14,6 +14,7 @@ from typing import TYPE_CHECKING, Any
 import torch
 from torch.autograd import forward_ad
 
+from qwenquest_amd import _lib
 from qwenquest_amd.attention.ops import (
     coded_extend_attention,
     extend_attention,
@@ -89,9 +90,8 @@ class AttentionBackend(ABC):
         """
         assert batch.out_cache_loc is not None and batch.extend_prefix_lens is not None
         pool = self.token_to_kv_pool
-        if self.coded and torch._C._get_tracing_state() is not None:
-            # neither the store nor the rows read back are torch operations
-            raise RuntimeError("a prefill over a pool of codes cannot be traced: a trace would keep its values, not its work")
+        if self.coded:  # neither the store nor the rows read back are torch operations
+            _lib.refuse_tracing("a prefill over a pool of codes")
         pool.set_kv_buffer(layer.layer_id, batch.out_cache_loc, k, v)
         if self.coded:
             return self._forward_extend_coded(q, layer, batch)

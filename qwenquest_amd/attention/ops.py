@@ -248,6 +248,7 @@ def coded_decode_plan(pool: CodedTokenToKVPool, block_table: torch.Tensor, req_p
                       seq_lens: torch.Tensor) -> DecodePlan:
     """What ``coded_decode_attention`` over whole contexts makes of a step's lengths, once for the step's
     layers, on the current stream."""
+    _lib.refuse_tracing("a decode step over a pool of codes")
     dev = pool.device
     bs = int(req_pool_indices.shape[0])
     table = _lib.table_args(block_table, dev)
@@ -287,6 +288,7 @@ def coded_decode_attention(
     the same graph capture or both in none, they run as without it.
     Returns ``[bs, H*D]`` in q's dtype (bf16 or fp32): zeros for an empty context, NaN for a request
     outside the table or a context past its blocks."""
+    _lib.refuse_tracing("a decode step over a pool of codes")
     dev = pool.device
     q = _queries(q, pool)
     bs, heads, dim = q.shape
@@ -346,6 +348,7 @@ def coded_quest_step(
     step's division of the work saves a launch; each new token lies in the last block of its own
     request's context and no two in one block (rows of block 0 aside).  ``phase``: 1 = scoring and selection, 2 = store and attention after phase 1, 3 = both.
     Returns ``[bs, H*D]`` (complete after phase 2)."""
+    _lib.refuse_tracing("a decode step over a pool of codes")
     dev, step = pool.device, quest._step
     if step is None:
         raise RuntimeError("decode_step_blocks() must be called once per decode step first")
@@ -402,6 +405,7 @@ def coded_extend_attention(
     positions ``0 .. prefix_lens[i] + t``.  Returns ``[n, H*D]``; the lengths are read on the device
     only.  NaN: a request outside the table, a query tile that attends a block which is not there,
     rows of q past the requests' tokens."""
+    _lib.refuse_tracing("a prefill over a pool of codes")
     dev = pool.device
     if q.dtype != torch.bfloat16:
         raise ValueError(f"unsupported dtype {q.dtype}; the prefill kernel takes bfloat16")

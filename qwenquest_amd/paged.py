@@ -226,6 +226,7 @@ class CodedTokenToKVPool:
         """Write ``k``/``v`` ``[n, kv_heads, head_dim]`` at rows ``loc`` (memory.py:114-120).  Rows of
         block 0 and outside the pool are skipped; the rows of one block stand next to each other in
         ``loc``, as a slot map has them."""
+        _lib.refuse_tracing("a store into a pool of codes")
         loc = _device_i64(loc, self.device, "loc")
         n = int(loc.numel())
         if n == 0:
@@ -239,6 +240,7 @@ class CodedTokenToKVPool:
                  dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
         """K and V values ``[n, kv_heads, head_dim]`` of rows ``loc``: exact in bf16 (and fp32); NaN
         for a row outside the pool."""
+        _lib.refuse_tracing("rows out of a pool of codes")
         code = _lib.dtype_code(dtype)
         loc = _device_i64(loc, self.device, "loc")
         n = int(loc.numel())

@@ -368,6 +368,7 @@ class QuestAlgorithm:
 
     def _page_bounds(self, pool: CodedTokenToKVPool, block_table, reqs, seq_lens, prefix_lens, decode: bool,
                      max_new: int) -> StepLayout | None:
+        _lib.refuse_tracing("page bounds over a pool of codes")
         if self.page_size != 64:
             raise ValueError(f"an 8- or 4-bit pool's pages are its blocks of 64 tokens, not of {self.page_size}")
         if pool.kv_heads != self.kv_heads or pool.head_dim != self.head_dim or pool.num_layers < self.end_layer:
