@@ -603,7 +603,8 @@ int qq_fp4_decode_plan(int num_blocks, int kv_heads, int head_dim, int block_tab
 /* qq_fp8_quest_step over the 4-bit cache.  Planned (by qq_fp4_page_bounds), bf16 queries of 128 channels,
  * up to 16 query heads per KV head, top_k of 512 to 2112 (of one request to 2624, in tables of more than 4096 pages to
  * 4160), up to 8192 pages and as many requests as the chip's blocks hold per head (256 / kv_heads) take two launches: the
- * scores; the selection with the store and the attention.  Others take three or four, as there. */
+ * scores; the selection with the store and the attention.  Others take three or four, as there.  With a plan of another bs or
+ * top_k every output is NaN, the new tokens are stored and positions may not be written (as there). */
 int qq_fp4_quest_step(const void* q, int q_dtype, int64_t q_batch_stride, int num_q_heads, const void* k_new,
                       const void* v_new, int new_dtype, const int64_t* out_cache_loc, uint8_t* k_codes,
                       uint8_t* v_codes, uint8_t* k_scale, uint8_t* v_scale, int num_blocks, int kv_heads, int head_dim,

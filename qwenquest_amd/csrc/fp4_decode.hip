@@ -36,6 +36,7 @@ struct Fp4Unit {
   struct BeginSmem {};
   static constexpr int kDim = D;
   static constexpr bool kOneFactor = true;
+  static constexpr bool kStoresSelecting = true;
   static constexpr int KW = D / 32, VL = D / 32;  // words a lane: of a token of K; 16-byte loads: of a block of V
   typedef uint32_t words_t __attribute__((ext_vector_type(KW)));
   words_t kr[4];

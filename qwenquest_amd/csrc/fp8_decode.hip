@@ -39,6 +39,7 @@ struct Fp8Unit {
   using BeginSmem = StoreSmem<D>;
   static constexpr int kDim = D;
   static constexpr bool kOneFactor = false;  // a block's scale is one
+  static constexpr bool kStoresSelecting = false;
   static constexpr int KL = D / 64, VL = D / 16;  // 16-byte loads a lane: per 16 tokens of K, per block of V
   float ks = 0.0f, vs = 0.0f, ks2 = 0.0f, vs2 = 0.0f;  // of this lane's unit
   float kscale, vscale, kscale2, vscale2;              // of the unit at hand

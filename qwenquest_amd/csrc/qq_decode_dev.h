@@ -38,6 +38,7 @@
 //   merge_window_scales(from2, g) (with kOneFactor, before weight), merge_window(from2, g)   both V of a window in one
 //   tile_of(st, x, y), place_of(x, y)   where the weight of element 2 x + y of step st lies in S^T
 //   values(i, st)                 operand of channels 16 i .. and step st
+//   kStoresSelecting              whether an attention that selects stores the new tokens
 //   store_tokens(st, i, on, h), BeginSmem, begin_blocks(st), begin_store<SRC>(st, smem, block)
 #pragma once
 
@@ -277,7 +278,13 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attend_kernel(DecArgs<typen
   const int m16 = lane & 15, g = lane >> 4;
   const int rows = min(a.G - tile * kTile, kTile);  // query heads of this tile
   const int q_head = h * a.G + tile * kTile;
-  if (plan.bs != a.bs || plan.top_k != a.top_k) {  // another batch's plan: no answer to any request
+  if (__builtin_expect(plan.bs != a.bs || plan.top_k != a.top_k, 0)) {  // another batch's plan: no answer to any request
+    if constexpr (KPT > 0 && U::kStoresSelecting) {  // (no launch before has stored the new tokens)
+      const int group = lane / (D / 4);
+      if (st.k && wave == 0)
+        for (int b0 = slice; b0 < a.bs; b0 += 256 / D * a.max_slices)
+          U::store_tokens(st, b0 + group * a.max_slices, b0 + group * a.max_slices < a.bs, h);
+    }
     const float nan = __builtin_nanf("");
     for (int b = slice; b < a.bs; b += a.max_slices)
       for (int i = tid; i < rows * (D / 4); i += 64 * kDecWaves)

@@ -1,4 +1,5 @@
-"""Steps over the pools of codes as a backend does not make them: operators under torch.jit.trace."""
+"""Steps over the pools of codes as a backend does not make them: a Quest step with another step's plan, operators
+under torch.jit.trace."""
 
 from __future__ import annotations
 
@@ -16,6 +17,8 @@ from tests.test_gpu_fp8_engine import i64
 
 pytestmark = pytest.mark.gpu
 
+CACHE = ("k_codes", "v_codes", "k_scale", "v_scale")
+
 
 def quest_step(monkeypatch, cuda, kind, had, top_k=512, heads=16, kv=4):
     monkeypatch.setattr(engine, "Fp8TokenToKVPool", kind)
@@ -31,6 +34,27 @@ def quest_step(monkeypatch, cuda, kind, had, top_k=512, heads=16, kv=4):
     batch = ForwardBatch(ForwardMode.DECODE, None, pos, rpi, seq, loc, e.rtp, e.kvp, e.be)
     e.be.init_forward_metadata(batch)
     return e, batch, [e.rand(len(had), h, 128) for h in (heads, kv, kv)]
+
+
+@pytest.mark.parametrize("kind, kv, had", [(Fp8TokenToKVPool, 4, [700, 63]), (Fp4TokenToKVPool, 4, [700, 63]),
+                                           (Fp4TokenToKVPool, 1, [600, 64, 900, 1, 127] * 9), (Fp4TokenToKVPool, 8, [1300] * 20)])
+def test_a_quest_step_with_another_plan_keeps_its_tokens(monkeypatch, cuda, kind, kv, had):
+    """No answer to any request, but the new tokens are in the cache as a step of its own plan leaves them there, and no
+    other row is touched."""
+    e, batch, (q, k, v) = quest_step(monkeypatch, cuda, kind, had, heads=4 * kv, kv=kv)
+    before = [getattr(e.kvp, x).clone() for x in CACHE]
+    dense = ops.coded_decode_plan(e.kvp, e.rtp.block_table, batch.req_pool_indices, batch.seq_lens)
+    plan = e.be.quest._step.plan
+    e.be.quest._step.plan = dense._replace(top_k=512)  # does not show what it is of
+    assert e.be.forward(q, k, v, e.mods[0], batch).isnan().all()
+    got = [getattr(e.kvp, x).clone() for x in CACHE]
+    for x, old in zip(CACHE, before):
+        getattr(e.kvp, x).copy_(old)
+    e.kvp.set_kv_buffer(0, batch.out_cache_loc, k, v)
+    assert all(torch.equal(getattr(e.kvp, x), y) for x, y in zip(CACHE, got))
+    assert not all(torch.equal(x, y) for x, y in zip(before, got))
+    e.be.quest._step.plan = plan
+    assert not e.be.forward(q, k, v, e.mods[0], batch).isnan().any()
 
 
 def test_operators_that_a_trace_would_lose_refuse_it(monkeypatch, cuda):
