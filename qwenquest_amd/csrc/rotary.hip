@@ -4,9 +4,9 @@
 // then of the pairs (a, b) of the first 2 P channels (b is P further on, or next to a) pair j turns by
 // the angle pos[axis_j] * f_j:  (a cos - b sin, b cos + a sin).  fp32, rounded once at the end.
 //
-// The angle is taken in quarter turns in fp64 (53 bits: at position 2^31 still to 2^-22 of a radian), its
-// fraction goes to fp32 at 1/2 of a quarter at most, so that sine and cosine are good to fp32's last
-// places at any position.
+// The angle is taken in quarter turns in fp64, a product of all its bits, and its fraction goes to fp32 at 1/2 of a quarter at most:
+// sine and cosine are good to fp32's last places but for what the frequency, rounded to fp64, leaves of the angle,
+// 2^-53 of it (2^-24 at 2^29 radians, 2^-22 at 2^31).
 //
 // A wave works on a token: a lane per pair for the angles, which meet the heads in the LDS, then D / 8 lanes
 // (to the next power of two) per head, 8 channels a lane, whose cosines and sines stay in registers over the
@@ -138,10 +138,10 @@ __global__ __launch_bounds__(64 * kRotWaves) void rotary_kernel(RotaryArgs a) {
   float *cs = turned + wave * 2 * a.pairs, *sn = cs + a.pairs;
   for (int j = lane; j < a.pairs; j += 64) {
     const int64_t at = a.pos[(a.axes == 1 ? 0 : min(a.axis[j], a.axes - 1)) * a.pos_stride + token];
-    const double t = (double)at * a.quarters[j], whole = rint(t);
+    const double f = a.quarters[j], t = (double)at * f, whole = rint(t), rest = __builtin_fma((double)at, f, -t);
     const int quarter = (int)(whole - 4.0 * floor(whole * 0.25));  // 0 .. 3
     float s, c;
-    sincospif(0.5f * (float)(t - whole), &s, &c);
+    sincospif(0.5f * (float)(t - whole + rest), &s, &c);
     if (at >= (int64_t)1 << 31 || at <= -((int64_t)1 << 31)) s = c = __builtin_nanf("");
     cs[j] = quarter & 1 ? (quarter & 2 ? s : -s) : (quarter & 2 ? -c : c);
     sn[j] = quarter & 1 ? (quarter & 2 ? -c : c) : (quarter & 2 ? -s : s);

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import math
 from collections.abc import Sequence
+from fractions import Fraction
 
 import torch
 from torch.autograd import forward_ad
@@ -17,6 +18,8 @@ from qwenquest_amd.paged import _indexed
 
 __all__ = ["QKNormRotary"]
 
+#: quarter turns of a radian, 2 / pi
+_QUARTERS = 2 / Fraction("3.14159265358979323846264338327950288419716939937510582097494459")
 _ORDERS = ("blocks", "cycled")
 _PAIRS = ("halves", "neighbours")
 
@@ -26,8 +29,9 @@ class QKNormRotary:
 
     A head x becomes ``y = x / sqrt(mean(x^2) + eps) * weight`` (``q_weight`` / ``k_weight [head_dim]``, copied;
     None: no norm), then of the first ``rotary_dim`` channels pair j turns by ``position * inv_freq[j]``:
-    ``(a, b) -> (a cos - b sin, b cos + a sin)``.  In float32, angles exact to its last places at any position
-    under 2^31, rounded once to the input's type (bfloat16 or float32).
+    ``(a, b) -> (a cos - b sin, b cos + a sin)``.  In float32, rounded once to the input's type (bfloat16 or float32); an angle
+    is off by 2^-53 of itself at most, so that sine and cosine are good to float32's last places up to 2^29 radians
+    and to 2^-22 at 2^31.  A token at a position of 2^31 or beyond, either way, gets NaN where it would turn.
 
     ``inv_freq [rotary_dim / 2]``: by default ``base ** (-2 j / rotary_dim)``.  ``pairs``: "halves" (channel j with
     j + rotary_dim / 2) or "neighbours" (2 j with 2 j + 1).  ``sections``: the number of pairs that turn by each of several
@@ -81,8 +85,8 @@ class QKNormRotary:
             raise ValueError(f"sections {tuple(left)} must add up to the {count} pairs")
         self.num_heads, self.kv_heads, self.head_dim, self.rotary_dim = num_heads, kv_heads, head_dim, rotary_dim
         self.eps, self.axes, self.neighbours = float(eps), len(left), pairs == "neighbours"
-        # in quarter turns, as the kernel takes angles
-        self._quarters = (freq * (2.0 / math.pi)).to(self.device)
+        # in quarter turns, as the kernel takes angles, each rounded once
+        self._quarters = torch.tensor([float(Fraction(f) * _QUARTERS) for f in freq.tolist()], dtype=torch.float64).to(self.device)
         self._axis = torch.tensor(_deal(left, section_order == "cycled"), dtype=torch.int32, device=self.device)
         self._weights = [self._weight(w, what) for w, what in ((q_weight, "q_weight"), (k_weight, "k_weight"))]
         # what every call passes, of tensors that stay where they are
