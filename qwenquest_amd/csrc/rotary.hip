@@ -170,12 +170,23 @@ __global__ __launch_bounds__(64 * kRotWaves) void rotary_kernel(RotaryArgs a) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(x[i], x[i], sum);
     sum = lanes_sum<L>(in ? sum : 0.0f, lane);
-    const bool key = h >= a.H;
-    const float mean = __builtin_fmaf(sum, share, a.eps);
+    const bool key = h >= a.H, normed = key ? a.wk != nullptr : a.wq != nullptr;
+    float mean = __builtin_fmaf(sum, share, a.eps);
+    // Squares that leave float32's range, or all but do: the row in other units
+    const bool large = !(sum <= 0x1p100f), small = mean < 0x1p-100f;
+    if (__builtin_expect(__any(normed && (large || small)), 0)) {
+      const float unit = !normed ? 1.0f : large ? 0x1p-96f : small ? 0x1p96f : 1.0f;
+      sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i] *= unit;
+        sum = __builtin_fmaf(x[i], x[i], sum);
+      }
+      mean = __builtin_fmaf(lanes_sum<L>(in ? sum : 0.0f, lane), share, a.eps * unit * unit);
+    }
     float f = __builtin_amdgcn_rsqf(mean);
     // a Newton step: the instruction is off by up to 2^-23
     f = mean < INFINITY && mean > 1e-37f ? f + 0.5f * f * __builtin_fmaf(-mean * f, f, 1.0f) : f;
-    const bool normed = key ? a.wk != nullptr : a.wq != nullptr;
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = normed ? x[i] * f * (key ? wk[i] : wq[i]) : x[i];
 #pragma unroll
