@@ -155,6 +155,7 @@ extern "C" int qq_fp4_decode_attention(const void* q, int q_dtype, int64_t q_bat
   QQ_REQUIRE(!planned || !positions, "%s: a plan is of whole contexts, not of selected pages", what);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool one = planned && a.tiles == 1;
+  QQ_REQUIRE(one || (head_dim == 128 ? begin_fits<Fp4Unit<128>>(a, st) : begin_fits<Fp4Unit<64>>(a, st)), "%s: bad sizes", what);
   if (head_dim == 128) launch_decode<Fp4Unit<128>>(a, st, SelectArgs{}, one, q_dtype, s);
   else launch_decode<Fp4Unit<64>>(a, st, SelectArgs{}, one, q_dtype, s);
   return check_launch(what);
@@ -199,6 +200,7 @@ extern "C" int qq_fp4_quest_step(const void* q, int q_dtype, int64_t q_batch_str
                           block_table_stride, block_table_rows, block_table_cols, req_pool_indices, seq_lens, bs, positions,
                           top_k, top_k, scale, out, workspace, workspace_bytes);
   if (ok != QQ_OK || bs == 0) return ok;
+  QQ_REQUIRE(phase == 1 || (head_dim == 128 ? begin_fits<Fp4Unit<128>>(a, st) : begin_fits<Fp4Unit<64>>(a, st)), "%s: bad sizes", what);
   const int C = kv_heads * head_dim, k_sel = top_k / 64 - 1;
   QQ_REQUIRE(C <= kMaxC, "%s: kv_heads*head_dim %d exceeds %d", what, C, kMaxC);
   QQ_REQUIRE(k_sel <= 1024, "%s: %d selected pages exceed 1024", what, k_sel);

@@ -443,7 +443,7 @@ extern "C" int qq_fp4_extend_attention(const void* q, int num_q_heads, const uin
   const int64_t tiles = extend_tiles(n, bs, G);
   a.splits = extend_splits(tiles, kv_heads, (int64_t)block_table_cols * kCacheTokens);
   const int64_t grid = (tiles * a.splits + 1) * kv_heads;
-  QQ_REQUIRE(grid < (int64_t)1 << 31, "%s: too many query rows", what);
+  QQ_REQUIRE(grid < (int64_t)1 << 24, "%s: too many query rows", what);  // (a launch holds fewer than 2^32 threads)
   a.tiles = (int)tiles;
   a.q_factor = scale < 0x1p-60f ? 0x1p-64f : scale > 0x1p60f ? 0x1p64f : 1.0f;
   a.sl2 = scale / a.q_factor * kLog2e;

@@ -763,6 +763,13 @@ void attend(const DecArgs<typename U::Cache>& a, const typename U::Store& st, co
 
 constexpr int kBeginPages = 16 * 256;  // pages that a begin launch selects of, at most
 
+// A call that is not divided begins with a launch of one block, one for every request and those of the new tokens, of 256
+// threads, where a launch holds fewer than 2^32.
+template <typename U>
+bool begin_fits(const DecArgs<typename U::Cache>& a, const typename U::Store& st) {
+  return 1 + (int64_t)a.bs + (st.k ? (int64_t)U::begin_blocks(st) : 0) < (int64_t)1 << 24;
+}
+
 // `sel`: with k_sel > 0 the pages are selected first, from scores that are there.  planned: the
 // workspace holds the slices, and nothing of another head tile waits for the new tokens.
 template <typename U>
