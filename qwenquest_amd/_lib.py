@@ -249,6 +249,11 @@ def table_args(block_table: torch.Tensor, device: torch.device) -> tuple:
     return ptr(block_table), max(block_table.stride(0), cols), rows, cols
 
 
+def pool_kind(pool) -> str:
+    """The C entries' prefix for a pool of codes; one that names none holds 8-bit blocks."""
+    return getattr(pool, "kind", "fp8")
+
+
 def dtype_code(dt: torch.dtype) -> int:
     if dt == torch.bfloat16:
         return DTYPE_BF16

@@ -235,11 +235,11 @@ def _queries(q: torch.Tensor, pool: CodedTokenToKVPool) -> torch.Tensor:
 
 
 def _entry(pool: CodedTokenToKVPool, name: str):
-    return getattr(_lib.load(), f"qq_{pool.kind}_{name}")
+    return getattr(_lib.load(), f"qq_{_lib.pool_kind(pool)}_{name}")
 
 
 def _of_kind(pool: CodedTokenToKVPool, kind: str) -> CodedTokenToKVPool:
-    if pool.kind != kind:
+    if _lib.pool_kind(pool) != kind:
         raise ValueError(f"expected an {kind.capitalize()}TokenToKVPool, got an {type(pool).__name__}")
     return pool
 
@@ -258,7 +258,7 @@ def coded_decode_plan(pool: CodedTokenToKVPool, block_table: torch.Tensor, req_p
     ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
     stream = _lib.stream(dev)
     with _lib.on(dev):
-        _lib.call(f"qq_{pool.kind}_decode_plan", pool.num_blocks, pool.kv_heads, pool.head_dim, table[2], table[3],
+        _lib.call(f"qq_{_lib.pool_kind(pool)}_decode_plan", pool.num_blocks, pool.kv_heads, pool.head_dim, table[2], table[3],
                   _lib.ptr(rpi), _lib.ptr(seq), bs, _lib.ptr(ws), need, stream)
     return DecodePlan(bs, ws, stream, _lib.capture_id(dev, stream))
 
@@ -318,7 +318,7 @@ def coded_decode_attention(
         ws, plan = torch.empty(max(need, 1), dtype=torch.uint8, device=dev), None
     with _lib.on(dev):
         _lib.call(
-            f"qq_{pool.kind}_decode_attention", _lib.ptr(q), _lib.dtype_code(q.dtype), q.stride(0), heads, _lib.ptr(kn),
+            f"qq_{_lib.pool_kind(pool)}_decode_attention", _lib.ptr(q), _lib.dtype_code(q.dtype), q.stride(0), heads, _lib.ptr(kn),
             _lib.ptr(vn), _lib.DTYPE_BF16 if kn is None else _lib.dtype_code(kn.dtype), _lib.ptr(loc),
             *pool.layer_args(layer_id), *table, _lib.ptr(rpi), _lib.ptr(seq), bs, _lib.ptr(positions),
             0 if positions is None else max(positions.stride(0), positions.shape[1]), int(top_k), float(scaling),
@@ -379,7 +379,7 @@ def coded_quest_step(
         raise ValueError("the step's plan is not decode_step_blocks' of this batch and pool")
     with _lib.on(dev):
         _lib.call(
-            f"qq_{pool.kind}_quest_step", _lib.ptr(q), _lib.dtype_code(q.dtype), q.stride(0), heads, _lib.ptr(kn), _lib.ptr(vn),
+            f"qq_{_lib.pool_kind(pool)}_quest_step", _lib.ptr(q), _lib.dtype_code(q.dtype), q.stride(0), heads, _lib.ptr(kn), _lib.ptr(vn),
             _lib.dtype_code(kn.dtype), _lib.ptr(loc), *pool.layer_args(layer_id), *table,
             _lib.ptr(quest.page_k_bounds), layer_id - quest.start_layer, _lib.ptr(rpi), _lib.ptr(step.seq_lens),
             _lib.ptr(step.candidate_limit_i32), bs, quest.max_reqs, quest.max_pages_per_req, quest.top_k, float(scaling),
@@ -423,7 +423,7 @@ def coded_extend_attention(
     out = torch.empty((n, heads * dim), dtype=q.dtype, device=dev)
     with _lib.on(dev):
         _lib.call(
-            f"qq_{pool.kind}_extend_attention", _lib.ptr(q), heads, *pool.layer_args(layer_id), *table, _lib.ptr(rpi),
+            f"qq_{_lib.pool_kind(pool)}_extend_attention", _lib.ptr(q), heads, *pool.layer_args(layer_id), *table, _lib.ptr(rpi),
             _lib.ptr(seq), _lib.ptr(prefix), _lib.ptr(ext), bs, n, float(scaling), _lib.ptr(out), _lib.ptr(ws), need,
             _lib.stream(dev),
         )

@@ -386,13 +386,13 @@ class QuestAlgorithm:
         actual = limit = ws = None
         if decode:
             actual, limit = torch.empty((2, bs), dtype=torch.int32, device=dev).unbind(0)
-            need = int(getattr(_lib.load(), f"qq_{pool.kind}_decode_workspace_bytes")(bs, self.kv_heads, self.kv_heads, self.head_dim))
+            need = int(getattr(_lib.load(), f"qq_{_lib.pool_kind(pool)}_decode_workspace_bytes")(bs, self.kv_heads, self.kv_heads, self.head_dim))
             # of this step alone: a graph's replay must not find another step's division in it
             ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
         stream = _lib.stream(dev)
         with _lib.on(dev):
             _lib.call(
-                f"qq_{pool.kind}_page_bounds", codes, pool.k_codes.stride(0), scale, pool.k_scale.stride(0), *geometry,
+                f"qq_{_lib.pool_kind(pool)}_page_bounds", codes, pool.k_codes.stride(0), scale, pool.k_scale.stride(0), *geometry,
                 *table, *(_lib.ptr(t) for t in lens), bs, int(decode), int(max_new), self.num_layers,
                 _lib.ptr(self.page_k_bounds), self.max_reqs, self.max_pages_per_req, self.top_k,
                 int(self.avoid_recent_overlap), _lib.ptr(actual), _lib.ptr(limit), _lib.ptr(ws),

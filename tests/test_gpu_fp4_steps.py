@@ -1,5 +1,5 @@
-"""Steps over the pools of codes as a backend does not make them: a Quest step with another step's plan, operators
-under torch.jit.trace."""
+"""Steps over the 4-bit pool that go wrong or go through the functions of one kind of pool: a Quest step with another
+step's plan, the functions by their pools, operators under torch.jit.trace."""
 
 from __future__ import annotations
 
@@ -8,7 +8,7 @@ from types import SimpleNamespace
 import pytest
 import torch
 
-from qwenquest_amd import QKNormRotary
+from qwenquest_amd import QKNormRotary, QuestAlgorithm
 from qwenquest_amd.attention import ops
 from qwenquest_amd.batch import ForwardBatch, ForwardMode
 from qwenquest_amd.paged import Fp4TokenToKVPool, Fp8TokenToKVPool
@@ -55,6 +55,49 @@ def test_a_quest_step_with_another_plan_keeps_its_tokens(monkeypatch, cuda, kind
     assert not all(torch.equal(x, y) for x, y in zip(before, got))
     e.be.quest._step.plan = plan
     assert not e.be.forward(q, k, v, e.mods[0], batch).isnan().any()
+
+
+def test_quest_steps_by_their_kind_of_pool(monkeypatch, cuda):
+    """fp8_quest_step and fp4_quest_step are the backend's step, and refuse the other pool."""
+    for kind, own, other in ((Fp8TokenToKVPool, ops.fp8_quest_step, ops.fp4_quest_step), (Fp4TokenToKVPool, ops.fp4_quest_step, ops.fp8_quest_step)):
+        e, b, (q, k, v) = quest_step(monkeypatch, cuda, kind, [700, 63])
+        want = e.be.forward(q, k, v, e.mods[0], b)
+        pos = torch.empty_like(e.be._positions)
+        args = (q, k, v, b.out_cache_loc, e.kvp, 0, e.rtp.block_table, e.be.quest, b.req_pool_indices, pos, e.mods[0].scaling)
+        assert torch.equal(own(*args), want) and torch.equal(pos[:2], e.be._positions[:2])
+        with pytest.raises(ValueError, match="TokenToKVPool"):
+            other(*args)
+
+
+def test_a_pool_that_names_no_kind_holds_8_bit_blocks(cuda):
+    """Any object with an 8-bit pool's attributes serves the 8-bit functions."""
+    pool = Fp8TokenToKVPool(6, 1, 2, 128, cuda)
+    gen = torch.Generator(device=cuda).manual_seed(0)
+    rand = lambda *shape: torch.empty(shape, device=cuda).normal_(generator=gen).bfloat16()  # noqa: E731
+    pool.set_kv_buffer(0, torch.arange(64, 364, device=cuda), rand(300, 2, 128), rand(300, 2, 128))
+    plain = SimpleNamespace(**{x: getattr(pool, x) for x in ("device", "num_blocks", "kv_heads", "head_dim", "num_layers", "k_codes", "k_scale",
+                                                             "layer_args", "new_rows")})
+    table, rpi, n = torch.arange(1, 6, dtype=torch.int32, device=cuda)[None], i64([0], cuda), i64([290], cuda)
+    q = rand(1, 8, 128)
+    want = ops.fp8_decode_attention(q, pool, 0, table, rpi, n, 0.1)
+    plan = ops.fp8_decode_plan(plain, table, rpi, n)
+    assert torch.equal(ops.fp8_decode_attention(q, plain, 0, table, rpi, n, 0.1), want)
+    assert torch.equal(ops.fp8_decode_attention(q, plain, 0, table, rpi, n, 0.1, plan=plan), want)
+    q = rand(20, 8, 128)
+    assert torch.equal(*(ops.fp8_extend_attention(q, p, 0, table, rpi, n, n - 20, i64([20], cuda), 0.1) for p in (pool, plain)))
+    quests = []
+    for p in (pool, plain):
+        quest = QuestAlgorithm(128, 64, cuda)
+        quest.init_storage(0, 1, 1, 320, 2, 128)
+        quest.update_prefill_representations_blocks(rpi, n, p, table)
+        quest.decode_step_blocks(rpi, n, p, table)
+        quests.append(quest)
+    assert torch.equal(quests[0].page_k_bounds[0, 0, :4], quests[1].page_k_bounds[0, 0, :4])
+    args = (q[:1], rand(1, 2, 128), rand(1, 2, 128), i64([64 + 289], cuda))
+    outs = [ops.fp8_quest_step(*args, p, 0, table, x, rpi, torch.empty((1, 128), dtype=torch.int32, device=cuda), 0.1) for p, x in zip((pool, plain), quests)]
+    assert torch.equal(*outs)
+    with pytest.raises(ValueError, match="Fp4TokenToKVPool"):
+        ops.fp4_decode_attention(q[:1], plain, 0, table, rpi, n, 0.1)
 
 
 def test_operators_that_a_trace_would_lose_refuse_it(monkeypatch, cuda):
