@@ -21,7 +21,7 @@ from qwenquest_amd.attention.ops import (
     extend_attention_batch,
     extend_attention_batch_checked,
 )
-from qwenquest_amd.paged import BlockReqToTokenPool, CodedTokenToKVPool, Fp8TokenToKVPool
+from qwenquest_amd.paged import BlockReqToTokenPool, CodedTokenToKVPool
 
 if TYPE_CHECKING:
     from qwenquest_amd.batch import ForwardBatch
@@ -48,9 +48,8 @@ class AttentionBackend(ABC):
     def __init__(self, req_to_token_pool: ReqToTokenPool, token_to_kv_pool: MHATokenToKVPool):
         self.req_to_token_pool = req_to_token_pool
         self.token_to_kv_pool = token_to_kv_pool
-        #: whether the pool holds blocks of codes, in 8 or 4 bits; whether in 8
+        #: whether the pool holds blocks of codes, in 8 or 4 bits
         self.coded = isinstance(token_to_kv_pool, CodedTokenToKVPool)
-        self.fp8 = isinstance(token_to_kv_pool, Fp8TokenToKVPool)
         if self.coded:
             if not isinstance(req_to_token_pool, BlockReqToTokenPool):
                 raise ValueError(f"an {type(token_to_kv_pool).__name__} needs a BlockReqToTokenPool")

@@ -30,7 +30,7 @@
 //   look_up(c, h, blk, blk2, w)   of this lane's unit what there is one word of (w: also of blk2)
 //   load_k(c, h, lane, blk, blk2, from2), load_v(c, h, lane, blk)
 //                                 codes of one unit; K's of tokens before from2 from blk2
-//   load_window_v(c, h, lane, blk2)   a window's second V, over K's registers
+//   load_window_v(c, h, lane, blk2)   a window's second V, in K's registers or its own
 //   kOneFactor                    whether all products take the factor sl2, and weights what weight(t, i, ..) says
 //   begin(j, win, sl2)            the factors of lane j's unit
 //   keys(t, i, k0, k1)            operands of steps 2 i and 2 i + 1 for tokens 16 t ..
@@ -472,7 +472,8 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attend_kernel(DecArgs<typen
       }
     }
     if (!last && u + 1 == c1) load_q(b + 1);
-    // the next unit's K under this one's softmax and values; a window's second V goes there instead
+    // the next unit's K under this one's softmax and values; a window loads its second V instead (which some caches keep
+    // in K's registers)
     if (win) unit.load_window_v(a.c, h, lane, __builtin_amdgcn_readlane(blk2, j));
     else if (!last && !next_set) load_k(j + 1);
     float mx = -INFINITY;
