@@ -18,8 +18,8 @@ from qwenquest_amd.paged import _indexed
 
 __all__ = ["QKNormRotary"]
 
-#: quarter turns of a radian, 2 / pi
-_QUARTERS = 2 / Fraction("3.14159265358979323846264338327950288419716939937510582097494459")
+#: quarter turns of a radian, 2 / pi, by 2^160
+_QUARTERS = round(2**161 / Fraction("3.14159265358979323846264338327950288419716939937510582097494459"))
 _ORDERS = ("blocks", "cycled")
 _PAIRS = ("halves", "neighbours")
 
@@ -85,8 +85,8 @@ class QKNormRotary:
             raise ValueError(f"sections {tuple(left)} must add up to the {count} pairs")
         self.num_heads, self.kv_heads, self.head_dim, self.rotary_dim = num_heads, kv_heads, head_dim, rotary_dim
         self.eps, self.axes, self.neighbours = float(eps), len(left), pairs == "neighbours"
-        # in quarter turns, as the kernel takes angles, each rounded once
-        self._quarters = torch.tensor([float(Fraction(f) * _QUARTERS) for f in freq.tolist()], dtype=torch.float64).to(self.device)
+        # in quarter turns, as the kernel takes angles
+        self._quarters = torch.tensor([_quarter_turns(f) for f in freq.tolist()], dtype=torch.float64).to(self.device)
         self._axis = torch.tensor(_deal(left, section_order == "cycled"), dtype=torch.int32, device=self.device)
         self._weights = [self._weight(w, what) for w, what in ((q_weight, "q_weight"), (k_weight, "k_weight"))]
         # what every call passes, of tensors that stay where they are
@@ -157,6 +157,12 @@ class QKNormRotary:
             _lib.call("qq_qk_norm_rotary", *rows, code, self.num_heads, self.kv_heads, self.head_dim, n, *self._args,
                       pos.data_ptr(), n, self.axes, *(o.data_ptr() for o in outs), *([None] * (3 - outputs)), _lib.stream(dev))
         return outs
+
+
+def _quarter_turns(radians: float) -> float:
+    """``radians`` in quarter turns, by a product of whole numbers: rounded once."""
+    mantissa, exponent = math.frexp(radians)
+    return math.ldexp(float(int(mantissa * 2**53) * _QUARTERS), exponent - 53 - 160)
 
 
 def _deal(left: list[int], cycled: bool) -> list[int]:
