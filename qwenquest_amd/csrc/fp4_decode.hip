@@ -7,9 +7,9 @@
 // scale in the conversion (exact: a code has 2 significand bits), two at a time, NaN for a lost token; V's
 // become bf16 as they are, and a weight takes its token's scale, exact in fp32, before it is cut into three
 // bf16 pieces.  Every product takes the same factor (kOneFactor), so that only units at an edge mask, and the maximum may lag.
-// Bound: 16 requests of 131072 tokens, 4 heads of 128, 207 us, 5.4 TB/s of codes and scales, with the vector units 63 % busy
+// Bound: 16 requests of 131072 tokens, 4 heads of 128, 207 to 211 us, 5.4 TB/s of codes and scales, with the vector units 63 % busy
 // and waves waiting 40 %; 228 with the masks and rescalings in every unit.  A small batch by the chain of round trips, as
-// over the 8-bit cache: one request of 2000 tokens 11.1 us a layer (waiting 80 %), 48 of up to 20000 in fp32 23.0.
+// over the 8-bit cache: one request of 2000 tokens 10.9 us a layer (waiting 79 %), 48 of up to 20000 in fp32 23.1.
 // Quest, 16 requests' 31 pages and window of 131072 tokens 16.8 us with the selection.  Not taken: the next two
 // units in flight instead of one (226 us where this took 214; fp32 spills), rescaling in every unit without the branch (slower), the sign of a
 // negative factor on the queries (3 % at one request: another step before the first product).

@@ -24,12 +24,13 @@
 // rescaling: that goes in two halves, and a tile with an E below kLowE, values under 2^-27, adds weights of their own, 2^kUp times as
 // large (then a token is missing only under 2^-88 of another one; above kLowE under 2^-44).
 //
-// Bound: the matrix cores, near the clock that they hold: 8192 tokens behind 8192, 32 heads on 4 of 128, 1555 to 1615 us (by
-// card): 36 matrix instructions a tile and wave are 1.19 PFLOP/s, where a plain product of 8192^3 reaches 1.225; of the
-// formula's 1.02 to 1.06.  E and 2^(1 - E) by lane exchanges instead of matrix instructions 1953; weights and products one
+// Bound: the matrix cores, near the clock that they hold: 8192 tokens behind 8192, 32 heads on 4 of 128, 1592 to 1664 us (by
+// card): 36 matrix instructions a tile and wave are 1.11 to 1.16 PFLOP/s, where a plain product of 8192^3 reaches 1.225; of the
+// formula's 0.99 to 1.04.  (The sum's range, V scale bytes behind a context and scores past 2^22 take 0.2 %; at 64 channels, 1068 us,
+// where the vector units are the bound, 2 %.)  E and 2^(1 - E) by lane exchanges instead of matrix instructions 1953; weights and products one
 // after the other 1690.  Not taken: the next tile's scores between this one's products (256 registers, 1693), three
 // blocks a CU with the queries in the LDS (1635), wave priorities (no change).  A short batch by its longest request's
-// tiles: 3440 new of 8330 tokens 174 us with the store.
+// tiles: 3440 new of 8330 tokens 174 to 179 us with the store.
 #include "qq_extend_dev.h"
 #include "qq_fp4.h"
 
