@@ -185,10 +185,20 @@ class CodedTokenToKVPool:
         self.head_dim = head_dim
         self.size = num_blocks * BLOCK_TOKENS - 1
         self._allocate((num_layers, num_blocks, kv_heads))
-        # one layer's codes and scales with the geometry, as the C entries take them; the tensors
-        # stay where they are
+        self._bind()
+
+    def _bind(self) -> None:
+        """One layer's codes and scales with the geometry, as the C entries take them; the tensors stay where they are."""
         steps = [(_lib.ptr(t), t.stride(0) * t.element_size()) for t in (self.k_codes, self.v_codes, self.k_scale, self.v_scale)]
-        self._layers = [(*(base + i * step for base, step in steps), num_blocks, kv_heads, head_dim) for i in range(num_layers)]
+        self._layers = [(*(base + i * step for base, step in steps), self.num_blocks, self.kv_heads, self.head_dim)
+                        for i in range(self.num_layers)]
+
+    def __getstate__(self) -> dict:  # addresses hold for this pool's own tensors, not for a copy's or a pickle's
+        return {name: value for name, value in self.__dict__.items() if name != "_layers"}
+
+    def __setstate__(self, state: dict) -> None:
+        self.__dict__.update(state)
+        self._bind()
 
     def _allocate(self, shape: tuple[int, int, int]) -> None:
         raise NotImplementedError

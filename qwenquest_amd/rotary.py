@@ -89,9 +89,19 @@ class QKNormRotary:
         self._quarters = torch.tensor([_quarter_turns(f) for f in freq.tolist()], dtype=torch.float64).to(self.device)
         self._axis = torch.tensor(_deal(left, section_order == "cycled"), dtype=torch.int32, device=self.device)
         self._weights = [self._weight(w, what) for w, what in ((q_weight, "q_weight"), (k_weight, "k_weight"))]
-        # what every call passes, of tensors that stay where they are
-        self._args = (*(_lib.ptr(w) for w in self._weights), self.eps, _lib.ptr(self._quarters), _lib.ptr(self._axis), count,
-                      int(self.neighbours))
+        self._bind()
+
+    def _bind(self) -> None:
+        """What every call passes, of tensors that stay where they are."""
+        self._args = (*(_lib.ptr(w) for w in self._weights), self.eps, _lib.ptr(self._quarters), _lib.ptr(self._axis),
+                      self.rotary_dim // 2, int(self.neighbours))
+
+    def __getstate__(self) -> dict:  # addresses hold for this object's own tensors, not for a copy's or a pickle's
+        return {name: value for name, value in self.__dict__.items() if name != "_args"}
+
+    def __setstate__(self, state: dict) -> None:
+        self.__dict__.update(state)
+        self._bind()
 
     def _weight(self, w: torch.Tensor | None, what: str) -> torch.Tensor | None:
         if w is None:
