@@ -74,13 +74,24 @@ class BlockReqToTokenPool(ReqToTokenPool):
         self.free_count = torch.full((1,), num_blocks - 1, dtype=torch.int32, device=dev)
         # refused calls by reason, never set back; what has been raised of them
         self._err = torch.zeros(len(_REFUSALS), dtype=torch.int32, device=dev)
-        self._err_host = pinned_zeros((len(_REFUSALS),), torch.int32)
         self._raised = [0] * len(_REFUSALS)
+        self._bind()
+
+    def _bind(self) -> None:
+        """The C entries' view of the pool, whose tensors stay where they are, and the counts' mirror."""
+        self._err_host = pinned_zeros((len(_REFUSALS),), torch.int32)
+        self._err_host.copy_(self._err)
         self._err_host_dev = HiSparseCoordinator._device_address(self._err_host)
-        # the C entries' view of the pool, whose tensors stay where they are
         r2t, bt = self.req_to_token, self.block_table
         self._args = (_lib.ptr(bt), bt.stride(0), _lib.ptr(r2t), r2t.stride(0), r2t.shape[1], r2t.shape[0],
                       _lib.ptr(self.held), _lib.ptr(self.free_blocks), _lib.ptr(self.free_count), self.free_blocks.numel())
+
+    def __getstate__(self) -> dict:  # addresses hold for this pool's own tensors, not for a copy's or a pickle's
+        return {name: value for name, value in self.__dict__.items() if name not in ("_args", "_err_host", "_err_host_dev")}
+
+    def __setstate__(self, state: dict) -> None:
+        self.__dict__.update(state)
+        self._bind()
 
     def available_blocks(self) -> int:
         """Free blocks (reads the device: a synchronisation)."""

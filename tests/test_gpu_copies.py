@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from qwenquest_amd import QKNormRotary
-from qwenquest_amd.paged import Fp4TokenToKVPool, Fp8TokenToKVPool
+from qwenquest_amd.paged import BlockReqToTokenPool, Fp4TokenToKVPool, Fp8TokenToKVPool
 
 pytestmark = pytest.mark.gpu
 
@@ -56,3 +56,25 @@ def test_pools(cuda, kind, how):
     pool.set_kv_buffer(1, loc, v, k)
     assert not torch.equal(other.get_rows(1, loc)[0], pool.get_rows(1, loc)[0])
     assert torch.equal(other.get_rows(1, loc)[1], want[1])
+
+
+@pytest.mark.parametrize("how", COPIES)
+def test_request_pools(cuda, how):
+    pool = BlockReqToTokenPool(3, 400, 12, cuda)
+    i64 = lambda *x: torch.tensor(x, device=cuda)  # noqa: E731
+    pool.assign(i64(0, 1), i64(0, 0), i64(100, 70), 170)
+    other = COPIES[how](pool)
+    for x in (pool, other):
+        assert x.available_blocks() == 7 and x.held.tolist() == [2, 2, 0]
+    loc, pos = other.assign(i64(2), i64(0), i64(200), 200)
+    assert other.available_blocks() == 3 and other.held.tolist() == [2, 2, 4] and pos.tolist() == list(range(200))
+    assert torch.equal(other.req_to_token[2, :200].long(), loc) and (loc > 0).all()
+    assert pool.available_blocks() == 7 and pool.held.tolist() == [2, 2, 0] and not pool.block_table[2].any()
+    pool.release(i64(0))
+    assert pool.available_blocks() == 9 and other.available_blocks() == 3 and other.block_table[0, 0] > 0
+    other.assign(i64(0), i64(100), i64(301), 301)  # past its table
+    pool.check_errors()
+    torch.cuda.synchronize()
+    with pytest.raises(ValueError):
+        other.poll_errors()
+    pool.poll_errors()
