@@ -553,8 +553,9 @@ int64_t qq_fp8_extend_workspace_bytes(int64_t n, int bs, int num_q_heads, int kv
  * order (csrc/qq_fp4.h), and scales, each the byte of a power of two's exponent: k_scale
  * [num_blocks, kv_heads, 2 * head_dim], one for each token and 32 channels, v_scale
  * [num_blocks, kv_heads, 64], one for each token; a value is code * 2^(scale - 127).  head_dim 64
- * or 128.  Pool row r is token r % 64 of block r / 64.  What is not said here is as in the 8-bit
- * cache's entry of the same name. */
+ * or 128.  Pool row r is token r % 64 of block r / 64.  The bytes of rows that nobody has written may be
+ * any: they reach no answer but of who attends them.  What is not said here is as in the 8-bit cache's entry of the
+ * same name. */
 
 /* k[i], v[i] ([n, kv_heads, head_dim] bf16 or fp32, 16-byte aligned) go to row loc[i].  The scale
  * of values with largest magnitude m is 2^e, e the least with m <= 7 * 2^e, of K -96 to 125, of V -50 to
